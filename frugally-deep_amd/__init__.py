@@ -37,6 +37,23 @@ class GemmBatch(ctypes.Structure):
         (n, ctypes.c_int64) for n in ("a_outer", "a_inner", "b_outer", "b_inner", "c_outer", "c_inner")]
 
 
+KV_TYPES = {"f32": 0, "bf16": 1}
+
+
+class KvPages(ctypes.Structure):
+    """fdx_kv_pages: a key / value cache in pages.  k, v, table and lens are DevBuf objects (anything with a `ptr`), which the
+    structure keeps alive; kind "f32" or "bf16"."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("type", ctypes.c_int), ("n_pages", ctypes.c_int),
+                ("page_size", ctypes.c_int), ("kv_heads", ctypes.c_int), ("dk", ctypes.c_int), ("dv", ctypes.c_int),
+                ("table", ctypes.c_void_p), ("table_width", ctypes.c_int), ("lens", ctypes.c_void_p), ("n_seqs", ctypes.c_int),
+                ("max_len", ctypes.c_int)]
+
+    def __init__(self, k, v, kind, n_pages, page_size, kv_heads, dk, dv, table, table_width, lens, n_seqs, max_len):
+        super().__init__(k.ptr, v.ptr, KV_TYPES[kind], n_pages, page_size, kv_heads, dk, dv, table.ptr, table_width, lens.ptr, n_seqs,
+                         max_len)
+        self._kept = (k, v, table, lens)
+
+
 class FdxError(RuntimeError):
     pass
 
@@ -56,7 +73,8 @@ def _load():
 lib = _load()
 lib.fdx_last_error.restype = ctypes.c_char_p
 lib.fdx_set_last_error.restype = None
-lib.fdx_mha_scratch_bytes.restype = ctypes.c_size_t
+for _name in ("fdx_mha_scratch_bytes", "fdx_mha_packed_scratch_bytes", "fdx_mha_paged_scratch_bytes", "fdx_token_logprobs_scratch_bytes"):
+    getattr(lib, _name).restype = ctypes.c_size_t
 
 
 def check(status):
@@ -584,6 +602,115 @@ def mha_decode(q, k_cache, v_cache, heads, dk, dv, length):
     out = DevBuf(4 * b * heads * dv)
     check(lib.fdx_mha_decode_f32(_dp(dq), _dp(dkc), _dp(dvc), b, heads, dk, dv, length, max_len, _dp(out)))
     return out.to_host((b, heads * dv))
+
+
+def _row_starts(lengths):
+    return DevBuf.from_host(np.concatenate([[0], np.cumsum(lengths)]).astype(np.int32), np.int32)
+
+
+def _raise_if_set(flag, message):
+    if flag.to_host((1,), np.int32)[0]:
+        raise FdxError(message)
+
+
+def mha_packed(q, k, v, lengths, heads, kv_heads, dk, dv, causal=True):
+    """q [tokens,heads*dk], k [tokens,kv_heads*dk], v [tokens,kv_heads*dv]: sequences of `lengths` rows, one behind the other."""
+    q, k, v = (np.ascontiguousarray(a, np.float32) for a in (q, k, v))
+    tokens = q.shape[0]
+    dq, dk_, dv_, starts = DevBuf.from_host(q), DevBuf.from_host(k), DevBuf.from_host(v), _row_starts(lengths)
+    scratch = DevBuf(lib.fdx_mha_packed_scratch_bytes(tokens, len(lengths), heads, kv_heads, dk, dv))
+    out, flag = DevBuf.from_host(np.zeros((tokens, heads * dv), np.float32)), DevBuf.from_host(np.zeros(1, np.int32), np.int32)
+    i64 = ctypes.c_int64
+    check(lib.fdx_mha_packed_f32(_dp(dq), i64(heads * dk), _dp(dk_), i64(kv_heads * dk), _dp(dv_), i64(kv_heads * dv), starts.ptr,
+                                 len(lengths), tokens, heads, kv_heads, dk, dv, int(causal), _dp(out), i64(heads * dv), scratch.ptr, flag.ptr))
+    _raise_if_set(flag, "lengths of the packed sequences exceed the rows")
+    return out.to_host((tokens, heads * dv))
+
+
+class PagedCache:
+    """Keys and values of several sequences in pages of device memory, for kv_append and mha_paged.  A sequence takes pages as it
+    grows and gives them back with release(); the page table lives on the host and goes to the device when it has changed."""
+
+    def __init__(self, n_pages, page_size, kv_heads, dk, dv, n_seqs, max_len, kind="f32"):
+        self.n_pages, self.page_size, self.kv_heads, self.dk, self.dv = n_pages, page_size, kv_heads, dk, dv
+        self.n_seqs, self.max_len, self.kind = n_seqs, max_len, kind
+        size = 4 if kind == "f32" else 2
+        rows = n_pages * page_size * kv_heads
+        self.k, self.v = (DevBuf.from_host(np.zeros(rows * d * size, np.uint8), np.uint8) for d in (dk, dv))
+        self.table = np.full((n_seqs, -(-max_len // page_size)), -1, np.int32)
+        self.lens = np.zeros(n_seqs, np.int32)
+        self.free = list(range(n_pages - 1, -1, -1))
+
+    def grow(self, lengths):
+        """Makes room for lengths[i] more positions of sequence i."""
+        want = self.lens + np.asarray(lengths, np.int32)
+        if want.max() > self.max_len:
+            raise FdxError("a sequence of %d positions in a cache of at most %d" % (want.max(), self.max_len))
+        need = [max(0, -(-int(w) // self.page_size) - int((row >= 0).sum())) for w, row in zip(want, self.table)]
+        if sum(need) > len(self.free):
+            raise FdxError("the cache has %d free pages, %d are needed" % (len(self.free), sum(need)))
+        for row, count in zip(self.table, need):
+            used = int((row >= 0).sum())
+            for j in range(used, used + count):
+                row[j] = self.free.pop()
+        self.lens = want
+
+    def release(self, seq):
+        self.free += [int(page) for page in self.table[seq] if page >= 0]
+        self.table[seq], self.lens[seq] = -1, 0
+
+    def pages(self):
+        """The cache as the entry points take it (fdx_kv_pages)."""
+        return KvPages(self.k, self.v, self.kind, self.n_pages, self.page_size, self.kv_heads, self.dk, self.dv,
+                       DevBuf.from_host(self.table, np.int32), self.table.shape[1], DevBuf.from_host(self.lens, np.int32), self.n_seqs,
+                       self.max_len)
+
+
+def kv_append(cache, k, v, lengths):
+    """Adds lengths[i] rows of k [tokens,kv_heads*dk] and v [tokens,kv_heads*dv] to sequence i of a PagedCache."""
+    k, v = np.ascontiguousarray(k, np.float32), np.ascontiguousarray(v, np.float32)
+    cache.grow(lengths)
+    dk_, dv_, starts, pages = DevBuf.from_host(k), DevBuf.from_host(v), _row_starts(lengths), cache.pages()
+    flag = DevBuf.from_host(np.zeros(1, np.int32), np.int32)
+    check(lib.fdx_kv_append_f32(_dp(dk_), ctypes.c_int64(k.shape[1]), _dp(dv_), ctypes.c_int64(v.shape[1]), starts.ptr, k.shape[0],
+                                ctypes.byref(pages), flag.ptr))
+    _raise_if_set(flag, "rows outside the cache")
+
+
+def mha_paged(cache, q, lengths, heads):
+    """Attention of the last lengths[i] positions of sequence i, whose queries are rows of q [tokens,heads*dk], over its pages."""
+    q = np.ascontiguousarray(q, np.float32)
+    tokens, most = q.shape[0], int(max(lengths))
+    dq, starts, pages = DevBuf.from_host(q), _row_starts(lengths), cache.pages()
+    scratch = DevBuf(lib.fdx_mha_paged_scratch_bytes(tokens, most, heads, ctypes.byref(pages)))
+    out = DevBuf.from_host(np.zeros((tokens, heads * cache.dv), np.float32))
+    flag = DevBuf.from_host(np.zeros(1, np.int32), np.int32)
+    check(lib.fdx_mha_paged_f32(_dp(dq), ctypes.c_int64(q.shape[1]), starts.ptr, tokens, most, heads, ctypes.byref(pages), _dp(out),
+                                ctypes.c_int64(heads * cache.dv), scratch.ptr, flag.ptr))
+    _raise_if_set(flag, "positions outside the cache")
+    return out.to_host((tokens, heads * cache.dv))
+
+
+def token_logprobs(logits, ids=None, top=0):
+    """logits [rows,vocab]; returns a dict of logprobs [rows] (if ids are given; 0 where an id is negative), entropy [rows],
+    top_ids and top_logprobs [rows,top] (if top > 0)."""
+    logits = np.ascontiguousarray(logits, np.float32)
+    rows, vocab = logits.shape
+    dx = DevBuf.from_host(logits)
+    di = None if ids is None else DevBuf.from_host(ids, np.int32)
+    dl, de = (None if ids is None else DevBuf(4 * rows)), DevBuf(4 * rows)
+    dti, dtl = (DevBuf(4 * rows * top), DevBuf(4 * rows * top)) if top else (None, None)
+    scratch = DevBuf(lib.fdx_token_logprobs_scratch_bytes(ctypes.c_int64(rows), vocab, top))
+    flag = DevBuf.from_host(np.zeros(1, np.int32), np.int32)
+    check(lib.fdx_token_logprobs_f32(_dp(dx), ctypes.c_int64(vocab), ctypes.c_int64(rows), vocab, di and di.ptr, top, _dp(dl), _dp(de),
+                                     dti and dti.ptr, _dp(dtl), scratch.ptr, flag.ptr))
+    _raise_if_set(flag, "token ids must be less than the number of logits")
+    out = {"entropy": de.to_host((rows,))}
+    if ids is not None:
+        out["logprobs"] = dl.to_host((rows,))
+    if top:
+        out.update(top_ids=dti.to_host((rows, top), np.int32), top_logprobs=dtl.to_host((rows, top)))
+    return out
 
 
 # ------------------------------------------------------------------ whole models

@@ -1,0 +1,95 @@
+// Where the rows of ragged batches lie: spans of packed rows, tiles of them, places in a paged cache.  Plain integer
+// arithmetic on numbers that device memory holds and nobody has checked: whatever they are, what comes out is in range.
+#pragma once
+#include <cstdint>
+
+#if defined(__HIPCC__)
+#define FDX_HD __host__ __device__ __forceinline__
+#else
+#define FDX_HD inline
+#endif
+
+namespace fdx {
+
+struct Span {
+    int first, count;
+};
+
+// rows starts[i] .. starts[i + 1] - 1, cut to 0 .. tokens - 1
+FDX_HD Span packed_span(const int32_t* starts, int i, int tokens)
+{
+    int a = starts[i], b = starts[i + 1];
+    a = a < 0 ? 0 : (a > tokens ? tokens : a);
+    b = b < a ? a : (b > tokens ? tokens : b);
+    return { a, b - a };
+}
+
+FDX_HD bool packed_start_ok(const int32_t* starts, int i, int tokens)
+{
+    return starts[i] >= 0 && starts[i] <= starts[i + 1] && starts[i + 1] <= tokens;
+}
+
+// Tiles of `rows` rows over sequences that bring `per_token` rows a token, without a pass that adds up lengths: sequence i owns
+// the numbers from starts[i] * per_token / rows + i up to the next sequence's, which are at least as many as it has tiles
+// (floor(x + y) + 1 - floor(x) >= ceil(y)).  The numbers that are left over are no tile.
+FDX_HD int64_t first_tile(int start, int i, int per_token, int rows) { return (int64_t)start * per_token / rows + i; }
+
+FDX_HD int64_t tile_numbers(int tokens, int n_seqs, int per_token, int rows) { return first_tile(tokens, n_seqs, per_token, rows); }
+
+struct Tile {
+    int seq, index; // sequence (-1: no tile), tile inside it
+    Span span;
+};
+
+FDX_HD Tile find_tile(const int32_t* starts, int n_seqs, int tokens, int per_token, int rows, int64_t number)
+{
+    int lo = 0, hi = n_seqs; // the last sequence whose first number is not above `number`, if there is one
+    while (lo < hi) {
+        const int mid = lo + (hi - lo) / 2;
+        const int a = starts[mid];
+        if (first_tile(a < 0 ? 0 : (a > tokens ? tokens : a), mid, per_token, rows) <= number)
+            lo = mid + 1;
+        else
+            hi = mid;
+    }
+    Tile t { lo - 1, 0, { 0, 0 } };
+    if (t.seq < 0)
+        return t;
+    t.span = packed_span(starts, t.seq, tokens);
+    const int64_t index = number - first_tile(t.span.first, t.seq, per_token, rows);
+    if (index < 0 || index * rows >= (int64_t)t.span.count * per_token)
+        t.seq = -1;
+    t.index = (int)index;
+    return t;
+}
+
+// the sequence that row `row` belongs to, -1 if none
+FDX_HD int find_row(const int32_t* starts, int n_seqs, int tokens, int row)
+{
+    int lo = 0, hi = n_seqs;
+    while (lo < hi) {
+        const int mid = lo + (hi - lo) / 2;
+        if (starts[mid] <= row)
+            lo = mid + 1;
+        else
+            hi = mid;
+    }
+    if (lo == 0)
+        return -1;
+    const Span s = packed_span(starts, lo - 1, tokens);
+    return row >= s.first && row - s.first < s.count ? lo - 1 : -1;
+}
+
+// row of position `pos` among the rows of all pages, -1 if the table does not reach it or names no page of the cache
+FDX_HD int page_row(const int32_t* table_row, int table_width, int n_pages, int page_size, int pos)
+{
+    if (pos < 0)
+        return -1;
+    const int at = (int)((uint32_t)pos / (uint32_t)page_size);
+    if (at >= table_width)
+        return -1;
+    const int page = table_row[at];
+    return page < 0 || page >= n_pages ? -1 : page * page_size + (pos - at * page_size);
+}
+
+} // namespace fdx

@@ -345,6 +345,86 @@ fdx_status fdx_mha_prefill_f32(const float* q, const float* k, const float* v, i
 fdx_status fdx_mha_decode_f32(const float* q, const float* k_cache, const float* v_cache, int batch, int heads,
     int dk, int dv, int len, int max_len, float* out);
 
+/*
+ * Attention inside each of several sequences whose rows lie one behind the other (packed prompts), without padding and with
+ * key / value heads shared by groups of query heads; no counterpart in the reference, whose layer takes one sequence at a
+ * time and as many key heads as query heads (layers/multi_head_attention_layer.hpp:74-95).
+ *   out[t][h][:] = sum_s softmax_s(q[t][h] . k[s][h'] / sqrt(dk)) * v[s][h'],  h' = h / (heads / kv_heads),
+ * s over the rows of t's sequence, up to t itself if `causal` is not 0.
+ * q [tokens][heads*dk], k [tokens][kv_heads*dk], v [tokens][kv_heads*dv], out [tokens][heads*dv], rows ldq / ldk / ldv / ldo
+ * floats apart.  starts: n_seqs + 1 row numbers in device memory, ascending; sequence i has rows starts[i] .. starts[i+1]-1,
+ * none if they are equal.  Rows of `out` that belong to no sequence stay as they are.  Depths up to 128.
+ * scratch_dev: fdx_mha_packed_scratch_bytes bytes, 16-byte aligned, left to the call until its work has completed; its
+ * contents before and after mean nothing.  Two calls that may overlap need two.
+ * error_flag_dev (may be NULL) is set to 1 on the device if `starts` descends or leaves 0 .. tokens; what it holds else is
+ * left alone.  Such starts are cut to the range, so nothing outside the tensors is read or written.
+ * `out` must not overlap an input.
+ */
+size_t fdx_mha_packed_scratch_bytes(int tokens, int n_seqs, int heads, int kv_heads, int dk, int dv);
+fdx_status fdx_mha_packed_f32(const float* q, int64_t ldq, const float* k, int64_t ldk, const float* v, int64_t ldv,
+    const int32_t* starts, int n_seqs, int tokens, int heads, int kv_heads, int dk, int dv, int causal, float* out, int64_t ldo,
+    void* scratch_dev, int* error_flag_dev);
+
+/*
+ * A key / value cache in pages.  Position p of sequence i lies in page table[i][p / page_size] at row p % page_size; a page
+ * holds page_size rows of kv_heads * dk keys (k) and of kv_heads * dv values (v), both of element type `type`: fp32, or bf16 for
+ * half the memory and half the traffic (rounded to nearest when written, widened when read; all sums stay fp32).  Sequences
+ * may share pages that hold the same prefix.  All pointers are device memory; the structure itself is read during the call.
+ * lens[i]: positions of sequence i, those of the call's new tokens included.  max_len: no sequence is longer; it sizes the
+ * launch and has to be covered by the table (max_len <= table_width * page_size).  n_pages * page_size < 2^31.
+ */
+enum { FDX_KV_F32 = 0, FDX_KV_BF16 = 1 };
+typedef struct fdx_kv_pages {
+    void* k;
+    void* v;
+    int type;                         /* FDX_KV_*                                    */
+    int n_pages, page_size;
+    int kv_heads, dk, dv;
+    const int32_t* table;             /* [n_seqs][table_width]                       */
+    int table_width;
+    const int32_t* lens;              /* [n_seqs]                                    */
+    int n_seqs, max_len;
+} fdx_kv_pages;
+/*
+ * Writes the keys and values of new tokens into the pages.  Sequence i brings rows starts[i] .. starts[i+1]-1 of k and v (none
+ * if they are equal), as its last positions: row starts[i] + j goes to position lens[i] - (starts[i+1] - starts[i]) + j.
+ * k [tokens][kv_heads*dk], v [tokens][kv_heads*dv], rows ldk / ldv floats apart.  No two rows of one call may have the same
+ * place.  A row whose position is negative or not below max_len, or whose page number is not one of the cache, is not
+ * written; error_flag_dev (may be NULL) is set to 1 on the device for it, and for `starts` as fdx_mha_packed_f32 does.
+ */
+fdx_status fdx_kv_append_f32(const float* k, int64_t ldk, const float* v, int64_t ldv, const int32_t* starts, int tokens,
+    const fdx_kv_pages* cache, int* error_flag_dev);
+/*
+ * Attention of every sequence's newest tokens (one in a decode step, more for a chunk of a prompt or for tokens to verify) over
+ * all of its positions in the pages: new token j of n sees positions 0 .. lens[i] - n + j, its own and those in front.
+ * q [tokens][heads*dk], out [tokens][heads*dv], rows ldq / ldo floats apart, sequence i's rows starts[i] .. starts[i+1]-1 as
+ * above; heads / kv_heads query heads share a key head.  max_new: no sequence has more new tokens; it sizes the launch.
+ * A token that sees no position (lens[i] < n) gets zeros; rows that belong to no sequence stay as they are.  Positions whose page
+ * number is not one of the cache are left out of the sums, lens beyond max_len and tokens beyond max_new are cut, and
+ * error_flag_dev (may be NULL) is set to 1 on the device.  Depths up to 128.  scratch_dev as for fdx_mha_packed_f32, of
+ * fdx_mha_paged_scratch_bytes bytes; `out` must not overlap an input.
+ */
+size_t fdx_mha_paged_scratch_bytes(int tokens, int max_new, int heads, const fdx_kv_pages* cache);
+fdx_status fdx_mha_paged_f32(const float* q, int64_t ldq, const int32_t* starts, int tokens, int max_new, int heads,
+    const fdx_kv_pages* cache, float* out, int64_t ldo, void* scratch_dev, int* error_flag_dev);
+
+/*
+ * What a program reports or decides with besides the greedy token: per row of logits, with p = softmax(row),
+ *   logprobs[r]          = log p[ids[r]]        (0 for a negative id, "no token here": a padded place of a batch)
+ *   entropy[r]           = -sum_i p[i] log p[i]
+ *   top_ids[r][0..top)   = the likeliest tokens, by descending logit, equal logits by ascending id
+ *   top_logprobs[r][j]   = log p[top_ids[r][j]]
+ * logits [rows][vocab], rows ld floats apart.  ids and logprobs are both NULL or both given, entropy may be NULL, top_ids and
+ * top_logprobs are NULL exactly if top is 0; top <= 32 and top <= vocab.  Logits of -infinity are tokens ruled out: probability
+ * 0, no share of the entropy; a row of nothing else has entropy 0 and log probabilities of -infinity.  A row that holds a NaN or
+ * +infinity gets NaN everywhere but in top_ids (NaN counts as the lowest logit there).  An id of vocab or more gets NaN and sets
+ * error_flag_dev (may be NULL) to 1 on the device.  scratch_dev as for fdx_mha_packed_f32, of
+ * fdx_token_logprobs_scratch_bytes bytes.  (The reference's softmax and its log: include/fdeep/tensor.hpp:1165-1192.)
+ */
+size_t fdx_token_logprobs_scratch_bytes(int64_t rows, int vocab, int top);
+fdx_status fdx_token_logprobs_f32(const float* logits, int64_t ld, int64_t rows, int vocab, const int32_t* ids, int top,
+    float* logprobs, float* entropy, int32_t* top_ids, float* top_logprobs, void* scratch_dev, int* error_flag_dev);
+
 /* TF window geometry shared by conv and pooling (include/fdeep/convolution.hpp:320-396):
  * padding 0 valid, 1 same, 2 causal; geom = pad_top, pad_bottom, pad_left, pad_right, out_h, out_w */
 fdx_status fdx_window_geometry(int in_h, int in_w, int k_h, int k_w, int s_h, int s_w, int padding, int* geom);

@@ -1,0 +1,101 @@
+// The arithmetic of ragged batches and page tables on host memory, with whatever numbers a caller's device memory might hold: run
+// under the address sanitizer, every array exactly as long as the device's.
+#include <climits>
+#include <cstdio>
+#include <random>
+#include <vector>
+
+#include "kv_pages.hpp"
+
+using namespace fdx;
+
+#define CHECK(c)                                                                                                                          \
+    do {                                                                                                                                  \
+        if (!(c)) {                                                                                                                       \
+            std::printf("failed at line %d: %s\n", __LINE__, #c);                                                                         \
+            return 1;                                                                                                                     \
+        }                                                                                                                                 \
+    } while (0)
+
+int main()
+{
+    std::mt19937 rng(7);
+    auto upto = [&](int n) { return (int)(rng() % (unsigned)(n + 1)); };
+    // ascending starts: every tile of every sequence has exactly one number, every row its sequence
+    for (int round = 0; round < 3000; ++round) {
+        const int n = 1 + upto(9), per_token = 1 + upto(7), rows = 1 << upto(7);
+        std::vector<int32_t> starts(n + 1);
+        starts[0] = upto(3) == 0 ? upto(20) : 0;
+        for (int i = 0; i < n; ++i)
+            starts[i + 1] = starts[i] + (upto(2) == 0 ? 0 : upto(1 << upto(9)));
+        const int tokens = starts[n] + (upto(1) ? upto(30) : 0);
+        std::vector<std::vector<int>> seen(n);
+        for (int i = 0; i < n; ++i)
+            seen[i].assign((((int64_t)starts[i + 1] - starts[i]) * per_token + rows - 1) / rows, 0);
+        for (int64_t number = 0; number < tile_numbers(tokens, n, per_token, rows); ++number) {
+            const Tile t = find_tile(starts.data(), n, tokens, per_token, rows, number);
+            if (t.seq >= 0) {
+                CHECK(t.index >= 0 && t.index < (int)seen[t.seq].size());
+                CHECK(t.span.first == starts[t.seq] && t.span.count == starts[t.seq + 1] - starts[t.seq]);
+                ++seen[t.seq][t.index];
+            }
+        }
+        for (const auto& s : seen)
+            for (int count : s)
+                CHECK(count == 1);
+        for (int row = 0; row < tokens; ++row) {
+            const int s = find_row(starts.data(), n, tokens, row);
+            bool any = false;
+            for (int i = 0; i < n; ++i)
+                any = any || (row >= starts[i] && row < starts[i + 1]);
+            CHECK(any == (s >= 0));
+            if (s >= 0)
+                CHECK(row >= starts[s] && row < starts[s + 1]);
+        }
+        for (int i = 0; i < n; ++i)
+            CHECK(packed_start_ok(starts.data(), i, tokens));
+    }
+    // any starts at all: what comes out lies in the tensors
+    const int32_t odd[] = { INT_MIN, -1, 0, 1, 5, 17, 64, 65, 1000, INT_MAX };
+    for (int round = 0; round < 20000; ++round) {
+        const int n = 1 + upto(5), per_token = 1 + upto(7), rows = 1 << upto(7), tokens = 1 + upto(70);
+        std::vector<int32_t> starts(n + 1);
+        for (auto& s : starts)
+            s = odd[upto(9)];
+        for (int64_t number = 0; number < tile_numbers(tokens, n, per_token, rows); ++number) {
+            const Tile t = find_tile(starts.data(), n, tokens, per_token, rows, number);
+            if (t.seq < 0)
+                continue;
+            CHECK(t.seq < n && t.index >= 0 && t.span.first >= 0 && t.span.count > 0 && t.span.first + t.span.count <= tokens);
+            CHECK((int64_t)t.index * rows < (int64_t)t.span.count * per_token);
+        }
+        for (int row = 0; row < tokens; ++row) {
+            const int s = find_row(starts.data(), n, tokens, row);
+            CHECK(s < n);
+            if (s >= 0) {
+                const Span span = packed_span(starts.data(), s, tokens);
+                CHECK(row >= span.first && row < span.first + span.count && span.first + span.count <= tokens);
+            }
+        }
+    }
+    // any page numbers and positions: a row of the cache or -1
+    for (int round = 0; round < 20000; ++round) {
+        const int width = 1 + upto(6), page_size = 1 + upto(70), n_pages = 1 + upto(9);
+        std::vector<int32_t> table(width);
+        for (auto& t : table)
+            t = upto(3) == 0 ? odd[upto(9)] : upto(n_pages);
+        const int32_t positions[] = { INT_MIN, -1, 0, page_size - 1, page_size, width * page_size - 1, width * page_size, INT_MAX, upto(500) };
+        for (int pos : positions) {
+            const int row = page_row(table.data(), width, n_pages, page_size, pos);
+            const bool there = pos >= 0 && pos / page_size < width && table[pos / page_size] >= 0 && table[pos / page_size] < n_pages;
+            CHECK(there == (row >= 0));
+            if (there)
+                CHECK(row == table[pos / page_size] * page_size + pos % page_size && row < n_pages * page_size);
+        }
+    }
+    // the largest cache
+    const int32_t last[] = { (1 << 27) - 1 };
+    CHECK(page_row(last, 1, (1 << 27) - 1 + 1, 15, 14) == (int)(((int64_t)(1 << 27) - 1) * 15 + 14));
+    std::printf("kv_pages done\n");
+    return 0;
+}

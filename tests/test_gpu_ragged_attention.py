@@ -1,0 +1,423 @@
+"""Attention over packed prompts and over paged caches, and the writing of such caches, against plain sums in 64 bits.
+
+Bounds.  fp32 operands may be held as two fp16 numbers (22 bits) for the matrix instructions: a product is off by at most
+3 * 2^-22 of its size, a score of dk products of unit operands by about 0.64 sqrt(dk) 2^-22 * 3 / sqrt(dk) (independent signs) = 5e-7
+absolute, which is the relative error of a probability; the sums of the output add as much again, and both average out over the
+keys.  1e-6 in the 2-norm, and 1e-5 of the largest value for any single output, leave a factor of two over that.  Scores k times
+larger carry k times the error.  bf16 caches: the reference takes the rounded keys and values, so the bounds are the same."""
+import ctypes
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+def bf16(x):
+    """fp32 values rounded to the nearest bf16, ties to even"""
+    b = np.ascontiguousarray(x, np.float32).view(np.uint32)
+    return ((b + 0x7fff + ((b >> 16) & 1)) & 0xffff0000).astype(np.uint32).view(np.float32)
+
+
+def attend(q, k, v, heads, kv_heads, sees):
+    """q [n][heads*dk], k [keys][kv*dk], v [keys][kv*dv]; query i sees the first sees[i] keys; in 64 bits"""
+    n, keys = q.shape[0], k.shape[0]
+    q = q.astype(np.float64).reshape(n, heads, q.shape[1] // heads)
+    k, v = (a.astype(np.float64).reshape(keys, kv_heads, a.shape[1] // kv_heads) for a in (k, v))
+    out = np.zeros((n, heads, v.shape[2]))
+    for h in range(heads):
+        kh, vh = k[:, h * kv_heads // heads], v[:, h * kv_heads // heads]
+        x = q[:, h] @ kh.T / np.sqrt(q.shape[2])
+        for i in range(n):
+            if sees[i] > 0:
+                e = np.exp(x[i, :sees[i]] - x[i, :sees[i]].max())
+                out[i, h] = e / e.sum() @ vh[:sees[i]]
+    return out.reshape(n, heads * v.shape[2])
+
+
+def close(got, want, bound=1e-6):
+    norm = np.linalg.norm(want)
+    err, worst = np.linalg.norm(got - want) / max(norm, 1e-30), np.abs(got - want).max() / max(np.abs(want).max(), 1e-30)
+    print("relative error %.2e, largest %.2e" % (err, worst), flush=True)
+    assert err <= bound and worst <= 10 * bound, (err, worst)
+
+
+def packed_reference(q, k, v, lengths, heads, kv_heads, causal):
+    out, at = [], 0
+    for n in lengths:
+        rows = slice(at, at + n)
+        out.append(attend(q[rows], k[rows], v[rows], heads, kv_heads, np.arange(n) + 1 if causal else np.full(n, n)))
+        at += n
+    return np.concatenate(out)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lengths,heads,kv_heads,dk,dv", [
+    ([1], 1, 1, 64, 64), ([2, 1, 1], 3, 1, 64, 64), ([37], 12, 12, 64, 64), ([0, 5, 0, 0, 64, 65, 1, 0], 8, 2, 64, 64),
+    ([129, 31, 200], 4, 4, 128, 128), ([300], 7, 1, 128, 128), ([127, 128, 129], 10, 5, 80, 80), ([63, 190], 6, 6, 32, 32),
+    ([70, 11], 4, 2, 96, 64), ([70, 11], 4, 2, 40, 128), ([33, 90], 3, 1, 1, 1), ([33, 90], 6, 2, 13, 7), ([400], 2, 2, 127, 125),
+    ([600, 10, 513], 2, 1, 64, 64)])
+def test_packed(fdx, lengths, heads, kv_heads, dk, dv, causal):
+    print("packed", lengths, heads, kv_heads, dk, dv, causal, flush=True)
+    r, tokens = np.random.default_rng(sum(lengths) + dk), sum(lengths)
+    q, k, v = (r.standard_normal((tokens, h * d)).astype(np.float32) for h, d in ((heads, dk), (kv_heads, dk), (kv_heads, dv)))
+    close(fdx.mha_packed(q, k, v, lengths, heads, kv_heads, dk, dv, causal), packed_reference(q, k, v, lengths, heads, kv_heads, causal))
+
+
+def test_packed_scores_of_a_few_hundred(fdx):
+    """The running maximum moves from tile to tile; scores 40 times larger, errors too."""
+    r, lengths = np.random.default_rng(3), [333, 50]
+    q, k, v = (r.standard_normal((383, h * 64)).astype(np.float32) for h in (8, 2, 2))
+    close(fdx.mha_packed(40 * q, k, v, lengths, 8, 2, 64, 64), packed_reference(40 * q, k, v, lengths, 8, 2, True), 4e-5)
+    # and one that climbs all the way: every key beats those in front of it
+    k[:, :64] = q[:, :64] * 0 + 1
+    k[:, 0] = np.arange(383) * 8
+    q[:, ::64] = 1
+    close(fdx.mha_packed(q, k, v, lengths, 8, 2, 64, 64), packed_reference(q, k, v, lengths, 8, 2, True), 4e-5)
+
+
+@pytest.mark.parametrize("eq,ek,ev", [(0, 0, 0), (60, -60, 0), (-60, 60, 0), (-100, 100, 0), (0, 0, 100), (0, 0, -100), (-40, -80, 5), (110, -110, 110)])
+def test_packed_sizes_of_operands(fdx, eq, ek, ev):
+    """Operands far from one in size: scaled by powers of two, the result scales."""
+    r, lengths = np.random.default_rng(5), [200, 41]
+    q, k, v = (r.standard_normal((241, h * 64)).astype(np.float32) for h in (4, 2, 2))
+    q, k, v = (np.ldexp(a, e).astype(np.float32) for a, e in ((q, eq), (k, ek), (v, ev)))
+    got = fdx.mha_packed(q, k, v, lengths, 4, 2, 64, 64)
+    close(np.ldexp(got.astype(np.float64), -ev), packed_reference(q, k, np.ldexp(v.astype(np.float64), -ev), lengths, 4, 2, True))
+
+
+def test_packed_rows_of_mixed_sizes(fdx):
+    """Keys and values whose sizes differ by 2^15 from row to row and by 2^12 from depth to depth keep the bound of their own size:
+    every query sees its own key only (scores of +-200 apart), so a result is one row of values."""
+    r, n = np.random.default_rng(6), 160
+    q, k = np.zeros((n, 64), np.float32), np.zeros((n, 64), np.float32)
+    angle = 2 * np.pi * np.arange(n) / n
+    q[:, 0], q[:, 1] = np.cos(angle), np.sin(angle)
+    k[:, :2], q = q[:, :2] * 1000, q * 10000
+    v = (r.standard_normal((n, 64)) * 2.0 ** r.integers(-7, 8, (n, 1)) * 2.0 ** r.integers(-6, 7, (1, 64))).astype(np.float32)
+    got, want = fdx.mha_packed(q, k, v, [n], 1, 1, 64, 64, False), packed_reference(q, k, v, [n], 1, 1, False)
+    size = np.abs(want).max(1, keepdims=True)
+    print("worst row", (np.abs(got - want) / size).max(), flush=True)
+    assert (np.abs(got - want) <= 1e-6 * size).all()
+
+
+def test_packed_infinities_and_nan(fdx):
+    """A NaN or infinity reaches the queries that see it and no other, whatever tile they share."""
+    r, lengths, heads, kv = np.random.default_rng(8), [90, 150, 40], 4, 2
+    q, k, v = (r.standard_normal((280, h * 64)).astype(np.float32) for h in (heads, kv, kv))
+    base = packed_reference(q, k, v, lengths, heads, kv, True)
+    for what in (np.nan, np.inf, -np.inf):
+        for name, row, first, last in (("v", 120, 120, 240), ("k", 120, 120, 240), ("q", 100, 100, 101), ("v", 279, 279, 280), ("k", 0, 0, 90)):
+            print("packed odd", what, name, row, flush=True)
+            qq, kk, vv = q.copy(), k.copy(), v.copy()
+            dict(q=qq, k=kk, v=vv)[name][row, 64 + 3] = what   # query head 1 / key head 1
+            got = fdx.mha_packed(qq, kk, vv, lengths, heads, kv, 64, 64).reshape(280, heads, 64)
+            hit = np.zeros((280, heads, 64), bool)
+            if name == "v":
+                hit[first:last, 2:, 3] = True
+            else:
+                hit[first:last, (slice(1, 2) if name == "q" else slice(2, 4))] = True
+            with np.errstate(all="ignore"):
+                want = packed_reference(qq, kk, vv, lengths, heads, kv, True).reshape(280, heads, 64)
+            close(got[~hit], base.reshape(280, heads, 64)[~hit])
+            seen = want[hit]
+            if name == "v":
+                assert np.array_equal(np.isnan(got[hit]), np.isnan(seen)) and np.array_equal(got[hit][np.isinf(seen)], seen[np.isinf(seen)])
+            else:   # scores of -infinity drop a key, those of +infinity and NaN leave nothing
+                assert np.array_equal(np.isnan(got[hit]), np.isnan(seen))
+                close(got[hit][~np.isnan(seen)], seen[~np.isnan(seen)]) if (~np.isnan(seen)).any() else None
+
+
+def call_packed(fdx, q, ldq, k, ldk, v, ldv, starts, tokens, heads, kv, dk, dv, out, ldo, causal=True):
+    """The entry point itself: byte offsets of 4 behind the buffers' starts are kept."""
+    i64, n_seqs = ctypes.c_int64, len(starts) - 1
+    d_starts, flag = fdx.DevBuf.from_host(np.asarray(starts, np.int32), np.int32), fdx.DevBuf.from_host(np.zeros(1, np.int32), np.int32)
+    scratch = fdx.DevBuf(fdx.lib.fdx_mha_packed_scratch_bytes(tokens, n_seqs, heads, kv, dk, dv))
+    fdx.check(fdx.lib.fdx_mha_packed_f32(q, i64(ldq), k, i64(ldk), v, i64(ldv), d_starts.ptr, n_seqs, tokens, heads, kv, dk, dv, int(causal), out,
+                                         i64(ldo), scratch.ptr, flag.ptr))
+    fdx.sync()
+    return int(flag.to_host((1,), np.int32)[0])
+
+
+@pytest.mark.parametrize("shift,pad", [(0, 4), (1, 4), (0, 3), (2, 1), (3, 0)])
+@pytest.mark.parametrize("dk,dv", [(64, 64), (128, 128)])
+def test_packed_strides_and_alignment(fdx, shift, pad, dk, dv):
+    """q, k and v as column blocks of one projection that starts `shift` floats behind an aligned address, rows `pad` floats apart;
+    rows in front of and behind the sequences, and the gaps between rows of the output, stay as they were."""
+    heads, kv, lengths, before, behind = 4, 2, [70, 0, 135], 3, 5
+    r, tokens = np.random.default_rng(shift), before + 205 + behind
+    width = (heads + kv) * dk + kv * dv + pad
+    x = r.standard_normal((tokens, width)).astype(np.float32)
+    buf = fdx.DevBuf.from_host(np.concatenate([np.zeros(shift, np.float32), x.ravel()]))
+    ldo = heads * dv + pad
+    out = fdx.DevBuf.from_host(np.full(shift + tokens * ldo, 7, np.float32))
+    at = lambda b, floats: ctypes.c_void_p(b.ptr.value + 4 * floats)
+    flag = call_packed(fdx, at(buf, shift), width, at(buf, shift + heads * dk), width, at(buf, shift + (heads + kv) * dk), width,
+                       [before, before + 70, before + 70, before + 205], tokens, heads, kv, dk, dv, at(out, shift), ldo)
+    got = out.to_host((shift + tokens * ldo,))[shift:].reshape(tokens, ldo)
+    q, k, v = x[before:-behind, :heads * dk], x[before:-behind, heads * dk:(heads + kv) * dk], x[before:-behind, (heads + kv) * dk:(heads + kv) * dk + kv * dv]
+    assert flag == 0
+    close(got[before:-behind, :heads * dv], packed_reference(q, k, v, lengths, heads, kv, True))
+    assert (got[:before] == 7).all() and (got[-behind:] == 7).all() and (got[:, heads * dv:] == 7).all()
+
+
+@pytest.mark.parametrize("starts", [[0, 50, 20, 60], [0, 10, 61], [-5, 30], [0, 40, 2**31 - 1], [40, 20, 0], [-2**31, 2**31 - 1]])
+def test_packed_starts_that_are_none(fdx, starts):
+    """Reported, nothing outside the tensors touched: what lies behind the output stays."""
+    r, tokens = np.random.default_rng(1), 60
+    q, k, v = (fdx.DevBuf.from_host(r.standard_normal((tokens, 128)).astype(np.float32)) for _ in range(3))
+    out = fdx.DevBuf.from_host(np.full((tokens + 100) * 128, 3, np.float32))
+    print("packed starts", starts, flush=True)
+    assert call_packed(fdx, q.ptr, 128, k.ptr, 128, v.ptr, 128, starts, tokens, 2, 2, 64, 64, out.ptr, 128) == 1
+    assert (out.to_host(((tokens + 100) * 128,))[tokens * 128:] == 3).all()
+
+
+def test_packed_runs_are_equal(fdx):
+    r, lengths = np.random.default_rng(2), [300, 20, 1, 77]
+    q, k, v = (r.standard_normal((398, h * 64)).astype(np.float32) for h in (8, 2, 2))
+    first = fdx.mha_packed(q, k, v, lengths, 8, 2, 64, 64)
+    for _ in range(3):
+        assert np.array_equal(first, fdx.mha_packed(q, k, v, lengths, 8, 2, 64, 64))
+
+
+# ---------------------------------------------------------------- paged caches
+
+class Filled:
+    """A cache with `context` positions per sequence written by kv_append in `steps` calls, and the rows that went in."""
+
+    def __init__(self, fdx, context, kv, dk, dv, page, kind, seed=0, extra=4, steps=2, max_len=None):
+        r = np.random.default_rng(seed)
+        self.keys = [r.standard_normal((n, kv * dk)).astype(np.float32) for n in context]
+        self.values = [r.standard_normal((n, kv * dv)).astype(np.float32) for n in context]
+        n_pages = sum(-(-n // page) for n in context) + extra
+        self.cache = fdx.PagedCache(n_pages, page, kv, dk, dv, len(context), max_len or max(max(context), 1), kind)
+        r.shuffle(self.cache.free)   # pages of a sequence lie apart
+        done = [0] * len(context)
+        for step in range(steps):
+            upto = [n if step == steps - 1 else n // 2 for n in context]
+            part = [b - a for a, b in zip(done, upto)]
+            if sum(part):
+                fdx.kv_append(self.cache, *(np.concatenate([x[a:b] for x, a, b in zip(xs, done, upto)]) for xs in (self.keys, self.values)), part)
+            done = upto
+        if kind == "bf16":
+            self.keys, self.values = [bf16(x) for x in self.keys], [bf16(x) for x in self.values]
+
+    def reference(self, q, new, heads):
+        out, at = [], 0
+        for s, n in enumerate(new):
+            length = len(self.keys[s])
+            out.append(attend(q[at:at + n], self.keys[s], self.values[s], heads, self.cache.kv_heads, np.arange(length - n, length) + 1))
+            at += n
+        return np.concatenate(out)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("kv,dk,dv,page", [(2, 64, 64, 16), (3, 128, 128, 5), (1, 80, 80, 64), (2, 13, 7, 3), (2, 96, 64, 1), (1, 32, 128, 200)])
+def test_append(fdx, kv, dk, dv, page, kind):
+    """Every position holds its row, rounded to nearest in bf16, and no other place of the pages has changed."""
+    context = [1, 0, 77, 16, 130]
+    print("append", kv, dk, dv, page, kind, flush=True)
+    f = Filled(fdx, context, kv, dk, dv, page, kind, steps=3)
+    c, rows = f.cache, f.cache.n_pages * page
+    for buf, d, want in ((c.k, dk, f.keys), (c.v, dv, f.values)):
+        held = buf.to_host((rows, kv * d), np.float32) if kind == "f32" else \
+            (buf.to_host((rows, kv * d), np.uint16).astype(np.uint32) << 16).view(np.float32)
+        used = np.zeros(rows, bool)
+        for s, n in enumerate(context):
+            pos = np.arange(n)
+            at = c.table[s][pos // page] * page + pos % page
+            assert np.array_equal(held[at], want[s])
+            used[at] = True
+        assert (held[~used] == 0).all()
+
+
+def test_append_rounds_to_nearest(fdx):
+    x = np.array([1, 1 + 2**-8, 1 + 3 * 2**-8, 1 + 2**-8 + 2**-20, -1 - 2**-8, 3.4e38, -3.4e38, 1e-40, 2**-133, 0.0, -0.0, np.inf, -np.inf, np.nan,
+                  65504, 1e-38], np.float32)
+    c = fdx.PagedCache(1, 1, 1, 16, 16, 1, 1, "bf16")
+    fdx.kv_append(c, x[None], x[None], [1])
+    held = (c.k.to_host((16,), np.uint16).astype(np.uint32) << 16).view(np.float32)
+    want = bf16(x)
+    ok = ~np.isnan(x)
+    assert np.array_equal(held[ok].view(np.uint32), want[ok].view(np.uint32)) and np.isnan(held[~ok]).all()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("context,new,heads,kv,dk,dv,page", [
+    ([1], [1], 1, 1, 64, 64, 16), ([201], [1], 12, 12, 64, 64, 16), ([5, 300, 64, 17], [1, 1, 1, 1], 8, 2, 64, 64, 16),
+    ([700, 33, 1], [1, 1, 1], 32, 8, 128, 128, 16), ([100, 260, 31], [1, 0, 1], 16, 1, 128, 128, 7), ([100, 50], [1, 1], 32, 1, 64, 64, 32),
+    ([130, 90], [1, 1], 10, 5, 80, 80, 13), ([60, 61, 62], [1, 1, 1], 6, 2, 13, 7, 3), ([90], [1], 40, 1, 64, 64, 16), ([70], [1], 4, 2, 96, 64, 1),
+    ([200, 77, 16], [3, 5, 16], 4, 4, 64, 64, 16), ([400, 90, 2], [7, 1, 2], 8, 2, 128, 128, 16), ([300, 200], [40, 1], 8, 2, 64, 64, 16),
+    ([500, 129, 40, 3], [129, 129, 1, 3], 8, 2, 64, 64, 24), ([450, 260], [300, 17], 7, 1, 128, 128, 64), ([140], [140], 3, 3, 32, 32, 200),
+    ([77, 190], [60, 33], 5, 1, 33, 127, 11), ([2100, 1900], [1, 2], 4, 1, 64, 64, 16), ([2300, 5, 1030], [70, 5, 1], 4, 2, 128, 128, 32)])
+def test_paged(fdx, context, new, heads, kv, dk, dv, page, kind):
+    print("paged", context, new, heads, kv, dk, dv, page, kind, flush=True)
+    f = Filled(fdx, context, kv, dk, dv, page, kind, seed=sum(context))
+    q = np.random.default_rng(dk).standard_normal((sum(new), heads * dk)).astype(np.float32)
+    close(fdx.mha_paged(f.cache, q, new, heads), f.reference(q, new, heads))
+
+
+def call_paged(fdx, cache, q, ldq, starts, tokens, max_new, heads, out, ldo, **change):
+    c = cache.pages()
+    for key, value in change.items():
+        if key in ("table", "lens"):
+            value = fdx.DevBuf.from_host(value, np.int32)
+            c._kept += (value,)
+            value = value.ptr
+        setattr(c, key, value)
+    d_starts, flag = fdx.DevBuf.from_host(np.asarray(starts, np.int32), np.int32), fdx.DevBuf.from_host(np.zeros(1, np.int32), np.int32)
+    scratch = fdx.DevBuf(fdx.lib.fdx_mha_paged_scratch_bytes(tokens, max_new, heads, ctypes.byref(c)))
+    fdx.check(fdx.lib.fdx_mha_paged_f32(q, ctypes.c_int64(ldq), d_starts.ptr, tokens, max_new, heads, ctypes.byref(c), out, ctypes.c_int64(ldo),
+                                        scratch.ptr, flag.ptr))
+    fdx.sync()
+    return int(flag.to_host((1,), np.int32)[0])
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [3, 1, 2], [40, 9, 70]])
+def test_paged_tokens_that_see_nothing(fdx, new):
+    """More new tokens than positions: the first ones see none and get zeros, none of it is an error."""
+    f = Filled(fdx, [50, 2, 30], 2, 64, 64, 16, "f32")
+    lens = np.array([50, 0, min(30, new[2])], np.int32) if new[0] == 1 else np.array([50, 1, 1], np.int32)
+    tokens, heads = sum(new), 4
+    q = np.random.default_rng(1).standard_normal((tokens, heads * 64)).astype(np.float32)
+    out, dq, starts = fdx.DevBuf.from_host(np.full((tokens, heads * 64), 9, np.float32)), fdx.DevBuf.from_host(q), np.concatenate([[0], np.cumsum(new)])
+    print("paged empty", new, lens, flush=True)
+    flag = call_paged(fdx, f.cache, dq.ptr, heads * 64, starts, tokens, max(new), heads, out.ptr, heads * 64, lens=lens)
+    got = out.to_host((tokens, heads * 64))
+    want = np.concatenate([attend(q[starts[s]:starts[s + 1]], f.keys[s], f.values[s], heads, 2, np.arange(lens[s] - n, lens[s]) + 1)
+                           for s, n in enumerate(new)])
+    assert flag == 0
+    close(got, want)
+    assert (got[want == 0] == 0).all()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("shift,pad", [(0, 4), (1, 0), (0, 3)])
+@pytest.mark.parametrize("new", [[1, 1], [2, 30]])
+def test_paged_strides_and_alignment(fdx, shift, pad, kind, new):
+    heads, kv, d = 4, 2, 64
+    f = Filled(fdx, [90, 131], kv, d, d, 16, kind)
+    tokens = 2 + sum(new) + 3
+    ld = heads * d + pad
+    x = np.random.default_rng(4).standard_normal((tokens, ld)).astype(np.float32)
+    dq, out = fdx.DevBuf.from_host(np.concatenate([np.zeros(shift, np.float32), x.ravel()])), fdx.DevBuf.from_host(np.full(shift + tokens * ld, 7, np.float32))
+    at = lambda b: ctypes.c_void_p(b.ptr.value + 4 * shift)
+    print("paged strides", shift, pad, kind, new, flush=True)
+    assert call_paged(fdx, f.cache, at(dq), ld, [2, 2 + new[0], 2 + sum(new)], tokens, max(new), heads, at(out), ld) == 0
+    got = out.to_host((shift + tokens * ld,))[shift:].reshape(tokens, ld)
+    close(got[2:-3, :heads * d], f.reference(x[2:-3, :heads * d], new, heads))
+    assert (got[:2] == 7).all() and (got[-3:] == 7).all() and (got[:, heads * d:] == 7).all()
+
+
+@pytest.mark.parametrize("new", [[1, 1], [4, 3], [60, 9]])
+def test_paged_pages_that_are_none(fdx, new):
+    """Positions of pages that the cache does not have are left out and reported; so are lengths and tokens beyond what was said."""
+    heads, kv, d, page = 4, 2, 64, 16
+    f = Filled(fdx, [90, 131], kv, d, d, page, "f32")
+    q = np.random.default_rng(4).standard_normal((sum(new), heads * d)).astype(np.float32)
+    dq, starts = fdx.DevBuf.from_host(q), [0, new[0], sum(new)]
+    out = fdx.DevBuf.from_host(np.zeros((sum(new) + 50, heads * d), np.float32))
+    for bad in (-1, f.cache.n_pages, 2**31 - 1, -2**31):
+        table = f.cache.table.copy()
+        table[1, 2] = bad
+        print("paged bad page", new, bad, flush=True)
+        assert call_paged(fdx, f.cache, dq.ptr, heads * d, starts, sum(new), max(new), heads, out.ptr, heads * d, table=table) == 1
+        got = out.to_host((sum(new), heads * d))
+        keep = np.r_[0:32, 48:131]
+        sees = np.array([(keep < 131 - new[1] + j + 1).sum() for j in range(new[1])])
+        close(got[new[0]:], attend(q[new[0]:], f.keys[1][keep], f.values[1][keep], heads, kv, sees))
+        close(got[:new[0]], attend(q[:new[0]], f.keys[0], f.values[0], heads, kv, np.arange(90 - new[0], 90) + 1))
+    for lens, flag in (([90, 132], 1), ([90, 2**31 - 1], 1), ([-1, 131], 1), ([-2**31, 131], 1), ([90, 131], 0)):
+        print("paged lens", lens, flush=True)
+        assert call_paged(fdx, f.cache, dq.ptr, heads * d, starts, sum(new), max(new), heads, out.ptr, heads * d, lens=lens) == flag
+        got = out.to_host((sum(new), heads * d))
+        close(got[new[0]:], attend(q[new[0]:], f.keys[1], f.values[1], heads, kv, np.arange(131 - new[1], 131) + 1))
+        if lens[0] < 0:
+            assert (got[:new[0]] == 0).all()
+    for starts in ([0, 2**31 - 1, 5], [-4, 1, sum(new)], [1, 0, 1]):
+        print("paged starts", starts, flush=True)
+        assert call_paged(fdx, f.cache, dq.ptr, heads * d, starts, sum(new), max(new), heads, out.ptr, heads * d) == 1
+    assert (out.to_host((sum(new) + 50, heads * d))[sum(new):] == 0).all()
+
+
+def test_paged_more_new_tokens_than_said(fdx):
+    f, heads = Filled(fdx, [90, 131], 2, 64, 64, 16, "f32"), 4
+    q = np.random.default_rng(4).standard_normal((45, heads * 64)).astype(np.float32)
+    dq, out = fdx.DevBuf.from_host(q), fdx.DevBuf.from_host(np.full((45, heads * 64), 5, np.float32))
+    assert call_paged(fdx, f.cache, dq.ptr, heads * 64, [0, 5, 45], 45, 5, heads, out.ptr, heads * 64) == 1
+    got = out.to_host((45, heads * 64))
+    close(got[:5], attend(q[:5], f.keys[0], f.values[0], heads, 2, np.arange(85, 90) + 1))
+    close(got[5:10], attend(q[5:10], f.keys[1], f.values[1], heads, 2, np.arange(131 - 40, 131 - 35) + 1))
+    assert (got[10:] == 5).all()
+
+
+def test_append_outside_the_cache(fdx):
+    """Positions below zero, from max_len on and of pages that are none: not written, reported; the others are."""
+    kv, d, page = 1, 8, 4
+    x = np.arange(1, 6 * 8 + 1, dtype=np.float32).reshape(6, 8)
+    for lens, table, want in (([2, 3], [[0, 1], [2, 3]], {8: 3, 9: 4, 10: 5, 0: 1, 1: 2}), ([9, 3], [[0, 1], [2, 3]], {6: 0, 7: 1, 8: 3, 9: 4, 10: 5}),
+                              ([3, 5], [[0, 1], [2, 9]], {0: 0, 1: 1, 2: 2, 10: 3, 11: 4}), ([3, 3], [[-1, 1], [2, 3]], {8: 3, 9: 4, 10: 5})):
+        c = fdx.PagedCache(4, page, kv, d, d, 2, 8)
+        c.table, c.lens = np.array(table, np.int32), np.array(lens, np.int32)
+        pages, dx, starts = c.pages(), fdx.DevBuf.from_host(x), fdx.DevBuf.from_host(np.array([0, 3, 6], np.int32), np.int32)
+        flag = fdx.DevBuf.from_host(np.zeros(1, np.int32), np.int32)
+        fdx.check(fdx.lib.fdx_kv_append_f32(dx.ptr, ctypes.c_int64(8), dx.ptr, ctypes.c_int64(8), starts.ptr, 6, ctypes.byref(pages), flag.ptr))
+        assert flag.to_host((1,), np.int32)[0] == 1
+        rows = np.zeros((16, 8), np.float32)
+        for row, of in want.items():
+            rows[row] = x[of]
+        assert np.array_equal(c.k.to_host((16, 8)), rows) and np.array_equal(c.v.to_host((16, 8)), rows)
+
+
+def test_paged_nan_that_only_later_tokens_see(fdx):
+    """Keys and values that a chunk's later tokens see and its earlier ones do not: a NaN there stays with the later ones."""
+    for new in ([4], [16], [50], [100]):
+        f = Filled(fdx, [150], 2, 64, 64, 16, "f32")
+        q = np.random.default_rng(4).standard_normal((new[0], 256)).astype(np.float32)
+        base = f.reference(q, new, 4)
+        for buf, name in ((f.cache.v, "v"), (f.cache.k, "k")):
+            rows = buf.to_host((f.cache.n_pages * 16, 128))
+            at = f.cache.table[0][148 // 16] * 16 + 148 % 16
+            keep = rows[at, 64].copy()
+            rows[at, 64] = np.nan
+            odd = fdx.DevBuf.from_host(rows)
+            setattr(f.cache, name, odd)
+            got = fdx.mha_paged(f.cache, q, new, 4).reshape(new[0], 4, 64)
+            setattr(f.cache, name, buf)
+            print("paged nan", new, name, flush=True)
+            hit = np.zeros(got.shape, bool)
+            hit[-2:, 2:, (slice(0, 1) if name == "v" else slice(0, 64))] = True
+            assert np.isnan(got[hit]).all()
+            close(got[~hit], base.reshape(got.shape)[~hit])
+
+
+def test_prompts_then_tokens(fdx):
+    """The operators as a serving program uses them: prompts at once, their keys and values into the cache, then steps of one token,
+    a chunk for one sequence beside them, and the scores of the tokens: the same as one pass over each whole sequence."""
+    heads, kv, d, vocab = 8, 2, 64, 501
+    r = np.random.default_rng(11)
+    prompts, steps = [40, 7, 1, 129], [[1, 1, 1, 1], [1, 30, 0, 1], [1, 1, 1, 1]]
+    total = [p + sum(s[i] for s in steps) for i, p in enumerate(prompts)]
+    q, k, v = ([r.standard_normal((n, h * d)).astype(np.float32) for n in total] for h in (heads, kv, kv))
+    head = r.standard_normal((vocab, heads * d)).astype(np.float32) / 10
+    whole = np.split(fdx.mha_packed(np.concatenate(q), np.concatenate(k), np.concatenate(v), total, heads, kv, d, d), np.cumsum(total)[:-1])
+    for kind in ("f32", "bf16"):
+        cache = fdx.PagedCache(40, 16, kv, d, d, 4, max(total), kind)
+        done = [0] * 4
+        for new in [prompts] + steps:
+            part = lambda xs: np.concatenate([x[a:a + n] for x, a, n in zip(xs, done, new)])
+            fdx.kv_append(cache, part(k), part(v), new)
+            got = fdx.mha_paged(cache, part(q), new, heads)
+            if new is prompts:
+                close(got, fdx.mha_packed(part(q), part(k), part(v), new, heads, kv, d, d), 1e-6 if kind == "f32" else 1e-2)
+            close(got, part(whole), 2e-6 if kind == "f32" else 1e-2)   # bf16: keys off by 2^-9 a score, values by 2^-9
+            logits = fdx.gemm(got, head)
+            scores = fdx.token_logprobs(logits, ids=np.arange(len(got)) % vocab, top=3)
+            x = logits.astype(np.float64)
+            lp = x - np.log(np.exp(x - x.max(1, keepdims=True)).sum(1, keepdims=True)) - x.max(1, keepdims=True)
+            assert np.abs(scores["logprobs"] - lp[np.arange(len(got)), np.arange(len(got)) % vocab]).max() < 1e-5
+            assert np.array_equal(scores["top_ids"][:, 0], fdx.argmax(logits)[0])
+            done = [a + n for a, n in zip(done, new)]
+        for s in range(4):
+            cache.release(s)
+        assert sorted(cache.free) == list(range(40))

@@ -1,0 +1,118 @@
+"""What the entry points for packed prompts, paged caches and token scores refuse, and the arithmetic their kernels find rows and
+pages with, without a GPU: arguments are checked before anything is launched."""
+import ctypes
+import os
+import subprocess
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+P = ctypes.c_void_p(1 << 20)   # never followed: the calls below are refused
+I64 = ctypes.c_int64
+INVALID, UNSUPPORTED = 1, 4
+
+
+class Ptr:
+    ptr = P
+
+
+def pages(fdx, **change):
+    args = dict(k=Ptr, v=Ptr, kind="f32", n_pages=10, page_size=16, kv_heads=2, dk=64, dv=64, table=Ptr, table_width=4, lens=Ptr, n_seqs=3,
+                max_len=64)
+    raw = {key: change.pop(key) for key in list(change) if key not in args}
+    args.update(change)
+    c = fdx.KvPages(**args)
+    for key, value in raw.items():
+        setattr(c, key, value)
+    return c
+
+
+def refused(fdx, status, code, text):
+    assert status == code, (status, fdx.lib.fdx_last_error())
+    assert text in fdx.lib.fdx_last_error().decode()
+
+
+class Null:
+    ptr = None
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(k=Null), "null"), (dict(v=Null), "null"), (dict(table=Null), "null"), (dict(lens=Null), "null"), (dict(type=2), "type 2"),
+    (dict(type=-1), "type -1"), (dict(n_pages=0), "shape"), (dict(page_size=0), "shape"), (dict(kv_heads=-1), "shape"), (dict(dk=0), "shape"),
+    (dict(dv=0), "shape"), (dict(n_seqs=0), "shape"), (dict(table_width=0), "shape"), (dict(max_len=0), "shape"), (dict(max_len=65), "reach"),
+    (dict(n_pages=1 << 27), "2^31"), (dict(k=type("Odd", (), dict(ptr=ctypes.c_void_p((1 << 20) + 2)))), "aligned")])
+def test_caches(fdx, change, text):
+    c = ctypes.byref(pages(fdx, **change))
+    refused(fdx, fdx.lib.fdx_kv_append_f32(P, I64(128), P, I64(128), P, 5, c, None), INVALID, text)
+    refused(fdx, fdx.lib.fdx_mha_paged_f32(P, I64(256), P, 5, 2, 4, c, P, I64(256), P, None), INVALID, text)
+
+
+def test_append(fdx):
+    c = ctypes.byref(pages(fdx))
+
+    def call(k=P, ldk=128, v=P, ldv=128, starts=P, tokens=5, cache=c):
+        return fdx.lib.fdx_kv_append_f32(k, I64(ldk), v, I64(ldv), starts, tokens, cache, None)
+    for change, text in ((dict(k=None), "null"), (dict(v=None), "null"), (dict(starts=None), "null"), (dict(cache=None), "null"),
+                         (dict(ldk=127), "overlap"), (dict(ldv=0), "overlap"), (dict(tokens=0), "tokens"), (dict(tokens=-4), "tokens"),
+                         (dict(tokens=(1 << 25) + 1), "tokens")):
+        refused(fdx, call(**change), INVALID, text)
+
+
+def test_paged(fdx):
+    def call(q=P, ldq=256, starts=P, tokens=5, max_new=2, heads=4, cache=None, out=P, ldo=256, scratch=P):
+        return fdx.lib.fdx_mha_paged_f32(q, I64(ldq), starts, tokens, max_new, heads, ctypes.byref(cache or pages(fdx)), out, I64(ldo), scratch,
+                                         None)
+    for change, text in ((dict(q=None), "null"), (dict(out=None), "null"), (dict(starts=None), "null"), (dict(ldq=255), "overlap"),
+                         (dict(ldo=255), "overlap"), (dict(tokens=0), "shape"), (dict(max_new=0), "shape"), (dict(heads=0), "shape"),
+                         (dict(heads=3, ldq=256), "share"), (dict(tokens=1 << 25, heads=4), "too many")):
+        refused(fdx, call(**change), INVALID, text)
+    for change in (dict(dk=129), dict(dv=192)):
+        refused(fdx, call(cache=pages(fdx, **change), ldq=1024, ldo=1024), UNSUPPORTED, "depths up to 128")
+
+
+def test_packed(fdx):
+    def call(q=P, ldq=256, k=P, ldk=128, v=P, ldv=128, starts=P, n_seqs=3, tokens=5, heads=4, kv_heads=2, dk=64, dv=64, out=P, ldo=256):
+        return fdx.lib.fdx_mha_packed_f32(q, I64(ldq), k, I64(ldk), v, I64(ldv), starts, n_seqs, tokens, heads, kv_heads, dk, dv, 1, out,
+                                          I64(ldo), P, None)
+    for change, text in ((dict(q=None), "null"), (dict(k=None), "null"), (dict(v=None), "null"), (dict(starts=None), "null"),
+                         (dict(out=None), "null"), (dict(n_seqs=0), "shape"), (dict(tokens=0), "shape"), (dict(heads=0), "shape"),
+                         (dict(kv_heads=0), "shape"), (dict(dk=0), "shape"), (dict(dv=-1), "shape"), (dict(kv_heads=3, ldk=256, ldv=256), "share"),
+                         (dict(kv_heads=8, ldk=1024, ldv=1024), "share"), (dict(ldq=255), "overlap"), (dict(ldk=1), "overlap"),
+                         (dict(ldv=127), "overlap"), (dict(ldo=128), "overlap"), (dict(tokens=1 << 25), "too many"),
+                         (dict(n_seqs=(1 << 22) + 1), "too many")):
+        refused(fdx, call(**change), INVALID, text)
+    refused(fdx, call(dk=130, ldq=600, ldk=300), UNSUPPORTED, "depths up to 128, not 130 and 64")
+
+
+def test_scores(fdx):
+    def call(x=P, ld=100, rows=3, vocab=100, ids=P, top=5, logprobs=P, entropy=P, top_ids=P, top_logprobs=P):
+        return fdx.lib.fdx_token_logprobs_f32(x, I64(ld), I64(rows), vocab, ids, top, logprobs, entropy, top_ids, top_logprobs, P, None)
+    for change, text in ((dict(x=None), "null"), (dict(rows=0), "rows"), (dict(rows=(1 << 23) + 1), "rows"), (dict(vocab=0), "rows"),
+                         (dict(vocab=(1 << 24) + 1, ld=1 << 25), "rows"), (dict(ld=99), "overlap"), (dict(ids=None), "together"),
+                         (dict(logprobs=None), "together"), (dict(top=-1), "alternatives"), (dict(top=33), "alternatives"),
+                         (dict(top=8, vocab=7), "alternatives"), (dict(top_ids=None), "with top"), (dict(top_logprobs=None), "with top"),
+                         (dict(top=0), "with top"),
+                         (dict(ids=None, logprobs=None, entropy=None, top=0, top_ids=None, top_logprobs=None), "nothing asked")):
+        refused(fdx, call(**change), INVALID, text)
+
+
+def test_scratch_sizes_of_refused_calls_are_zero(fdx):
+    """A size for arguments that the call itself refuses: an answer, not a crash."""
+    assert fdx.lib.fdx_mha_packed_scratch_bytes(0, 1, 1, 1, 64, 64) == 0
+    assert fdx.lib.fdx_mha_packed_scratch_bytes(5, 1, 4, 0, 64, 64) == 0
+    assert fdx.lib.fdx_mha_paged_scratch_bytes(5, 1, 4, None) == 0
+    for change in (dict(kv_heads=0), dict(max_len=0), dict(n_seqs=-3), dict(dk=0), dict(dv=0)):
+        assert fdx.lib.fdx_mha_paged_scratch_bytes(5, 1, 4, ctypes.byref(pages(fdx, **change))) == 0
+    assert fdx.lib.fdx_mha_paged_scratch_bytes(0, 1, 4, ctypes.byref(pages(fdx))) == 0
+    assert fdx.lib.fdx_mha_paged_scratch_bytes(5, 0, 4, ctypes.byref(pages(fdx))) == 0
+    assert fdx.lib.fdx_token_logprobs_scratch_bytes(I64(0), 100, 5) == 0
+    assert fdx.lib.fdx_token_logprobs_scratch_bytes(I64(5), -1, 5) == 0
+
+
+def test_rows_and_pages_on_the_host(tmp_path):
+    exe = str(tmp_path / "kv_pages_test.bin")
+    subprocess.check_call(["g++", "-std=c++17", "-O1", "-g", "-fsanitize=address,undefined", "-fno-sanitize-recover=undefined",
+                           "-I" + os.path.join(ROOT, "frugally-deep_amd", "csrc"), os.path.join(ROOT, "tests", "cpp", "kv_pages_test.cpp"),
+                           "-o", exe])
+    out = subprocess.run([exe], capture_output=True, text=True, timeout=300, env=dict(os.environ, ASAN_OPTIONS="detect_leaks=0"))
+    assert out.returncode == 0 and "kv_pages done" in out.stdout, (out.stdout, out.stderr[-3000:])
