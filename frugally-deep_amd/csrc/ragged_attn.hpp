@@ -25,7 +25,22 @@ struct RaggedParams {
     const int32_t *table, *lens; // paged only
     int table_width, n_pages, page_size, max_len, max_new;
     int* error_flag;
+    float* part;          // rows that see more than split_keys keys: sums of each range of split_keys, met by ragged_join_kernel
+    int splits, split_keys;
+    int tile_from;        // sequences that bring fewer rows to a key head are another launch's
 };
+
+// The sums of a row over one range of keys as they lie in p.part: [range][row][m, l], then [range][row][depth] of o / l.  m is
+// -infinity where the range has no key, -FLT_MAX where all its scores are -infinity.
+__device__ __forceinline__ float* part_size(const RaggedParams& p, int range, int64_t row)
+{
+    return p.part + 2 * (range * ((int64_t)p.tokens * p.heads) + row);
+}
+__device__ __forceinline__ float* part_out(const RaggedParams& p, int range, int64_t row)
+{
+    const int64_t rows = (int64_t)p.tokens * p.heads;
+    return p.part + 2 * p.splits * rows + (range * rows + row) * p.dv;
+}
 
 template <int KIND>
 struct KvElement {
@@ -86,7 +101,7 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // 64 + lane of the output.  m is the largest score in units of log2, l the sum of 2^(score - m), o the weighted values.
 template <int KIND>
 __device__ __forceinline__ void plain_row(const RaggedParams& p, const Sequence& s, const float* q, int kv_head, int first, int last, float& m,
-    float& l, float (&o)[2], bool& missing)
+    float& l, float (&o)[2], bool& seen, bool& missing)
 {
     typedef typename KvElement<KIND>::type T;
     const int lane = threadIdx.x & 63;
@@ -95,11 +110,12 @@ __device__ __forceinline__ void plain_row(const RaggedParams& p, const Sequence&
     const float scale = p.scale * kLog2e;
     m = -INFINITY;
     l = o[0] = o[1] = 0.f;
+    seen = missing = false;
 #pragma clang loop unroll(disable)
     for (int j0 = first; j0 < last; j0 += 64) {
         const int row = j0 + lane < last ? key_row<KIND>(p, s, j0 + lane) : -1;
-        if (j0 + lane < last && row < 0)
-            missing = true;
+        seen = seen || __any(row >= 0);
+        missing = missing || __any(j0 + lane < last && row < 0);
         float sc = -INFINITY;
         if (row >= 0) {
             const T* kr = kb + (int64_t)row * p.ldk;
