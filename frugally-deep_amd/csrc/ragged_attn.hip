@@ -104,7 +104,7 @@ __global__ __launch_bounds__(256, 2) void ragged_tile_kernel(RaggedParams p)
         raise_flag(p, s.cut);
     const int count = s.span.count * p.group; // rows
     const int r_first = tile.index * 128;
-    if (r_first >= count || s.span.count * p.group < p.tile_from)
+    if (r_first >= count || count <= p.few_rows)
         return;
     const int r = r_first + wave * 32 + c;
     const bool q_ok = r < count;
@@ -426,9 +426,291 @@ __global__ __launch_bounds__(256, 2) void ragged_tile_kernel(RaggedParams p)
     }
 }
 
+// ---- few query rows: keys and values pass once, straight from memory to the fp32 matrix instructions ----
+//
+// A workgroup takes all rows (up to 16 R) that a sequence brings to one key head, over one range of its keys; its four waves take every
+// fourth block of 16 keys, each with sums of its own, and meet at the end.  Bound by memory: a lane's loads are the operands of
+// the 16x16x4 fp32 products, nothing is staged, and a block's loads are on their way while the block before is worked on.
+//  * S^T = K Q^T: lane (c, g) of 16 x 4 loads chunks of key c, chunk i at depth 4 W i + W g (W elements are 16 bytes), and has scores of keys
+//    4 g .. 4 g + 3 of row c.
+//  * O^T = V^T P^T: lane (c, g) loads depths V c .. V c + V - 1 of keys 4 g .. + 3, so the probabilities it has are the operand, and gets
+//    depths V (4 g + i) + e of row c.  The products are exact in fp32; what they cost, 32 cycles per 16 keys, 16 rows and 4 depths, is less
+//    than the memory's share of a CU needs for the keys.
+template <typename T, int W, bool WIDE>
+__device__ __forceinline__ auto load_chunk(const T* row, int d, int depth)
+{
+    typedef T tv __attribute__((ext_vector_type(W)));
+    tv v;
+#pragma unroll
+    for (int e = 0; e < W; ++e)
+        v[e] = (T)0.f;
+    if (WIDE) {
+        if (d < depth)
+            v = *reinterpret_cast<const tv*>(row + d);
+    } else {
+#pragma unroll
+        for (int e = 0; e < W; ++e)
+            if (d + e < depth)
+                v[e] = row[d + e];
+    }
+    return v;
+}
+
+template <int D, int KIND, int R, bool WIDE>
+__global__ __launch_bounds__(256) void ragged_few_kernel(RaggedParams p)
+{
+    typedef typename KvElement<KIND>::type T;
+    constexpr int W = 16 / (int)sizeof(T), NK = D / (4 * W); // elements of a key chunk, chunks of a lane
+    constexpr int DL = D / 16, VW = DL < W ? DL : W, NV = DL / VW; // depths of a lane, in NV loads of VW
+    typedef T kvec __attribute__((ext_vector_type(W)));
+    typedef T vvec __attribute__((ext_vector_type(VW)));
+    struct Block {
+        kvec k[NK];
+        vvec v[4][NV];
+        int row;
+    };
+    __shared__ float meet_o[4][16][D + 4];
+    __shared__ float meet_m[4][16 * R], meet_l[4][16 * R];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c = lane & 15, g = lane >> 4;
+    const int seq = blockIdx.x / p.kv_heads, kv_head = blockIdx.x % p.kv_heads;
+    if (p.error_flag && blockIdx.x == 0 && blockIdx.y == 0)
+        for (int i = tid; i < p.n_seqs; i += 256)
+            raise_flag(p, !packed_start_ok(p.starts, i, p.tokens));
+    const Sequence s = sequence_of<KIND>(p, seq, packed_span(p.starts, seq, p.tokens));
+    if (tid == 0)
+        raise_flag(p, s.cut);
+    const int count = s.span.count * p.group;
+    if (count == 0 || count > p.few_rows)
+        return;
+    const int k_first = blockIdx.y * p.split_keys;
+    int k_end = visible_keys(p, s, s.span.count - 1);
+    if (blockIdx.y > 0 && k_first >= k_end)
+        return;
+    if (k_end - k_first > p.split_keys)
+        k_end = k_first + p.split_keys;
+    const int blocks = k_end > k_first ? (k_end - k_first + 15) / 16 : 0;
+
+    const T* kbase = static_cast<const T*>(p.k) + (int64_t)kv_head * p.dk;
+    const T* vbase = static_cast<const T*>(p.v) + (int64_t)kv_head * p.dv;
+    auto look_up = [&](int blk) { // the place of key c of a block; positions behind the range repeat its last one
+        const int at = k_first + blk * 16 + c;
+        return key_row<KIND>(p, s, at < k_end ? at : k_end - 1);
+    };
+    auto fetch = [&](Block& b, int row) {
+        b.row = row;
+        const T* kr = kbase + (int64_t)(row < 0 ? 0 : row) * p.ldk;
+#pragma unroll
+        for (int i = 0; i < NK; ++i)
+            b.k[i] = load_chunk<T, W, WIDE>(kr, 4 * W * i + W * g, p.dk);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int vrow = __shfl(row, 4 * g + i, 64);
+            const T* vr = vbase + (int64_t)(vrow < 0 ? 0 : vrow) * p.ldv;
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+                b.v[i][j] = load_chunk<T, VW, WIDE>(vr, 16 * VW * j + VW * c, p.dv);
+        }
+    };
+    Block a, b;
+    int row_b = 0;
+    if (wave < blocks) {
+        const int row_a = look_up(wave);
+        row_b = look_up(wave + 4);
+        fetch(a, row_a);
+    }
+
+    float q[R][NK][W];
+    int visible[R];
+    float m_run[R], l_run[R];
+    f32x4 oacc[R][DL];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const bool ok = 16 * r + c < count;
+        const int at = ok ? 16 * r + c : 0, token = at / p.group;
+        visible[r] = ok ? visible_keys(p, s, token) : 0;
+        const float* from = p.q + (int64_t)(s.span.first + token) * p.ldq + (int64_t)(kv_head * p.group + at - token * p.group) * p.dk;
+#pragma unroll
+        for (int i = 0; i < NK; ++i)
+#pragma unroll
+            for (int h = 0; h < W; h += 4) {
+                const f32x4 x = load_chunk<float, 4, WIDE>(from, 4 * W * i + W * g + h, p.dk);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    q[r][i][h + e] = x[e] * (p.scale * kLog2e);
+            }
+        m_run[r] = -INFINITY;
+        l_run[r] = 0.f;
+#pragma unroll
+        for (int e = 0; e < DL; ++e)
+            oacc[r][e] = f32x4 { 0.f, 0.f, 0.f, 0.f };
+    }
+    // keys that the first row sees are seen by all
+    const int first_sees = visible_keys(p, s, 0), all_see = first_sees < k_end ? first_sees : k_end;
+    bool missing = false;
+    auto work = [&](const Block& x, int blk) {
+        f32x4 sc[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            sc[r] = f32x4 { 0.f, 0.f, 0.f, 0.f };
+#pragma unroll
+            for (int i = 0; i < NK; ++i)
+#pragma unroll
+                for (int e = 0; e < W; ++e)
+                    sc[r] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)x.k[i][e], q[r][i][e], sc[r], 0, 0, 0);
+        }
+        const int at = k_first + blk * 16;
+        if (at + 16 > all_see) {
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (at + 4 * g + i >= (visible[r] < k_end ? visible[r] : k_end))
+                        sc[r][i] = -INFINITY;
+        }
+        if (__any(x.row < 0)) {
+            missing = true;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const bool none = __shfl(x.row, 4 * g + i, 64) < 0;
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+                    sc[r][i] = none ? -INFINITY : sc[r][i];
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float mx = fmaxf(fmaxf(sc[r][0], sc[r][1]), fmaxf(sc[r][2], sc[r][3]));
+            mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            if (__any(mx > m_run[r] + 8.f)) { // the maximum moves when a score passes it by 2^8
+                const float m_new = fmaxf(m_run[r], mx);
+                const float corr = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run[r] - m_new);
+                m_run[r] = m_new;
+                l_run[r] *= corr;
+#pragma unroll
+                for (int e = 0; e < DL; ++e)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        oacc[r][e][i] *= corr;
+            }
+            const float base = m_run[r] == -INFINITY ? 0.f : m_run[r];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                sc[r][i] = __builtin_amdgcn_exp2f(sc[r][i] - base);
+                l_run[r] += sc[r][i];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < NV; ++j)
+#pragma unroll
+                    for (int e = 0; e < VW; ++e)
+                        oacc[r][j * VW + e] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)x.v[i][j][e], sc[r][i], oacc[r][j * VW + e], 0, 0, 0);
+        }
+    };
+    for (int blk = wave; blk < blocks; blk += 8) {
+        const bool more = blk + 4 < blocks;
+        int row_a = 0;
+        if (more) {
+            fetch(b, row_b);
+            row_a = look_up(blk + 8);
+        }
+        work(a, blk);
+        if (!more)
+            break;
+        if (blk + 8 < blocks) {
+            fetch(a, row_a);
+            row_b = look_up(blk + 12);
+        }
+        work(b, blk + 4);
+    }
+    raise_flag(p, missing);
+
+    // the waves' sums meet, 16 rows at a time: 16 threads a row, DL depths each
+    uint32_t odd = 0; // of this wave's rows those whose sums are not finite, or empty though there are keys
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        l_run[r] += __shfl_xor(l_run[r], 16, 64);
+        l_run[r] += __shfl_xor(l_run[r], 32, 64);
+        if (r > 0)
+            __syncthreads();
+        if (g == 0) {
+            meet_m[wave][16 * r + c] = m_run[r];
+            meet_l[wave][16 * r + c] = l_run[r];
+        }
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < VW; ++e)
+                    meet_o[wave][c][16 * VW * j + VW * (4 * g + i) + e] = oacc[r][j * VW + e][i];
+        __syncthreads();
+        const int at = 16 * r + (tid >> 4), d0 = (tid & 15) * DL;
+        const float top = fmaxf(fmaxf(meet_m[0][at], meet_m[1][at]), fmaxf(meet_m[2][at], meet_m[3][at]));
+        const float m = top == -INFINITY ? 0.f : top;
+        float l = 0.f, o[DL], size;
+#pragma unroll
+        for (int e = 0; e < DL; ++e)
+            o[e] = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float f = __builtin_amdgcn_exp2f(meet_m[w][at] - m);
+            l += f * meet_l[w][at];
+#pragma unroll
+            for (int e = 0; e < DL; ++e)
+                o[e] += f * meet_o[w][tid >> 4][d0 + e];
+        }
+        size = l;
+#pragma unroll
+        for (int e = 0; e < DL; ++e)
+            size += fabsf(o[e]);
+        const int token = (at < count ? at : 0) / p.group, head = kv_head * p.group + (at < count ? at : 0) - token * p.group;
+        const int sees = visible_keys(p, s, token);
+        const bool in_parts = sees > p.split_keys, mine = at < count && (in_parts ? k_first < sees : blockIdx.y == 0);
+        const uint64_t bad = __ballot(mine && (!(size < INFINITY) || (l == 0.f && k_first < sees)));
+        if (mine && (bad >> (lane & 48) & 0xffff) == 0) {
+            const int64_t q_row = s.span.first + token, id = q_row * p.heads + head;
+            const float f = l > 0.f ? 1.f / l : 0.f; // no key: zeros
+            float* to = in_parts ? part_out(p, blockIdx.y, id) : p.out + q_row * p.ldo + (int64_t)head * p.dv;
+            if (in_parts && (tid & 15) == 0) {
+                float* size_at = part_size(p, blockIdx.y, id);
+                size_at[0] = top;
+                size_at[1] = l;
+            }
+#pragma unroll
+            for (int e = 0; e < DL; e += 4) {
+                if (WIDE) {
+                    if (d0 + e < p.dv)
+                        *reinterpret_cast<f32x4*>(to + d0 + e) = f32x4 { o[e] * f, o[e + 1] * f, o[e + 2] * f, o[e + 3] * f };
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (d0 + e + i < p.dv)
+                            to[d0 + e + i] = o[e + i] * f;
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) // rows 4 wave .. 4 wave + 3 of the sixteen
+            if (bad >> (16 * k) & 0xffff)
+                odd |= 1u << (16 * r + 4 * wave + k);
+    }
+    if (__builtin_expect(odd == 0, 1))
+        return;
+#pragma clang loop unroll(disable)
+    while (odd) {
+        const int r1 = __builtin_ctz(odd);
+        odd &= odd - 1;
+        const int token = r1 / p.group;
+        store_plain_row<KIND>(p, s, token, kv_head * p.group + r1 - token * p.group, kv_head, blockIdx.y, lane);
+    }
+}
+
 // Rows that more than one range of keys was summed for: sum of 2^(m - M) l o over the ranges, divided by that of 2^(m - M) l.
 template <int KIND>
-__global__ __launch_bounds__(256) void ragged_join_kernel(RaggedParams p)
+__global__ __launch_bounds__(256) void ragged_join_kernel(RaggedParams p, int few_keys, int tile_keys)
 {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t id = (int64_t)blockIdx.x * 4 + wave;
@@ -442,9 +724,10 @@ __global__ __launch_bounds__(256) void ragged_join_kernel(RaggedParams p)
     if (row - s.span.first >= s.span.count)
         return;
     const int visible = visible_keys(p, s, row - s.span.first);
-    if (visible <= p.split_keys)
+    const int keys = s.span.count * p.group <= p.few_rows ? few_keys : tile_keys;
+    if (visible <= keys)
         return;
-    const int parts = (visible + p.split_keys - 1) / p.split_keys;
+    const int parts = (visible + keys - 1) / keys;
     float top = -INFINITY;
     for (int i = 0; i < parts; ++i)
         top = fmaxf(top, part_size(p, i, id)[0]);
@@ -467,37 +750,105 @@ __global__ __launch_bounds__(256) void ragged_join_kernel(RaggedParams p)
         to[64 + lane] = finish(o1, l, top != -INFINITY);
 }
 
-template <int D, int KIND>
-static void tile_launch(const RaggedParams& p, bool wide)
+// How a call is cut: sequences of few rows (up to `few_rows`) go to ragged_few_kernel in ranges of few_keys keys, the others to
+// ragged_tile_kernel in ranges of tile_keys.
+struct RaggedPlan {
+    int few_rows, few_ranges, few_keys; // few_ranges 0: no such launch
+    int tile_ranges, tile_keys;
+    int64_t tiles;
+    int ranges() const { return few_ranges > tile_ranges ? few_ranges : tile_ranges; }
+    size_t scratch(int tokens, int heads, int dv) const
+    {
+        return ranges() > 1 ? sizeof(float) * (size_t)ranges() * tokens * heads * (2 + (size_t)dv) : 0;
+    }
+};
+
+static int ranges_of(int64_t keys, int64_t want, int least, int* range_keys)
 {
-    const int64_t tiles = KIND == kPackedF32
-        ? tile_numbers(p.tokens, p.n_seqs, p.group, 128)
-        : tile_numbers(p.tokens, p.n_seqs, p.group, 128);
-    const dim3 grid((unsigned)(tiles * p.kv_heads), (unsigned)p.splits);
-    if (wide)
-        hipLaunchKernelGGL((ragged_tile_kernel<D, KIND, true>), grid, dim3(256), 0, stream(), p);
-    else
-        hipLaunchKernelGGL((ragged_tile_kernel<D, KIND, false>), grid, dim3(256), 0, stream(), p);
+    int64_t per = (keys + want - 1) / want;
+    per = (per < least ? least : per) + 63 & ~(int64_t)63;
+    *range_keys = per > INT_MAX - 64 ? INT_MAX - 64 : (int)per;
+    return (int)((keys + *range_keys - 1) / *range_keys);
 }
 
-// rows of every tensor start on vectors of four elements
-static bool wide_rows(const RaggedParams& p, int size)
+static RaggedPlan paged_plan(int tokens, int max_new, int heads, const fdx_kv_pages* c)
 {
-    const uintptr_t f = reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.out);
-    const uintptr_t kv = reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v);
-    return (f & 15) == 0 && (kv & (4 * size - 1)) == 0 && ((p.ldq | p.ldo | p.ldk | p.ldv | p.dk | p.dv) & 3) == 0;
+    RaggedPlan r {};
+    const int group = heads / c->kv_heads;
+    const int64_t most = (int64_t)(max_new < tokens ? max_new : tokens) * group; // rows of a sequence
+    r.few_rows = most <= 16 ? 16 : 32;
+    if (group <= r.few_rows) {
+        const int64_t items = (int64_t)c->n_seqs * c->kv_heads;
+        r.few_ranges = ranges_of(c->max_len, (4096 + items - 1) / items, 256, &r.few_keys);
+    }
+    if (most > r.few_rows || r.few_ranges == 0) {
+        r.tiles = tile_numbers(tokens, c->n_seqs, group, 128) * c->kv_heads;
+        const int64_t full = ((int64_t)tokens * group + 127) / 128 * c->kv_heads;
+        r.tile_ranges = ranges_of(c->max_len, full >= 256 ? 1 : (512 + full - 1) / full, 512, &r.tile_keys);
+    }
+    if (r.few_ranges == 0)
+        r.few_rows = 0;
+    return r;
+}
+
+static RaggedPlan packed_plan(int tokens, int n_seqs, int heads, int kv_heads)
+{
+    RaggedPlan r {};
+    r.tiles = tile_numbers(tokens, n_seqs, heads / kv_heads, 128) * kv_heads;
+    r.tile_ranges = 1;
+    r.tile_keys = INT_MAX - 64;
+    return r;
+}
+
+// rows of every tensor start on vectors of four elements (eight in bf16 pages)
+template <int KIND>
+static bool wide_rows(const RaggedParams& p)
+{
+    const uintptr_t all = reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.k)
+        | reinterpret_cast<uintptr_t>(p.v);
+    const int64_t unit = KIND == kPagedBf16 ? 7 : 3;
+    return (all & 15) == 0 && ((p.ldq | p.ldo | p.ldk | p.ldv | p.dk | p.dv) & unit) == 0;
+}
+
+template <int D, int KIND, bool WIDE>
+static void ragged_launch(RaggedParams p, const RaggedPlan& plan)
+{
+    p.few_rows = plan.few_rows;
+    p.ranges = plan.ranges();
+    if constexpr (KIND != kPackedF32) {
+        if (plan.few_ranges > 0) {
+            p.split_keys = plan.few_keys;
+            const dim3 grid((unsigned)(p.n_seqs * p.kv_heads), (unsigned)plan.few_ranges);
+            if (plan.few_rows <= 16)
+                hipLaunchKernelGGL((ragged_few_kernel<D, KIND, 1, WIDE>), grid, dim3(256), 0, stream(), p);
+            else
+                hipLaunchKernelGGL((ragged_few_kernel<D, KIND, 2, WIDE>), grid, dim3(256), 0, stream(), p);
+        }
+    }
+    if (plan.tiles > 0) {
+        p.split_keys = plan.tile_keys;
+        hipLaunchKernelGGL((ragged_tile_kernel<D, KIND, WIDE>), dim3((unsigned)plan.tiles, (unsigned)plan.tile_ranges), dim3(256), 0, stream(), p);
+    }
+    if (plan.ranges() > 1)
+        hipLaunchKernelGGL(ragged_join_kernel<KIND>, dim3((unsigned)(((int64_t)p.tokens * p.heads + 3) / 4)), dim3(256), 0, stream(), p, plan.few_keys,
+            plan.tile_keys);
 }
 
 template <int KIND>
-static void ragged_launch(const RaggedParams& p)
+static void ragged_dispatch(const RaggedParams& p, const RaggedPlan& plan)
 {
-    const bool wide = wide_rows(p, KIND == kPagedBf16 ? 2 : 4);
-    if (p.dk <= 64 && p.dv <= 64)
-        tile_launch<64, KIND>(p, wide);
-    else
-        tile_launch<128, KIND>(p, wide);
-    if (p.splits > 1)
-        hipLaunchKernelGGL(ragged_join_kernel<KIND>, dim3((unsigned)(((int64_t)p.tokens * p.heads + 3) / 4)), dim3(256), 0, stream(), p);
+    const bool small = p.dk <= 64 && p.dv <= 64;
+    if (wide_rows<KIND>(p)) {
+        if (small)
+            ragged_launch<64, KIND, true>(p, plan);
+        else
+            ragged_launch<128, KIND, true>(p, plan);
+    } else {
+        if (small)
+            ragged_launch<64, KIND, false>(p, plan);
+        else
+            ragged_launch<128, KIND, false>(p, plan);
+    }
 }
 
 static fdx_status check_ragged(const char* who, const RaggedParams& p, const void* scratch, size_t need)
@@ -524,8 +875,10 @@ using namespace fdx;
 
 extern "C" size_t fdx_mha_packed_scratch_bytes(int tokens, int n_seqs, int heads, int kv_heads, int dk, int dv)
 {
-    (void)tokens; (void)n_seqs; (void)heads; (void)kv_heads; (void)dk; (void)dv;
-    return 0;
+    (void)dk;
+    if (tokens <= 0 || n_seqs <= 0 || heads <= 0 || kv_heads <= 0 || dv <= 0)
+        return 0;
+    return packed_plan(tokens, n_seqs, heads, kv_heads).scratch(tokens, heads, dv);
 }
 
 extern "C" fdx_status fdx_mha_packed_f32(const float* q, int64_t ldq, const float* k, int64_t ldk, const float* v, int64_t ldv,
@@ -537,24 +890,24 @@ extern "C" fdx_status fdx_mha_packed_f32(const float* q, int64_t ldq, const floa
     p.starts = starts; p.n_seqs = n_seqs; p.tokens = tokens;
     p.heads = heads; p.kv_heads = kv_heads; p.group = kv_heads > 0 ? heads / kv_heads : 0;
     p.dk = dk; p.dv = dv; p.causal = causal != 0;
-    p.error_flag = error_flag_dev;
+    p.error_flag = error_flag_dev; p.part = static_cast<float*>(scratch_dev);
     const fdx_status st = check_ragged("mha_packed", p, scratch_dev, fdx_mha_packed_scratch_bytes(tokens, n_seqs, heads, kv_heads, dk, dv));
     if (st != FDX_OK)
         return st;
     p.scale = (float)(1.0 / std::sqrt((double)dk));
     profile_begin();
-    p.splits = 1;
-    p.split_keys = INT_MAX;
-    ragged_launch<kPackedF32>(p);
+    ragged_dispatch<kPackedF32>(p, packed_plan(tokens, n_seqs, heads, kv_heads));
     profile_end("mha_packed_f32", 0.0, 4.0 * tokens * ((double)heads + kv_heads) * (dk + dv));
     FDX_LAUNCH_CHECK();
     return FDX_OK;
 }
 
-extern "C" size_t fdx_mha_paged_scratch_bytes(int tokens, int max_new, int heads, const fdx_kv_pages* cache)
+extern "C" size_t fdx_mha_paged_scratch_bytes(int tokens, int max_new, int heads, const fdx_kv_pages* c)
 {
-    (void)tokens; (void)max_new; (void)heads; (void)cache;
-    return 0;
+    if (!c || tokens <= 0 || max_new <= 0 || heads <= 0 || c->kv_heads <= 0 || heads % c->kv_heads != 0 || c->dk <= 0 || c->dv <= 0 || c->n_seqs <= 0
+        || c->max_len <= 0)
+        return 0;
+    return paged_plan(tokens, max_new, heads, c).scratch(tokens, heads, c->dv);
 }
 
 extern "C" fdx_status fdx_mha_paged_f32(const float* q, int64_t ldq, const int32_t* starts, int tokens, int max_new, int heads,
@@ -572,18 +925,18 @@ extern "C" fdx_status fdx_mha_paged_f32(const float* q, int64_t ldq, const int32
     p.dk = cache->dk; p.dv = cache->dv; p.causal = 1;
     p.table = cache->table; p.lens = cache->lens; p.table_width = cache->table_width; p.n_pages = cache->n_pages;
     p.page_size = cache->page_size; p.max_len = cache->max_len; p.max_new = max_new < tokens ? max_new : tokens;
-    p.error_flag = error_flag_dev;
+    p.error_flag = error_flag_dev; p.part = static_cast<float*>(scratch_dev);
     st = check_ragged("mha_paged", p, scratch_dev, fdx_mha_paged_scratch_bytes(tokens, max_new, heads, cache));
     if (st != FDX_OK)
         return st;
+    FDX_REQUIRE((int64_t)p.n_seqs * p.kv_heads <= (1 << 22), "mha_paged: sequences * key heads too many for one launch");
     p.scale = (float)(1.0 / std::sqrt((double)p.dk));
+    const RaggedPlan plan = paged_plan(tokens, max_new, heads, cache);
     profile_begin();
-    p.splits = 1;
-    p.split_keys = INT_MAX;
     if (cache->type == FDX_KV_F32)
-        ragged_launch<kPagedF32>(p);
+        ragged_dispatch<kPagedF32>(p, plan);
     else
-        ragged_launch<kPagedBf16>(p);
+        ragged_dispatch<kPagedBf16>(p, plan);
     profile_end("mha_paged_f32", 0.0, 4.0 * tokens * heads * (double)(p.dk + p.dv));
     FDX_LAUNCH_CHECK();
     return FDX_OK;

@@ -26,20 +26,21 @@ struct RaggedParams {
     int table_width, n_pages, page_size, max_len, max_new;
     int* error_flag;
     float* part;          // rows that see more than split_keys keys: sums of each range of split_keys, met by ragged_join_kernel
-    int splits, split_keys;
-    int tile_from;        // sequences that bring fewer rows to a key head are another launch's
+    int ranges;           // ranges that p.part has room for
+    int split_keys;
+    int few_rows;         // sequences that bring up to this many rows to a key head are ragged_few_kernel's, others ragged_tile_kernel's
 };
 
-// The sums of a row over one range of keys as they lie in p.part: [range][row][m, l], then [range][row][depth] of o / l.  m is
+// The sums of a row over one range of keys as they lie in p.part: [range][row][depth] of o / l, then [range][row][m, l].  m is
 // -infinity where the range has no key, -FLT_MAX where all its scores are -infinity.
-__device__ __forceinline__ float* part_size(const RaggedParams& p, int range, int64_t row)
-{
-    return p.part + 2 * (range * ((int64_t)p.tokens * p.heads) + row);
-}
 __device__ __forceinline__ float* part_out(const RaggedParams& p, int range, int64_t row)
 {
+    return p.part + (range * ((int64_t)p.tokens * p.heads) + row) * p.dv;
+}
+__device__ __forceinline__ float* part_size(const RaggedParams& p, int range, int64_t row)
+{
     const int64_t rows = (int64_t)p.tokens * p.heads;
-    return p.part + 2 * p.splits * rows + (range * rows + row) * p.dv;
+    return p.part + p.ranges * rows * p.dv + 2 * (range * rows + row);
 }
 
 template <int KIND>

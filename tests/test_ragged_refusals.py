@@ -70,6 +70,14 @@ def test_paged(fdx):
         refused(fdx, call(cache=pages(fdx, **change), ldq=1024, ldo=1024), UNSUPPORTED, "depths up to 128")
 
 
+def test_paged_scratch(fdx):
+    """Long caches of few sequences are summed in ranges, which takes memory of the caller's."""
+    c = ctypes.byref(pages(fdx, page_size=4096, max_len=16384))
+    assert fdx.lib.fdx_mha_paged_scratch_bytes(5, 2, 4, c) > 0
+    for scratch in (None, ctypes.c_void_p((1 << 20) + 4)):
+        refused(fdx, fdx.lib.fdx_mha_paged_f32(P, I64(256), P, 5, 2, 4, c, P, I64(256), scratch, None), INVALID, "scratch")
+
+
 def test_packed(fdx):
     def call(q=P, ldq=256, k=P, ldk=128, v=P, ldv=128, starts=P, n_seqs=3, tokens=5, heads=4, kv_heads=2, dk=64, dv=64, out=P, ldo=256):
         return fdx.lib.fdx_mha_packed_f32(q, I64(ldq), k, I64(ldk), v, I64(ldv), starts, n_seqs, tokens, heads, kv_heads, dk, dv, 1, out,
