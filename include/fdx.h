@@ -417,7 +417,7 @@ fdx_status fdx_mha_paged_f32(const float* q, int64_t ldq, const int32_t* starts,
  * logits [rows][vocab], rows ld floats apart.  ids and logprobs are both NULL or both given, entropy may be NULL, top_ids and
  * top_logprobs are NULL exactly if top is 0; top <= 32 and top <= vocab.  Logits of -infinity are tokens ruled out: probability
  * 0, no share of the entropy; a row of nothing else has entropy 0 and log probabilities of -infinity.  A row that holds a NaN or
- * +infinity gets NaN everywhere but in top_ids (NaN counts as the lowest logit there).  An id of vocab or more gets NaN and sets
+ * +infinity gets NaN everywhere but in top_ids (NaN counts as -infinity there).  An id of vocab or more gets NaN and sets
  * error_flag_dev (may be NULL) to 1 on the device.  scratch_dev as for fdx_mha_packed_f32, of
  * fdx_token_logprobs_scratch_bytes bytes.  (The reference's softmax and its log: include/fdeep/tensor.hpp:1165-1192.)
  */
