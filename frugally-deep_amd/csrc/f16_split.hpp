@@ -24,13 +24,55 @@ __device__ __forceinline__ Pow2 pow2_for(float largest)
     return { __builtin_bit_cast(float, (uint32_t)field << 23), __builtin_bit_cast(float, (uint32_t)(254 - field) << 23) };
 }
 
+// Two instructions a value: the mixed-precision multiply-add rounds x s to h, and x s - h to l, without a register for either in fp32
+// (the compiler takes three, a product among them).
 __device__ __forceinline__ void split2x8(const float (&x)[8], float s, f16x8& h, f16x8& l)
 {
+    typedef uint32_t u32x4_ __attribute__((ext_vector_type(4)));
+    u32x4_ hw, lw;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        h[i] = (_Float16)(x[i] * s);
-        l[i] = (_Float16)__builtin_fmaf(x[i], s, -(float)h[i]);
+    for (int i = 0; i < 4; ++i) {
+        uint32_t a, b;
+        asm("v_fma_mixlo_f16 %0, %1, %2, 0" : "=v"(a) : "v"(x[2 * i]), "v"(s));
+        asm("v_fma_mixhi_f16 %0, %1, %2, 0" : "+v"(a) : "v"(x[2 * i + 1]), "v"(s));
+        asm("v_fma_mixlo_f16 %0, %1, %2, -%3 op_sel_hi:[0,0,1]" : "=v"(b) : "v"(x[2 * i]), "v"(s), "v"(a));
+        asm("v_fma_mixhi_f16 %0, %1, %2, -%3 op_sel:[0,0,1] op_sel_hi:[0,0,1]" : "+v"(b) : "v"(x[2 * i + 1]), "v"(s), "v"(a));
+        hw[i] = a;
+        lw[i] = b;
     }
+    h = __builtin_bit_cast(f16x8, hw);
+    l = __builtin_bit_cast(f16x8, lw);
+}
+// the same for values that need no power
+__device__ __forceinline__ void split2x8(const float (&x)[8], f16x8& h, f16x8& l)
+{
+    typedef uint32_t u32x4_ __attribute__((ext_vector_type(4)));
+    u32x4_ hw, lw;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t a = __builtin_bit_cast(uint32_t, f16x2 { (_Float16)x[2 * i], (_Float16)x[2 * i + 1] });
+        uint32_t b;
+        asm("v_fma_mixlo_f16 %0, %1, 1.0, -%2 op_sel_hi:[0,0,1]" : "=v"(b) : "v"(x[2 * i]), "v"(a));
+        asm("v_fma_mixhi_f16 %0, %1, 1.0, -%2 op_sel:[0,0,1] op_sel_hi:[0,0,1]" : "+v"(b) : "v"(x[2 * i + 1]), "v"(a));
+        hw[i] = a;
+        lw[i] = b;
+    }
+    h = __builtin_bit_cast(f16x8, hw);
+    l = __builtin_bit_cast(f16x8, lw);
+}
+// max(a, b, c) and max(a, |b|, |c|) as one instruction each: the compiler's maximum of values that it has not computed itself takes another
+// one a value, for NaNs
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+__device__ __forceinline__ float max3_abs(float a, float b, float c)
+{
+    float r;
+    asm("v_max3_f32 %0, %1, abs(%2), abs(%3)" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
 }
 
 } // namespace fdx

@@ -39,12 +39,15 @@ __device__ __forceinline__ void store_plain_row(const RaggedParams& p, const Seq
 //
 // A workgroup takes 128 rows of one key head of one sequence, rows counting through the query heads of the group first (row = token *
 // group + head), so that short sequences fill a tile and a key is read once for all heads that share it; a wave takes 32 of them.
-// Keys and values pass through LDS in tiles of 64, split in two fp16 planes on the way (f16_split.hpp).  Products are taken
+// Keys and values pass through LDS in tiles of 4096 / D keys, split in two fp16 planes on the way (f16_split.hpp).  Products are taken
 // transposed, S^T = K Q^T: a query is a lane's column and keys are the accumulator's registers, so the softmax's running maximum and sum
 // are one register a lane, and the probabilities lie as the second product O^T = V^T P^T takes them.
+//  * LDS holds two tiles: while one is multiplied the next one is split and written beside the first product's matrix instructions and the
+//    one behind it is on its way to registers, one barrier a tile.  (One tile in LDS and two barriers: the vector units' and the matrix units' times
+//    added up instead of passing side by side.)
 //  * LDS holds blocks of eight contraction indices: keys [plane][depth block][key][16 bytes], values [plane][key block][depth][16 bytes].
-//    Depth block 4 g + l holds depths 32 g + 4 l .. + 3 and 32 g + 16 + 4 l .. + 3, the two 16-byte chunks that lane l of four fetches
-//    of a key row; a key block the eight keys whose probabilities one lane half has in eight consecutive accumulator registers.
+//    N = D / 16 threads fetch a key: depth block N g + l holds the 16-byte chunks 2 N g + l and 2 N g + N + l of the row, which lane l of the N
+//    has; a key block the eight keys whose probabilities one lane half has in eight consecutive accumulator registers.
 //  * A query row, a tile's keys and the values so far are each brought to fp16's range by a power of two; a tile whose values are larger than
 //    any before lowers the sums' power (a test a tile, rare).
 //  * The maximum that a row's exponentials refer to moves only when a score passes it by 2^4, so sums are rescaled a few times a row
@@ -52,21 +55,16 @@ __device__ __forceinline__ void store_plain_row(const RaggedParams& p, const Seq
 //  * Rows whose sums are not finite (infinite or NaN operands, whether the row sees them or not) are taken again by plain_row.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-template <typename T, int W>
-__device__ __forceinline__ void load_depths(const T* row, int d, int depth, bool wide, float (&x)[W])
+// W elements of a row from depth d on, zeros behind `depth`; EXACT: all are there and lie on vectors
+template <typename T, int W, bool EXACT>
+__device__ __forceinline__ void load_depths(const T* row, int d, int depth, int wide, float* x)
 {
     typedef T tv __attribute__((ext_vector_type(W)));
-    if (wide) {
-        if (d < depth) {
-            const tv v = *reinterpret_cast<const tv*>(row + d);
+    if (EXACT || (wide && d < depth)) {
+        const tv v = *reinterpret_cast<const tv*>(row + d);
 #pragma unroll
-            for (int e = 0; e < W; ++e)
-                x[e] = (float)v[e];
-        } else {
-#pragma unroll
-            for (int e = 0; e < W; ++e)
-                x[e] = 0.f;
-        }
+        for (int e = 0; e < W; ++e)
+            x[e] = (float)v[e];
     } else {
 #pragma unroll
         for (int e = 0; e < W; ++e)
@@ -76,18 +74,19 @@ __device__ __forceinline__ void load_depths(const T* row, int d, int depth, bool
 
 constexpr float kShift = 10.f; // exponentials are 2^kShift times the probability's numerator
 
-template <int D, int KIND, bool WIDE>
+template <int D, int KIND, bool EXACT>
 __global__ __launch_bounds__(256, 2) void ragged_tile_kernel(RaggedParams p)
 {
     typedef typename KvElement<KIND>::type T;
-    constexpr int KB = D / 8, STEPS = D / 16, KL = D / 32, VD = D / 32, DB = D / 32;
-    constexpr int KBLK = 64 * 16 + 32, VBLK = D * 16 + 32; // bytes of a block, offset against each other
+    constexpr int KT = 4096 / D, HALVES = KT / 32, N = D / 16; // keys of a tile, in accumulators of 32; threads that fetch a key
+    constexpr int KB = D / 8, VB = KT / 8, STEPS = D / 16, DB = D / 32;
+    constexpr int KBLK = KT * 16 + 32, VBLK = D * 16 + 32; // bytes of a block, offset against each other
     constexpr bool kPaged = KIND != kPackedF32;
-    __shared__ __attribute__((aligned(16))) unsigned char ks[2 * KB * KBLK];
-    __shared__ __attribute__((aligned(16))) unsigned char vs[2 * 8 * VBLK];
-    __shared__ float largest[2][4];
-    __shared__ int rows_of[2][64];
-    __shared__ uint64_t absent[2];
+    __shared__ __attribute__((aligned(16))) unsigned char ks0[2 * KB * KBLK], ks1[2 * KB * KBLK];
+    __shared__ __attribute__((aligned(16))) unsigned char vs0[2 * VB * VBLK], vs1[2 * VB * VBLK];
+    __shared__ float largest[2][2][4];
+    __shared__ int rows_of[4][KT];
+    __shared__ uint64_t absent[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 31, half = lane >> 5;
     if (p.error_flag && blockIdx.x == 0 && blockIdx.y == 0)
@@ -117,12 +116,13 @@ __global__ __launch_bounds__(256, 2) void ragged_tile_kernel(RaggedParams p)
     int k_end = visible_keys(p, s, r_last / p.group); // of the workgroup's last row
     if (blockIdx.y > 0 && k_first >= k_end)
         return;
-    if (k_end > k_first + p.split_keys)
+    if (k_end - k_first > p.split_keys)
         k_end = k_first + p.split_keys;
-    const int tiles = k_end > k_first ? (k_end - k_first + 63) / 64 : 0;
+    const int tiles = k_end > k_first ? (k_end - k_first + KT - 1) / KT : 0;
     // what the wave's rows see: all of them the first `wave_all_see`, some the first `wave_any`
     const int w_first = r_first + wave * 32, w_last = w_first + 31 < count ? w_first + 31 : count - 1;
-    const int wave_all_see = visible_keys(p, s, (w_first < count ? w_first : count - 1) / p.group), wave_any = visible_keys(p, s, w_last / p.group);
+    const int wave_all_see = visible_keys(p, s, (w_first < count ? w_first : count - 1) / p.group);
+    const int wave_any = visible_keys(p, s, w_last / p.group);
 
     // the query: depth block 2 u + half
     f16x8 qh[STEPS], ql[STEPS];
@@ -132,15 +132,9 @@ __global__ __launch_bounds__(256, 2) void ragged_tile_kernel(RaggedParams p)
         const float* from = p.q + q_row * p.ldq + (int64_t)head * p.dk;
 #pragma unroll
         for (int u = 0; u < STEPS; ++u) {
-            const int blk = 2 * u + half, d0 = 32 * (blk >> 2) + 4 * (blk & 3);
-            float lo[4], hi[4];
-            load_depths<float, 4>(from, d0, p.dk, WIDE, lo);
-            load_depths<float, 4>(from, d0 + 16, p.dk, WIDE, hi);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                x[u][e] = lo[e];
-                x[u][4 + e] = hi[e];
-            }
+            const int blk = 2 * u + half, d0 = 8 * N * (blk / N) + 4 * (blk % N);
+            load_depths<float, 4, EXACT>(from, d0, p.dk, p.wide, x[u]);
+            load_depths<float, 4, EXACT>(from, d0 + 4 * N, p.dk, p.wide, x[u] + 4);
 #pragma unroll
             for (int e = 0; e < 8; ++e)
                 top = fmaxf(top, fabsf(x[u][e]));
@@ -155,77 +149,91 @@ __global__ __launch_bounds__(256, 2) void ragged_tile_kernel(RaggedParams p)
 
     const T* kbase = static_cast<const T*>(p.k) + (int64_t)kv_head * p.dk;
     const T* vbase = static_cast<const T*>(p.v) + (int64_t)kv_head * p.dv;
-    const int krow = tid >> 2, kl = tid & 3, vblk = tid >> 5, vd = (tid & 31) * VD;
-    float kst[KL][8], vst[8][VD];
+    const int krow = tid / N, kl = tid % N, vblk = tid / (D / 2), vd = tid % (D / 2) * 2;
+    float kst[2][8], vst[8][2];
     // positions behind the range repeat its last one: masked, and as finite as it is
-    auto place = [&](int j0, int key, int buf) -> int64_t {
-        if constexpr (kPaged)
-            return rows_of[buf][key];
-        else
-            return s.span.first + (j0 + key < k_end ? j0 + key : k_end - 1);
+    auto place = [&](int t, int key) -> int64_t {
+        if constexpr (kPaged) {
+            return rows_of[t & 3][key];
+        } else {
+            const int at = k_first + t * KT + key;
+            return s.span.first + (at < k_end ? at : k_end - 1);
+        }
     };
-    auto look_up = [&](int j0) { // lane of wave 0: the place of key j0 + lane
-        return key_row<KIND>(p, s, j0 + lane < k_end ? j0 + lane : k_end - 1);
+    auto look_up = [&](int t) { // lane of wave 0: the place of a key of tile t
+        const int at = k_first + t * KT + (lane & (KT - 1));
+        return key_row<KIND>(p, s, at < k_end ? at : k_end - 1);
     };
-    auto keep_place = [&](int row, int buf) {
-        rows_of[buf][lane] = row < 0 ? 0 : row;
+    auto keep_place = [&](int row, int t) {
+        if (lane < KT)
+            rows_of[t & 3][lane] = row < 0 ? 0 : row;
         const uint64_t none = __ballot(row < 0);
         if (lane == 0) {
-            absent[buf] = none;
+            absent[t & 3] = none;
             raise_flag(p, none != 0);
         }
     };
-    auto fetch = [&](int j0, int buf) {
-        const T* kr = kbase + place(j0, krow, buf) * p.ldk;
+    const uint32_t ld_k = (uint32_t)p.ldk, ld_v = (uint32_t)p.ldv;
+    const int vkey = 16 * (vblk >> 1) + 4 * (vblk & 1); // the first of the eight keys, the others 1, 2, 3, 8, 9, 10, 11 behind it
+    auto fetch = [&](int t) {
+        if (EXACT && !kPaged && k_first + (t + 1) * KT <= k_end) { // a whole tile: one base, offsets that stay
+            const int64_t row = s.span.first + k_first + t * KT;
+            const T *kr = kbase + row * p.ldk, *vr = vbase + row * p.ldv;
+            const uint32_t ko = krow * ld_k + 4 * kl, vo = vkey * ld_v + vd;
 #pragma unroll
-        for (int g = 0; g < KL; ++g) {
-            float lo[4], hi[4];
-            load_depths<T, 4>(kr, 32 * g + 4 * kl, p.dk, WIDE, lo);
-            load_depths<T, 4>(kr, 32 * g + 16 + 4 * kl, p.dk, WIDE, hi);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                kst[g][e] = lo[e];
-                kst[g][4 + e] = hi[e];
+            for (int g = 0; g < 2; ++g) {
+                load_depths<T, 4, EXACT>(kr + (ko + 8 * N * g), 0, 0, 1, kst[g]);
+                load_depths<T, 4, EXACT>(kr + (ko + 8 * N * g + 4 * N), 0, 0, 1, kst[g] + 4);
             }
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                load_depths<T, 2, EXACT>(vr + (vo + (8 * (j >> 2) + (j & 3)) * ld_v), 0, 0, 1, vst[j]);
+            return;
+        }
+        const T* kr = kbase + place(t, krow) * p.ldk;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            load_depths<T, 4, EXACT>(kr, 8 * N * g + 4 * kl, p.dk, p.wide, kst[g]);
+            load_depths<T, 4, EXACT>(kr, 8 * N * g + 4 * N + 4 * kl, p.dk, p.wide, kst[g] + 4);
+        }
+        if (EXACT && kPaged && p.page_size % 16 == 0) { // the eight keys lie in one page
+            const T* vr = vbase + place(t, vkey) * p.ldv + vd;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                load_depths<T, 2, EXACT>(vr + (8 * (j >> 2) + (j & 3)) * ld_v, 0, 0, 1, vst[j]);
+            return;
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            load_depths<T, VD>(vbase + place(j0, 16 * (vblk >> 1) + 4 * (vblk & 1) + 8 * (j >> 2) + (j & 3), buf) * p.ldv, vd, p.dv, WIDE, vst[j]);
+            load_depths<T, 2, EXACT>(vbase + place(t, vkey + 8 * (j >> 2) + (j & 3)) * p.ldv, vd, p.dv, p.wide, vst[j]);
     };
-    auto measure = [&] { // the largest finite key and value of the fetched tile
+    auto measure = [&](int t) { // the largest finite key and value of the fetched tile
         float km = 0.f, vm = 0.f;
 #pragma unroll
-        for (int g = 0; g < KL; ++g)
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                km = fmaxf(km, fabsf(kst[g][e]));
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-#pragma unroll
-            for (int d = 0; d < VD; ++d)
-                vm = fmaxf(vm, fabsf(vst[j][d]));
+        for (int e = 0; e < 8; ++e) {
+            km = max3_abs(km, kst[0][e], kst[1][e]);
+            vm = max3_abs(vm, vst[e][0], vst[e][1]);
+        }
         km = wave_all<true>(km);
         vm = wave_all<true>(vm);
         if (__builtin_expect(km == INFINITY || vm == INFINITY, 0)) { // rows that do not see the infinity keep their sums
             km = vm = 0.f;
 #pragma unroll
-            for (int g = 0; g < KL; ++g)
+            for (int e = 0; e < 8; ++e)
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
+                for (int g = 0; g < 2; ++g) {
                     km = fmaxf(km, fabsf(kst[g][e]) < INFINITY ? fabsf(kst[g][e]) : 0.f);
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-#pragma unroll
-                for (int d = 0; d < VD; ++d)
-                    vm = fmaxf(vm, fabsf(vst[j][d]) < INFINITY ? fabsf(vst[j][d]) : 0.f);
+                    vm = fmaxf(vm, fabsf(vst[e][g]) < INFINITY ? fabsf(vst[e][g]) : 0.f);
+                }
             km = wave_all<true>(km);
             vm = wave_all<true>(vm);
         }
         if (lane == 0) {
-            largest[0][wave] = km;
-            largest[1][wave] = vm;
+            largest[t & 1][0][wave] = km;
+            largest[t & 1][1][wave] = vm;
         }
     };
+    auto four = [](const float* v) { return fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])); };
     auto mfma = [](f16x8 a, f16x8 b, const f32x16& acc) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, acc, 0, 0, 0); };
     constexpr f32x16 kZero = { 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f };
 
@@ -234,91 +242,78 @@ __global__ __launch_bounds__(256, 2) void ragged_tile_kernel(RaggedParams p)
     for (int d = 0; d < DB; ++d)
         oacc[d] = kZero;
     float m_run = -INFINITY, l_run = 0.f, v_top = 0.f;
-    Pow2 sv = pow2_for(0.f);
+    Pow2 sk = pow2_for(0.f), sv = sk, sk_next = sk, sv_next = sk; // of the tile at work (sv: of the sums) and of the one behind it
     int next_row = 0;
-
-    if (tiles > 0) {
-        if constexpr (kPaged) {
-            if (wave == 0) {
-                keep_place(look_up(k_first), 0);
-                next_row = look_up(k_first + 64);
-            }
-            __syncthreads();
-        }
-        fetch(k_first, 0);
-        measure();
-    }
-    for (int t = 0; t < tiles; ++t) {
-        const int j0 = k_first + t * 64;
-        __syncthreads(); // every wave is done with the previous tile
-        const Pow2 sk = pow2_for(fmaxf(fmaxf(largest[0][0], largest[0][1]), fmaxf(largest[0][2], largest[0][3])));
-        const float vm = fmaxf(fmaxf(largest[1][0], largest[1][1]), fmaxf(largest[1][2], largest[1][3]));
-        if (vm > v_top) { // the same for the whole workgroup
-            v_top = vm;
-            const Pow2 now = pow2_for(vm);
-            const float f = now.up * sv.down;
-            sv = now;
-            if (f != 1.f) {
+    auto scale_next = [&](int t) {
+        sk_next = pow2_for(four(largest[t & 1][0]));
+        v_top = fmaxf(v_top, four(largest[t & 1][1]));
+        sv_next = pow2_for(v_top);
+    };
+    auto stage = [&](unsigned char* ks, unsigned char* vs) {
 #pragma unroll
-                for (int d = 0; d < DB; ++d)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        oacc[d][e] *= f;
-            }
-        }
-#pragma unroll
-        for (int g = 0; g < KL; ++g) {
+        for (int g = 0; g < 2; ++g) {
             f16x8 h, l;
-            split2x8(kst[g], sk.up, h, l);
-            *reinterpret_cast<f16x8*>(&ks[(4 * g + kl) * KBLK + krow * 16]) = h;
-            *reinterpret_cast<f16x8*>(&ks[(KB + 4 * g + kl) * KBLK + krow * 16]) = l;
+            split2x8(kst[g], sk_next.up, h, l);
+            *reinterpret_cast<f16x8*>(&ks[(N * g + kl) * KBLK + krow * 16]) = h;
+            *reinterpret_cast<f16x8*>(&ks[(KB + N * g + kl) * KBLK + krow * 16]) = l;
         }
 #pragma unroll
-        for (int d = 0; d < VD; ++d) {
+        for (int d = 0; d < 2; ++d) {
             const float x[8] = { vst[0][d], vst[1][d], vst[2][d], vst[3][d], vst[4][d], vst[5][d], vst[6][d], vst[7][d] };
             f16x8 h, l;
-            split2x8(x, sv.up, h, l);
+            split2x8(x, sv_next.up, h, l);
             *reinterpret_cast<f16x8*>(&vs[vblk * VBLK + (vd + d) * 16]) = h;
-            *reinterpret_cast<f16x8*>(&vs[(8 + vblk) * VBLK + (vd + d) * 16]) = l;
+            *reinterpret_cast<f16x8*>(&vs[(VB + vblk) * VBLK + (vd + d) * 16]) = l;
         }
-        if constexpr (kPaged)
-            if (wave == 0 && t + 1 < tiles)
-                keep_place(next_row, (t + 1) & 1);
-        __syncthreads();
-        if (t + 1 < tiles) {
-            fetch(j0 + 64, (t + 1) & 1); // in flight while this tile is worked on
-            if (kPaged && wave == 0 && t + 2 < tiles)
-                next_row = look_up(j0 + 128);
-        }
-        if (j0 < wave_any) { // some row of this wave sees some key of the tile
-            // S^T: 64 keys x 32 rows
-            f32x16 sacc[2];
+    };
+    auto turn = [&](int t, const unsigned char* ks, const unsigned char* vs, unsigned char* ks_next, unsigned char* vs_next) {
+        const int j0 = k_first + t * KT;
+        const bool work = j0 < wave_any; // some row of this wave sees some key of the tile
+        const float f = sv_next.up * sv.down;
+        sk = sk_next;
+        if (work)
+            sv = sv_next; // a wave that is through keeps its sums as they are
+        if (t + 1 < tiles)
+            scale_next(t + 1);
+        // S^T: KT keys x 32 rows, for a wave that sees none of them too; beside it tile t + 1 goes to LDS (the last time what the
+        // registers still hold, for nobody)
+        f32x16 sacc[HALVES];
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb) {
-                sacc[kb] = kZero;
+        for (int kb = 0; kb < HALVES; ++kb) {
+            sacc[kb] = kZero;
 #pragma unroll
-                for (int u = 0; u < STEPS; ++u) {
-                    const f16x8 kh = *reinterpret_cast<const f16x8*>(&ks[(2 * u + half) * KBLK + (kb * 32 + c) * 16]);
-                    const f16x8 kw = *reinterpret_cast<const f16x8*>(&ks[(KB + 2 * u + half) * KBLK + (kb * 32 + c) * 16]);
-                    sacc[kb] = mfma(kw, qh[u], sacc[kb]);
-                    sacc[kb] = mfma(kh, ql[u], sacc[kb]);
-                    sacc[kb] = mfma(kh, qh[u], sacc[kb]);
-                }
+            for (int u = 0; u < STEPS; ++u) {
+                const f16x8 kh = *reinterpret_cast<const f16x8*>(&ks[(2 * u + half) * KBLK + (kb * 32 + c) * 16]);
+                const f16x8 kw = *reinterpret_cast<const f16x8*>(&ks[(KB + 2 * u + half) * KBLK + (kb * 32 + c) * 16]);
+                sacc[kb] = mfma(kw, qh[u], sacc[kb]);
+                sacc[kb] = mfma(kh, ql[u], sacc[kb]);
+                sacc[kb] = mfma(kh, qh[u], sacc[kb]);
             }
+        }
+        stage(ks_next, vs_next);
+        if constexpr (kPaged)
+            if (wave == 0 && t + 3 < tiles)
+                keep_place(next_row, t + 3);
+        if (t + 2 < tiles) {
+            fetch(t + 2);
+            if (kPaged && wave == 0 && t + 4 < tiles)
+                next_row = look_up(t + 4);
+        }
+        if (work) {
             const int limit = (visible < k_end ? visible : k_end) - j0; // keys of the tile that this lane's row sees
-            if (j0 + 64 > wave_all_see || j0 + 64 > k_end) {
+            if (j0 + KT > wave_all_see || j0 + KT > k_end) {
 #pragma unroll
-                for (int kb = 0; kb < 2; ++kb)
+                for (int kb = 0; kb < HALVES; ++kb)
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
                         if (kb * 32 + 8 * (e >> 2) + 4 * half + (e & 3) >= limit)
                             sacc[kb][e] = -INFINITY;
             }
             if constexpr (kPaged) {
-                const uint64_t none = absent[t & 1];
+                const uint64_t none = absent[t & 3];
                 if (none != 0) {
 #pragma unroll
-                    for (int kb = 0; kb < 2; ++kb)
+                    for (int kb = 0; kb < HALVES; ++kb)
 #pragma unroll
                         for (int e = 0; e < 16; ++e)
                             if (none >> (kb * 32 + 8 * (e >> 2) + 4 * half + (e & 3)) & 1)
@@ -327,15 +322,15 @@ __global__ __launch_bounds__(256, 2) void ragged_tile_kernel(RaggedParams p)
             }
             float mx = -INFINITY;
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
+            for (int kb = 0; kb < HALVES; ++kb)
 #pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    mx = fmaxf(mx, sacc[kb][e]);
+                for (int e = 0; e < 16; e += 2)
+                    mx = max3(mx, sacc[kb][e], sacc[kb][e + 1]);
             mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
             const float to_log2 = fmaxf(q_down * sk.down, 1.17549435e-38f); // above zero: -infinity stays what it is
             mx *= to_log2;
-            if (__any(mx > m_run + 4.f)) {
-                const float m_new = fmaxf(m_run, mx);
+            if (__any(mx > m_run + 4.f) || f != 1.f) {
+                const float m_new = mx > m_run + 4.f ? mx : m_run;
                 const float corr = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
                 m_run = m_new;
                 l_run *= corr;
@@ -343,12 +338,12 @@ __global__ __launch_bounds__(256, 2) void ragged_tile_kernel(RaggedParams p)
                 for (int d = 0; d < DB; ++d)
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
-                        oacc[d][e] *= corr;
+                        oacc[d][e] *= corr * f;
             }
             const float base = kShift - (m_run == -INFINITY ? 0.f : m_run); // a row that has seen no key yet adds zeros
             float rs = 0.f;
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
+            for (int kb = 0; kb < HALVES; ++kb)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     sacc[kb][e] = __builtin_amdgcn_exp2f(fmaf(sacc[kb][e], to_log2, base));
@@ -357,25 +352,55 @@ __global__ __launch_bounds__(256, 2) void ragged_tile_kernel(RaggedParams p)
             l_run += rs; // the other half of the tile's keys lies in lane + 32: they meet at the end
             // O^T += V^T P^T
 #pragma unroll
-            for (int u = 0; u < 4; ++u) { // keys of block 2 u + half: registers 8 (u % 2) .. + 7 of half tile u / 2
+            for (int u = 0; u < KT / 16; ++u) { // keys of block 2 u + half: registers 8 (u % 2) .. + 7 of accumulator u / 2
                 float x[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
                     x[j] = sacc[u >> 1][8 * (u & 1) + j];
                 f16x8 ph, pl;
-                split2x8(x, 1.f, ph, pl);
+                split2x8(x, ph, pl);
 #pragma unroll
                 for (int d = 0; d < DB; ++d) {
                     const f16x8 vh = *reinterpret_cast<const f16x8*>(&vs[(2 * u + half) * VBLK + (d * 32 + c) * 16]);
-                    const f16x8 vl = *reinterpret_cast<const f16x8*>(&vs[(8 + 2 * u + half) * VBLK + (d * 32 + c) * 16]);
+                    const f16x8 vl = *reinterpret_cast<const f16x8*>(&vs[(VB + 2 * u + half) * VBLK + (d * 32 + c) * 16]);
                     oacc[d] = mfma(vl, ph, oacc[d]);
                     oacc[d] = mfma(vh, pl, oacc[d]);
                     oacc[d] = mfma(vh, ph, oacc[d]);
                 }
             }
         }
+        if (t + 2 < tiles)
+            measure(t + 2);
+        __syncthreads();
+    };
+
+    if (tiles > 0) {
+        if constexpr (kPaged) {
+            if (wave == 0) {
+                const int row0 = look_up(0), row1 = look_up(1), row2 = look_up(2);
+                next_row = look_up(3);
+                keep_place(row0, 0);
+                keep_place(row1, 1);
+                keep_place(row2, 2);
+            }
+            __syncthreads();
+        }
+        fetch(0);
+        measure(0);
+        __syncthreads();
+        scale_next(0);
+        stage(ks0, vs0);
+        if (tiles > 1) {
+            fetch(1);
+            measure(1);
+        }
+        __syncthreads();
+        sv = sv_next;
+    }
+    for (int t = 0; t < tiles; t += 2) {
+        turn(t, ks0, vs0, ks1, vs1);
         if (t + 1 < tiles)
-            measure();
+            turn(t + 1, ks1, vs1, ks0, vs0);
     }
 
     l_run += __shfl_xor(l_run, 32, 64);
@@ -404,9 +429,8 @@ __global__ __launch_bounds__(256, 2) void ragged_tile_kernel(RaggedParams p)
             for (int g = 0; g < 4; ++g) {
                 const int depth = 32 * d + 8 * g + 4 * half;
                 const f32x4 o = { oacc[d][4 * g] * f, oacc[d][4 * g + 1] * f, oacc[d][4 * g + 2] * f, oacc[d][4 * g + 3] * f };
-                if (WIDE) {
-                    if (depth < p.dv)
-                        *reinterpret_cast<f32x4*>(to + depth) = o;
+                if (EXACT || (p.wide && depth < p.dv)) {
+                    *reinterpret_cast<f32x4*>(to + depth) = o;
                 } else {
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
@@ -814,6 +838,7 @@ template <int D, int KIND, bool WIDE>
 static void ragged_launch(RaggedParams p, const RaggedPlan& plan)
 {
     p.few_rows = plan.few_rows;
+    p.wide = WIDE;
     p.ranges = plan.ranges();
     if constexpr (KIND != kPackedF32) {
         if (plan.few_ranges > 0) {
@@ -827,7 +852,11 @@ static void ragged_launch(RaggedParams p, const RaggedPlan& plan)
     }
     if (plan.tiles > 0) {
         p.split_keys = plan.tile_keys;
-        hipLaunchKernelGGL((ragged_tile_kernel<D, KIND, WIDE>), dim3((unsigned)plan.tiles, (unsigned)plan.tile_ranges), dim3(256), 0, stream(), p);
+        const dim3 grid((unsigned)plan.tiles, (unsigned)plan.tile_ranges);
+        if (WIDE && p.dk == D && p.dv == D && p.ldk < (1 << 24) && p.ldv < (1 << 24)) // offsets inside a tile in 32 bits
+            hipLaunchKernelGGL((ragged_tile_kernel<D, KIND, true>), grid, dim3(256), 0, stream(), p);
+        else
+            hipLaunchKernelGGL((ragged_tile_kernel<D, KIND, false>), grid, dim3(256), 0, stream(), p);
     }
     if (plan.ranges() > 1)
         hipLaunchKernelGGL(ragged_join_kernel<KIND>, dim3((unsigned)(((int64_t)p.tokens * p.heads + 3) / 4)), dim3(256), 0, stream(), p, plan.few_keys,

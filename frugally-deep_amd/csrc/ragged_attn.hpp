@@ -28,6 +28,7 @@ struct RaggedParams {
     float* part;          // rows that see more than split_keys keys: sums of each range of split_keys, met by ragged_join_kernel
     int ranges;           // ranges that p.part has room for
     int split_keys;
+    int wide;             // rows of every tensor lie on 16-byte vectors, and depths are whole ones
     int few_rows;         // sequences that bring up to this many rows to a key head are ragged_few_kernel's, others ragged_tile_kernel's
 };
 
