@@ -18,6 +18,7 @@ struct AppendParams {
     const int32_t* starts;
     int tokens;
     fdx_kv_pages c;
+    Divisor page_size;
     int* error_flag;
 };
 
@@ -50,7 +51,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendParams p)
     const int64_t pos = (int64_t)p.c.lens[s] - span.count + (row - span.first);
     const int at = pos < 0 || pos >= p.c.max_len
         ? -1
-        : page_row(p.c.table + (int64_t)s * p.c.table_width, p.c.table_width, p.c.n_pages, p.c.page_size, (int)pos);
+        : page_row(p.c.table + (int64_t)s * p.c.table_width, p.c.table_width, p.c.n_pages, p.page_size, (int)pos);
     if (at < 0) {
         if (p.error_flag && lane == 0)
             *p.error_flag = 1;
@@ -74,6 +75,7 @@ fdx_status check_kv_pages(const char* who, const fdx_kv_pages* c)
     FDX_REQUIRE((int64_t)c->n_pages * c->page_size < ((int64_t)1 << 31), "%s: more than 2^31 positions in the cache", who);
     FDX_REQUIRE((int64_t)c->kv_heads * c->dk < ((int64_t)1 << 31) && (int64_t)c->kv_heads * c->dv < ((int64_t)1 << 31),
         "%s: rows of the cache too long", who);
+    FDX_REQUIRE(c->max_len <= (1 << 30), "%s: sequences of more than 2^30 positions", who);
     FDX_REQUIRE((int64_t)c->table_width * c->page_size >= c->max_len, "%s: the table does not reach max_len", who);
     const uintptr_t size = c->type == FDX_KV_BF16 ? 2 : 4;
     FDX_REQUIRE(((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & (size - 1)) == 0,
@@ -95,7 +97,7 @@ extern "C" fdx_status fdx_kv_append_f32(const float* k, int64_t ldk, const float
     FDX_REQUIRE(tokens > 0 && tokens <= (1 << 25), "kv_append: 1 to 2^25 tokens");
     const int64_t nk = (int64_t)cache->kv_heads * cache->dk, nv = (int64_t)cache->kv_heads * cache->dv;
     FDX_REQUIRE(ldk >= nk && ldv >= nv, "kv_append: rows overlap");
-    const AppendParams p { k, v, ldk, ldv, starts, tokens, *cache, error_flag_dev };
+    const AppendParams p { k, v, ldk, ldv, starts, tokens, *cache, make_divisor(cache->page_size), error_flag_dev };
     const dim3 grid((unsigned)((2 * (int64_t)tokens + 3) / 4));
     // vectors of four wherever every row of the four tensors starts on one
     const uintptr_t rows = reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)

@@ -11,6 +11,21 @@
 
 namespace fdx {
 
+// Quotients by a number that a launch does not change, as a product: with 2^l >= by, mul = floor(2^(31+l) / by) + 1 is off from 2^(31+l) / by
+// by at most 1, so n mul / 2^(31+l) from n / by by less than 1 / by for n < 2^31.
+struct Divisor {
+    uint32_t by, mul;
+    int shift;
+};
+inline Divisor make_divisor(int by)
+{
+    int l = 0;
+    while (((int64_t)1 << l) < by)
+        ++l;
+    return { (uint32_t)by, (uint32_t)(((uint64_t)1 << (31 + l)) / (uint32_t)by + 1), 31 + l };
+}
+FDX_HD int quotient(int n, const Divisor& d) { return (int)((uint64_t)(uint32_t)n * d.mul >> d.shift); }
+
 struct Span {
     int first, count;
 };
@@ -81,15 +96,15 @@ FDX_HD int find_row(const int32_t* starts, int n_seqs, int tokens, int row)
 }
 
 // row of position `pos` among the rows of all pages, -1 if the table does not reach it or names no page of the cache
-FDX_HD int page_row(const int32_t* table_row, int table_width, int n_pages, int page_size, int pos)
+FDX_HD int page_row(const int32_t* table_row, int table_width, int n_pages, const Divisor& page_size, int pos)
 {
     if (pos < 0)
         return -1;
-    const int at = (int)((uint32_t)pos / (uint32_t)page_size);
+    const int at = quotient(pos, page_size);
     if (at >= table_width)
         return -1;
     const int page = table_row[at];
-    return page < 0 || page >= n_pages ? -1 : page * page_size + (pos - at * page_size);
+    return page < 0 || page >= n_pages ? -1 : page * (int)page_size.by + (pos - at * (int)page_size.by);
 }
 
 } // namespace fdx

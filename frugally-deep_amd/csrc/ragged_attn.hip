@@ -14,25 +14,31 @@ template <int KIND>
 __device__ __forceinline__ void store_plain_row(const RaggedParams& p, const Sequence& s, int token, int head, int kv_head, int range, int lane)
 {
     const int visible = visible_keys(p, s, token);
-    const bool in_parts = visible > p.split_keys;
-    const int first = range * p.split_keys;
+    const bool in_parts = visible > s.range;
+    const int first = in_parts ? range * s.range : 0;
     if (in_parts ? first >= visible : range > 0)
         return;
-    const int last = in_parts && visible - first > p.split_keys ? first + p.split_keys : visible;
-    const int64_t row = s.span.first + token, id = row * p.heads + head;
+    const int last = in_parts && visible - first > s.range ? first + s.range : visible;
+    const int64_t row = s.span.first + token;
     float m, l, o[2];
     bool seen, missing;
     plain_row<KIND>(p, s, p.q + row * p.ldq + (int64_t)head * p.dk, kv_head, first, last, m, l, o, seen, missing);
     raise_flag(p, missing);
-    float* to = in_parts ? part_out(p, range, id) : p.out + row * p.ldo + (int64_t)head * p.dv;
-    if (in_parts && lane == 0) {
-        part_size(p, range, id)[0] = seen && m == -INFINITY ? -FLT_MAX : m;
-        part_size(p, range, id)[1] = l;
+    float* to = p.out + row * p.ldo + (int64_t)head * p.dv;
+    if (in_parts) {
+        const PartSums& part = s.few ? p.few : p.tile;
+        const int64_t id = part_row(p, s, token, head);
+        to = part.out(range, id, p.dv);
+        if (lane == 0) {
+            float* at = part.size(range, id, p.dv);
+            at[0] = seen && m == -INFINITY ? -FLT_MAX : m;
+            at[1] = l;
+        }
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i)
         if (64 * i + lane < p.dv)
-            to[64 * i + lane] = in_parts ? finish(o[i], l, false) : finish(o[i], l, seen);
+            to[64 * i + lane] = finish(o[i], l, seen && !in_parts);
 }
 
 // ---- many query rows: tiles on the fp16 matrix instructions ----
@@ -45,14 +51,16 @@ __device__ __forceinline__ void store_plain_row(const RaggedParams& p, const Seq
 //  * LDS holds two tiles: while one is multiplied the next one is split and written beside the first product's matrix instructions and the
 //    one behind it is on its way to registers, one barrier a tile.  (One tile in LDS and two barriers: the vector units' and the matrix units' times
 //    added up instead of passing side by side.)
-//  * LDS holds blocks of eight contraction indices: keys [plane][depth block][key][16 bytes], values [plane][key block][depth][16 bytes].
-//    N = D / 16 threads fetch a key: depth block N g + l holds the 16-byte chunks 2 N g + l and 2 N g + N + l of the row, which lane l of the N
-//    has; a key block the eight keys whose probabilities one lane half has in eight consecutive accumulator registers.
-//  * A query row, a tile's keys and the values so far are each brought to fp16's range by a power of two; a tile whose values are larger than
-//    any before lowers the sums' power (a test a tile, rare).
+//  * N = D / 16 threads fetch a key's row of either: block N g + l of eight depths holds the 16-byte chunks 2 N g + l and 2 N g + N + l of it,
+//    which lane l of the N has.  Keys lie as [plane][depth block][key][16 bytes], which the first product reads as it is; values as
+//    [plane][key][depth], and the transposing LDS read gives the second product four keys of a depth at a time.
+//  * A query row, a tile's keys and its values are each brought to fp16's range by a power of two.  The sums have the power of the last
+//    tile's values, which changes with one that is another multiple of four.  A tile whose rows are too far apart in size for one power
+//    (spread_fits; a row of 10^30 behind the mask) is left to plain sums.
 //  * The maximum that a row's exponentials refer to moves only when a score passes it by 2^4, so sums are rescaled a few times a row
 //    instead of every tile; exponentials carry 2^10 to stay clear of fp16's small end, at most 2^14.
-//  * Rows whose sums are not finite (infinite or NaN operands, whether the row sees them or not) are taken again by plain_row.
+//  * Rows whose sums are not finite (infinite or NaN operands, whether the row sees them or not, and tiles left out above) are taken again by
+//    plain_row.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 // W elements of a row from depth d on, zeros behind `depth`; EXACT: all are there and lie on vectors
@@ -72,6 +80,17 @@ __device__ __forceinline__ void load_depths(const T* row, int d, int depth, int 
     }
 }
 
+// a workgroup's row: its token, the row of q and out, its head (rows behind the last one: the last one's)
+struct QueryRow {
+    int token, head;
+    int64_t row;
+};
+__device__ __forceinline__ QueryRow row_of(const RaggedParams& p, const Sequence& s, int kv_head, int count, int r)
+{
+    const int at = r < count ? r : count - 1, token = quotient(at, p.by_group);
+    return { token, kv_head * p.group + at - token * p.group, (int64_t)s.span.first + token };
+}
+
 constexpr float kShift = 10.f; // exponentials are 2^kShift times the probability's numerator
 
 template <int D, int KIND, bool EXACT>
@@ -79,14 +98,15 @@ __global__ __launch_bounds__(256, 2) void ragged_tile_kernel(RaggedParams p)
 {
     typedef typename KvElement<KIND>::type T;
     constexpr int KT = 4096 / D, HALVES = KT / 32, N = D / 16; // keys of a tile, in accumulators of 32; threads that fetch a key
-    constexpr int KB = D / 8, VB = KT / 8, STEPS = D / 16, DB = D / 32;
-    constexpr int KBLK = KT * 16 + 32, VBLK = D * 16 + 32; // bytes of a block, offset against each other
+    constexpr int KB = D / 8, STEPS = D / 16, DB = D / 32;
+    constexpr int KBLK = KT * 16 + 32, VROW = D * 2 + 32; // bytes of a block of keys, of a row of values, offset against each other
     constexpr bool kPaged = KIND != kPackedF32;
     __shared__ __attribute__((aligned(16))) unsigned char ks0[2 * KB * KBLK], ks1[2 * KB * KBLK];
-    __shared__ __attribute__((aligned(16))) unsigned char vs0[2 * VB * VBLK], vs1[2 * VB * VBLK];
-    __shared__ float largest[2][2][4];
-    __shared__ int rows_of[4][KT];
-    __shared__ uint64_t absent[4];
+    __shared__ __attribute__((aligned(16))) unsigned char vs0[2 * KT * VROW], vs1[2 * KT * VROW];
+    __shared__ Spread spread[2][4];
+    constexpr int kAhead = 512; // places of two halves of as many positions are looked up ahead, all threads at once
+    __shared__ int rows_of[kPaged ? 2 * kAhead : 1];
+    __shared__ int some_absent;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 31, half = lane >> 5;
     if (p.error_flag && blockIdx.x == 0 && blockIdx.y == 0)
@@ -95,7 +115,9 @@ __global__ __launch_bounds__(256, 2) void ragged_tile_kernel(RaggedParams p)
     // key heads next to each other: consecutive workgroups go to the eight XCDs in turn, so that an XCD's cache holds few heads'
     // keys; later tiles of a sequence, which see more keys, first
     const int kv_head = blockIdx.x % p.kv_heads;
-    const Tile tile = find_tile(p.starts, p.n_seqs, p.tokens, p.group, 128, gridDim.x / p.kv_heads - 1 - blockIdx.x / p.kv_heads);
+    const int64_t number = blockIdx.x / p.kv_heads;
+    const Tile tile = p.causal && p.n_seqs <= 64 ? late_tile_wave(p.starts, p.n_seqs, p.tokens, p.group, 128, number)
+                                                 : find_tile_wave(p.starts, p.n_seqs, p.tokens, p.group, 128, gridDim.x / p.kv_heads - 1 - number);
     if (tile.seq < 0)
         return;
     const Sequence s = sequence_of<KIND>(p, tile.seq, tile.span);
@@ -103,33 +125,31 @@ __global__ __launch_bounds__(256, 2) void ragged_tile_kernel(RaggedParams p)
         raise_flag(p, s.cut);
     const int count = s.span.count * p.group; // rows
     const int r_first = tile.index * 128;
-    if (r_first >= count || count <= p.few_rows)
+    if (r_first >= count || (KIND != kPackedF32 && s.few))
         return;
-    const int r = r_first + wave * 32 + c;
-    const bool q_ok = r < count;
-    const int token = (q_ok ? r : count - 1) / p.group, head = kv_head * p.group + (q_ok ? r : count - 1) - token * p.group;
-    const int64_t q_row = s.span.first + token;
-    const int visible = visible_keys(p, s, token);
+    const int visible = visible_keys(p, s, row_of(p, s, kv_head, count, r_first + wave * 32 + c).token);
 
     const int r_last = r_first + 128 < count ? r_first + 127 : count - 1;
-    const int k_first = blockIdx.y * p.split_keys;
-    int k_end = visible_keys(p, s, r_last / p.group); // of the workgroup's last row
-    if (blockIdx.y > 0 && k_first >= k_end)
+    int k_end = visible_keys(p, s, quotient(r_last, p.by_group)); // of the workgroup's last row
+    const int64_t k_from = (int64_t)blockIdx.y * s.range;
+    if (blockIdx.y > 0 && k_from >= k_end)
         return;
-    if (k_end - k_first > p.split_keys)
-        k_end = k_first + p.split_keys;
+    const int k_first = (int)k_from;
+    if (k_end - k_first > s.range)
+        k_end = k_first + s.range;
     const int tiles = k_end > k_first ? (k_end - k_first + KT - 1) / KT : 0;
     // what the wave's rows see: all of them the first `wave_all_see`, some the first `wave_any`
     const int w_first = r_first + wave * 32, w_last = w_first + 31 < count ? w_first + 31 : count - 1;
-    const int wave_all_see = visible_keys(p, s, (w_first < count ? w_first : count - 1) / p.group);
-    const int wave_any = visible_keys(p, s, w_last / p.group);
+    const int wave_all_see = visible_keys(p, s, quotient(w_first < count ? w_first : count - 1, p.by_group));
+    const int wave_any = visible_keys(p, s, quotient(w_last, p.by_group));
 
     // the query: depth block 2 u + half
     f16x8 qh[STEPS], ql[STEPS];
     float q_down;
     {
         float x[STEPS][8], top = 0.f;
-        const float* from = p.q + q_row * p.ldq + (int64_t)head * p.dk;
+        const QueryRow at = row_of(p, s, kv_head, count, r_first + wave * 32 + c);
+        const float* from = p.q + at.row * p.ldq + (int64_t)at.head * p.dk;
 #pragma unroll
         for (int u = 0; u < STEPS; ++u) {
             const int blk = 2 * u + half, d0 = 8 * N * (blk / N) + 4 * (blk % N);
@@ -139,8 +159,7 @@ __global__ __launch_bounds__(256, 2) void ragged_tile_kernel(RaggedParams p)
             for (int e = 0; e < 8; ++e)
                 top = fmaxf(top, fabsf(x[u][e]));
         }
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
-        const Pow2 sq = pow2_for(top);
+        const Pow2 sq = pow2_for<1>(exponent(max_halves(top)));
         q_down = sq.down * (p.scale * kLog2e);
 #pragma unroll
         for (int u = 0; u < STEPS; ++u)
@@ -149,91 +168,80 @@ __global__ __launch_bounds__(256, 2) void ragged_tile_kernel(RaggedParams p)
 
     const T* kbase = static_cast<const T*>(p.k) + (int64_t)kv_head * p.dk;
     const T* vbase = static_cast<const T*>(p.v) + (int64_t)kv_head * p.dv;
-    const int krow = tid / N, kl = tid % N, vblk = tid / (D / 2), vd = tid % (D / 2) * 2;
-    float kst[2][8], vst[8][2];
+    const int krow = tid / N, kl = tid % N;
+    float kst[2][8], vst[2][8];
     // positions behind the range repeat its last one: masked, and as finite as it is
     auto place = [&](int t, int key) -> int64_t {
         if constexpr (kPaged) {
-            return rows_of[t & 3][key];
+            const int row = rows_of[(t * KT + key) & (2 * kAhead - 1)];
+            return row < 0 ? 0 : row;
         } else {
             const int at = k_first + t * KT + key;
             return s.span.first + (at < k_end ? at : k_end - 1);
         }
     };
-    auto look_up = [&](int t) { // lane of wave 0: the place of a key of tile t
-        const int at = k_first + t * KT + (lane & (KT - 1));
-        return key_row<KIND>(p, s, at < k_end ? at : k_end - 1);
-    };
-    auto keep_place = [&](int row, int t) {
-        if (lane < KT)
-            rows_of[t & 3][lane] = row < 0 ? 0 : row;
-        const uint64_t none = __ballot(row < 0);
-        if (lane == 0) {
-            absent[t & 3] = none;
-            raise_flag(p, none != 0);
-        }
-    };
-    const uint32_t ld_k = (uint32_t)p.ldk, ld_v = (uint32_t)p.ldv;
-    const int vkey = 16 * (vblk >> 1) + 4 * (vblk & 1); // the first of the eight keys, the others 1, 2, 3, 8, 9, 10, 11 behind it
-    auto fetch = [&](int t) {
-        if (EXACT && !kPaged && k_first + (t + 1) * KT <= k_end) { // a whole tile: one base, offsets that stay
-            const int64_t row = s.span.first + k_first + t * KT;
-            const T *kr = kbase + row * p.ldk, *vr = vbase + row * p.ldv;
-            const uint32_t ko = krow * ld_k + 4 * kl, vo = vkey * ld_v + vd;
+    auto look_up = [&](int first) { // places of positions first .. first + kAhead - 1 of the range
 #pragma unroll
-            for (int g = 0; g < 2; ++g) {
-                load_depths<T, 4, EXACT>(kr + (ko + 8 * N * g), 0, 0, 1, kst[g]);
-                load_depths<T, 4, EXACT>(kr + (ko + 8 * N * g + 4 * N), 0, 0, 1, kst[g] + 4);
+        for (int i = 0; i < kAhead; i += 256) {
+            const int at = k_first + first + i + tid;
+            const int row = key_row<KIND>(p, s, at < k_end ? at : k_end - 1);
+            rows_of[(first + i + tid) & (2 * kAhead - 1)] = row;
+            if (row < 0) {
+                some_absent = 1;
+                raise_flag(p, true);
             }
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                load_depths<T, 2, EXACT>(vr + (vo + (8 * (j >> 2) + (j & 3)) * ld_v), 0, 0, 1, vst[j]);
-            return;
         }
-        const T* kr = kbase + place(t, krow) * p.ldk;
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-            load_depths<T, 4, EXACT>(kr, 8 * N * g + 4 * kl, p.dk, p.wide, kst[g]);
-            load_depths<T, 4, EXACT>(kr, 8 * N * g + 4 * N + 4 * kl, p.dk, p.wide, kst[g] + 4);
-        }
-        if (EXACT && kPaged && p.page_size % 16 == 0) { // the eight keys lie in one page
-            const T* vr = vbase + place(t, vkey) * p.ldv + vd;
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                load_depths<T, 2, EXACT>(vr + (8 * (j >> 2) + (j & 3)) * ld_v, 0, 0, 1, vst[j]);
-            return;
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            load_depths<T, 2, EXACT>(vbase + place(t, vkey + 8 * (j >> 2) + (j & 3)) * p.ldv, vd, p.dv, p.wide, vst[j]);
     };
-    auto measure = [&](int t) { // the largest finite key and value of the fetched tile
+    auto fetch = [&](int t) {
+        const int64_t row = place(t, krow);
+        const T *kr = kbase + row * p.ldk, *vr = vbase + row * p.ldv;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            load_depths<T, 4, EXACT>(kr, 4 * N * i + 4 * kl, p.dk, p.wide, kst[i >> 1] + 4 * (i & 1));
+            load_depths<T, 4, EXACT>(vr, 4 * N * i + 4 * kl, p.dv, p.wide, vst[i >> 1] + 4 * (i & 1));
+        }
+    };
+    // A turn is shorter than a trip to memory under load: the tile behind the next fetch is brought to the cache, an element of each
+    // thread's part of a row (its chunks lie within 64 N bytes), looked at a turn later.
+    float asked[2] = { 0.f, 0.f };
+    auto ask = [&](int t) {
+        asm volatile("" ::"v"(asked[0]), "v"(asked[1]));
+        const int64_t row = place(t, krow);
+        const int d = 16 * kl; // 16 elements apart
+        asked[0] = (float)kbase[row * p.ldk + (EXACT || d < p.dk ? d : 0)];
+        asked[1] = (float)vbase[row * p.ldv + (EXACT || d < p.dv ? d : 0)];
+    };
+    auto measure = [&](int t) { // sizes of the fetched rows, infinities and NaN aside
         float km = 0.f, vm = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            km = max3_abs(km, kst[0][e], kst[1][e]);
-            vm = max3_abs(vm, vst[e][0], vst[e][1]);
+            km = max3(km, fabsf(kst[0][e]), fabsf(kst[1][e]));
+            vm = max3(vm, fabsf(vst[0][e]), fabsf(vst[1][e]));
         }
-        km = wave_all<true>(km);
-        vm = wave_all<true>(vm);
-        if (__builtin_expect(km == INFINITY || vm == INFINITY, 0)) { // rows that do not see the infinity keep their sums
+        if (__builtin_expect(__any(!(km < INFINITY && vm < INFINITY)), 0)) { // rows that do not see the infinity keep their sums
             km = vm = 0.f;
 #pragma unroll
             for (int e = 0; e < 8; ++e)
 #pragma unroll
                 for (int g = 0; g < 2; ++g) {
                     km = fmaxf(km, fabsf(kst[g][e]) < INFINITY ? fabsf(kst[g][e]) : 0.f);
-                    vm = fmaxf(vm, fabsf(vst[e][g]) < INFINITY ? fabsf(vst[e][g]) : 0.f);
+                    vm = fmaxf(vm, fabsf(vst[g][e]) < INFINITY ? fabsf(vst[g][e]) : 0.f);
                 }
-            km = wave_all<true>(km);
-            vm = wave_all<true>(vm);
         }
-        if (lane == 0) {
-            largest[t & 1][0][wave] = km;
-            largest[t & 1][1][wave] = vm;
+        km = fmaxf(km, dpp_move<0xB1>(km));
+        km = fmaxf(km, dpp_move<0x4E>(km));
+        vm = fmaxf(vm, dpp_move<0xB1>(vm));
+        vm = fmaxf(vm, dpp_move<0x4E>(vm));
+        if (N == 8) {
+            km = fmaxf(km, dpp_move<0x141>(km));
+            vm = fmaxf(vm, dpp_move<0x141>(vm));
         }
+        Spread r = row_spread(km, vm);
+        r.top = most_of_wave<N>(r.top);
+        r.low = most_of_wave<N>(r.low);
+        if (lane == 0)
+            spread[t & 1][wave] = r;
     };
-    auto four = [](const float* v) { return fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])); };
     auto mfma = [](f16x8 a, f16x8 b, const f32x16& acc) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, acc, 0, 0, 0); };
     constexpr f32x16 kZero = { 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f };
 
@@ -241,13 +249,16 @@ __global__ __launch_bounds__(256, 2) void ragged_tile_kernel(RaggedParams p)
 #pragma unroll
     for (int d = 0; d < DB; ++d)
         oacc[d] = kZero;
-    float m_run = -INFINITY, l_run = 0.f, v_top = 0.f;
-    Pow2 sk = pow2_for(0.f), sv = sk, sk_next = sk, sv_next = sk; // of the tile at work (sv: of the sums) and of the one behind it
-    int next_row = 0;
+    float m_run = -INFINITY, l_run = 0.f;
+    // of the tile at work (sv: of the sums) and of the one behind it
+    Pow2 sk = pow2_for<1>(0), sv = pow2_for<4>(0), sk_next = sk, sv_next = sv;
+    bool fits = true, fits_next = true;
     auto scale_next = [&](int t) {
-        sk_next = pow2_for(four(largest[t & 1][0]));
-        v_top = fmaxf(v_top, four(largest[t & 1][1]));
-        sv_next = pow2_for(v_top);
+        const Spread* r = spread[t & 1];
+        const u16x2 top = most(most(r[0].top, r[1].top), most(r[2].top, r[3].top)), low = most(most(r[0].low, r[1].low), most(r[2].low, r[3].low));
+        fits_next = spread_fits(top, low);
+        sk_next = pow2_for<1>(top[0]);
+        sv_next = pow2_for<4>(top[1]);
     };
     auto stage = [&](unsigned char* ks, unsigned char* vs) {
 #pragma unroll
@@ -258,21 +269,33 @@ __global__ __launch_bounds__(256, 2) void ragged_tile_kernel(RaggedParams p)
             *reinterpret_cast<f16x8*>(&ks[(KB + N * g + kl) * KBLK + krow * 16]) = l;
         }
 #pragma unroll
-        for (int d = 0; d < 2; ++d) {
-            const float x[8] = { vst[0][d], vst[1][d], vst[2][d], vst[3][d], vst[4][d], vst[5][d], vst[6][d], vst[7][d] };
+        for (int g = 0; g < 2; ++g) {
             f16x8 h, l;
-            split2x8(x, sv_next.up, h, l);
-            *reinterpret_cast<f16x8*>(&vs[vblk * VBLK + (vd + d) * 16]) = h;
-            *reinterpret_cast<f16x8*>(&vs[(VB + vblk) * VBLK + (vd + d) * 16]) = l;
+            split2x8(vst[g], sv_next.up, h, l);
+            *reinterpret_cast<f16x8*>(&vs[krow * VROW + (N * g + kl) * 16]) = h;
+            *reinterpret_cast<f16x8*>(&vs[(KT + krow) * VROW + (N * g + kl) * 16]) = l;
         }
+    };
+    // values of four keys for this lane's depth: sixteen lanes address four rows of sixteen depths
+    const int v_at = (4 * half + ((c & 15) >> 2)) * VROW + (16 * (c >> 4) + 4 * (c & 3)) * 2;
+    auto values = [&](const unsigned char* vs, int key, int d) {
+        typedef short s16x4 __attribute__((ext_vector_type(4)));
+        struct {
+            s16x4 a, b;
+        } r;
+        r.a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(vs + v_at + key * VROW + d * 64));
+        r.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(vs + v_at + (key + 8) * VROW + d * 64));
+        return __builtin_bit_cast(f16x8, r);
     };
     auto turn = [&](int t, const unsigned char* ks, const unsigned char* vs, unsigned char* ks_next, unsigned char* vs_next) {
         const int j0 = k_first + t * KT;
         const bool work = j0 < wave_any; // some row of this wave sees some key of the tile
-        const float f = sv_next.up * sv.down;
+        float f = sv_next.up * sv.down;
+        f = t == 0 || (f > 1e-18f && f < 1e18f) ? f : NAN; // sums that would leave fp32's range
         sk = sk_next;
         if (work)
             sv = sv_next; // a wave that is through keeps its sums as they are
+        fits = fits_next;
         if (t + 1 < tiles)
             scale_next(t + 1);
         // S^T: KT keys x 32 rows, for a wave that sees none of them too; beside it tile t + 1 goes to LDS (the last time what the
@@ -291,13 +314,16 @@ __global__ __launch_bounds__(256, 2) void ragged_tile_kernel(RaggedParams p)
             }
         }
         stage(ks_next, vs_next);
-        if constexpr (kPaged)
-            if (wave == 0 && t + 3 < tiles)
-                keep_place(next_row, t + 3);
+        int absent = 0;
+        if constexpr (kPaged) {
+            absent = some_absent;
+            if ((t * KT & (kAhead - 1)) == 0 && t > 0 && (t + kAhead / KT) < tiles)
+                look_up(t * KT + kAhead); // into the half that is done with
+        }
         if (t + 2 < tiles) {
             fetch(t + 2);
-            if (kPaged && wave == 0 && t + 4 < tiles)
-                next_row = look_up(t + 4);
+            if (kPaged && t + 3 < tiles)
+                ask(t + 3);
         }
         if (work) {
             const int limit = (visible < k_end ? visible : k_end) - j0; // keys of the tile that this lane's row sees
@@ -309,16 +335,13 @@ __global__ __launch_bounds__(256, 2) void ragged_tile_kernel(RaggedParams p)
                         if (kb * 32 + 8 * (e >> 2) + 4 * half + (e & 3) >= limit)
                             sacc[kb][e] = -INFINITY;
             }
-            if constexpr (kPaged) {
-                const uint64_t none = absent[t & 3];
-                if (none != 0) {
+            if (kPaged && __builtin_amdgcn_readfirstlane(absent)) {
 #pragma unroll
-                    for (int kb = 0; kb < HALVES; ++kb)
+                for (int kb = 0; kb < HALVES; ++kb)
 #pragma unroll
-                        for (int e = 0; e < 16; ++e)
-                            if (none >> (kb * 32 + 8 * (e >> 2) + 4 * half + (e & 3)) & 1)
-                                sacc[kb][e] = -INFINITY;
-                }
+                    for (int e = 0; e < 16; ++e)
+                        if (rows_of[(t * KT + kb * 32 + 8 * (e >> 2) + 4 * half + (e & 3)) & (2 * kAhead - 1)] < 0)
+                            sacc[kb][e] = -INFINITY;
             }
             float mx = -INFINITY;
 #pragma unroll
@@ -326,9 +349,10 @@ __global__ __launch_bounds__(256, 2) void ragged_tile_kernel(RaggedParams p)
 #pragma unroll
                 for (int e = 0; e < 16; e += 2)
                     mx = max3(mx, sacc[kb][e], sacc[kb][e + 1]);
-            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            mx = max_halves(mx);
             const float to_log2 = fmaxf(q_down * sk.down, 1.17549435e-38f); // above zero: -infinity stays what it is
             mx *= to_log2;
+            l_run = fits ? l_run : NAN;
             if (__any(mx > m_run + 4.f) || f != 1.f) {
                 const float m_new = mx > m_run + 4.f ? mx : m_run;
                 const float corr = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
@@ -361,8 +385,7 @@ __global__ __launch_bounds__(256, 2) void ragged_tile_kernel(RaggedParams p)
                 split2x8(x, ph, pl);
 #pragma unroll
                 for (int d = 0; d < DB; ++d) {
-                    const f16x8 vh = *reinterpret_cast<const f16x8*>(&vs[(2 * u + half) * VBLK + (d * 32 + c) * 16]);
-                    const f16x8 vl = *reinterpret_cast<const f16x8*>(&vs[(VB + 2 * u + half) * VBLK + (d * 32 + c) * 16]);
+                    const f16x8 vh = values(vs, 16 * u, d), vl = values(vs, KT + 16 * u, d);
                     oacc[d] = mfma(vl, ph, oacc[d]);
                     oacc[d] = mfma(vh, pl, oacc[d]);
                     oacc[d] = mfma(vh, ph, oacc[d]);
@@ -376,13 +399,12 @@ __global__ __launch_bounds__(256, 2) void ragged_tile_kernel(RaggedParams p)
 
     if (tiles > 0) {
         if constexpr (kPaged) {
-            if (wave == 0) {
-                const int row0 = look_up(0), row1 = look_up(1), row2 = look_up(2);
-                next_row = look_up(3);
-                keep_place(row0, 0);
-                keep_place(row1, 1);
-                keep_place(row2, 2);
-            }
+            if (tid == 0)
+                some_absent = 0;
+            __syncthreads();
+            look_up(0);
+            if (tiles > kAhead / KT)
+                look_up(kAhead);
             __syncthreads();
         }
         fetch(0);
@@ -403,6 +425,12 @@ __global__ __launch_bounds__(256, 2) void ragged_tile_kernel(RaggedParams p)
             turn(t + 1, ks1, vs1, ks0, vs0);
     }
 
+    int again = r_first + wave * 32 + c; // found out once more, so that no registers hold it during the loop
+    asm volatile("" : "+v"(again));
+    const bool q_ok = again < count;
+    const QueryRow at_row = row_of(p, s, kv_head, count, again);
+    const int64_t q_row = at_row.row;
+    const int head = at_row.head;
     l_run += __shfl_xor(l_run, 32, 64);
     float size = l_run;
 #pragma unroll
@@ -413,21 +441,24 @@ __global__ __launch_bounds__(256, 2) void ragged_tile_kernel(RaggedParams p)
     // a row's two lanes hold half of its depths each
     const uint64_t odd_lanes = __ballot(q_ok && !(size < INFINITY));
     uint32_t odd = (uint32_t)odd_lanes | (uint32_t)(odd_lanes >> 32);
-    const bool in_parts = visible > p.split_keys;
-    const int64_t id = q_row * p.heads + head;
+    const bool in_parts = visible > s.range;
     if (q_ok && !(odd >> c & 1) && (in_parts ? k_first < visible : blockIdx.y == 0)) {
         const float f = l_run > 0.f ? sv.down / l_run : 0.f; // no key: zeros
-        float* to = in_parts ? part_out(p, blockIdx.y, id) : p.out + q_row * p.ldo + (int64_t)head * p.dv;
-        if (in_parts && half == 0) {
-            float* at = part_size(p, blockIdx.y, id);
-            at[0] = m_run - kShift;
-            at[1] = l_run;
+        float* to = p.out + q_row * p.ldo + (int64_t)head * p.dv;
+        if (in_parts) {
+            const int64_t id = part_row(p, s, at_row.token, head);
+            to = p.tile.out(blockIdx.y, id, p.dv);
+            float* at = p.tile.size(blockIdx.y, id, p.dv);
+            if (half == 0) {
+                at[0] = m_run - kShift;
+                at[1] = l_run;
+            }
         }
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const int depth = 32 * d + 8 * g + 4 * half;
+                const int blk = 4 * d + g, depth = 8 * N * (blk / N) + 4 * N * half + 4 * (blk % N); // what columns 8 blk + 4 half hold
                 const f32x4 o = { oacc[d][4 * g] * f, oacc[d][4 * g + 1] * f, oacc[d][4 * g + 2] * f, oacc[d][4 * g + 3] * f };
                 if (EXACT || (p.wide && depth < p.dv)) {
                     *reinterpret_cast<f32x4*>(to + depth) = o;
@@ -445,14 +476,322 @@ __global__ __launch_bounds__(256, 2) void ragged_tile_kernel(RaggedParams p)
     while (odd) {
         const int r1 = r_first + wave * 32 + __builtin_ctz(odd);
         odd &= odd - 1;
-        const int t1 = r1 / p.group, h1 = kv_head * p.group + r1 - t1 * p.group;
+        const int t1 = quotient(r1, p.by_group), h1 = kv_head * p.group + r1 - t1 * p.group;
         store_plain_row<KIND>(p, s, t1, h1, kv_head, blockIdx.y, lane);
+    }
+}
+
+// ---- packed prompts: keys and values split once, in tiles as the products read them ----
+//
+// In ragged_tile_kernel the vector units are busier than the matrix units: of some 430 issue slots a wave spends on a tile of 64 keys and 32 rows
+// at depth 64, 150 go into splitting keys and values, which every workgroup does again for its 128 rows.  Where sequences are long enough to
+// fill tiles, ragged_ready_kernel splits them once, into the order that LDS holds: [tile][key head][keys, then values][plane][block][key or
+// depth][16 bytes], 16 KB each (as many bytes as fp32), with the powers of two beside them.  ragged_packed_kernel's loads then go from memory to
+// LDS past the registers, and the registers hold two tiles' scores: the first product of tile t + 1 runs beside the softmax of tile t.
+__device__ __forceinline__ int64_t ready_tile(const RaggedParams& p, int seq, int first, int keys_a_tile) { return first_tile(first, seq, 1, keys_a_tile); }
+
+template <int D, bool EXACT>
+__global__ __launch_bounds__(256) void ragged_ready_kernel(RaggedParams p)
+{
+    constexpr int KT = 4096 / D, N = D / 16, KB = D / 8, VB = KT / 8;
+    __shared__ __attribute__((aligned(16))) unsigned char out[32768];
+    __shared__ Spread spread[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int kv_head = blockIdx.x % p.kv_heads;
+    const int64_t number = blockIdx.x / p.kv_heads;
+    const Tile tile = find_tile_wave(p.starts, p.n_seqs, p.tokens, 1, KT, number);
+    if (tile.seq < 0)
+        return;
+    const int krow = tid / N, kl = tid % N, vblk = tid / (D / 2), vd = tid % (D / 2) * 2;
+    const int left = tile.span.count - tile.index * KT; // keys behind the sequence's last are zeros
+    const int64_t row = tile.span.first + tile.index * KT;
+    const float* kr = static_cast<const float*>(p.k) + (row + (krow < left ? krow : 0)) * p.ldk + (int64_t)kv_head * p.dk;
+    const float* vr = static_cast<const float*>(p.v) + row * p.ldv + (int64_t)kv_head * p.dv;
+    float k[2][8], v[2][8];
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+        load_depths<float, 4, EXACT>(kr, 8 * N * g + 4 * kl, p.dk, p.wide, k[g]);
+        load_depths<float, 4, EXACT>(kr, 8 * N * g + 4 * N + 4 * kl, p.dk, p.wide, k[g] + 4);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int key = 16 * (vblk >> 1) + 4 * (vblk & 1) + 8 * (j >> 2) + (j & 3);
+        float x[2];
+        load_depths<float, 2, EXACT>(vr + (key < left ? key : 0) * p.ldv, vd, p.dv, p.wide, x);
+        v[0][j] = key < left ? x[0] : 0.f;
+        v[1][j] = key < left ? x[1] : 0.f;
+    }
+    // sizes of the rows, infinities and NaN aside: queries that do not see those keep their sums
+    float km = 0.f, vm[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            k[g][e] = krow < left ? k[g][e] : 0.f;
+            km = fmaxf(km, fabsf(k[g][e]) < INFINITY ? fabsf(k[g][e]) : 0.f);
+        }
+        const float a = fabsf(v[0][e]), b = fabsf(v[1][e]);
+        vm[e] = fmaxf(a < INFINITY ? a : 0.f, b < INFINITY ? b : 0.f);
+    }
+    km = N == 4 ? fmaxf(km, dpp_move<0xB1>(km)) : half_row_all<true>(km);
+    km = N == 4 ? fmaxf(km, dpp_move<0x4E>(km)) : km;
+    Spread r { u16x2 { 0, 0 }, u16x2 { 0, 0 } };
+#pragma unroll
+    for (int e = 0; e < 8; ++e) { // D / 2 lanes have a row of values
+        vm[e] = fmaxf(half_row_all<true>(vm[e]), dpp_move<0x140>(half_row_all<true>(vm[e])));
+        vm[e] = fmaxf(vm[e], __shfl_xor(vm[e], 16, 64));
+        if (D == 128)
+            vm[e] = fmaxf(vm[e], __shfl_xor(vm[e], 32, 64));
+        const Spread one = row_spread(km, vm[e]);
+        r.top = most(r.top, one.top);
+        r.low = most(r.low, one.low);
+    }
+    r.top = most_of_wave<N>(r.top);
+    r.low = most_of_wave<N>(r.low);
+    if (lane == 0)
+        spread[wave] = r;
+    __syncthreads();
+    const u16x2 top = most(most(spread[0].top, spread[1].top), most(spread[2].top, spread[3].top));
+    const u16x2 low = most(most(spread[0].low, spread[1].low), most(spread[2].low, spread[3].low));
+    const Pow2 sk = pow2_for<1>(top[0]), sv = pow2_for<4>(top[1]);
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+        f16x8 h, l;
+        split2x8(k[g], sk.up, h, l);
+        *reinterpret_cast<f16x8*>(&out[((N * g + kl) * KT + krow) * 16]) = h;
+        *reinterpret_cast<f16x8*>(&out[((KB + N * g + kl) * KT + krow) * 16]) = l;
+        split2x8(v[g], sv.up, h, l);
+        *reinterpret_cast<f16x8*>(&out[16384 + (vblk * D + vd + g) * 16]) = h;
+        *reinterpret_cast<f16x8*>(&out[16384 + ((VB + vblk) * D + vd + g) * 16]) = l;
+    }
+    if (tid == 0)
+        p.powers[blockIdx.x] = { spread_fits(top, low) ? sk.down : NAN, sv.down };
+    __syncthreads();
+    unsigned char* to = p.ready + (int64_t)blockIdx.x * 32768;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        *reinterpret_cast<f32x4*>(to + (i * 256 + tid) * 16) = *reinterpret_cast<const f32x4*>(&out[(i * 256 + tid) * 16]);
+}
+
+// 16 KB from memory to LDS, a kilobyte a wave and instruction
+__device__ __forceinline__ void load_to_lds(const unsigned char* from, unsigned char* to, int wave, int lane)
+{
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + (wave * 4 + i) * 1024 + lane * 16),
+            (__attribute__((address_space(3))) void*)(to + (wave * 4 + i) * 1024), 16, 0, 0);
+}
+
+template <int D>
+__global__ __launch_bounds__(256, 2) void ragged_packed_kernel(RaggedParams p)
+{
+    constexpr int KT = 4096 / D, HALVES = KT / 32, N = D / 16;
+    constexpr int KB = D / 8, VB = KT / 8, STEPS = D / 16, DB = D / 32;
+    __shared__ __attribute__((aligned(1024))) unsigned char ks0[16384], ks1[16384], vs0[16384], vs1[16384];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c = lane & 31, half = lane >> 5;
+    if (p.error_flag && blockIdx.x == 0)
+        for (int i = tid; i < p.n_seqs; i += 256)
+            raise_flag(p, !packed_start_ok(p.starts, i, p.tokens));
+    const int kv_head = blockIdx.x % p.kv_heads; // the order of ragged_tile_kernel
+    const int64_t number = blockIdx.x / p.kv_heads;
+    const Tile tile = p.causal && p.n_seqs <= 64 ? late_tile_wave(p.starts, p.n_seqs, p.tokens, p.group, 128, number)
+                                                 : find_tile_wave(p.starts, p.n_seqs, p.tokens, p.group, 128, gridDim.x / p.kv_heads - 1 - number);
+    if (tile.seq < 0)
+        return;
+    const Sequence s = sequence_of<kPackedF32>(p, tile.seq, tile.span);
+    const int count = s.span.count * p.group, r_first = tile.index * 128;
+    const int r = r_first + wave * 32 + c;
+    const bool q_ok = r < count;
+    const int token = quotient(q_ok ? r : count - 1, p.by_group), head = kv_head * p.group + (q_ok ? r : count - 1) - token * p.group;
+    const int64_t q_row = s.span.first + token;
+    const int visible = visible_keys(p, s, token);
+    const int r_last = r_first + 128 < count ? r_first + 127 : count - 1;
+    const int tiles = (visible_keys(p, s, quotient(r_last, p.by_group)) + KT - 1) / KT; // at least one
+    const int w_first = r_first + wave * 32, w_last = w_first + 31 < count ? w_first + 31 : count - 1;
+    const int wave_all_see = visible_keys(p, s, quotient(w_first < count ? w_first : count - 1, p.by_group));
+    const int wave_any = visible_keys(p, s, quotient(w_last, p.by_group));
+
+    const int64_t tile0 = ready_tile(p, tile.seq, s.span.first, KT) * p.kv_heads + kv_head;
+    const unsigned char* ready = p.ready + tile0 * 32768;
+    const f32x2_pow* powers = p.powers + tile0;
+    const int64_t tile_bytes = (int64_t)p.kv_heads * 32768;
+    load_to_lds(ready, ks0, wave, lane);
+    load_to_lds(ready + 16384, vs0, wave, lane);
+    if (tiles > 1)
+        load_to_lds(ready + tile_bytes, ks1, wave, lane);
+
+    f16x8 qh[STEPS], ql[STEPS]; // depth block 2 u + half
+    float q_down;
+    {
+        float x[STEPS][8], top = 0.f;
+        const float* from = p.q + q_row * p.ldq + (int64_t)head * p.dk;
+#pragma unroll
+        for (int u = 0; u < STEPS; ++u) {
+            const int blk = 2 * u + half, d0 = 8 * N * (blk / N) + 4 * (blk % N);
+            load_depths<float, 4, false>(from, d0, p.dk, p.wide, x[u]);
+            load_depths<float, 4, false>(from, d0 + 4 * N, p.dk, p.wide, x[u] + 4);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                top = fmaxf(top, fabsf(x[u][e]));
+        }
+        const Pow2 sq = pow2_for<1>(exponent(max_halves(top)));
+        q_down = sq.down * (p.scale * kLog2e);
+#pragma unroll
+        for (int u = 0; u < STEPS; ++u)
+            split2x8(x[u], sq.up, qh[u], ql[u]);
+    }
+
+    auto mfma = [](f16x8 a, f16x8 b, const f32x16& acc) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, acc, 0, 0, 0); };
+    constexpr f32x16 kZero = { 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f };
+    f32x16 oacc[DB], sa[HALVES], sb[HALVES];
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+        oacc[d] = kZero;
+    float m_run = -INFINITY, l_run = 0.f;
+    float v_down = 0.f; // what takes the sums' power back: that of the last tile's values
+
+    auto scores = [&](f32x16 (&sc)[HALVES], const unsigned char* ks) {
+#pragma unroll
+        for (int kb = 0; kb < HALVES; ++kb) {
+            sc[kb] = kZero;
+#pragma unroll
+            for (int u = 0; u < STEPS; ++u) {
+                const f16x8 kh = *reinterpret_cast<const f16x8*>(&ks[((2 * u + half) * KT + kb * 32 + c) * 16]);
+                const f16x8 kw = *reinterpret_cast<const f16x8*>(&ks[((KB + 2 * u + half) * KT + kb * 32 + c) * 16]);
+                sc[kb] = mfma(kw, qh[u], sc[kb]);
+                sc[kb] = mfma(kh, ql[u], sc[kb]);
+                sc[kb] = mfma(kh, qh[u], sc[kb]);
+            }
+        }
+    };
+    // tile t: its scores are in sc; ks holds the keys of tile t + 1 and vs the values of tile t; the keys of tile t + 2 go to ks_to, the values of
+    // tile t + 1 to vs_to
+    auto turn = [&](int t, f32x16 (&sc)[HALVES], f32x16 (&next)[HALVES], const unsigned char* ks, const unsigned char* vs, unsigned char* ks_to,
+                    unsigned char* vs_to) {
+        const int j0 = t * KT;
+        if (t + 1 < tiles)
+            load_to_lds(ready + (t + 1) * tile_bytes + 16384, vs_to, wave, lane);
+        if (t + 2 < tiles)
+            load_to_lds(ready + (t + 2) * tile_bytes, ks_to, wave, lane);
+        const f32x2_pow down = powers[(int64_t)t * p.kv_heads];
+        if (j0 < wave_any) { // some row of this wave sees some key of the tile
+            const int limit = visible - j0; // keys of the tile that this lane's row sees
+            if (j0 + KT > wave_all_see) {
+#pragma unroll
+                for (int kb = 0; kb < HALVES; ++kb)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (kb * 32 + 8 * (e >> 2) + 4 * half + (e & 3) >= limit)
+                            sc[kb][e] = -INFINITY;
+            }
+            float mx = -INFINITY;
+#pragma unroll
+            for (int kb = 0; kb < HALVES; ++kb)
+#pragma unroll
+                for (int e = 0; e < 16; e += 2)
+                    mx = max3(mx, sc[kb][e], sc[kb][e + 1]);
+            const float to_log2 = fmaxf(q_down * down.k_down, 1.17549435e-38f); // above zero: -infinity stays what it is
+            mx = max_halves(mx) * to_log2;
+            l_run = down.k_down == down.k_down ? l_run : NAN; // a tile that is left to plain sums
+            if (__any(mx > m_run + 4.f) || down.v_down != v_down) {
+                const float m_new = mx > m_run + 4.f ? mx : m_run;
+                const float corr = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
+                const float f = v_down / down.v_down;
+                m_run = m_new;
+                v_down = down.v_down;
+                l_run *= corr;
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        oacc[d][e] *= t == 0 || (f > 1e-18f && f < 1e18f) ? corr * f : NAN; // NAN: sums that would leave fp32's range
+            }
+            const float base = kShift - (m_run == -INFINITY ? 0.f : m_run);
+            float rs = 0.f;
+#pragma unroll
+            for (int kb = 0; kb < HALVES; ++kb)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    sc[kb][e] = __builtin_amdgcn_exp2f(fmaf(sc[kb][e], to_log2, base));
+                    rs += sc[kb][e];
+                }
+            l_run += rs;
+            scores(next, ks);
+#pragma unroll
+            for (int u = 0; u < KT / 16; ++u) { // keys of block 2 u + half: registers 8 (u % 2) .. + 7 of accumulator u / 2
+                float x[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    x[j] = sc[u >> 1][8 * (u & 1) + j];
+                f16x8 ph, pl;
+                split2x8(x, ph, pl);
+#pragma unroll
+                for (int d = 0; d < DB; ++d) {
+                    const f16x8 vh = *reinterpret_cast<const f16x8*>(&vs[((2 * u + half) * D + d * 32 + c) * 16]);
+                    const f16x8 vl = *reinterpret_cast<const f16x8*>(&vs[((VB + 2 * u + half) * D + d * 32 + c) * 16]);
+                    oacc[d] = mfma(vl, ph, oacc[d]);
+                    oacc[d] = mfma(vh, pl, oacc[d]);
+                    oacc[d] = mfma(vh, ph, oacc[d]);
+                }
+            }
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+    };
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // this wave's part of the tiles is in LDS
+    __syncthreads();
+    scores(sa, ks0);
+    __syncthreads(); // ks0 is done with
+    for (int t = 0; t < tiles; t += 2) {
+        turn(t, sa, sb, ks1, vs0, ks0, vs1);
+        if (t + 1 < tiles)
+            turn(t + 1, sb, sa, ks0, vs1, ks1, vs0);
+    }
+
+    l_run += __shfl_xor(l_run, 32, 64);
+    float size = l_run;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            size += fabsf(oacc[d][e]);
+    // a row's two lanes hold half of its depths each
+    const uint64_t odd_lanes = __ballot(q_ok && !(size < INFINITY));
+    uint32_t odd = (uint32_t)odd_lanes | (uint32_t)(odd_lanes >> 32);
+    if (q_ok && !(odd >> c & 1)) {
+        const float f = v_down / l_run;
+        float* to = p.out + q_row * p.ldo + (int64_t)head * p.dv;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int depth = 32 * d + 8 * g + 4 * half;
+                const f32x4 o = { oacc[d][4 * g] * f, oacc[d][4 * g + 1] * f, oacc[d][4 * g + 2] * f, oacc[d][4 * g + 3] * f };
+                if (p.wide && depth < p.dv) {
+                    *reinterpret_cast<f32x4*>(to + depth) = o;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (depth + e < p.dv)
+                            to[depth + e] = o[e];
+                }
+            }
+    }
+    if (__builtin_expect(odd == 0, 1))
+        return;
+#pragma clang loop unroll(disable)
+    while (odd) {
+        const int r1 = r_first + wave * 32 + __builtin_ctz(odd);
+        odd &= odd - 1;
+        const int t1 = quotient(r1, p.by_group), h1 = kv_head * p.group + r1 - t1 * p.group;
+        store_plain_row<kPackedF32>(p, s, t1, h1, kv_head, 0, lane);
     }
 }
 
 // ---- few query rows: keys and values pass once, straight from memory to the fp32 matrix instructions ----
 //
-// A workgroup takes all rows (up to 16 R) that a sequence brings to one key head, over one range of its keys; its four waves take every
+// A workgroup takes sixteen of the rows that a sequence brings to one key head, over one range of its keys; its four waves take every
 // fourth block of 16 keys, each with sums of its own, and meet at the end.  Bound by memory: a lane's loads are the operands of
 // the 16x16x4 fp32 products, nothing is staged, and a block's loads are on their way while the block before is worked on.
 //  * S^T = K Q^T: lane (c, g) of 16 x 4 loads chunks of key c, chunk i at depth 4 W i + W g (W elements are 16 bytes), and has scores of keys
@@ -480,8 +819,8 @@ __device__ __forceinline__ auto load_chunk(const T* row, int d, int depth)
     return v;
 }
 
-template <int D, int KIND, int R, bool WIDE>
-__global__ __launch_bounds__(256) void ragged_few_kernel(RaggedParams p)
+template <int D, int KIND, bool WIDE>
+__global__ __launch_bounds__(256, 2) void ragged_few_kernel(RaggedParams p)
 {
     typedef typename KvElement<KIND>::type T;
     constexpr int W = 16 / (int)sizeof(T), NK = D / (4 * W); // elements of a key chunk, chunks of a lane
@@ -494,7 +833,7 @@ __global__ __launch_bounds__(256) void ragged_few_kernel(RaggedParams p)
         int row;
     };
     __shared__ float meet_o[4][16][D + 4];
-    __shared__ float meet_m[4][16 * R], meet_l[4][16 * R];
+    __shared__ float meet_m[4][16], meet_l[4][16];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 15, g = lane >> 4;
     const int seq = blockIdx.x / p.kv_heads, kv_head = blockIdx.x % p.kv_heads;
@@ -505,14 +844,16 @@ __global__ __launch_bounds__(256) void ragged_few_kernel(RaggedParams p)
     if (tid == 0)
         raise_flag(p, s.cut);
     const int count = s.span.count * p.group;
-    if (count == 0 || count > p.few_rows)
+    const int r_first = blockIdx.z * 16;
+    if (r_first >= count || !s.few)
         return;
-    const int k_first = blockIdx.y * p.split_keys;
     int k_end = visible_keys(p, s, s.span.count - 1);
-    if (blockIdx.y > 0 && k_first >= k_end)
+    const int64_t k_from = (int64_t)blockIdx.y * s.range;
+    if (blockIdx.y > 0 && k_from >= k_end)
         return;
-    if (k_end - k_first > p.split_keys)
-        k_end = k_first + p.split_keys;
+    const int k_first = (int)k_from;
+    if (k_end - k_first > s.range)
+        k_end = k_first + s.range;
     const int blocks = k_end > k_first ? (k_end - k_first + 15) / 16 : 0;
 
     const T* kbase = static_cast<const T*>(p.k) + (int64_t)kv_head * p.dk;
@@ -544,16 +885,13 @@ __global__ __launch_bounds__(256) void ragged_few_kernel(RaggedParams p)
         fetch(a, row_a);
     }
 
-    float q[R][NK][W];
-    int visible[R];
-    float m_run[R], l_run[R];
-    f32x4 oacc[R][DL];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const bool ok = 16 * r + c < count;
-        const int at = ok ? 16 * r + c : 0, token = at / p.group;
-        visible[r] = ok ? visible_keys(p, s, token) : 0;
-        const float* from = p.q + (int64_t)(s.span.first + token) * p.ldq + (int64_t)(kv_head * p.group + at - token * p.group) * p.dk;
+    float q[NK][W];
+    const bool q_ok = r_first + c < count;
+    const int q_token = quotient(q_ok ? r_first + c : 0, p.by_group);
+    const int visible = q_ok ? visible_keys(p, s, q_token) : 0;
+    {
+        const float* from = p.q + (int64_t)(s.span.first + q_token) * p.ldq
+            + (int64_t)(kv_head * p.group + (q_ok ? r_first + c : 0) - q_token * p.group) * p.dk;
 #pragma unroll
         for (int i = 0; i < NK; ++i)
 #pragma unroll
@@ -561,77 +899,64 @@ __global__ __launch_bounds__(256) void ragged_few_kernel(RaggedParams p)
                 const f32x4 x = load_chunk<float, 4, WIDE>(from, 4 * W * i + W * g + h, p.dk);
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    q[r][i][h + e] = x[e] * (p.scale * kLog2e);
+                    q[i][h + e] = x[e] * (p.scale * kLog2e);
             }
-        m_run[r] = -INFINITY;
-        l_run[r] = 0.f;
-#pragma unroll
-        for (int e = 0; e < DL; ++e)
-            oacc[r][e] = f32x4 { 0.f, 0.f, 0.f, 0.f };
     }
+    float m_run = -INFINITY, l_run = 0.f;
+    f32x4 oacc[DL];
+#pragma unroll
+    for (int e = 0; e < DL; ++e)
+        oacc[e] = f32x4 { 0.f, 0.f, 0.f, 0.f };
     // keys that the first row sees are seen by all
-    const int first_sees = visible_keys(p, s, 0), all_see = first_sees < k_end ? first_sees : k_end;
+    const int first_sees = visible_keys(p, s, quotient(r_first, p.by_group)), all_see = first_sees < k_end ? first_sees : k_end;
     bool missing = false;
     auto work = [&](const Block& x, int blk) {
-        f32x4 sc[R];
+        f32x4 sc = { 0.f, 0.f, 0.f, 0.f };
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            sc[r] = f32x4 { 0.f, 0.f, 0.f, 0.f };
+        for (int i = 0; i < NK; ++i)
 #pragma unroll
-            for (int i = 0; i < NK; ++i)
-#pragma unroll
-                for (int e = 0; e < W; ++e)
-                    sc[r] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)x.k[i][e], q[r][i][e], sc[r], 0, 0, 0);
-        }
+            for (int e = 0; e < W; ++e)
+                sc = __builtin_amdgcn_mfma_f32_16x16x4f32((float)x.k[i][e], q[i][e], sc, 0, 0, 0);
         const int at = k_first + blk * 16;
         if (at + 16 > all_see) {
 #pragma unroll
-            for (int r = 0; r < R; ++r)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (at + 4 * g + i >= (visible[r] < k_end ? visible[r] : k_end))
-                        sc[r][i] = -INFINITY;
+            for (int i = 0; i < 4; ++i)
+                if (at + 4 * g + i >= (visible < k_end ? visible : k_end))
+                    sc[i] = -INFINITY;
         }
         if (__any(x.row < 0)) {
             missing = true;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const bool none = __shfl(x.row, 4 * g + i, 64) < 0;
-#pragma unroll
-                for (int r = 0; r < R; ++r)
-                    sc[r][i] = none ? -INFINITY : sc[r][i];
-            }
-        }
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            float mx = fmaxf(fmaxf(sc[r][0], sc[r][1]), fmaxf(sc[r][2], sc[r][3]));
-            mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-            if (__any(mx > m_run[r] + 8.f)) { // the maximum moves when a score passes it by 2^8
-                const float m_new = fmaxf(m_run[r], mx);
-                const float corr = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run[r] - m_new);
-                m_run[r] = m_new;
-                l_run[r] *= corr;
-#pragma unroll
-                for (int e = 0; e < DL; ++e)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        oacc[r][e][i] *= corr;
-            }
-            const float base = m_run[r] == -INFINITY ? 0.f : m_run[r];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                sc[r][i] = __builtin_amdgcn_exp2f(sc[r][i] - base);
-                l_run[r] += sc[r][i];
-            }
-#pragma unroll
             for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < NV; ++j)
-#pragma unroll
-                    for (int e = 0; e < VW; ++e)
-                        oacc[r][j * VW + e] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)x.v[i][j][e], sc[r][i], oacc[r][j * VW + e], 0, 0, 0);
+                sc[i] = __shfl(x.row, 4 * g + i, 64) < 0 ? -INFINITY : sc[i];
         }
+        float mx = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mx = max_halves(mx);
+        if (__any(mx > m_run + 8.f)) { // the maximum moves when a score passes it by 2^8
+            const float m_new = fmaxf(m_run, mx);
+            const float corr = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
+            m_run = m_new;
+            l_run *= corr;
+#pragma unroll
+            for (int e = 0; e < DL; ++e)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    oacc[e][i] *= corr;
+        }
+        const float base = m_run == -INFINITY ? 0.f : m_run;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            sc[i] = __builtin_amdgcn_exp2f(sc[i] - base);
+            l_run += sc[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+#pragma unroll
+                for (int e = 0; e < VW; ++e)
+                    oacc[j * VW + e] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)x.v[i][j][e], sc[i], oacc[j * VW + e], 0, 0, 0);
     };
     for (int blk = wave; blk < blocks; blk += 8) {
         const bool more = blk + 4 < blocks;
@@ -651,116 +976,120 @@ __global__ __launch_bounds__(256) void ragged_few_kernel(RaggedParams p)
     }
     raise_flag(p, missing);
 
-    // the waves' sums meet, 16 rows at a time: 16 threads a row, DL depths each
-    uint32_t odd = 0; // of this wave's rows those whose sums are not finite, or empty though there are keys
+    // the waves' sums meet: 16 threads a row, DL depths each
+    l_run += __shfl_xor(l_run, 16, 64);
+    l_run += __shfl_xor(l_run, 32, 64);
+    if (g == 0) {
+        meet_m[wave][c] = m_run;
+        meet_l[wave][c] = l_run;
+    }
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        l_run[r] += __shfl_xor(l_run[r], 16, 64);
-        l_run[r] += __shfl_xor(l_run[r], 32, 64);
-        if (r > 0)
-            __syncthreads();
-        if (g == 0) {
-            meet_m[wave][16 * r + c] = m_run[r];
-            meet_l[wave][16 * r + c] = l_run[r];
-        }
+    for (int j = 0; j < NV; ++j)
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int e = 0; e < VW; ++e)
+                meet_o[wave][c][16 * VW * j + VW * (4 * g + i) + e] = oacc[j * VW + e][i];
+    __syncthreads();
+    // found out anew, so that no registers keep these through the loop
+    const int lane2 = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0)), tid2 = wave * 64 + lane2;
+    const int at = tid2 >> 4, d0 = (tid2 & 15) * DL, mine_row = r_first + at;
+    const float top = fmaxf(fmaxf(meet_m[0][at], meet_m[1][at]), fmaxf(meet_m[2][at], meet_m[3][at]));
+    const float m = top == -INFINITY ? 0.f : top;
+    float l = 0.f, o[DL];
 #pragma unroll
-                for (int e = 0; e < VW; ++e)
-                    meet_o[wave][c][16 * VW * j + VW * (4 * g + i) + e] = oacc[r][j * VW + e][i];
-        __syncthreads();
-        const int at = 16 * r + (tid >> 4), d0 = (tid & 15) * DL;
-        const float top = fmaxf(fmaxf(meet_m[0][at], meet_m[1][at]), fmaxf(meet_m[2][at], meet_m[3][at]));
-        const float m = top == -INFINITY ? 0.f : top;
-        float l = 0.f, o[DL], size;
+    for (int e = 0; e < DL; ++e)
+        o[e] = 0.f;
 #pragma unroll
-        for (int e = 0; e < DL; ++e)
-            o[e] = 0.f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const float f = __builtin_amdgcn_exp2f(meet_m[w][at] - m);
-            l += f * meet_l[w][at];
-#pragma unroll
-            for (int e = 0; e < DL; ++e)
-                o[e] += f * meet_o[w][tid >> 4][d0 + e];
-        }
-        size = l;
+    for (int w = 0; w < 4; ++w) {
+        const float f = __builtin_amdgcn_exp2f(meet_m[w][at] - m);
+        l += f * meet_l[w][at];
 #pragma unroll
         for (int e = 0; e < DL; ++e)
-            size += fabsf(o[e]);
-        const int token = (at < count ? at : 0) / p.group, head = kv_head * p.group + (at < count ? at : 0) - token * p.group;
-        const int sees = visible_keys(p, s, token);
-        const bool in_parts = sees > p.split_keys, mine = at < count && (in_parts ? k_first < sees : blockIdx.y == 0);
-        const uint64_t bad = __ballot(mine && (!(size < INFINITY) || (l == 0.f && k_first < sees)));
-        if (mine && (bad >> (lane & 48) & 0xffff) == 0) {
-            const int64_t q_row = s.span.first + token, id = q_row * p.heads + head;
-            const float f = l > 0.f ? 1.f / l : 0.f; // no key: zeros
-            float* to = in_parts ? part_out(p, blockIdx.y, id) : p.out + q_row * p.ldo + (int64_t)head * p.dv;
-            if (in_parts && (tid & 15) == 0) {
-                float* size_at = part_size(p, blockIdx.y, id);
+            o[e] += f * meet_o[w][at][d0 + e];
+    }
+    float size = l;
+#pragma unroll
+    for (int e = 0; e < DL; ++e)
+        size += fabsf(o[e]);
+    const bool there = mine_row < count;
+    const int token = quotient(there ? mine_row : 0, p.by_group), head = kv_head * p.group + (there ? mine_row : 0) - token * p.group;
+    const int sees = visible_keys(p, s, token);
+    const bool in_parts = sees > s.range, mine = there && (in_parts ? k_first < sees : blockIdx.y == 0);
+    // rows whose sums are not finite, or empty though there are keys; a row's 16 threads agree
+    const uint64_t bad = __ballot(mine && (!(size < INFINITY) || (l == 0.f && k_first < sees)));
+    if (mine && (bad >> (lane2 & 48) & 0xffff) == 0) {
+        const float f = l > 0.f ? 1.f / l : 0.f; // no key: zeros
+        float* to = p.out + (int64_t)(s.span.first + token) * p.ldo + (int64_t)head * p.dv;
+        if (in_parts) {
+            const int64_t id = part_row(p, s, token, head);
+            to = p.few.out(blockIdx.y, id, p.dv);
+            float* size_at = p.few.size(blockIdx.y, id, p.dv);
+            if ((tid2 & 15) == 0) {
                 size_at[0] = top;
                 size_at[1] = l;
             }
-#pragma unroll
-            for (int e = 0; e < DL; e += 4) {
-                if (WIDE) {
-                    if (d0 + e < p.dv)
-                        *reinterpret_cast<f32x4*>(to + d0 + e) = f32x4 { o[e] * f, o[e + 1] * f, o[e + 2] * f, o[e + 3] * f };
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (d0 + e + i < p.dv)
-                            to[d0 + e + i] = o[e + i] * f;
-                }
-            }
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) // rows 4 wave .. 4 wave + 3 of the sixteen
-            if (bad >> (16 * k) & 0xffff)
-                odd |= 1u << (16 * r + 4 * wave + k);
+        for (int e = 0; e < DL; e += 4) {
+            if (WIDE) {
+                if (d0 + e < p.dv)
+                    *reinterpret_cast<f32x4*>(to + d0 + e) = f32x4 { o[e] * f, o[e + 1] * f, o[e + 2] * f, o[e + 3] * f };
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (d0 + e + i < p.dv)
+                        to[d0 + e + i] = o[e + i] * f;
+            }
+        }
     }
+    uint32_t odd = 0; // of this wave's four rows
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        if (bad >> (16 * k) & 0xffff)
+            odd |= 1u << (4 * wave + k);
     if (__builtin_expect(odd == 0, 1))
         return;
 #pragma clang loop unroll(disable)
     while (odd) {
-        const int r1 = __builtin_ctz(odd);
+        const int r1 = r_first + __builtin_ctz(odd);
         odd &= odd - 1;
-        const int token = r1 / p.group;
-        store_plain_row<KIND>(p, s, token, kv_head * p.group + r1 - token * p.group, kv_head, blockIdx.y, lane);
+        const int t1 = quotient(r1, p.by_group);
+        store_plain_row<KIND>(p, s, t1, kv_head * p.group + r1 - t1 * p.group, kv_head, blockIdx.y, lane2);
     }
 }
 
 // Rows that more than one range of keys was summed for: sum of 2^(m - M) l o over the ranges, divided by that of 2^(m - M) l.
 template <int KIND>
-__global__ __launch_bounds__(256) void ragged_join_kernel(RaggedParams p, int few_keys, int tile_keys)
+__global__ __launch_bounds__(256) void ragged_join_kernel(RaggedParams p)
 {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t id = (int64_t)blockIdx.x * 4 + wave;
-    const int row = (int)(id / p.heads), head = (int)(id % p.heads);
+    const int64_t item = (int64_t)blockIdx.x * 4 + wave;
+    const int row = (int)((uint64_t)item / (uint32_t)p.heads), head = (int)(item - (int64_t)row * p.heads);
     if (row >= p.tokens)
         return;
     const int index = find_row(p.starts, p.n_seqs, p.tokens, row);
     if (index < 0)
         return;
     const Sequence s = sequence_of<KIND>(p, index, packed_span(p.starts, index, p.tokens));
-    if (row - s.span.first >= s.span.count)
+    const int token = row - s.span.first;
+    if (token >= s.span.count)
         return;
-    const int visible = visible_keys(p, s, row - s.span.first);
-    const int keys = s.span.count * p.group <= p.few_rows ? few_keys : tile_keys;
-    if (visible <= keys)
+    const int visible = visible_keys(p, s, token);
+    if (visible <= s.range)
         return;
-    const int parts = (visible + keys - 1) / keys;
+    const int parts = (visible + s.range - 1) / s.range;
+    const PartSums& part = s.few ? p.few : p.tile;
+    const int64_t id = part_row(p, s, token, head);
     float top = -INFINITY;
     for (int i = 0; i < parts; ++i)
-        top = fmaxf(top, part_size(p, i, id)[0]);
+        top = fmaxf(top, part.size(i, id, p.dv)[0]);
     const float m = top == -INFINITY ? 0.f : top;
     float l = 0.f, o0 = 0.f, o1 = 0.f;
     for (int i = 0; i < parts; ++i) {
-        const float* at = part_size(p, i, id);
+        const float* at = part.size(i, id, p.dv);
         const float w = at[1] * __builtin_amdgcn_exp2f(at[0] - m);
-        const float* from = part_out(p, i, id);
+        const float* from = part.out(i, id, p.dv);
         l += w;
         if (lane < p.dv)
             o0 = fmaf(w, from[lane], o0);
@@ -774,25 +1103,23 @@ __global__ __launch_bounds__(256) void ragged_join_kernel(RaggedParams p, int fe
         to[64 + lane] = finish(o1, l, top != -INFINITY);
 }
 
-// How a call is cut: sequences of few rows (up to `few_rows`) go to ragged_few_kernel in ranges of few_keys keys, the others to
-// ragged_tile_kernel in ranges of tile_keys.
+// How a call is cut: sequences of few rows (up to `few_rows`) go to ragged_few_kernel in ranges of up to few_keys keys, the others to
+// ragged_tile_kernel in ranges of up to tile_keys.
 struct RaggedPlan {
     int few_rows, few_ranges, few_keys; // few_ranges 0: no such launch
     int tile_ranges, tile_keys;
+    int64_t few_part, tile_part; // rows whose sums may be kept
     int64_t tiles;
-    int ranges() const { return few_ranges > tile_ranges ? few_ranges : tile_ranges; }
-    size_t scratch(int tokens, int heads, int dv) const
-    {
-        return ranges() > 1 ? sizeof(float) * (size_t)ranges() * tokens * heads * (2 + (size_t)dv) : 0;
-    }
+    int64_t ready; // tiles of split keys and values, for all key heads; 0: none are laid out
+    size_t ready_bytes() const { return (size_t)ready * (32768 + sizeof(f32x2_pow)); }
+    size_t few_floats(int dv) const { return few_ranges > 1 ? ((size_t)few_ranges * few_part * (2 + (size_t)dv) + 3) & ~(size_t)3 : 0; }
+    size_t tile_floats(int dv) const { return tile_ranges > 1 ? (size_t)tile_ranges * tile_part * (2 + (size_t)dv) : 0; }
 };
 
-static int ranges_of(int64_t keys, int64_t want, int least, int* range_keys)
+static int ranges_of(int keys, int64_t most, int* range_keys)
 {
-    int64_t per = (keys + want - 1) / want;
-    per = (per < least ? least : per) + 63 & ~(int64_t)63;
-    *range_keys = per > INT_MAX - 64 ? INT_MAX - 64 : (int)per;
-    return (int)((keys + *range_keys - 1) / *range_keys);
+    *range_keys = (int)(most > keys ? keys : (most + 63) & ~(int64_t)63);
+    return (keys + *range_keys - 1) / *range_keys;
 }
 
 static RaggedPlan paged_plan(int tokens, int max_new, int heads, const fdx_kv_pages* c)
@@ -803,24 +1130,30 @@ static RaggedPlan paged_plan(int tokens, int max_new, int heads, const fdx_kv_pa
     r.few_rows = most <= 16 ? 16 : 32;
     if (group <= r.few_rows) {
         const int64_t items = (int64_t)c->n_seqs * c->kv_heads;
-        r.few_ranges = ranges_of(c->max_len, (4096 + items - 1) / items, 256, &r.few_keys);
-    }
-    if (most > r.few_rows || r.few_ranges == 0) {
-        r.tiles = tile_numbers(tokens, c->n_seqs, group, 128) * c->kv_heads;
-        const int64_t full = ((int64_t)tokens * group + 127) / 128 * c->kv_heads;
-        r.tile_ranges = ranges_of(c->max_len, full >= 256 ? 1 : (512 + full - 1) / full, 512, &r.tile_keys);
+        const int64_t keys = c->max_len * items / 4096;
+        r.few_ranges = ranges_of(c->max_len, keys < 512 ? 512 : keys, &r.few_keys);
+        r.few_part = items * (most < r.few_rows ? most : r.few_rows);
     }
     if (r.few_ranges == 0)
         r.few_rows = 0;
+    if (most > r.few_rows) {
+        r.tiles = tile_numbers(tokens, c->n_seqs, group, 128) * c->kv_heads;
+        const int64_t full = ((int64_t)tokens * group + 127) / 128 * c->kv_heads;
+        int64_t keys = c->max_len * full / 1024;
+        keys = keys < 512 ? 512 : (keys > 4096 ? 4096 : keys);
+        r.tile_ranges = ranges_of(c->max_len, keys < c->max_len / 16 ? c->max_len / 16 : keys, &r.tile_keys);
+        r.tile_part = (int64_t)tokens * heads;
+    }
     return r;
 }
 
-static RaggedPlan packed_plan(int tokens, int n_seqs, int heads, int kv_heads)
+static RaggedPlan packed_plan(int tokens, int n_seqs, int heads, int kv_heads, int dk, int dv)
 {
     RaggedPlan r {};
+    const int keys_a_tile = dk <= 64 && dv <= 64 ? 64 : 32;
+    if (tokens >= 512 && tokens / n_seqs >= keys_a_tile)
+        r.ready = tile_numbers(tokens, n_seqs, 1, keys_a_tile) * kv_heads;
     r.tiles = tile_numbers(tokens, n_seqs, heads / kv_heads, 128) * kv_heads;
-    r.tile_ranges = 1;
-    r.tile_keys = INT_MAX - 64;
     return r;
 }
 
@@ -837,30 +1170,32 @@ static bool wide_rows(const RaggedParams& p)
 template <int D, int KIND, bool WIDE>
 static void ragged_launch(RaggedParams p, const RaggedPlan& plan)
 {
-    p.few_rows = plan.few_rows;
     p.wide = WIDE;
-    p.ranges = plan.ranges();
-    if constexpr (KIND != kPackedF32) {
-        if (plan.few_ranges > 0) {
-            p.split_keys = plan.few_keys;
-            const dim3 grid((unsigned)(p.n_seqs * p.kv_heads), (unsigned)plan.few_ranges);
-            if (plan.few_rows <= 16)
-                hipLaunchKernelGGL((ragged_few_kernel<D, KIND, 1, WIDE>), grid, dim3(256), 0, stream(), p);
+    const bool exact = WIDE && p.dk == D && p.dv == D;
+    const dim3 block(256);
+    if constexpr (KIND == kPackedF32) {
+        if (plan.ready > 0) {
+            if (exact)
+                hipLaunchKernelGGL((ragged_ready_kernel<D, true>), dim3((unsigned)plan.ready), block, 0, stream(), p);
             else
-                hipLaunchKernelGGL((ragged_few_kernel<D, KIND, 2, WIDE>), grid, dim3(256), 0, stream(), p);
+                hipLaunchKernelGGL((ragged_ready_kernel<D, false>), dim3((unsigned)plan.ready), block, 0, stream(), p);
+            hipLaunchKernelGGL(ragged_packed_kernel<D>, dim3((unsigned)plan.tiles), block, 0, stream(), p);
+            return;
         }
+    } else if (plan.few_ranges > 0) {
+        const dim3 grid((unsigned)(p.n_seqs * p.kv_heads), (unsigned)plan.few_ranges, (unsigned)(plan.few_rows / 16));
+        hipLaunchKernelGGL((ragged_few_kernel<D, KIND, WIDE>), grid, block, 0, stream(), p);
     }
     if (plan.tiles > 0) {
-        p.split_keys = plan.tile_keys;
-        const dim3 grid((unsigned)plan.tiles, (unsigned)plan.tile_ranges);
-        if (WIDE && p.dk == D && p.dv == D && p.ldk < (1 << 24) && p.ldv < (1 << 24)) // offsets inside a tile in 32 bits
-            hipLaunchKernelGGL((ragged_tile_kernel<D, KIND, true>), grid, dim3(256), 0, stream(), p);
+        const dim3 grid((unsigned)plan.tiles, (unsigned)(plan.tile_ranges > 0 ? plan.tile_ranges : 1));
+        if (exact)
+            hipLaunchKernelGGL((ragged_tile_kernel<D, KIND, true>), grid, block, 0, stream(), p);
         else
-            hipLaunchKernelGGL((ragged_tile_kernel<D, KIND, false>), grid, dim3(256), 0, stream(), p);
+            hipLaunchKernelGGL((ragged_tile_kernel<D, KIND, false>), grid, block, 0, stream(), p);
     }
-    if (plan.ranges() > 1)
-        hipLaunchKernelGGL(ragged_join_kernel<KIND>, dim3((unsigned)(((int64_t)p.tokens * p.heads + 3) / 4)), dim3(256), 0, stream(), p, plan.few_keys,
-            plan.tile_keys);
+    if constexpr (KIND != kPackedF32)
+        if (plan.few_ranges > 1 || plan.tile_ranges > 1)
+            hipLaunchKernelGGL(ragged_join_kernel<KIND>, dim3((unsigned)(((int64_t)p.tokens * p.heads + 3) / 4)), block, 0, stream(), p);
 }
 
 template <int KIND>
@@ -904,10 +1239,9 @@ using namespace fdx;
 
 extern "C" size_t fdx_mha_packed_scratch_bytes(int tokens, int n_seqs, int heads, int kv_heads, int dk, int dv)
 {
-    (void)dk;
-    if (tokens <= 0 || n_seqs <= 0 || heads <= 0 || kv_heads <= 0 || dv <= 0)
+    if (tokens <= 0 || n_seqs <= 0 || heads <= 0 || kv_heads <= 0 || dk <= 0 || dv <= 0)
         return 0;
-    return packed_plan(tokens, n_seqs, heads, kv_heads).scratch(tokens, heads, dv);
+    return packed_plan(tokens, n_seqs, heads, kv_heads, dk, dv).ready_bytes();
 }
 
 extern "C" fdx_status fdx_mha_packed_f32(const float* q, int64_t ldq, const float* k, int64_t ldk, const float* v, int64_t ldv,
@@ -919,13 +1253,17 @@ extern "C" fdx_status fdx_mha_packed_f32(const float* q, int64_t ldq, const floa
     p.starts = starts; p.n_seqs = n_seqs; p.tokens = tokens;
     p.heads = heads; p.kv_heads = kv_heads; p.group = kv_heads > 0 ? heads / kv_heads : 0;
     p.dk = dk; p.dv = dv; p.causal = causal != 0;
-    p.error_flag = error_flag_dev; p.part = static_cast<float*>(scratch_dev);
+    p.error_flag = error_flag_dev;
     const fdx_status st = check_ragged("mha_packed", p, scratch_dev, fdx_mha_packed_scratch_bytes(tokens, n_seqs, heads, kv_heads, dk, dv));
     if (st != FDX_OK)
         return st;
     p.scale = (float)(1.0 / std::sqrt((double)dk));
+    p.by_group = make_divisor(p.group);
     profile_begin();
-    ragged_dispatch<kPackedF32>(p, packed_plan(tokens, n_seqs, heads, kv_heads));
+    const RaggedPlan plan = packed_plan(tokens, n_seqs, heads, kv_heads, dk, dv);
+    p.ready = static_cast<unsigned char*>(scratch_dev);
+    p.powers = reinterpret_cast<f32x2_pow*>(p.ready + plan.ready * 32768);
+    ragged_dispatch<kPackedF32>(p, plan);
     profile_end("mha_packed_f32", 0.0, 4.0 * tokens * ((double)heads + kv_heads) * (dk + dv));
     FDX_LAUNCH_CHECK();
     return FDX_OK;
@@ -936,7 +1274,8 @@ extern "C" size_t fdx_mha_paged_scratch_bytes(int tokens, int max_new, int heads
     if (!c || tokens <= 0 || max_new <= 0 || heads <= 0 || c->kv_heads <= 0 || heads % c->kv_heads != 0 || c->dk <= 0 || c->dv <= 0 || c->n_seqs <= 0
         || c->max_len <= 0)
         return 0;
-    return paged_plan(tokens, max_new, heads, c).scratch(tokens, heads, c->dv);
+    const RaggedPlan plan = paged_plan(tokens, max_new, heads, c);
+    return sizeof(float) * (plan.few_floats(c->dv) + plan.tile_floats(c->dv));
 }
 
 extern "C" fdx_status fdx_mha_paged_f32(const float* q, int64_t ldq, const int32_t* starts, int tokens, int max_new, int heads,
@@ -953,14 +1292,19 @@ extern "C" fdx_status fdx_mha_paged_f32(const float* q, int64_t ldq, const int32
     p.heads = heads; p.kv_heads = cache->kv_heads; p.group = heads / cache->kv_heads;
     p.dk = cache->dk; p.dv = cache->dv; p.causal = 1;
     p.table = cache->table; p.lens = cache->lens; p.table_width = cache->table_width; p.n_pages = cache->n_pages;
-    p.page_size = cache->page_size; p.max_len = cache->max_len; p.max_new = max_new < tokens ? max_new : tokens;
-    p.error_flag = error_flag_dev; p.part = static_cast<float*>(scratch_dev);
+    p.page_size = make_divisor(cache->page_size); p.max_len = cache->max_len; p.max_new = max_new < tokens ? max_new : tokens;
+    p.error_flag = error_flag_dev;
     st = check_ragged("mha_paged", p, scratch_dev, fdx_mha_paged_scratch_bytes(tokens, max_new, heads, cache));
     if (st != FDX_OK)
         return st;
     FDX_REQUIRE((int64_t)p.n_seqs * p.kv_heads <= (1 << 22), "mha_paged: sequences * key heads too many for one launch");
     p.scale = (float)(1.0 / std::sqrt((double)p.dk));
     const RaggedPlan plan = paged_plan(tokens, max_new, heads, cache);
+    float* part = static_cast<float*>(scratch_dev);
+    p.by_group = make_divisor(p.group);
+    p.few_rows = plan.few_rows;
+    p.few = { part, plan.few_part, plan.few_ranges, plan.few_keys, (int)(plan.few_part / ((int64_t)p.n_seqs * p.kv_heads)) };
+    p.tile = { part + plan.few_floats(p.dv), plan.tile_part, plan.tile_ranges, plan.tile_keys, 0 };
     profile_begin();
     if (cache->type == FDX_KV_F32)
         ragged_dispatch<kPagedF32>(p, plan);

@@ -13,6 +13,22 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 // where keys and values come from
 enum { kPackedF32 = 0, kPagedF32 = 1, kPagedBf16 = 2 };
 
+// Rows that see more keys than one workgroup takes: their sums over each range of keys, for ragged_join_kernel.  [range][row][depth] of
+// o / l, then [range][row][m, l].  m is -infinity where the range has no key, -FLT_MAX where all its scores are -infinity.
+struct PartSums {
+    float* at;
+    int64_t rows;
+    int ranges, keys; // of the longest sequence; keys: what a range has at most
+    int a_head;       // few rows: rows of a sequence and key head
+
+    __device__ __forceinline__ float* out(int range, int64_t row, int dv) const { return at + (range * rows + row) * dv; }
+    __device__ __forceinline__ float* size(int range, int64_t row, int dv) const { return at + ranges * rows * dv + 2 * (range * rows + row); }
+};
+
+struct f32x2_pow {
+    float k_down, v_down; // what takes a tile's power of two back
+};
+
 struct RaggedParams {
     const float* q;
     float* out;
@@ -21,28 +37,17 @@ struct RaggedParams {
     int64_t ldk, ldv;
     const int32_t* starts;
     int n_seqs, tokens, heads, kv_heads, group, dk, dv, causal;
+    Divisor by_group, page_size;
     float scale;
     const int32_t *table, *lens; // paged only
-    int table_width, n_pages, page_size, max_len, max_new;
+    int table_width, n_pages, max_len, max_new;
     int* error_flag;
-    float* part;          // rows that see more than split_keys keys: sums of each range of split_keys, met by ragged_join_kernel
-    int ranges;           // ranges that p.part has room for
-    int split_keys;
-    int wide;             // rows of every tensor lie on 16-byte vectors, and depths are whole ones
+    PartSums few, tile;   // of the launch for few rows and of the one for tiles
     int few_rows;         // sequences that bring up to this many rows to a key head are ragged_few_kernel's, others ragged_tile_kernel's
+    int wide;             // rows of every tensor lie on 16-byte vectors, and depths are whole ones
+    unsigned char* ready; // packed prompts: tiles of split keys and values, [tile][key head][32 KB], and their powers [tile][key head]
+    f32x2_pow* powers;
 };
-
-// The sums of a row over one range of keys as they lie in p.part: [range][row][depth] of o / l, then [range][row][m, l].  m is
-// -infinity where the range has no key, -FLT_MAX where all its scores are -infinity.
-__device__ __forceinline__ float* part_out(const RaggedParams& p, int range, int64_t row)
-{
-    return p.part + (range * ((int64_t)p.tokens * p.heads) + row) * p.dv;
-}
-__device__ __forceinline__ float* part_size(const RaggedParams& p, int range, int64_t row)
-{
-    const int64_t rows = (int64_t)p.tokens * p.heads;
-    return p.part + p.ranges * rows * p.dv + 2 * (range * rows + row);
-}
 
 template <int KIND>
 struct KvElement {
@@ -59,13 +64,15 @@ struct Sequence {
     int keys;     // positions that its last new token sees (all of them without a causal mask)
     int ahead;    // position of its first new token; may be negative: tokens that see nothing
     int index;
+    bool few;     // its rows are few enough for ragged_few_kernel
+    int range;    // keys of a range: as many ranges as its keys need, of the same length
     bool cut;     // lens or the number of new tokens beyond what the call was told
 };
 
 template <int KIND>
 __device__ __forceinline__ Sequence sequence_of(const RaggedParams& p, int index, Span span)
 {
-    Sequence s { span, span.count, 0, index, false };
+    Sequence s { span, span.count, 0, index, false, 0x7fffffff, false };
     if constexpr (KIND != kPackedF32) {
         const int len = p.lens[index];
         s.keys = len < 0 ? 0 : (len > p.max_len ? p.max_len : len);
@@ -73,8 +80,23 @@ __device__ __forceinline__ Sequence sequence_of(const RaggedParams& p, int index
         s.cut = len != s.keys || span.count > p.max_new;
         if (span.count > p.max_new)
             s.span.count = p.max_new;
+        s.few = s.span.count * p.group <= p.few_rows;
+        const int most = s.few ? p.few.keys : p.tile.keys;
+        if (s.keys > most) {
+            const int parts = (s.keys + most - 1) / most;
+            s.range = ((s.keys + parts - 1) / parts + 63) & ~63;
+        }
     }
     return s;
+}
+
+// where the sums of a row are kept, rows as the launches number them
+__device__ __forceinline__ int64_t part_row(const RaggedParams& p, const Sequence& s, int token, int head)
+{
+    if (!s.few)
+        return (int64_t)(s.span.first + token) * p.heads + head;
+    const int kv_head = quotient(head, p.by_group);
+    return ((int64_t)s.index * p.kv_heads + kv_head) * p.few.a_head + token * p.group + head - kv_head * p.group;
 }
 
 // row of a position in k and v, -1 for one that is not there
@@ -96,11 +118,74 @@ __device__ __forceinline__ int visible_keys(const RaggedParams& p, const Sequenc
     return n < 0 ? 0 : n;
 }
 
+// find_tile by a whole wave: sixty-four sequences are looked at together, where a binary search waits for memory once a step
+__device__ __forceinline__ Tile find_tile_wave(const int32_t* starts, int n_seqs, int tokens, int per_token, int rows, int64_t number)
+{
+    const int lane = threadIdx.x & 63;
+    int lo = 0, hi = n_seqs;
+    while (lo < hi) {
+        const int step = (hi - lo + 63) >> 6, i = lo + lane * step;
+        bool not_above = false;
+        if (i < hi) {
+            const int a = starts[i];
+            not_above = first_tile(a < 0 ? 0 : (a > tokens ? tokens : a), i, per_token, rows) <= number;
+        }
+        const int count = __builtin_popcountll(__ballot(not_above));
+        const int next = lo + count * step;
+        if (step == 1) {
+            lo = hi = next;
+        } else {
+            hi = next < hi ? next : hi;
+            lo = count > 0 ? next - step + 1 : hi;
+        }
+    }
+    Tile t { lo - 1, 0, { 0, 0 } };
+    if (t.seq < 0)
+        return t;
+    t.span = packed_span(starts, t.seq, tokens);
+    const int64_t index = number - first_tile(t.span.first, t.seq, per_token, rows);
+    if (index < 0 || index * rows >= (int64_t)t.span.count * per_token)
+        t.seq = -1;
+    t.index = (int)index;
+    return t;
+}
+
+// The same for up to sixty-four sequences, numbered the other way: tiles furthest inside their sequences first, which see most keys.
+// before(j) = tiles of index j and more; the tile with `number` tiles in front of it has the index j with before(j + 1) <= number < before(j).
+__device__ __forceinline__ Tile late_tile_wave(const int32_t* starts, int n_seqs, int tokens, int per_token, int rows, int64_t number)
+{
+    const int lane = threadIdx.x & 63;
+    Span span { 0, 0 };
+    if (lane < n_seqs)
+        span = packed_span(starts, lane, tokens);
+    const int tiles = (int)(((int64_t)span.count * per_token + rows - 1) / rows);
+    auto before = [&](int j) { return (int64_t)wave_all<false>((float)(tiles > j ? tiles - j : 0)); }; // below 2^24: tokens * heads is at most 2^26
+    Tile t { -1, 0, { 0, 0 } };
+    if (number >= before(0))
+        return t;
+    int lo = 0, hi = (int)wave_all<true>((float)tiles); // before(lo) > number >= before(hi)
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (before(mid) > number)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    uint64_t of = __ballot(tiles > lo);
+    for (int skip = (int)(number - before(lo + 1)); skip > 0; --skip)
+        of &= of - 1;
+    t.seq = __builtin_ctzll(of);
+    t.index = lo;
+    t.span = packed_span(starts, t.seq, tokens);
+    return t;
+}
+
 // exponentials are taken to base two on scores that carry log2(e)
 constexpr float kLog2e = 1.44269504088896340736f;
 
 // One query row over the keys first .. last - 1 by one whole wave, in fp32: a lane has a key's score, then depths lane and
-// 64 + lane of the output.  m is the largest score in units of log2, l the sum of 2^(score - m), o the weighted values.
+// 64 + lane of the output.  m - 24 is the largest score in units of log2, l the sum of 2^(score - m), o the weighted values: with 2^-24 in every
+// weight the sums of values near fp32's end stay below it.
 template <int KIND>
 __device__ __forceinline__ void plain_row(const RaggedParams& p, const Sequence& s, const float* q, int kv_head, int first, int last, float& m,
     float& l, float (&o)[2], bool& seen, bool& missing)
@@ -129,7 +214,7 @@ __device__ __forceinline__ void plain_row(const RaggedParams& p, const Sequence&
         float mx = sc;
         for (int w = 32; w > 0; w >>= 1)
             mx = fmaxf(mx, __shfl_xor(mx, w, 64));
-        const float m_new = fmaxf(m, mx), m_use = m_new == -INFINITY ? 0.f : m_new, corr = __builtin_amdgcn_exp2f(m - m_use);
+        const float m_new = fmaxf(m, mx + 24.f), m_use = m_new == -INFINITY ? 0.f : m_new, corr = __builtin_amdgcn_exp2f(m - m_use);
         const float pr = row >= 0 ? __builtin_amdgcn_exp2f(sc - m_use) : 0.f;
         float rs = pr;
         for (int w = 32; w > 0; w >>= 1)

@@ -78,6 +78,15 @@ int main()
             }
         }
     }
+    // quotients: every divisor's multiples and their neighbours, small and large
+    for (int round = 0; round < 200000; ++round) {
+        const int by = round < 3000 ? round + 1 : 1 + (int)(rng() % (upto(3) == 0 ? 2147483647u : 100000u));
+        const Divisor d = make_divisor(by);
+        const int64_t multiple = (int64_t)by * (1 + (int64_t)(rng() % (2147483647u / (unsigned)by)));
+        for (int64_t n : { (int64_t)0, (int64_t)by - 1, (int64_t)by, multiple - 1, multiple, multiple + 1, (int64_t)2147483647, (int64_t)(rng() >> 1) })
+            if (n >= 0 && n <= 2147483647)
+                CHECK(quotient((int)n, d) == (int)(n / by));
+    }
     // any page numbers and positions: a row of the cache or -1
     for (int round = 0; round < 20000; ++round) {
         const int width = 1 + upto(6), page_size = 1 + upto(70), n_pages = 1 + upto(9);
@@ -86,7 +95,7 @@ int main()
             t = upto(3) == 0 ? odd[upto(9)] : upto(n_pages);
         const int32_t positions[] = { INT_MIN, -1, 0, page_size - 1, page_size, width * page_size - 1, width * page_size, INT_MAX, upto(500) };
         for (int pos : positions) {
-            const int row = page_row(table.data(), width, n_pages, page_size, pos);
+            const int row = page_row(table.data(), width, n_pages, make_divisor(page_size), pos);
             const bool there = pos >= 0 && pos / page_size < width && table[pos / page_size] >= 0 && table[pos / page_size] < n_pages;
             CHECK(there == (row >= 0));
             if (there)
@@ -95,7 +104,7 @@ int main()
     }
     // the largest cache
     const int32_t last[] = { (1 << 27) - 1 };
-    CHECK(page_row(last, 1, (1 << 27) - 1 + 1, 15, 14) == (int)(((int64_t)(1 << 27) - 1) * 15 + 14));
+    CHECK(page_row(last, 1, (1 << 27) - 1 + 1, make_divisor(15), 14) == (int)(((int64_t)(1 << 27) - 1) * 15 + 14));
     std::printf("kv_pages done\n");
     return 0;
 }

@@ -64,6 +64,58 @@ def test_packed(fdx, lengths, heads, kv_heads, dk, dv, causal):
     close(fdx.mha_packed(q, k, v, lengths, heads, kv_heads, dk, dv, causal), packed_reference(q, k, v, lengths, heads, kv_heads, causal))
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lengths,heads,kv_heads,dk,dv", [
+    ([513, 130], 4, 2, 128, 128), ([700], 5, 5, 80, 80), ([520, 1, 0, 300], 2, 1, 33, 127), ([64] * 9, 3, 3, 64, 64), ([512], 1, 1, 64, 64),
+    ([33, 600, 95, 32, 31], 8, 1, 128, 128), ([1, 1200, 2], 6, 2, 32, 32), ([300, 300], 7, 7, 64, 40), ([900], 16, 2, 64, 64)])
+def test_packed_of_many_tokens(fdx, lengths, heads, kv_heads, dk, dv, causal):
+    test_packed(fdx, lengths, heads, kv_heads, dk, dv, causal)
+
+
+@pytest.mark.parametrize("lengths", [[90, 150, 40], [640, 200]])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("power", [12, 18, 30, 70, 124])
+def test_packed_sizes_behind_the_mask(fdx, lengths, d, power):
+    """Keys and values of later tokens 2^power times larger: the tokens in front of them do not see them and keep their bound, also
+    those that share a tile with them."""
+    r, heads, kv, total = np.random.default_rng(power), 4, 2, sum(lengths)
+    q, k, v = (r.standard_normal((total, h * d)).astype(np.float32) for h in (heads, kv, kv))
+    base = packed_reference(q, k, v, lengths, heads, kv, True)
+    for name, first in (("k", 41), ("v", 41), ("v", lengths[0] - 1), ("k", 2), ("v", 3)):
+        print("packed behind the mask", lengths, d, power, name, first, flush=True)
+        kk, vv = k.copy(), v.copy()
+        dict(k=kk, v=vv)[name][first:lengths[0]] *= np.float32(2.0 ** power)
+        got = fdx.mha_packed(q, kk, vv, lengths, heads, kv, d, d)
+        keep = np.r_[0:first, lengths[0]:total]
+        close(got[keep], base[keep])
+        if name == "v":   # and the rows that see them: their result is as large as the largest they see
+            with np.errstate(all="ignore"):
+                want = packed_reference(q, kk, vv, lengths, heads, kv, True)[first:lengths[0]]
+            # one probability with nothing to average over: its score is a chain of d sums of up to 3 sqrt(d) = 34, each off by up to
+            # half of 2^-19 and by a quarter on average, 0.25 * 2^-19 * sqrt(d) / sqrt(d) = 5e-7 in all as a standard deviation, over a few rows
+            close(got[first:lengths[0]].astype(np.float64), want, 2e-6)
+
+
+def test_packed_many_tokens_infinities_and_nan(fdx):
+    """As above where keys and values are split in a pass of their own."""
+    r, n, heads, kv = np.random.default_rng(8), 700, 2, 1
+    q, k, v = (r.standard_normal((n, h * 64)).astype(np.float32) for h in (heads, kv, kv))
+    base = packed_reference(q, k, v, [n], heads, kv, True)
+    for what in (np.nan, np.inf, -np.inf):
+        for name, row in (("v", 333), ("k", 333), ("v", n - 1), ("k", 640)):
+            print("packed many odd", what, name, row, flush=True)
+            kk, vv = k.copy(), v.copy()
+            dict(k=kk, v=vv)[name][row, 7] = what
+            got = fdx.mha_packed(q, kk, vv, [n], heads, kv, 64, 64)
+            close(got[:row], base[:row])
+            with np.errstate(all="ignore"):
+                want = packed_reference(q, kk, vv, [n], heads, kv, True)[row:]
+            assert np.array_equal(np.isnan(got[row:]), np.isnan(want)) and np.array_equal(np.isinf(got[row:]), np.isinf(want))
+            ok = np.isfinite(want)
+            if ok.any():
+                close(got[row:][ok], want[ok])
+
+
 def test_packed_scores_of_a_few_hundred(fdx):
     """The running maximum moves from tile to tile; scores 40 times larger, errors too."""
     r, lengths = np.random.default_rng(3), [333, 50]
@@ -391,6 +443,23 @@ def test_paged_nan_that_only_later_tokens_see(fdx):
             close(got[~hit], base.reshape(got.shape)[~hit])
 
 
+@pytest.mark.parametrize("new", [[4], [60], [140]])
+@pytest.mark.parametrize("power", [14, 40, 124])
+def test_paged_sizes_behind_the_mask(fdx, new, power):
+    """A chunk whose last tokens' keys and values are 2^power times larger than the others'."""
+    for name in ("v", "k"):
+        f = Filled(fdx, [150], 2, 64, 64, 16, "f32")
+        q = np.random.default_rng(4).standard_normal((new[0], 256)).astype(np.float32)
+        base = f.reference(q, new, 4)
+        buf = f.cache.v if name == "v" else f.cache.k
+        rows = buf.to_host((f.cache.n_pages * 16, 128))
+        at = f.cache.table[0][np.arange(147, 150) // 16] * 16 + np.arange(147, 150) % 16
+        rows[at] *= np.float32(2.0 ** power)
+        setattr(f.cache, name, fdx.DevBuf.from_host(rows))
+        print("paged behind the mask", new, power, name, flush=True)
+        close(fdx.mha_paged(f.cache, q, new, 4)[:-3], base[:-3])
+
+
 def test_prompts_then_tokens(fdx):
     """The operators as a serving program uses them: prompts at once, their keys and values into the cache, then steps of one token,
     a chunk for one sequence beside them, and the scores of the tokens: the same as one pass over each whole sequence."""
@@ -421,3 +490,35 @@ def test_prompts_then_tokens(fdx):
         for s in range(4):
             cache.release(s)
         assert sorted(cache.free) == list(range(40))
+
+
+@pytest.mark.parametrize("n_seqs", [63, 64, 65, 300])
+def test_many_sequences(fdx, n_seqs):
+    """Lengths of 0 to 9 and two longer ones somewhere, as prompts and as the newest tokens of caches."""
+    r = np.random.default_rng(n_seqs)
+    lengths = r.integers(0, 10, n_seqs).tolist()
+    lengths[n_seqs // 3], lengths[n_seqs - 2] = 150, 70
+    heads, kv, d = 4, 2, 64
+    print("many sequences", n_seqs, flush=True)
+    q, k, v = (r.standard_normal((sum(lengths), h * d)).astype(np.float32) for h in (heads, kv, kv))
+    for causal in (True, False):
+        close(fdx.mha_packed(q, k, v, lengths, heads, kv, d, d, causal), packed_reference(q, k, v, lengths, heads, kv, causal))
+    new = [min(n, int(m)) for n, m in zip(lengths, r.integers(0, 12, n_seqs))]
+    new[n_seqs // 3] = 90
+    f = Filled(fdx, lengths, kv, d, d, 8, "f32", seed=1, max_len=2000)
+    q = r.standard_normal((sum(new), heads * d)).astype(np.float32)
+    close(fdx.mha_paged(f.cache, q, new, heads), f.reference(q, new, heads))
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("context,new,heads,kv,d", [([5000, 40], [1, 1], 4, 2, 64), ([3000, 2900, 700], [40, 1, 100], 8, 2, 128),
+                                                    ([2600, 1], [2, 1], 6, 6, 64), ([4500], [600], 2, 1, 128), ([1500, 0, 900], [33, 0, 3], 32, 1, 64)])
+def test_paged_long_contexts(fdx, context, new, heads, kv, d, kind):
+    """Keys in ranges over several workgroups; pages of sixteen, and of a size that divides nothing."""
+    for page in (16, 37):
+        print("paged long", context, new, heads, kv, d, page, kind, flush=True)
+        f = Filled(fdx, context, kv, d, d, page, kind, seed=sum(context), steps=1)
+        q = np.random.default_rng(d).standard_normal((sum(new), heads * d)).astype(np.float32)
+        close(fdx.mha_paged(f.cache, q, new, heads), f.reference(q, new, heads))
+        first = fdx.mha_paged(f.cache, q, new, heads)
+        assert np.array_equal(first, fdx.mha_paged(f.cache, q, new, heads))
