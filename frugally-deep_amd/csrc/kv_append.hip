@@ -4,12 +4,10 @@
 // launch for a decode step.
 #include <cstdint>
 
-#include "common.hpp"
-#include "kv_pages.hpp"
+#include "ragged_attn.hpp"
 
 namespace fdx {
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 
 struct AppendParams {
@@ -44,7 +42,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendParams p)
     const int row = (int)(item >> 1);
     if (row >= p.tokens)
         return;
-    const int s = find_row(p.starts, p.c.n_seqs, p.tokens, row);
+    const int s = find_row_wave(p.starts, p.c.n_seqs, p.tokens, row);
     if (s < 0)
         return;
     const Span span = packed_span(p.starts, s, p.tokens);

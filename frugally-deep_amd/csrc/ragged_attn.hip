@@ -2,6 +2,7 @@
 #include <cfloat>
 #include <climits>
 
+#include "bf16_split.hpp"
 #include "f16_split.hpp"
 #include "ragged_attn.hpp"
 
@@ -797,8 +798,10 @@ __global__ __launch_bounds__(256, 2) void ragged_packed_kernel(RaggedParams p)
 //  * S^T = K Q^T: lane (c, g) of 16 x 4 loads chunks of key c, chunk i at depth 4 W i + W g (W elements are 16 bytes), and has scores of keys
 //    4 g .. 4 g + 3 of row c.
 //  * O^T = V^T P^T: lane (c, g) loads depths V c .. V c + V - 1 of keys 4 g .. + 3, so the probabilities it has are the operand, and gets
-//    depths V (4 g + i) + e of row c.  The products are exact in fp32; what they cost, 32 cycles per 16 keys, 16 rows and 4 depths, is less
-//    than the memory's share of a CU needs for the keys.
+//    depths V (4 g + i) + e of row c.
+//  * fp32 pages: the 16x16x4 fp32 products, 32 cycles per 16 keys, 16 rows and 4 depths, which is half of what the memory's share of a CU needs
+//    for the keys.  bf16 pages bring twice the keys in that time: the bf16 products take them as they are, queries and probabilities as the
+//    exact sum of three bf16 values (bf16_split.hpp), 576 cycles instead of 2048 for 16 keys at depth 128.
 template <typename T, int W, bool WIDE>
 __device__ __forceinline__ auto load_chunk(const T* row, int d, int depth)
 {
@@ -825,6 +828,7 @@ __global__ __launch_bounds__(256, 2) void ragged_few_kernel(RaggedParams p)
     typedef typename KvElement<KIND>::type T;
     constexpr int W = 16 / (int)sizeof(T), NK = D / (4 * W); // elements of a key chunk, chunks of a lane
     constexpr int DL = D / 16, VW = DL < W ? DL : W, NV = DL / VW; // depths of a lane, in NV loads of VW
+    constexpr bool kBf16 = KIND == kPagedBf16;
     typedef T kvec __attribute__((ext_vector_type(W)));
     typedef T vvec __attribute__((ext_vector_type(VW)));
     struct Block {
@@ -885,7 +889,8 @@ __global__ __launch_bounds__(256, 2) void ragged_few_kernel(RaggedParams p)
         fetch(a, row_a);
     }
 
-    float q[NK][W];
+    float q[kBf16 ? 1 : NK][W];
+    bf16x8 q3[kBf16 ? NK : 1][3];
     const bool q_ok = r_first + c < count;
     const int q_token = quotient(q_ok ? r_first + c : 0, p.by_group);
     const int visible = q_ok ? visible_keys(p, s, q_token) : 0;
@@ -893,14 +898,29 @@ __global__ __launch_bounds__(256, 2) void ragged_few_kernel(RaggedParams p)
         const float* from = p.q + (int64_t)(s.span.first + q_token) * p.ldq
             + (int64_t)(kv_head * p.group + (q_ok ? r_first + c : 0) - q_token * p.group) * p.dk;
 #pragma unroll
-        for (int i = 0; i < NK; ++i)
+        for (int i = 0; i < NK; ++i) {
+            float y[W];
 #pragma unroll
             for (int h = 0; h < W; h += 4) {
                 const f32x4 x = load_chunk<float, 4, WIDE>(from, 4 * W * i + W * g + h, p.dk);
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    q[i][h + e] = x[e] * (p.scale * kLog2e);
+                    y[h + e] = x[e] * (p.scale * kLog2e);
             }
+            if constexpr (kBf16) {
+                uint32_t w[3][4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    split3(y[2 * e], y[2 * e + 1], w[0][e], w[1][e], w[2][e]);
+#pragma unroll
+                for (int z = 0; z < 3; ++z)
+                    q3[i][z] = __builtin_bit_cast(bf16x8, (u32x4 { w[z][0], w[z][1], w[z][2], w[z][3] }));
+            } else {
+#pragma unroll
+                for (int e = 0; e < W; ++e)
+                    q[i][e] = y[e];
+            }
+        }
     }
     float m_run = -INFINITY, l_run = 0.f;
     f32x4 oacc[DL];
@@ -913,10 +933,17 @@ __global__ __launch_bounds__(256, 2) void ragged_few_kernel(RaggedParams p)
     auto work = [&](const Block& x, int blk) {
         f32x4 sc = { 0.f, 0.f, 0.f, 0.f };
 #pragma unroll
-        for (int i = 0; i < NK; ++i)
+        for (int i = 0; i < NK; ++i) {
+            if constexpr (kBf16) {
 #pragma unroll
-            for (int e = 0; e < W; ++e)
-                sc = __builtin_amdgcn_mfma_f32_16x16x4f32((float)x.k[i][e], q[i][e], sc, 0, 0, 0);
+                for (int z = 2; z >= 0; --z) // small ones first
+                    sc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x.k[i]), q3[i][z], sc, 0, 0, 0);
+            } else {
+#pragma unroll
+                for (int e = 0; e < W; ++e)
+                    sc = __builtin_amdgcn_mfma_f32_16x16x4f32(x.k[i][e], q[i][e], sc, 0, 0, 0);
+            }
+        }
         const int at = k_first + blk * 16;
         if (at + 16 > all_see) {
 #pragma unroll
@@ -950,13 +977,37 @@ __global__ __launch_bounds__(256, 2) void ragged_few_kernel(RaggedParams p)
             sc[i] = __builtin_amdgcn_exp2f(sc[i] - base);
             l_run += sc[i];
         }
+        if constexpr (kBf16) {
+            typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+            typedef short s16x4 __attribute__((ext_vector_type(4)));
+            typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+            u32x2 pr[3];
+            uint32_t w[3][2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < 2; ++i)
+                split3(sc[2 * i], sc[2 * i + 1], w[0][i], w[1][i], w[2][i]);
+#pragma unroll
+            for (int z = 0; z < 3; ++z)
+                pr[z] = u32x2 { w[z][0], w[z][1] };
 #pragma unroll
             for (int j = 0; j < NV; ++j)
 #pragma unroll
-                for (int e = 0; e < VW; ++e)
-                    oacc[j * VW + e] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)x.v[i][j][e], sc[i], oacc[j * VW + e], 0, 0, 0);
+                for (int e = 0; e < VW; ++e) {
+                    const bf16x4 v4 = { x.v[0][j][e], x.v[1][j][e], x.v[2][j][e], x.v[3][j][e] };
+#pragma unroll
+                    for (int z = 2; z >= 0; --z)
+                        oacc[j * VW + e] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, v4), __builtin_bit_cast(s16x4, pr[z]),
+                            oacc[j * VW + e], 0, 0, 0);
+                }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < NV; ++j)
+#pragma unroll
+                    for (int e = 0; e < VW; ++e)
+                        oacc[j * VW + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.v[i][j][e], sc[i], oacc[j * VW + e], 0, 0, 0);
+        }
     };
     for (int blk = wave; blk < blocks; blk += 8) {
         const bool more = blk + 4 < blocks;
@@ -1068,7 +1119,7 @@ __global__ __launch_bounds__(256) void ragged_join_kernel(RaggedParams p)
     const int row = (int)((uint64_t)item / (uint32_t)p.heads), head = (int)(item - (int64_t)row * p.heads);
     if (row >= p.tokens)
         return;
-    const int index = find_row(p.starts, p.n_seqs, p.tokens, row);
+    const int index = find_row_wave(p.starts, p.n_seqs, p.tokens, row);
     if (index < 0)
         return;
     const Sequence s = sequence_of<KIND>(p, index, packed_span(p.starts, index, p.tokens));
@@ -1081,20 +1132,37 @@ __global__ __launch_bounds__(256) void ragged_join_kernel(RaggedParams p)
     const int parts = (visible + s.range - 1) / s.range;
     const PartSums& part = s.few ? p.few : p.tile;
     const int64_t id = part_row(p, s, token, head);
+    // a lane a range for the sizes, then all lanes a range at a time for the rows, four of them on their way together
     float top = -INFINITY;
-    for (int i = 0; i < parts; ++i)
-        top = fmaxf(top, part.size(i, id, p.dv)[0]);
+    for (int i0 = 0; i0 < parts; i0 += 64)
+        if (i0 + lane < parts)
+            top = fmaxf(top, part.size(i0 + lane, id, p.dv)[0]);
+    top = wave_all<true>(top);
     const float m = top == -INFINITY ? 0.f : top;
     float l = 0.f, o0 = 0.f, o1 = 0.f;
-    for (int i = 0; i < parts; ++i) {
-        const float* at = part.size(i, id, p.dv);
-        const float w = at[1] * __builtin_amdgcn_exp2f(at[0] - m);
-        const float* from = part.out(i, id, p.dv);
-        l += w;
-        if (lane < p.dv)
-            o0 = fmaf(w, from[lane], o0);
-        if (64 + lane < p.dv)
-            o1 = fmaf(w, from[64 + lane], o1);
+    for (int i0 = 0; i0 < parts; i0 += 64) {
+        float w = 0.f;
+        if (i0 + lane < parts) {
+            const float* at = part.size(i0 + lane, id, p.dv);
+            w = at[1] * __builtin_amdgcn_exp2f(at[0] - m);
+        }
+        l += wave_all<false>(w);
+        const int count = parts - i0 < 64 ? parts - i0 : 64;
+        for (int i = 0; i < count; i += 4) {
+            float x0[4], x1[4];
+#pragma unroll
+            for (int z = 0; z < 4; ++z) {
+                const float* from = part.out(i0 + (i + z < count ? i + z : i), id, p.dv);
+                x0[z] = from[lane < p.dv ? lane : 0];
+                x1[z] = from[64 + lane < p.dv ? 64 + lane : 0];
+            }
+#pragma unroll
+            for (int z = 0; z < 4; ++z) {
+                const float wi = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), i + z < count ? i + z : i));
+                o0 = fmaf(i + z < count ? wi : 0.f, x0[z], o0);
+                o1 = fmaf(i + z < count ? wi : 0.f, x1[z], o1);
+            }
+        }
     }
     float* to = p.out + (int64_t)row * p.ldo + (int64_t)head * p.dv;
     if (lane < p.dv)

@@ -150,7 +150,29 @@ __device__ __forceinline__ Tile find_tile_wave(const int32_t* starts, int n_seqs
     return t;
 }
 
-// The same for up to sixty-four sequences, numbered the other way: tiles furthest inside their sequences first, which see most keys.
+// find_row the same way
+__device__ __forceinline__ int find_row_wave(const int32_t* starts, int n_seqs, int tokens, int row)
+{
+    const int lane = threadIdx.x & 63;
+    int lo = 0, hi = n_seqs;
+    while (lo < hi) {
+        const int step = (hi - lo + 63) >> 6, i = lo + lane * step;
+        const int count = __builtin_popcountll(__ballot(i < hi && starts[i < hi ? i : lo] <= row));
+        const int next = lo + count * step;
+        if (step == 1) {
+            lo = hi = next;
+        } else {
+            hi = next < hi ? next : hi;
+            lo = count > 0 ? next - step + 1 : hi;
+        }
+    }
+    if (lo == 0)
+        return -1;
+    const Span s = packed_span(starts, lo - 1, tokens);
+    return row >= s.first && row - s.first < s.count ? lo - 1 : -1;
+}
+
+// find_tile for up to sixty-four sequences, numbered the other way: tiles furthest inside their sequences first, which see most keys.
 // before(j) = tiles of index j and more; the tile with `number` tiles in front of it has the index j with before(j + 1) <= number < before(j).
 __device__ __forceinline__ Tile late_tile_wave(const int32_t* starts, int n_seqs, int tokens, int per_token, int rows, int64_t number)
 {

@@ -1,15 +1,16 @@
 // Log probabilities of given tokens, entropy and the likeliest tokens of each row of logits.
 //
-//   m = max x, Z = sum e^(x - m), W = sum e^(x - m) (x - m);  log p[i] = x[i] - m - log Z,  H = log Z - W / Z
+//   m = max x, t = (x - m) log2(e), Z = sum 2^t, W = sum 2^t t;  log p[i] = x[i] - m - ln2 log2 Z,  H = ln2 (log2 Z - W / Z)
 // Both terms of H are at least zero, so nothing cancels.  Bound by memory: every logit is read once and stays in registers for all
 // that is asked of it.
 //
-// A workgroup takes a row, or a part of one where rows are few, in chunks of 4 E vectors a thread; waves keep sums of their own, which
-// meet at the end (exp(m_w - m) each).  The likeliest `top` tokens of a wave are a sorted list in LDS.  Of a chunk, every lane finds its own
-// best token; the top-th best of these 64 is a threshold that no fewer than `top` tokens of the chunk reach, and only `top` lanes can hold
-// tokens that do: on random logits about as many as are asked for, and never more than fit.  Those and the list so far are
-// ordered by counting, for each, the better ones.  Lists of waves and of parts meet in pairs, an item's place being its place in its
-// own list plus the number of better ones in the other.
+// A workgroup takes a row, or a part of one, in chunks of 4 E logits a thread; waves keep sums of their own, which meet at the end.  The likeliest
+// `top` tokens of a wave are a sorted list in LDS.  Of a chunk, `top` lanes' largest logits are a threshold that no fewer than `top` tokens
+// reach: it is found bit by bit with votes on the lanes' largest, and stops as soon as not many more lanes than that pass.  On
+// random logits about as many tokens pass as are asked for; they and the list so far are ordered by counting, for each, the better ones.
+// Where more pass than there is room for (equal logits), the best are taken one at a time.  Only finite logits are listed: places that stay
+// empty are those of ruled-out tokens, the lowest ids that are not listed.  Lists of waves and of parts meet in pairs, an item's place being its
+// place in its own list plus the number of better ones in the other.
 #include <cmath>
 #include <cstdint>
 
@@ -17,10 +18,10 @@
 
 namespace fdx {
 
-constexpr int kMostTop = 32, kMostParts = 64;
+constexpr int kMostTop = 32, kMostParts = 64, kFound = 192;
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4))); // rows start at any multiple of four bytes
-constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
 
 struct ScoreParams {
     const float* x;
@@ -32,31 +33,26 @@ struct ScoreParams {
     int* error_flag;
     uint64_t* part_keys; // [row][part][top]
     f32x4* part_sums;    // [row][part]: m, Z, W
-    int parts, part_len; // part_len: logits of a part, a multiple of 1024
+    int parts, part_len, chunk; // logits of a part, and of a chunk: multiples of what the workgroup's threads load at once
 };
 
-// Order of the likeliest tokens: descending logit (NaN as -infinity), then ascending id.  Larger keys come first, 0 is no token.
-__device__ __forceinline__ uint64_t score_key(float x, int id)
+// Order of the likeliest tokens: descending logit, then ascending id.  Larger keys come first, 0 is no token.
+__device__ __forceinline__ uint32_t score_bits(float x)
 {
-    uint32_t b = __builtin_bit_cast(uint32_t, x == 0.f ? 0.f : x); // -0 and +0 are equal logits
-    b = b & 0x80000000u ? ~b : b | 0x80000000u;
-    return (uint64_t)b << 32 | (uint32_t)~id;
+    const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.f); // -0 and +0 are equal logits
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-__device__ __forceinline__ float key_score(uint64_t key)
-{
-    const uint32_t b = (uint32_t)(key >> 32);
-    return __builtin_bit_cast(float, b & 0x80000000u ? b & 0x7fffffffu : ~b);
-}
+__device__ __forceinline__ float bits_score(uint32_t b) { return __builtin_bit_cast(float, b & 0x80000000u ? b & 0x7fffffffu : ~b); }
 
 struct Sums {
-    float m, z, w;
+    float m, z, w; // w in units of log2
 };
 __device__ __forceinline__ void add_sums(Sums& a, float m, float z, float w)
 {
     const float top = fmaxf(a.m, m), use = top == -INFINITY ? 0.f : top;
     // a sum without a finite logit has z = w = 0, and its distance is taken as finite so that the products are 0
-    const float da = fmaxf(a.m - use, -1e30f), db = fmaxf(m - use, -1e30f);
-    const float fa = __builtin_amdgcn_exp2f(da * kLog2e), fb = __builtin_amdgcn_exp2f(db * kLog2e);
+    const float da = fmaxf((a.m - use) * kLog2e, -1e30f), db = fmaxf((m - use) * kLog2e, -1e30f);
+    const float fa = __builtin_amdgcn_exp2f(da), fb = __builtin_amdgcn_exp2f(db);
     a.w = fa * (a.w + a.z * da) + fb * (w + z * db);
     a.z = fa * a.z + fb * z;
     a.m = top;
@@ -68,12 +64,24 @@ __device__ __forceinline__ void wave_lds_fence()
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
+__device__ __forceinline__ uint64_t wave_max_key(uint64_t v)
+{
+    for (int w = 32; w > 0; w >>= 1) {
+        const uint32_t lo = __shfl_xor((int)(uint32_t)v, w, 64), hi = __shfl_xor((int)(v >> 32), w, 64);
+        const uint64_t o = (uint64_t)hi << 32 | lo;
+        v = o > v ? o : v;
+    }
+    return v;
+}
+__device__ __forceinline__ uint64_t uniform_key(uint64_t v)
+{
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)v);
+}
 
 // `lists` sorted lists of `top` keys, one behind the other in `from`, become one at the returned place (`from` or `to`, both in LDS)
 __device__ __forceinline__ uint64_t* join_lists(uint64_t* from, uint64_t* to, int lists, int top)
 {
     while (lists > 1) {
-        const int left = (lists + 1) / 2;
         __syncthreads();
         for (int i = threadIdx.x; i < lists * top; i += 256) {
             const int list = i / top, place = i - list * top, other = list ^ 1;
@@ -92,7 +100,7 @@ __device__ __forceinline__ uint64_t* join_lists(uint64_t* from, uint64_t* to, in
         uint64_t* t = from;
         from = to;
         to = t;
-        lists = left;
+        lists = (lists + 1) / 2;
     }
     __syncthreads();
     return from;
@@ -102,12 +110,29 @@ __device__ __forceinline__ uint64_t* join_lists(uint64_t* from, uint64_t* to, in
 __device__ __forceinline__ void score_results(const ScoreParams& p, int64_t row, const Sums& s, const uint64_t* list)
 {
     const float m = s.m == -INFINITY ? 0.f : s.m;
-    const float lz = s.z == 0.f ? 0.f : logf(s.z); // NaN where the row holds one, or an infinity
+    const float lz = s.z == 0.f ? 0.f : __log2f(s.z); // NaN where the row holds one, or an infinity
+    auto logprob = [&](float x) { return (x - m) - lz * kLn2; };
     const int tid = threadIdx.x;
     if (tid < p.top) {
-        const uint64_t key = list[tid];
-        p.top_ids[row * p.top + tid] = (int)~(uint32_t)key;
-        p.top_logprobs[row * p.top + tid] = (key_score(key) - m) - lz;
+        uint64_t key = list[tid];
+        int id = (int)~(uint32_t)key;
+        float x = bits_score((uint32_t)(key >> 32));
+        if (key == 0) { // the place of a token that is ruled out: of the ids that are not listed, the lowest come first
+            int listed = 0;
+            while (listed < tid && list[listed] != 0)
+                ++listed;
+            int left = tid - listed;
+            for (id = 0;; ++id) {
+                bool in = false;
+                for (int i = 0; i < listed; ++i)
+                    in = in || (int)~(uint32_t)list[i] == id;
+                if (!in && left-- == 0)
+                    break;
+            }
+            x = -INFINITY;
+        }
+        p.top_ids[row * p.top + tid] = id;
+        p.top_logprobs[row * p.top + tid] = logprob(x);
     }
     if (tid == 64 && p.ids) {
         const int id = p.ids[row];
@@ -117,139 +142,152 @@ __device__ __forceinline__ void score_results(const ScoreParams& p, int64_t row,
             if (p.error_flag)
                 *p.error_flag = 1;
         } else if (id >= 0) {
-            r = (p.x[row * p.ld + id] - m) - lz;
+            r = logprob(p.x[row * p.ld + id]);
         }
         p.logprobs[row] = r;
     }
     if (tid == 128 && p.entropy)
-        p.entropy[row] = s.z == 0.f ? 0.f : lz - s.w / s.z;
+        p.entropy[row] = s.z == 0.f ? 0.f : (lz - s.w / s.z) * kLn2;
 }
 
 template <int E, bool TOP>
 __global__ __launch_bounds__(256) void token_scores_kernel(ScoreParams p)
 {
-    extern __shared__ __attribute__((aligned(16))) uint64_t lds[]; // a wave: two lists, the chunk's candidates
+    __shared__ __attribute__((aligned(16))) uint64_t lists[TOP ? 8 * kMostTop : 1]; // a wave: its list and a spare one
+    __shared__ __attribute__((aligned(16))) uint64_t found_by[TOP ? 4 : 1][TOP ? kFound : 1];
     __shared__ Sums met[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t row = blockIdx.x / p.parts;
     const int part = blockIdx.x % p.parts;
     const int first = part * p.part_len, last = p.vocab - first < p.part_len ? p.vocab : first + p.part_len;
     const float* x = p.x + row * p.ld;
-    uint64_t* list = lds + wave * 2 * p.top;
-    uint64_t* spare = list + p.top;
-    uint64_t* found = lds + 8 * p.top + wave * 4 * E * p.top;
-    uint64_t worst = 0; // of a full list
+    uint64_t* list = lists + wave * 2 * kMostTop;
+    uint64_t* spare = list + kMostTop;
+    uint64_t* found = found_by[TOP ? wave : 0];
+    uint32_t worst = 0; // logit of a full list's last token
     if (TOP && lane < p.top)
         list[lane] = 0;
     Sums s { -INFINITY, 0.f, 0.f };
-    for (int c0 = first; c0 < last; c0 += 1024 * E) {
+    for (int c0 = first; c0 < last; c0 += p.chunk) {
+        const int end = last - c0 < p.chunk ? last : c0 + p.chunk;
         f32x4 v[E];
 #pragma unroll
         for (int j = 0; j < E; ++j) {
             const int at = c0 + (j * 256 + tid) * 4;
             v[j] = f32x4 { -INFINITY, -INFINITY, -INFINITY, -INFINITY };
-            if (at + 3 < last) {
-                v[j] = *reinterpret_cast<const f32x4_any*>(x + at);
-            } else {
+            if (c0 + j * 256 * 4 < end) { // the same for the workgroup
+                if (at + 3 < end) {
+                    v[j] = *reinterpret_cast<const f32x4_any*>(x + at);
+                } else {
 #pragma unroll
-                for (int e = 0; e < 3; ++e)
-                    if (at + e < last)
-                        v[j][e] = x[at + e];
+                    for (int e = 0; e < 3; ++e)
+                        if (at + e < end)
+                            v[j][e] = x[at + e];
+                }
             }
         }
         float best = -INFINITY;
-        int where = 0x7fffffff;
 #pragma unroll
         for (int j = 0; j < E; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (TOP) {
-                    const int at = c0 + (j * 256 + tid) * 4 + e;
-                    where = v[j][e] > best ? at : where;
-                }
-                best = fmaxf(best, v[j][e]);
-            }
+            if (c0 + j * 256 * 4 < end)
+                best = fmaxf(fmaxf(fmaxf(best, v[j][0]), fmaxf(v[j][1], v[j][2])), v[j][3]);
         const float m = wave_all<true>(best), use = m == -INFINITY ? 0.f : m;
-        float z = 0.f, w = 0.f;
+        float z[2] = { 0.f, 0.f }, w[2] = { 0.f, 0.f };
 #pragma unroll
         for (int j = 0; j < E; ++j)
+            if (c0 + j * 256 * 4 < end) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float d = fmaxf(v[j][e] - use, -1e30f); // finite, so that 0 times it is 0
-                const float f = __builtin_amdgcn_exp2f((v[j][e] - use) * kLog2e);
-                z += f;
-                w = fmaf(f, d, w);
+                for (int e = 0; e < 4; ++e) { // finite, so that 0 times it is 0; NaN stays NaN
+                    const float t = __builtin_elementwise_maximum((v[j][e] - use) * kLog2e, -1e30f), f = __builtin_amdgcn_exp2f(t);
+                    z[e & 1] += f;
+                    w[e & 1] = fmaf(f, t, w[e & 1]);
+                }
             }
-        add_sums(s, m, wave_all<false>(z), wave_all<false>(w));
+        add_sums(s, m, wave_all<false>(z[0] + z[1]), wave_all<false>(w[0] + w[1]));
         if constexpr (TOP) {
-            // a lane of nothing but -infinity and NaN: its first token that there is
-            if (where == 0x7fffffff && c0 + tid * 4 < last)
-                where = c0 + tid * 4;
-            const uint64_t mine = where == 0x7fffffff ? 0 : score_key(best, where);
-            int better = 0;
-#pragma unroll 8
-            for (int i = 0; i < 64; ++i) {
-                const uint64_t o = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(mine >> 32), i) << 32
-                    | (uint32_t)__builtin_amdgcn_readlane((int)mine, i);
-                better += o > mine;
-            }
-            const uint64_t is_cut = __ballot(better == p.top - 1 && mine != 0);
-            uint64_t cut = worst + 1;
-            if (is_cut) {
-                const int l = __builtin_ctzll(is_cut);
-                const uint64_t o = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(mine >> 32), l) << 32
-                    | (uint32_t)__builtin_amdgcn_readlane((int)mine, l);
-                cut = o > cut ? o : cut;
-            }
-            const float cut_score = cut >> 32 ? key_score(cut) : -INFINITY; // no token below it is better
-            int count = 0;
-#pragma unroll
-            for (int j = 0; j < E; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float score = fmaxf(v[j][e], -INFINITY); // NaN as -infinity
-                    if (__any(score >= cut_score)) {
-                        const int at = c0 + (j * 256 + tid) * 4 + e;
-                        const uint64_t key = at < last ? score_key(score, at) : 0;
-                        const uint64_t in = __ballot(key >= cut && key != 0);
-                        if (key >= cut && key != 0)
-                            found[count + __builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in, 0))] = key;
-                        count += __builtin_popcountll(in);
+            const uint32_t mine = best > -INFINITY ? score_bits(best) : 0;
+            if (__ballot(mine > worst)) {
+                uint32_t cut = worst + 1; // equal logits: those of lower ids are in the list already
+                if (worst == 0) {
+                    cut = 0;
+                    for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
+                        const int pass = __builtin_popcountll(__ballot(mine >= (cut | bit)));
+                        cut = pass >= p.top ? cut | bit : cut;
+                        if (pass >= p.top && pass <= p.top + 4)
+                            break;
                     }
                 }
-            if (count) {
-                wave_lds_fence();
-                for (int i = lane; i < p.top; i += 64)
-                    spare[i] = 0;
-                wave_lds_fence();
-                for (int i = lane; i < p.top + count; i += 64) {
-                    const uint64_t key = i < p.top ? list[i] : found[i - p.top];
-                    int place = 0;
-                    for (int k = 0; k < p.top; ++k)
-                        place += list[k] > key;
-                    for (int k = 0; k < count; ++k)
-                        place += found[k] > key;
-                    if (key != 0 && place < p.top)
-                        spare[place] = key;
+                const float cut_score = bits_score(cut > 0x00800000u ? cut : 0x00800000u); // no less than -FLT_MAX
+                int count = 0;
+#pragma unroll
+                for (int j = 0; j < E; ++j)
+                    if (c0 + j * 256 * 4 < end) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint64_t in = __ballot(v[j][e] >= cut_score);
+                            if (in) {
+                                const int at = count + __builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in, 0));
+                                if (v[j][e] >= cut_score && at < kFound)
+                                    found[at] = (uint64_t)score_bits(v[j][e]) << 32 | (uint32_t)~(c0 + (j * 256 + tid) * 4 + e);
+                                count += __builtin_popcountll(in);
+                            }
+                        }
+                    }
+                if (count > kFound) { // the best ones, one at a time
+                    uint64_t before = ~(uint64_t)0;
+                    count = 0;
+                    while (count < p.top) {
+                        uint64_t most = 0;
+#pragma unroll
+                        for (int j = 0; j < E; ++j)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const uint64_t key = (uint64_t)score_bits(v[j][e]) << 32 | (uint32_t)~(c0 + (j * 256 + tid) * 4 + e);
+                                most = v[j][e] >= cut_score && key < before && key > most ? key : most;
+                            }
+                        before = uniform_key(wave_max_key(most));
+                        if (before == 0)
+                            break;
+                        if (lane == 0)
+                            found[count] = before;
+                        ++count;
+                    }
                 }
-                wave_lds_fence();
-                uint64_t* t = list;
-                list = spare;
-                spare = t;
-                worst = list[p.top - 1];
-                worst = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(worst >> 32)) << 32
-                    | (uint32_t)__builtin_amdgcn_readfirstlane((int)worst);
+                if (count > 0) {
+                    wave_lds_fence();
+                    if (lane < p.top)
+                        spare[lane] = 0;
+                    wave_lds_fence();
+                    for (int i = lane; i < p.top + count; i += 64) {
+                        const uint64_t key = i < p.top ? list[i] : found[i - p.top];
+                        int place = 0;
+#pragma unroll 4
+                        for (int k = 0; k < p.top; ++k)
+                            place += list[k] > key;
+#pragma unroll 4
+                        for (int k = 0; k < count; ++k)
+                            place += found[k] > key;
+                        if (key != 0 && place < p.top)
+                            spare[place] = key;
+                    }
+                    wave_lds_fence();
+                    uint64_t* t = list;
+                    list = spare;
+                    spare = t;
+                    worst = (uint32_t)(uniform_key(list[p.top - 1]) >> 32);
+                }
             }
         }
     }
     if (lane == 0)
         met[wave] = s;
-    uint64_t* all = lds + 8 * p.top;
+    const uint64_t* all = nullptr;
     if constexpr (TOP) {
-        __syncthreads(); // candidates are done with
+        uint64_t* flat = found_by[0]; // candidates are done with
+        __syncthreads();
         if (lane < p.top)
-            all[wave * p.top + lane] = list[lane];
-        all = join_lists(all, all + 4 * p.top, 4, p.top);
+            flat[wave * p.top + lane] = list[lane];
+        all = join_lists(flat, flat + 4 * p.top, 4, p.top);
     } else {
         __syncthreads();
     }
@@ -269,32 +307,38 @@ __global__ __launch_bounds__(256) void token_scores_kernel(ScoreParams p)
 
 __global__ __launch_bounds__(256) void token_scores_join_kernel(ScoreParams p)
 {
-    extern __shared__ __attribute__((aligned(16))) uint64_t lds[]; // lists of all parts, twice
+    __shared__ uint64_t lds[2 * kMostParts * kMostTop];
     const int64_t row = blockIdx.x;
+    const int lane = threadIdx.x & 63;
+    f32x4 o = { -INFINITY, 0.f, 0.f, 0.f }; // a lane a part
+    if (lane < p.parts)
+        o = p.part_sums[row * p.parts + lane];
     for (int i = threadIdx.x; i < p.parts * p.top; i += 256)
         lds[i] = p.part_keys[row * p.parts * p.top + i];
-    Sums s { -INFINITY, 0.f, 0.f };
-    for (int i = 0; i < p.parts; ++i) {
-        const f32x4 o = p.part_sums[row * p.parts + i];
-        add_sums(s, o[0], o[1], o[2]);
-    }
+    Sums s { wave_all<true>(o[0]), 0.f, 0.f };
+    const float d = fmaxf((o[0] - (s.m == -INFINITY ? 0.f : s.m)) * kLog2e, -1e30f), f = __builtin_amdgcn_exp2f(d);
+    s.z = wave_all<false>(f * o[1]);
+    s.w = wave_all<false>(f * (o[2] + o[1] * d));
     const uint64_t* list = join_lists(lds, lds + p.parts * p.top, p.parts, p.top);
     score_results(p, row, s, list);
 }
 
-// Rows are cut in parts while there are fewer workgroups than the GPU takes at once.
+// Rows are cut in parts of 4096 logits or more while that makes no more workgroups than two for each CU.
 struct ScorePlan {
-    int parts, part_len;
+    int parts, part_len, chunk;
     size_t keys, sums; // bytes
 };
+constexpr int kScoreE = 13;
 static ScorePlan score_plan(int64_t rows, int vocab, int top)
 {
-    int64_t parts = 1024 / rows, most = (vocab + 4095) / 4096;
-    parts = parts < 1 ? 1 : (parts > most ? most : parts);
-    parts = parts > kMostParts ? kMostParts : parts;
     ScorePlan r {};
-    r.part_len = (int)((vocab + parts * 1024 - 1) / (parts * 1024) * 1024);
+    auto thousands = [&](int64_t n, int64_t into) { return (int)((n + into * 1024 - 1) / (into * 1024) * 1024); };
+    const int64_t most = ((int64_t)vocab + 4095) / 4096;
+    int64_t parts = 512 / rows < most ? 512 / rows : most;
+    parts = parts < 1 ? 1 : (parts > kMostParts ? kMostParts : parts);
+    r.part_len = thousands(vocab, parts);
     r.parts = (vocab + r.part_len - 1) / r.part_len;
+    r.chunk = thousands(r.part_len, (r.part_len + 1024 * kScoreE - 1) / (1024 * kScoreE)); // chunks of a part are of one length
     if (r.parts > 1) {
         r.keys = ((size_t)rows * r.parts * top * sizeof(uint64_t) + 15) & ~(size_t)15;
         r.sums = (size_t)rows * r.parts * sizeof(f32x4);
@@ -306,9 +350,8 @@ template <int E>
 static void score_launch(const ScoreParams& p)
 {
     const dim3 grid((unsigned)(p.rows * p.parts));
-    const size_t lds = sizeof(uint64_t) * p.top * (8 + 16 * E);
     if (p.top > 0)
-        hipLaunchKernelGGL((token_scores_kernel<E, true>), grid, dim3(256), lds, stream(), p);
+        hipLaunchKernelGGL((token_scores_kernel<E, true>), grid, dim3(256), 0, stream(), p);
     else
         hipLaunchKernelGGL((token_scores_kernel<E, false>), grid, dim3(256), 0, stream(), p);
 }
@@ -341,14 +384,14 @@ extern "C" fdx_status fdx_token_logprobs_f32(const float* logits, int64_t ld, in
     const ScorePlan plan = score_plan(rows, vocab, top);
     char* scratch = static_cast<char*>(scratch_dev);
     const ScoreParams p { logits, ld, rows, vocab, top, ids, logprobs, entropy, top_logprobs, top_ids, error_flag_dev,
-        reinterpret_cast<uint64_t*>(scratch), reinterpret_cast<f32x4*>(scratch + plan.keys), plan.parts, plan.part_len };
+        reinterpret_cast<uint64_t*>(scratch), reinterpret_cast<f32x4*>(scratch + plan.keys), plan.parts, plan.part_len, plan.chunk };
     profile_begin();
-    if (plan.part_len <= 4096)
+    if (plan.chunk <= 4096)
         score_launch<4>(p);
     else
-        score_launch<12>(p);
+        score_launch<kScoreE>(p);
     if (plan.parts > 1)
-        hipLaunchKernelGGL(token_scores_join_kernel, dim3((unsigned)rows), dim3(256), 2 * sizeof(uint64_t) * plan.parts * top, stream(), p);
+        hipLaunchKernelGGL(token_scores_join_kernel, dim3((unsigned)rows), dim3(256), 0, stream(), p);
     profile_end("token_logprobs_f32", 5.0 * rows * vocab, 4.0 * rows * ((double)vocab + 3 + 2 * top));
     FDX_LAUNCH_CHECK();
     return FDX_OK;
