@@ -328,7 +328,9 @@ struct ScorePlan {
     int parts, part_len, chunk;
     size_t keys, sums; // bytes
 };
-constexpr int kScoreE = 13;
+// A chunk's vectors a thread: chunks cost some 300 instructions each whatever their length, registers cost waves.  2048 rows of 50 257 and 1000 of
+// 131 072 with 20 alternatives, in us: 7 vectors 107 / 118, 9 108 / 115, 13 127 / 168, 17 118 / 145.
+constexpr int kScoreE = 8;
 static ScorePlan score_plan(int64_t rows, int vocab, int top)
 {
     ScorePlan r {};
