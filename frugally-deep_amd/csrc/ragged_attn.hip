@@ -792,8 +792,10 @@ __global__ __launch_bounds__(256, 2) void ragged_packed_kernel(RaggedParams p)
 
 // ---- few query rows: keys and values pass once, straight from memory to the fp32 matrix instructions ----
 //
-// A workgroup takes sixteen of the rows that a sequence brings to one key head, over one range of its keys; its four waves take every
-// fourth block of 16 keys, each with sums of its own, and meet at the end.  Bound by memory: a lane's loads are the operands of
+// A workgroup takes the rows that a sequence brings to one key head, over one range of its keys.  Up to sixteen rows: its four waves take every
+// fourth block of 16 keys; up to thirty-two: two waves for either half of the rows take every second block, and the later one of two that load
+// the same keys finds them in the CU's cache (20 rows each of 32 sequences of 3000 keys,
+// 32 / 8 heads of 128, 231 us with fp32 pages; a workgroup for either half 291).  Waves have sums of their own, which meet at the end.  Bound by memory: a lane's loads are the operands of
 // the 16x16x4 fp32 products, nothing is staged, and a block's loads are on their way while the block before is worked on.
 //  * S^T = K Q^T: lane (c, g) of 16 x 4 loads chunks of key c, chunk i at depth 4 W i + W g (W elements are 16 bytes), and has scores of keys
 //    4 g .. 4 g + 3 of row c.
@@ -848,9 +850,10 @@ __global__ __launch_bounds__(256, 2) void ragged_few_kernel(RaggedParams p)
     if (tid == 0)
         raise_flag(p, s.cut);
     const int count = s.span.count * p.group;
-    const int r_first = blockIdx.z * 16;
-    if (r_first >= count || !s.few)
+    if (count == 0 || !s.few)
         return;
+    const bool halves = count > 16;
+    const int step = halves ? 2 : 4, slot = halves ? wave & 1 : wave, r_first = halves ? (wave >> 1) * 16 : 0; // of this wave
     int k_end = visible_keys(p, s, s.span.count - 1);
     const int64_t k_from = (int64_t)blockIdx.y * s.range;
     if (blockIdx.y > 0 && k_from >= k_end)
@@ -863,7 +866,9 @@ __global__ __launch_bounds__(256, 2) void ragged_few_kernel(RaggedParams p)
     const T* kbase = static_cast<const T*>(p.k) + (int64_t)kv_head * p.dk;
     const T* vbase = static_cast<const T*>(p.v) + (int64_t)kv_head * p.dv;
     auto look_up = [&](int blk) { // the place of key c of a block; positions behind the range repeat its last one
-        const int at = k_first + blk * 16 + c;
+        int first = k_first + blk * 16;
+        asm("" : "+s"(first)); // no register keeps a part of the sum for the next time
+        const int at = first + c;
         return key_row<KIND>(p, s, at < k_end ? at : k_end - 1);
     };
     auto fetch = [&](Block& b, int row) {
@@ -883,9 +888,9 @@ __global__ __launch_bounds__(256, 2) void ragged_few_kernel(RaggedParams p)
     };
     Block a, b;
     int row_b = 0;
-    if (wave < blocks) {
-        const int row_a = look_up(wave);
-        row_b = look_up(wave + 4);
+    if (slot < blocks) {
+        const int row_a = look_up(slot);
+        row_b = look_up(slot + step);
         fetch(a, row_a);
     }
 
@@ -1009,21 +1014,21 @@ __global__ __launch_bounds__(256, 2) void ragged_few_kernel(RaggedParams p)
                         oacc[j * VW + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.v[i][j][e], sc[i], oacc[j * VW + e], 0, 0, 0);
         }
     };
-    for (int blk = wave; blk < blocks; blk += 8) {
-        const bool more = blk + 4 < blocks;
+    for (int blk = slot; blk < blocks; blk += 2 * step) {
+        const bool more = blk + step < blocks;
         int row_a = 0;
         if (more) {
             fetch(b, row_b);
-            row_a = look_up(blk + 8);
+            row_a = look_up(blk + 2 * step);
         }
         work(a, blk);
         if (!more)
             break;
-        if (blk + 8 < blocks) {
+        if (blk + 2 * step < blocks) {
             fetch(a, row_a);
-            row_b = look_up(blk + 12);
+            row_b = look_up(blk + 3 * step);
         }
-        work(b, blk + 4);
+        work(b, blk + step);
     }
     raise_flag(p, missing);
 
@@ -1042,68 +1047,73 @@ __global__ __launch_bounds__(256, 2) void ragged_few_kernel(RaggedParams p)
             for (int e = 0; e < VW; ++e)
                 meet_o[wave][c][16 * VW * j + VW * (4 * g + i) + e] = oacc[j * VW + e][i];
     __syncthreads();
-    // found out anew, so that no registers keep these through the loop
+    // found out anew, so that no register keeps it through the loop
     const int lane2 = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0)), tid2 = wave * 64 + lane2;
-    const int at = tid2 >> 4, d0 = (tid2 & 15) * DL, mine_row = r_first + at;
-    const float top = fmaxf(fmaxf(meet_m[0][at], meet_m[1][at]), fmaxf(meet_m[2][at], meet_m[3][at]));
-    const float m = top == -INFINITY ? 0.f : top;
-    float l = 0.f, o[DL];
-#pragma unroll
-    for (int e = 0; e < DL; ++e)
-        o[e] = 0.f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        const float f = __builtin_amdgcn_exp2f(meet_m[w][at] - m);
-        l += f * meet_l[w][at];
+    const int at = tid2 >> 4, d0 = (tid2 & 15) * DL;
+    uint32_t odd = 0; // of this wave's four rows, and of the four behind the next sixteen
+    for (int half = 0; half <= (halves ? 1 : 0); ++half) {
+        const int w_first = 2 * half, w_last = halves ? w_first + 1 : 3; // the waves that have these rows
+        float top = -INFINITY;
+        for (int w = w_first; w <= w_last; ++w)
+            top = fmaxf(top, meet_m[w][at]);
+        const float m = top == -INFINITY ? 0.f : top;
+        float l = 0.f, o[DL];
 #pragma unroll
         for (int e = 0; e < DL; ++e)
-            o[e] += f * meet_o[w][at][d0 + e];
-    }
-    float size = l;
+            o[e] = 0.f;
+        for (int w = w_first; w <= w_last; ++w) {
+            const float f = __builtin_amdgcn_exp2f(meet_m[w][at] - m);
+            l += f * meet_l[w][at];
 #pragma unroll
-    for (int e = 0; e < DL; ++e)
-        size += fabsf(o[e]);
-    const bool there = mine_row < count;
-    const int token = quotient(there ? mine_row : 0, p.by_group), head = kv_head * p.group + (there ? mine_row : 0) - token * p.group;
-    const int sees = visible_keys(p, s, token);
-    const bool in_parts = sees > s.range, mine = there && (in_parts ? k_first < sees : blockIdx.y == 0);
-    // rows whose sums are not finite, or empty though there are keys; a row's 16 threads agree
-    const uint64_t bad = __ballot(mine && (!(size < INFINITY) || (l == 0.f && k_first < sees)));
-    if (mine && (bad >> (lane2 & 48) & 0xffff) == 0) {
-        const float f = l > 0.f ? 1.f / l : 0.f; // no key: zeros
-        float* to = p.out + (int64_t)(s.span.first + token) * p.ldo + (int64_t)head * p.dv;
-        if (in_parts) {
-            const int64_t id = part_row(p, s, token, head);
-            to = p.few.out(blockIdx.y, id, p.dv);
-            float* size_at = p.few.size(blockIdx.y, id, p.dv);
-            if ((tid2 & 15) == 0) {
-                size_at[0] = top;
-                size_at[1] = l;
+            for (int e = 0; e < DL; ++e)
+                o[e] += f * meet_o[w][at][d0 + e];
+        }
+        float size = l;
+#pragma unroll
+        for (int e = 0; e < DL; ++e)
+            size += fabsf(o[e]);
+        const int r = 16 * half + at;
+        const bool there = r < count;
+        const int token = quotient(there ? r : 0, p.by_group), head = kv_head * p.group + (there ? r : 0) - token * p.group;
+        const int sees = visible_keys(p, s, token);
+        const bool in_parts = sees > s.range, mine = there && (in_parts ? k_first < sees : blockIdx.y == 0);
+        // rows whose sums are not finite, or empty though there are keys; a row's 16 threads agree
+        const uint64_t bad = __ballot(mine && (!(size < INFINITY) || (l == 0.f && k_first < sees)));
+        if (mine && (bad >> (lane2 & 48) & 0xffff) == 0) {
+            const float f = l > 0.f ? 1.f / l : 0.f; // no key: zeros
+            float* to = p.out + (int64_t)(s.span.first + token) * p.ldo + (int64_t)head * p.dv;
+            if (in_parts) {
+                const int64_t id = part_row(p, s, token, head);
+                to = p.few.out(blockIdx.y, id, p.dv);
+                float* size_at = p.few.size(blockIdx.y, id, p.dv);
+                if ((tid2 & 15) == 0) {
+                    size_at[0] = top;
+                    size_at[1] = l;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < DL; e += 4) {
+                if (WIDE) {
+                    if (d0 + e < p.dv)
+                        *reinterpret_cast<f32x4*>(to + d0 + e) = f32x4 { o[e] * f, o[e + 1] * f, o[e + 2] * f, o[e + 3] * f };
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (d0 + e + i < p.dv)
+                            to[d0 + e + i] = o[e + i] * f;
+                }
             }
         }
 #pragma unroll
-        for (int e = 0; e < DL; e += 4) {
-            if (WIDE) {
-                if (d0 + e < p.dv)
-                    *reinterpret_cast<f32x4*>(to + d0 + e) = f32x4 { o[e] * f, o[e + 1] * f, o[e + 2] * f, o[e + 3] * f };
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (d0 + e + i < p.dv)
-                        to[d0 + e + i] = o[e + i] * f;
-            }
-        }
+        for (int k = 0; k < 4; ++k)
+            if (bad >> (16 * k) & 0xffff)
+                odd |= 1u << (16 * half + 4 * wave + k);
     }
-    uint32_t odd = 0; // of this wave's four rows
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-        if (bad >> (16 * k) & 0xffff)
-            odd |= 1u << (4 * wave + k);
     if (__builtin_expect(odd == 0, 1))
         return;
 #pragma clang loop unroll(disable)
     while (odd) {
-        const int r1 = r_first + __builtin_ctz(odd);
+        const int r1 = __builtin_ctz(odd);
         odd &= odd - 1;
         const int t1 = quotient(r1, p.by_group);
         store_plain_row<KIND>(p, s, t1, kv_head * p.group + r1 - t1 * p.group, kv_head, blockIdx.y, lane2);
@@ -1198,8 +1208,13 @@ static RaggedPlan paged_plan(int tokens, int max_new, int heads, const fdx_kv_pa
     r.few_rows = most <= 16 ? 16 : 32;
     if (group <= r.few_rows) {
         const int64_t items = (int64_t)c->n_seqs * c->kv_heads;
-        const int64_t keys = c->max_len * items / 4096;
-        r.few_ranges = ranges_of(c->max_len, keys < 512 ? 512 : keys, &r.few_keys);
+        // Ranges enough for some 4096 workgroups when every sequence is as long as the longest, which leaves those of shorter ones to fill
+        // gaps; 256 keys or more, and 64 ranges or fewer, which one pass of ragged_join_kernel takes.  us with at least 128 / 192 / 256 / 384 / 512
+        // keys, fp32: one sequence of 8000, 32 / 8 heads of 128, 28.4 / 29.9 / 26.0 / 28.0 / 31.7; 16 of 1000, 12 heads of 64, 28.1 / 29.2 / 26.4 / 28.9 /
+        // 28.9; one of 2000, 12.9 / 13.0 / 13.9 / 16.4 / 18.8; four of 32 000, 8 / 1 heads of 128, 60.9 / 56.3 / 46.7 / 48.0 / 41.0.
+        int64_t keys = c->max_len * items / 4096;
+        keys = keys < 256 ? 256 : keys;
+        r.few_ranges = ranges_of(c->max_len, keys < c->max_len / 64 ? c->max_len / 64 : keys, &r.few_keys);
         r.few_part = items * (most < r.few_rows ? most : r.few_rows);
     }
     if (r.few_ranges == 0)
@@ -1255,7 +1270,7 @@ static void ragged_launch(RaggedParams p, const RaggedPlan& plan)
             return;
         }
     } else if (plan.few_ranges > 0) {
-        const dim3 grid((unsigned)(p.n_seqs * p.kv_heads), (unsigned)plan.few_ranges, (unsigned)(plan.few_rows / 16));
+        const dim3 grid((unsigned)(p.n_seqs * p.kv_heads), (unsigned)plan.few_ranges);
         hipLaunchKernelGGL((ragged_few_kernel<D, KIND, WIDE>), grid, block, 0, stream(), p);
     }
     if (plan.tiles > 0) {
