@@ -1222,7 +1222,10 @@ static RaggedPlan paged_plan(int tokens, int max_new, int heads, const fdx_kv_pa
     if (most > r.few_rows) {
         r.tiles = tile_numbers(tokens, c->n_seqs, group, 128) * c->kv_heads;
         const int64_t full = ((int64_t)tokens * group + 127) / 128 * c->kv_heads;
-        int64_t keys = c->max_len * full / 1024;
+        // Ranges while there are fewer tiles than the 512 workgroups that the GPU takes at once, of 512 to 4096 keys.  us with at most 512 / 1024 /
+        // 2048 / 4096 keys, fp32 pages: 128 new tokens at the end of 8000, 32 / 8 heads of 128 (32 tiles), 91 / 128 / 174 / 316; 512 (128 tiles) 310 / 289 /
+        // 279 / 398; twice 2000 of 3000, 16 / 4 heads of 64 (500 tiles) 206 / 197 / 190 / 166; four times 1000 of 4000 (1000 tiles) 1087 / 982 / 957 / 887.
+        int64_t keys = full < 512 ? c->max_len / (512 / full) : c->max_len;
         keys = keys < 512 ? 512 : (keys > 4096 ? 4096 : keys);
         r.tile_ranges = ranges_of(c->max_len, keys < c->max_len / 16 ? c->max_len / 16 : keys, &r.tile_keys);
         r.tile_part = (int64_t)tokens * heads;
