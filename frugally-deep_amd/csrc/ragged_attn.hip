@@ -94,31 +94,55 @@ __device__ __forceinline__ QueryRow row_of(const RaggedParams& p, const Sequence
 
 constexpr float kShift = 10.f; // exponentials are 2^kShift times the probability's numerator
 
+// where a workgroup stands in its launch
+struct Place {
+    unsigned x, y, nx;
+};
+
+template <int D, int KIND>
+struct TileSizes {
+    static constexpr int KT = 4096 / D, N = D / 16; // keys of a tile; threads that fetch a key
+    static constexpr int KBLK = KT * 16 + 32, VROW = D * 2 + 32; // bytes of a block of keys, of a row of values, offset against each other
+    static constexpr int kKeys = 2 * (D / 8) * KBLK, kValues = 2 * KT * VROW; // bytes of a tile
+    static constexpr int kAhead = 512; // places of two halves of as many positions are looked up ahead, all threads at once
+    static constexpr int kPlaces = KIND == kPackedF32 ? 1 : 2 * kAhead;
+};
+// its LDS: two tiles, apart so that the compiler sees that what is written is not what is read
+struct TileLds {
+    unsigned char *ks0, *ks1, *vs0, *vs1;
+    Spread (*spread)[4];
+    int *rows_of, *some_absent;
+};
+#define FDX_TILE_LDS(D, KIND, lds)                                                                                          \
+    __shared__ __attribute__((aligned(16))) unsigned char lds##_ks0[TileSizes<D, KIND>::kKeys], lds##_ks1[TileSizes<D, KIND>::kKeys]; \
+    __shared__ __attribute__((aligned(16))) unsigned char lds##_vs0[TileSizes<D, KIND>::kValues], lds##_vs1[TileSizes<D, KIND>::kValues]; \
+    __shared__ Spread lds##_spread[2][4];                                                                                   \
+    __shared__ int lds##_rows_of[TileSizes<D, KIND>::kPlaces];                                                              \
+    __shared__ int lds##_absent;                                                                                            \
+    const TileLds lds { lds##_ks0, lds##_ks1, lds##_vs0, lds##_vs1, lds##_spread, lds##_rows_of, &lds##_absent }
+
 template <int D, int KIND, bool EXACT>
-__global__ __launch_bounds__(256, 2) void ragged_tile_kernel(RaggedParams p)
+__device__ __forceinline__ void tile_body(const RaggedParams& p, const Place& place_in, const TileLds& lds)
 {
     typedef typename KvElement<KIND>::type T;
-    constexpr int KT = 4096 / D, HALVES = KT / 32, N = D / 16; // keys of a tile, in accumulators of 32; threads that fetch a key
-    constexpr int KB = D / 8, STEPS = D / 16, DB = D / 32;
-    constexpr int KBLK = KT * 16 + 32, VROW = D * 2 + 32; // bytes of a block of keys, of a row of values, offset against each other
+    typedef TileSizes<D, KIND> S;
+    constexpr int KT = S::KT, HALVES = KT / 32, N = S::N, KB = D / 8, STEPS = D / 16, DB = D / 32, KBLK = S::KBLK, VROW = S::VROW, kAhead = S::kAhead;
     constexpr bool kPaged = KIND != kPackedF32;
-    __shared__ __attribute__((aligned(16))) unsigned char ks0[2 * KB * KBLK], ks1[2 * KB * KBLK];
-    __shared__ __attribute__((aligned(16))) unsigned char vs0[2 * KT * VROW], vs1[2 * KT * VROW];
-    __shared__ Spread spread[2][4];
-    constexpr int kAhead = 512; // places of two halves of as many positions are looked up ahead, all threads at once
-    __shared__ int rows_of[kPaged ? 2 * kAhead : 1];
-    __shared__ int some_absent;
+    unsigned char *ks0 = lds.ks0, *ks1 = lds.ks1, *vs0 = lds.vs0, *vs1 = lds.vs1;
+    Spread (*spread)[4] = lds.spread;
+    int* rows_of = lds.rows_of;
+    int& some_absent = *lds.some_absent;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 31, half = lane >> 5;
-    if (p.error_flag && blockIdx.x == 0 && blockIdx.y == 0)
+    if (p.error_flag && place_in.x == 0 && place_in.y == 0)
         for (int i = tid; i < p.n_seqs; i += 256)
             raise_flag(p, !packed_start_ok(p.starts, i, p.tokens));
     // key heads next to each other: consecutive workgroups go to the eight XCDs in turn, so that an XCD's cache holds few heads'
     // keys; later tiles of a sequence, which see more keys, first
-    const int kv_head = blockIdx.x % p.kv_heads;
-    const int64_t number = blockIdx.x / p.kv_heads;
+    const int kv_head = place_in.x % p.kv_heads;
+    const int64_t number = place_in.x / p.kv_heads;
     const Tile tile = p.causal && p.n_seqs <= 64 ? late_tile_wave(p.starts, p.n_seqs, p.tokens, p.group, 128, number)
-                                                 : find_tile_wave(p.starts, p.n_seqs, p.tokens, p.group, 128, gridDim.x / p.kv_heads - 1 - number);
+                                                 : find_tile_wave(p.starts, p.n_seqs, p.tokens, p.group, 128, place_in.nx / p.kv_heads - 1 - number);
     if (tile.seq < 0)
         return;
     const Sequence s = sequence_of<KIND>(p, tile.seq, tile.span);
@@ -132,8 +156,8 @@ __global__ __launch_bounds__(256, 2) void ragged_tile_kernel(RaggedParams p)
 
     const int r_last = r_first + 128 < count ? r_first + 127 : count - 1;
     int k_end = visible_keys(p, s, quotient(r_last, p.by_group)); // of the workgroup's last row
-    const int64_t k_from = (int64_t)blockIdx.y * s.range;
-    if (blockIdx.y > 0 && k_from >= k_end)
+    const int64_t k_from = (int64_t)place_in.y * s.range;
+    if (place_in.y > 0 && k_from >= k_end)
         return;
     const int k_first = (int)k_from;
     if (k_end - k_first > s.range)
@@ -443,13 +467,13 @@ __global__ __launch_bounds__(256, 2) void ragged_tile_kernel(RaggedParams p)
     const uint64_t odd_lanes = __ballot(q_ok && !(size < INFINITY));
     uint32_t odd = (uint32_t)odd_lanes | (uint32_t)(odd_lanes >> 32);
     const bool in_parts = visible > s.range;
-    if (q_ok && !(odd >> c & 1) && (in_parts ? k_first < visible : blockIdx.y == 0)) {
+    if (q_ok && !(odd >> c & 1) && (in_parts ? k_first < visible : place_in.y == 0)) {
         const float f = l_run > 0.f ? sv.down / l_run : 0.f; // no key: zeros
         float* to = p.out + q_row * p.ldo + (int64_t)head * p.dv;
         if (in_parts) {
             const int64_t id = part_row(p, s, at_row.token, head);
-            to = p.tile.out(blockIdx.y, id, p.dv);
-            float* at = p.tile.size(blockIdx.y, id, p.dv);
+            to = p.tile.out(place_in.y, id, p.dv);
+            float* at = p.tile.size(place_in.y, id, p.dv);
             if (half == 0) {
                 at[0] = m_run - kShift;
                 at[1] = l_run;
@@ -478,8 +502,15 @@ __global__ __launch_bounds__(256, 2) void ragged_tile_kernel(RaggedParams p)
         const int r1 = r_first + wave * 32 + __builtin_ctz(odd);
         odd &= odd - 1;
         const int t1 = quotient(r1, p.by_group), h1 = kv_head * p.group + r1 - t1 * p.group;
-        store_plain_row<KIND>(p, s, t1, h1, kv_head, blockIdx.y, lane);
+        store_plain_row<KIND>(p, s, t1, h1, kv_head, place_in.y, lane);
     }
+}
+
+template <int D, int KIND, bool EXACT>
+__global__ __launch_bounds__(256, 2) void ragged_tile_kernel(RaggedParams p)
+{
+    FDX_TILE_LDS(D, KIND, lds);
+    tile_body<D, KIND, EXACT>(p, Place { blockIdx.x, blockIdx.y, gridDim.x }, lds);
 }
 
 // ---- packed prompts: keys and values split once, in tiles as the products read them ----
@@ -825,7 +856,7 @@ __device__ __forceinline__ auto load_chunk(const T* row, int d, int depth)
 }
 
 template <int D, int KIND, bool WIDE>
-__global__ __launch_bounds__(256, 2) void ragged_few_kernel(RaggedParams p)
+__device__ __forceinline__ void few_body(const RaggedParams& p, const Place& place_in, float* meet_01, float* meet_23, float* meet_ml)
 {
     typedef typename KvElement<KIND>::type T;
     constexpr int W = 16 / (int)sizeof(T), NK = D / (4 * W); // elements of a key chunk, chunks of a lane
@@ -838,12 +869,13 @@ __global__ __launch_bounds__(256, 2) void ragged_few_kernel(RaggedParams p)
         vvec v[4][NV];
         int row;
     };
-    __shared__ float meet_o[4][16][D + 4];
-    __shared__ float meet_m[4][16], meet_l[4][16];
+    // [wave][row][depth] of the sums o, two waves each, and [wave][row] of m, then of l
+    float (*meet_m)[16] = reinterpret_cast<float (*)[16]>(meet_ml), (*meet_l)[16] = meet_m + 4;
+    auto meet_o = [&](int w, int row) { return (w < 2 ? meet_01 : meet_23) + ((w & 1) * 16 + row) * (D + 4); };
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 15, g = lane >> 4;
-    const int seq = blockIdx.x / p.kv_heads, kv_head = blockIdx.x % p.kv_heads;
-    if (p.error_flag && blockIdx.x == 0 && blockIdx.y == 0)
+    const int seq = place_in.x / p.kv_heads, kv_head = place_in.x % p.kv_heads;
+    if (p.error_flag && place_in.x == 0 && place_in.y == 0)
         for (int i = tid; i < p.n_seqs; i += 256)
             raise_flag(p, !packed_start_ok(p.starts, i, p.tokens));
     const Sequence s = sequence_of<KIND>(p, seq, packed_span(p.starts, seq, p.tokens));
@@ -855,8 +887,8 @@ __global__ __launch_bounds__(256, 2) void ragged_few_kernel(RaggedParams p)
     const bool halves = count > 16;
     const int step = halves ? 2 : 4, slot = halves ? wave & 1 : wave, r_first = halves ? (wave >> 1) * 16 : 0; // of this wave
     int k_end = visible_keys(p, s, s.span.count - 1);
-    const int64_t k_from = (int64_t)blockIdx.y * s.range;
-    if (blockIdx.y > 0 && k_from >= k_end)
+    const int64_t k_from = (int64_t)place_in.y * s.range;
+    if (place_in.y > 0 && k_from >= k_end)
         return;
     const int k_first = (int)k_from;
     if (k_end - k_first > s.range)
@@ -1045,7 +1077,7 @@ __global__ __launch_bounds__(256, 2) void ragged_few_kernel(RaggedParams p)
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int e = 0; e < VW; ++e)
-                meet_o[wave][c][16 * VW * j + VW * (4 * g + i) + e] = oacc[j * VW + e][i];
+                meet_o(wave, c)[16 * VW * j + VW * (4 * g + i) + e] = oacc[j * VW + e][i];
     __syncthreads();
     // found out anew, so that no register keeps it through the loop
     const int lane2 = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0)), tid2 = wave * 64 + lane2;
@@ -1066,7 +1098,7 @@ __global__ __launch_bounds__(256, 2) void ragged_few_kernel(RaggedParams p)
             l += f * meet_l[w][at];
 #pragma unroll
             for (int e = 0; e < DL; ++e)
-                o[e] += f * meet_o[w][at][d0 + e];
+                o[e] += f * meet_o(w, at)[d0 + e];
         }
         float size = l;
 #pragma unroll
@@ -1076,7 +1108,7 @@ __global__ __launch_bounds__(256, 2) void ragged_few_kernel(RaggedParams p)
         const bool there = r < count;
         const int token = quotient(there ? r : 0, p.by_group), head = kv_head * p.group + (there ? r : 0) - token * p.group;
         const int sees = visible_keys(p, s, token);
-        const bool in_parts = sees > s.range, mine = there && (in_parts ? k_first < sees : blockIdx.y == 0);
+        const bool in_parts = sees > s.range, mine = there && (in_parts ? k_first < sees : place_in.y == 0);
         // rows whose sums are not finite, or empty though there are keys; a row's 16 threads agree
         const uint64_t bad = __ballot(mine && (!(size < INFINITY) || (l == 0.f && k_first < sees)));
         if (mine && (bad >> (lane2 & 48) & 0xffff) == 0) {
@@ -1084,8 +1116,8 @@ __global__ __launch_bounds__(256, 2) void ragged_few_kernel(RaggedParams p)
             float* to = p.out + (int64_t)(s.span.first + token) * p.ldo + (int64_t)head * p.dv;
             if (in_parts) {
                 const int64_t id = part_row(p, s, token, head);
-                to = p.few.out(blockIdx.y, id, p.dv);
-                float* size_at = p.few.size(blockIdx.y, id, p.dv);
+                to = p.few.out(place_in.y, id, p.dv);
+                float* size_at = p.few.size(place_in.y, id, p.dv);
                 if ((tid2 & 15) == 0) {
                     size_at[0] = top;
                     size_at[1] = l;
@@ -1116,7 +1148,29 @@ __global__ __launch_bounds__(256, 2) void ragged_few_kernel(RaggedParams p)
         const int r1 = __builtin_ctz(odd);
         odd &= odd - 1;
         const int t1 = quotient(r1, p.by_group);
-        store_plain_row<KIND>(p, s, t1, kv_head * p.group + r1 - t1 * p.group, kv_head, blockIdx.y, lane2);
+        store_plain_row<KIND>(p, s, t1, kv_head * p.group + r1 - t1 * p.group, kv_head, place_in.y, lane2);
+    }
+}
+
+template <int D, int KIND, bool WIDE>
+__global__ __launch_bounds__(256, WIDE ? 2 : 1) void ragged_few_kernel(RaggedParams p)
+{
+    __shared__ float meet[2][2 * 16 * (D + 4)], meet_ml[2 * 4 * 16];
+    few_body<D, KIND, WIDE>(p, Place { blockIdx.x, blockIdx.y, gridDim.x }, meet[0], meet[1], meet_ml);
+}
+
+// Both in one launch: what is bound by memory runs beside what is bound by the matrix and vector units.  Tiles, which take longest, come first.
+template <int D, int KIND>
+__global__ __launch_bounds__(256, 2) void ragged_mixed_kernel(RaggedParams p, unsigned tile_x, unsigned tile_wgs, unsigned few_x)
+{
+    FDX_TILE_LDS(D, KIND, lds);
+    if (blockIdx.x < tile_wgs) {
+        tile_body<D, KIND, true>(p, Place { blockIdx.x % tile_x, blockIdx.x / tile_x, tile_x }, lds);
+    } else {
+        static_assert(2 * 16 * (D + 4) * sizeof(float) <= sizeof(lds_ks0) && 2 * 4 * 16 * sizeof(float) <= sizeof(lds_vs0), "fits into the tiles' LDS");
+        const unsigned at = blockIdx.x - tile_wgs;
+        few_body<D, KIND, true>(p, Place { at % few_x, at / few_x, few_x }, reinterpret_cast<float*>(lds.ks0), reinterpret_cast<float*>(lds.ks1),
+            reinterpret_cast<float*>(lds.vs0));
     }
 }
 
@@ -1272,12 +1326,21 @@ static void ragged_launch(RaggedParams p, const RaggedPlan& plan)
             hipLaunchKernelGGL(ragged_packed_kernel<D>, dim3((unsigned)plan.tiles), block, 0, stream(), p);
             return;
         }
-    } else if (plan.few_ranges > 0) {
-        const dim3 grid((unsigned)(p.n_seqs * p.kv_heads), (unsigned)plan.few_ranges);
-        hipLaunchKernelGGL((ragged_few_kernel<D, KIND, WIDE>), grid, block, 0, stream(), p);
     }
-    if (plan.tiles > 0) {
-        const dim3 grid((unsigned)plan.tiles, (unsigned)(plan.tile_ranges > 0 ? plan.tile_ranges : 1));
+    const unsigned tile_x = (unsigned)plan.tiles, tile_y = (unsigned)(plan.tile_ranges > 0 ? plan.tile_ranges : 1);
+    bool mixed = false;
+    if constexpr (KIND != kPackedF32) {
+        const unsigned few_x = (unsigned)(p.n_seqs * p.kv_heads);
+        const uint64_t few_wgs = (uint64_t)few_x * plan.few_ranges, tile_wgs = (uint64_t)tile_x * tile_y;
+        mixed = exact && few_wgs > 0 && tile_wgs > 0 && few_wgs + tile_wgs < (1u << 23);
+        if (mixed)
+            hipLaunchKernelGGL((ragged_mixed_kernel<D, KIND>), dim3((unsigned)(few_wgs + tile_wgs)), block, 0, stream(), p, tile_x, (unsigned)tile_wgs,
+                few_x);
+        else if (few_wgs > 0)
+            hipLaunchKernelGGL((ragged_few_kernel<D, KIND, WIDE>), dim3(few_x, (unsigned)plan.few_ranges), block, 0, stream(), p);
+    }
+    if (!mixed && plan.tiles > 0) {
+        const dim3 grid(tile_x, tile_y);
         if (exact)
             hipLaunchKernelGGL((ragged_tile_kernel<D, KIND, true>), grid, block, 0, stream(), p);
         else
