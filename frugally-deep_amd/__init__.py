@@ -608,6 +608,12 @@ def _row_starts(lengths):
     return DevBuf.from_host(np.concatenate([[0], np.cumsum(lengths)]).astype(np.int32), np.int32)
 
 
+def _rows_of(rows, **arrays):
+    for name, (a, width) in arrays.items():
+        if a.shape != (rows, width):
+            raise FdxError("%s of shape %s where %d rows of %d are expected" % (name, a.shape, rows, width))
+
+
 def _raise_if_set(flag, message):
     if flag.to_host((1,), np.int32)[0]:
         raise FdxError(message)
@@ -617,6 +623,7 @@ def mha_packed(q, k, v, lengths, heads, kv_heads, dk, dv, causal=True):
     """q [tokens,heads*dk], k [tokens,kv_heads*dk], v [tokens,kv_heads*dv]: sequences of `lengths` rows, one behind the other."""
     q, k, v = (np.ascontiguousarray(a, np.float32) for a in (q, k, v))
     tokens = q.shape[0]
+    _rows_of(tokens, q=(q, heads * dk), k=(k, kv_heads * dk), v=(v, kv_heads * dv))
     dq, dk_, dv_, starts = DevBuf.from_host(q), DevBuf.from_host(k), DevBuf.from_host(v), _row_starts(lengths)
     scratch = DevBuf(lib.fdx_mha_packed_scratch_bytes(tokens, len(lengths), heads, kv_heads, dk, dv))
     out, flag = DevBuf.from_host(np.zeros((tokens, heads * dv), np.float32)), DevBuf.from_host(np.zeros(1, np.int32), np.int32)
@@ -669,7 +676,11 @@ class PagedCache:
 def kv_append(cache, k, v, lengths):
     """Adds lengths[i] rows of k [tokens,kv_heads*dk] and v [tokens,kv_heads*dv] to sequence i of a PagedCache."""
     k, v = np.ascontiguousarray(k, np.float32), np.ascontiguousarray(v, np.float32)
+    rows = int(np.sum(lengths))
+    _rows_of(rows, k=(k, cache.kv_heads * cache.dk), v=(v, cache.kv_heads * cache.dv))
     cache.grow(lengths)
+    if rows == 0:
+        return
     dk_, dv_, starts, pages = DevBuf.from_host(k), DevBuf.from_host(v), _row_starts(lengths), cache.pages()
     flag = DevBuf.from_host(np.zeros(1, np.int32), np.int32)
     check(lib.fdx_kv_append_f32(_dp(dk_), ctypes.c_int64(k.shape[1]), _dp(dv_), ctypes.c_int64(v.shape[1]), starts.ptr, k.shape[0],
@@ -681,6 +692,7 @@ def mha_paged(cache, q, lengths, heads):
     """Attention of the last lengths[i] positions of sequence i, whose queries are rows of q [tokens,heads*dk], over its pages."""
     q = np.ascontiguousarray(q, np.float32)
     tokens, most = q.shape[0], int(max(lengths))
+    _rows_of(int(np.sum(lengths)), q=(q, heads * cache.dk))
     dq, starts, pages = DevBuf.from_host(q), _row_starts(lengths), cache.pages()
     scratch = DevBuf(lib.fdx_mha_paged_scratch_bytes(tokens, most, heads, ctypes.byref(pages)))
     out = DevBuf.from_host(np.zeros((tokens, heads * cache.dv), np.float32))
@@ -696,6 +708,8 @@ def token_logprobs(logits, ids=None, top=0):
     top_ids and top_logprobs [rows,top] (if top > 0)."""
     logits = np.ascontiguousarray(logits, np.float32)
     rows, vocab = logits.shape
+    if ids is not None and np.shape(ids) != (rows,):
+        raise FdxError("ids of shape %s for %d rows" % (np.shape(ids), rows))
     dx = DevBuf.from_host(logits)
     di = None if ids is None else DevBuf.from_host(ids, np.int32)
     dl, de = (None if ids is None else DevBuf(4 * rows)), DevBuf(4 * rows)

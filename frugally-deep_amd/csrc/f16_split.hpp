@@ -29,7 +29,8 @@ __device__ __forceinline__ Pow2 pow2_for(int e)
 __device__ __forceinline__ int exponent(float x) { return (int)(__builtin_bit_cast(uint32_t, x) >> 23 & 255u); }
 
 // Sets of rows that share a power: keys and values of a tile.  A row keeps 22 bits of its own largest value as long as that is not below
-// 2^-16 of the set's (2^-12 with a power in steps of four); sets that reach further are not for these products.  Two rows' largest values,
+// 2^-17 of the set's (2^-14 with a power in steps of four: fp16's last bit is 2^-24, and half of that has to be 2^-22 of the row's); sets that
+// reach further are not for these products.  Two rows' largest values,
 // one in each half, as what the set's spread is found from: `top` has their exponents, `low` 255 less each, 0 for a row of zeros.
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 struct Spread {
@@ -62,7 +63,7 @@ __device__ __forceinline__ u16x2 most_of_wave(u16x2 v)
     return most(__builtin_bit_cast(u16x2, (uint32_t)q[0]), __builtin_bit_cast(u16x2, (uint32_t)q[1]));
 }
 // whether keys (first half) and values (second half, in steps of four) can share their powers
-__device__ __forceinline__ bool spread_fits(u16x2 top, u16x2 low) { return top[0] + low[0] <= 255 + 16 && top[1] + low[1] <= 255 + 12; }
+__device__ __forceinline__ bool spread_fits(u16x2 top, u16x2 low) { return top[0] + low[0] <= 255 + 17 && top[1] + low[1] <= 255 + 14; }
 
 // Both roundings are of mixed-precision multiply-adds, x s and x s - h, which take and give either type.
 __device__ __forceinline__ void split2x8(const float (&x)[8], float s, f16x8& h, f16x8& l)

@@ -92,7 +92,7 @@ extern "C" fdx_status fdx_kv_append_f32(const float* k, int64_t ldk, const float
     if (st != FDX_OK)
         return st;
     FDX_REQUIRE(k && v && starts, "kv_append: null pointer");
-    FDX_REQUIRE(tokens > 0 && tokens <= (1 << 25), "kv_append: 1 to 2^25 tokens");
+    FDX_REQUIRE(tokens > 0 && tokens <= (1 << 24), "kv_append: 1 to 2^24 tokens");
     const int64_t nk = (int64_t)cache->kv_heads * cache->dk, nv = (int64_t)cache->kv_heads * cache->dv;
     FDX_REQUIRE(ldk >= nk && ldv >= nv, "kv_append: rows overlap");
     const AppendParams p { k, v, ldk, ldv, starts, tokens, *cache, make_divisor(cache->page_size), error_flag_dev };

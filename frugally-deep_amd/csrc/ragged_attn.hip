@@ -1373,8 +1373,8 @@ static fdx_status check_ragged(const char* who, const RaggedParams& p, const voi
     FDX_REQUIRE(p.q && p.k && p.v && p.starts && p.out, "%s: null pointer", who);
     FDX_REQUIRE(p.n_seqs > 0 && p.tokens > 0 && p.heads > 0 && p.kv_heads > 0 && p.dk > 0 && p.dv > 0, "%s: bad shape", who);
     FDX_REQUIRE(p.heads % p.kv_heads == 0, "%s: %d query heads cannot share %d key heads", who, p.heads, p.kv_heads);
-    FDX_REQUIRE((int64_t)p.tokens * p.heads <= ((int64_t)1 << 26) && p.n_seqs <= (1 << 22) && p.heads <= 65535,
-        "%s: tokens * heads or sequences too many for one launch", who);
+    FDX_REQUIRE((int64_t)p.tokens * p.heads <= (1 << 25) && (int64_t)p.n_seqs * p.kv_heads <= (1 << 22),
+        "%s: tokens * heads or sequences * key heads too many for one launch", who);
     FDX_REQUIRE(p.ldq >= (int64_t)p.heads * p.dk && p.ldo >= (int64_t)p.heads * p.dv && p.ldk >= (int64_t)p.kv_heads * p.dk
             && p.ldv >= (int64_t)p.kv_heads * p.dv,
         "%s: rows overlap", who);
@@ -1450,7 +1450,6 @@ extern "C" fdx_status fdx_mha_paged_f32(const float* q, int64_t ldq, const int32
     st = check_ragged("mha_paged", p, scratch_dev, fdx_mha_paged_scratch_bytes(tokens, max_new, heads, cache));
     if (st != FDX_OK)
         return st;
-    FDX_REQUIRE((int64_t)p.n_seqs * p.kv_heads <= (1 << 22), "mha_paged: sequences * key heads too many for one launch");
     p.scale = (float)(1.0 / std::sqrt((double)p.dk));
     const RaggedPlan plan = paged_plan(tokens, max_new, heads, cache);
     float* part = static_cast<float*>(scratch_dev);

@@ -181,7 +181,7 @@ __device__ __forceinline__ Tile late_tile_wave(const int32_t* starts, int n_seqs
     if (lane < n_seqs)
         span = packed_span(starts, lane, tokens);
     const int tiles = (int)(((int64_t)span.count * per_token + rows - 1) / rows);
-    auto before = [&](int j) { return (int64_t)wave_all<false>((float)(tiles > j ? tiles - j : 0)); }; // below 2^24: tokens * heads is at most 2^26
+    auto before = [&](int j) { return (int64_t)wave_all<false>((float)(tiles > j ? tiles - j : 0)); }; // exact below 2^24: tokens * heads is at most 2^25
     Tile t { -1, 0, { 0, 0 } };
     if (number >= before(0))
         return t;
@@ -194,8 +194,10 @@ __device__ __forceinline__ Tile late_tile_wave(const int32_t* starts, int n_seqs
             hi = mid;
     }
     uint64_t of = __ballot(tiles > lo);
-    for (int skip = (int)(number - before(lo + 1)); skip > 0; --skip)
+    for (int skip = (int)(number - before(lo + 1)); skip > 0 && of; --skip)
         of &= of - 1;
+    if (of == 0) // sequences that overlap: more tiles than there are rows, too many to count
+        return t;
     t.seq = __builtin_ctzll(of);
     t.index = lo;
     t.span = packed_span(starts, t.seq, tokens);

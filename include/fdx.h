@@ -353,7 +353,8 @@ fdx_status fdx_mha_decode_f32(const float* q, const float* k_cache, const float*
  * s over the rows of t's sequence, up to t itself if `causal` is not 0.
  * q [tokens][heads*dk], k [tokens][kv_heads*dk], v [tokens][kv_heads*dv], out [tokens][heads*dv], rows ldq / ldk / ldv / ldo
  * floats apart.  starts: n_seqs + 1 row numbers in device memory, ascending; sequence i has rows starts[i] .. starts[i+1]-1,
- * none if they are equal.  Rows of `out` that belong to no sequence stay as they are.  Depths up to 128.
+ * none if they are equal.  Rows of `out` that belong to no sequence stay as they are.  Depths up to 128; tokens * heads up to
+ * 2^25, n_seqs * kv_heads up to 2^22.  fp32 precision: products of operands held to 22 bits, sums in fp32.
  * scratch_dev: fdx_mha_packed_scratch_bytes bytes, 16-byte aligned, left to the call until its work has completed; its
  * contents before and after mean nothing.  Two calls that may overlap need two.
  * error_flag_dev (may be NULL) is set to 1 on the device if `starts` descends or leaves 0 .. tokens; what it holds else is
@@ -371,7 +372,7 @@ fdx_status fdx_mha_packed_f32(const float* q, int64_t ldq, const float* k, int64
  * half the memory and half the traffic (rounded to nearest when written, widened when read; all sums stay fp32).  Sequences
  * may share pages that hold the same prefix.  All pointers are device memory; the structure itself is read during the call.
  * lens[i]: positions of sequence i, those of the call's new tokens included.  max_len: no sequence is longer; it sizes the
- * launch and has to be covered by the table (max_len <= table_width * page_size).  n_pages * page_size < 2^31.
+ * launch and has to be covered by the table (max_len <= table_width * page_size), up to 2^30.  n_pages * page_size < 2^31.
  */
 enum { FDX_KV_F32 = 0, FDX_KV_BF16 = 1 };
 typedef struct fdx_kv_pages {

@@ -183,11 +183,16 @@ def test_packed_infinities_and_nan(fdx):
                 close(got[hit][~np.isnan(seen)], seen[~np.isnan(seen)]) if (~np.isnan(seen)).any() else None
 
 
+def noise(fdx, size):
+    """Memory whose contents mean nothing: NaN in every place."""
+    return fdx.DevBuf.from_host(np.full(size + 16, 255, np.uint8), np.uint8)
+
+
 def call_packed(fdx, q, ldq, k, ldk, v, ldv, starts, tokens, heads, kv, dk, dv, out, ldo, causal=True):
     """The entry point itself: byte offsets of 4 behind the buffers' starts are kept."""
     i64, n_seqs = ctypes.c_int64, len(starts) - 1
     d_starts, flag = fdx.DevBuf.from_host(np.asarray(starts, np.int32), np.int32), fdx.DevBuf.from_host(np.zeros(1, np.int32), np.int32)
-    scratch = fdx.DevBuf(fdx.lib.fdx_mha_packed_scratch_bytes(tokens, n_seqs, heads, kv, dk, dv))
+    scratch = noise(fdx, fdx.lib.fdx_mha_packed_scratch_bytes(tokens, n_seqs, heads, kv, dk, dv))
     fdx.check(fdx.lib.fdx_mha_packed_f32(q, i64(ldq), k, i64(ldk), v, i64(ldv), d_starts.ptr, n_seqs, tokens, heads, kv, dk, dv, int(causal), out,
                                          i64(ldo), scratch.ptr, flag.ptr))
     fdx.sync()
@@ -321,7 +326,7 @@ def call_paged(fdx, cache, q, ldq, starts, tokens, max_new, heads, out, ldo, **c
             value = value.ptr
         setattr(c, key, value)
     d_starts, flag = fdx.DevBuf.from_host(np.asarray(starts, np.int32), np.int32), fdx.DevBuf.from_host(np.zeros(1, np.int32), np.int32)
-    scratch = fdx.DevBuf(fdx.lib.fdx_mha_paged_scratch_bytes(tokens, max_new, heads, ctypes.byref(c)))
+    scratch = noise(fdx, fdx.lib.fdx_mha_paged_scratch_bytes(tokens, max_new, heads, ctypes.byref(c)))
     fdx.check(fdx.lib.fdx_mha_paged_f32(q, ctypes.c_int64(ldq), d_starts.ptr, tokens, max_new, heads, ctypes.byref(c), out, ctypes.c_int64(ldo),
                                         scratch.ptr, flag.ptr))
     fdx.sync()
@@ -525,3 +530,71 @@ def test_paged_long_contexts(fdx, context, new, heads, kv, d, kind):
         close(fdx.mha_paged(f.cache, q, new, heads), f.reference(q, new, heads))
         first = fdx.mha_paged(f.cache, q, new, heads)
         assert np.array_equal(first, fdx.mha_paged(f.cache, q, new, heads))
+
+
+def test_scratch_holds_anything_before_a_call(fdx):
+    """Key ranges and split prompts in memory full of NaN; a second call in the same memory right behind the first."""
+    heads, kv, d = 16, 1, 64
+    f = Filled(fdx, [2500, 700], kv, d, d, 16, "f32", steps=1)
+    r = np.random.default_rng(3)
+    q = r.standard_normal((41, heads * d)).astype(np.float32)
+    dq, out, c = fdx.DevBuf.from_host(q), [fdx.DevBuf(q.nbytes) for _ in range(2)], f.cache.pages()
+    starts = fdx.DevBuf.from_host(np.array([0, 1, 41], np.int32), np.int32)
+    need = fdx.lib.fdx_mha_paged_scratch_bytes(41, 40, heads, ctypes.byref(c))
+    assert need > 0
+    scratch = noise(fdx, need)
+    for o in out:
+        fdx.check(fdx.lib.fdx_mha_paged_f32(dq.ptr, ctypes.c_int64(heads * d), starts.ptr, 41, 40, heads, ctypes.byref(c), o.ptr, ctypes.c_int64(heads * d),
+                                            scratch.ptr, None))
+    want = f.reference(q, [1, 40], heads)
+    close(out[0].to_host(q.shape), want)
+    assert np.array_equal(out[0].to_host(q.shape), out[1].to_host(q.shape))
+    n = 300
+    q, k, v = (r.standard_normal((n, h * d)).astype(np.float32) for h in (heads, kv, kv))
+    assert fdx.lib.fdx_mha_packed_scratch_bytes(n, 1, heads, kv, d, d) > 0
+    bufs, o = [fdx.DevBuf.from_host(x) for x in (q, k, v)], fdx.DevBuf(q.nbytes)
+    assert call_packed(fdx, bufs[0].ptr, heads * d, bufs[1].ptr, d, bufs[2].ptr, d, [0, n], n, heads, kv, d, d, o.ptr, heads * d) == 0
+    close(o.to_host(q.shape), packed_reference(q, k, v, [n], heads, kv, True))
+
+
+def test_two_threads(fdx):
+    """Calls of two host threads, each with memory of its own."""
+    import threading
+    f, heads = Filled(fdx, [1200, 90], 2, 64, 64, 16, "bf16", steps=1), 8
+    r = np.random.default_rng(5)
+    qs = [r.standard_normal((n, heads * 64)).astype(np.float32) for n in (2, 61)]
+    new = [[1, 1], [60, 1]]
+    want, got, wrong = [f.reference(q, n, heads) for q, n in zip(qs, new)], [[], []], []
+
+    def work(i):
+        try:
+            for _ in range(10):
+                got[i].append(fdx.mha_paged(f.cache, qs[i], new[i], heads))
+        except Exception as e:   # reported below, by the test's own thread
+            wrong.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not wrong, wrong
+    for i in range(2):
+        close(got[i][0], want[i])
+        assert all(np.array_equal(got[i][0], x) for x in got[i])
+
+
+def test_shapes_that_do_not_fit(fdx):
+    x = np.zeros((5, 128), np.float32)
+    with pytest.raises(fdx.FdxError, match="k of shape"):
+        fdx.mha_packed(x, x[:4], x, [5], 2, 2, 64, 64)
+    c = fdx.PagedCache(4, 16, 2, 64, 64, 1, 40)
+    with pytest.raises(fdx.FdxError, match="v of shape"):
+        fdx.kv_append(c, x, x[:, :64], [5])
+    with pytest.raises(fdx.FdxError, match="at most 40"):
+        fdx.kv_append(c, np.zeros((41, 128), np.float32), np.zeros((41, 128), np.float32), [41])
+    fdx.kv_append(c, x, x, [5])
+    with pytest.raises(fdx.FdxError, match="q of shape"):
+        fdx.mha_paged(c, x[:3], [5], 2)
+    with pytest.raises(fdx.FdxError, match="free pages"):
+        d = fdx.PagedCache(1, 16, 2, 64, 64, 2, 40)
+        d.grow([16, 1])
+    with pytest.raises(fdx.FdxError, match="overlap"):
+        fdx.check(fdx.lib.fdx_kv_append_f32(c.k.ptr, ctypes.c_int64(3), c.v.ptr, ctypes.c_int64(128), c.k.ptr, 1, ctypes.byref(c.pages()), None))

@@ -87,7 +87,8 @@ def test_packed(fdx):
                          (dict(kv_heads=0), "shape"), (dict(dk=0), "shape"), (dict(dv=-1), "shape"), (dict(kv_heads=3, ldk=256, ldv=256), "share"),
                          (dict(kv_heads=8, ldk=1024, ldv=1024), "share"), (dict(ldq=255), "overlap"), (dict(ldk=1), "overlap"),
                          (dict(ldv=127), "overlap"), (dict(ldo=128), "overlap"), (dict(tokens=1 << 25), "too many"),
-                         (dict(n_seqs=(1 << 22) + 1), "too many")):
+                         (dict(n_seqs=(1 << 22) + 1), "too many"), (dict(n_seqs=1 << 21, heads=8, kv_heads=4, ldq=512, ldk=256, ldv=256, ldo=512), "too many"),
+                         (dict(tokens=(1 << 23) + 1), "too many")):
         refused(fdx, call(**change), INVALID, text)
     refused(fdx, call(dk=130, ldq=600, ldk=300), UNSUPPORTED, "depths up to 128, not 130 and 64")
 
