@@ -42,7 +42,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendParams p)
     const int row = (int)(item >> 1);
     if (row >= p.tokens)
         return;
-    const int s = find_row_wave(p.starts, p.c.n_seqs, p.tokens, row);
+    const int s = find_row(SearchWave(), p.starts, p.c.n_seqs, p.tokens, row);
     if (s < 0)
         return;
     const Span span = packed_span(p.starts, s, p.tokens);

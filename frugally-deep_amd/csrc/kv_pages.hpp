@@ -56,18 +56,35 @@ struct Tile {
     Span span;
 };
 
-FDX_HD Tile find_tile(const int32_t* starts, int n_seqs, int tokens, int per_token, int rows, int64_t number)
+// The searches are a wave's: sixty-four places are looked at together, where a binary search waits for memory once a step.  Wave has
+// count(f), mask(f), sum(f) and most(f) over f(0) .. f(63), and kept(f), numbers that each lane has worked out once.
+//
+// how many of the places 0 .. n - 1 are not above, where those are the first ones; whatever they are, 0 .. n
+template <class Wave, class NotAbove>
+FDX_HD int not_above(const Wave& wave, int n, const NotAbove& f)
 {
-    int lo = 0, hi = n_seqs; // the last sequence whose first number is not above `number`, if there is one
+    int lo = 0, hi = n;
     while (lo < hi) {
-        const int mid = lo + (hi - lo) / 2;
-        const int a = starts[mid];
-        if (first_tile(a < 0 ? 0 : (a > tokens ? tokens : a), mid, per_token, rows) <= number)
-            lo = mid + 1;
-        else
-            hi = mid;
+        const int step = (hi - lo + 63) >> 6, from = lo, to = hi;
+        const int count = wave.count([&](int lane) { return from + lane * step < to && f(from + lane * step); });
+        const int next = lo + count * step;
+        if (step == 1)
+            return next;
+        hi = next < hi ? next : hi;
+        lo = count > 0 ? next - step + 1 : hi;
     }
-    Tile t { lo - 1, 0, { 0, 0 } };
+    return lo;
+}
+
+template <class Wave>
+FDX_HD Tile find_tile(const Wave& wave, const int32_t* starts, int n_seqs, int tokens, int per_token, int rows, int64_t number)
+{
+    Tile t { not_above(wave, n_seqs,
+                 [&](int i) {
+                     const int a = starts[i];
+                     return first_tile(a < 0 ? 0 : (a > tokens ? tokens : a), i, per_token, rows) <= number;
+                 }) - 1,
+        0, { 0, 0 } };
     if (t.seq < 0)
         return t;
     t.span = packed_span(starts, t.seq, tokens);
@@ -78,21 +95,47 @@ FDX_HD Tile find_tile(const int32_t* starts, int n_seqs, int tokens, int per_tok
     return t;
 }
 
-// the sequence that row `row` belongs to, -1 if none
-FDX_HD int find_row(const int32_t* starts, int n_seqs, int tokens, int row)
+// find_tile for up to sixty-four sequences, numbered the other way: tiles furthest inside their sequences first, which see most keys.
+// before(j) = tiles of index j and more; the tile with `number` tiles in front of it has the index j with before(j + 1) <= number < before(j).
+template <class Wave>
+FDX_HD Tile late_tile(const Wave& wave, const int32_t* starts, int n_seqs, int tokens, int per_token, int rows, int64_t number)
 {
-    int lo = 0, hi = n_seqs;
-    while (lo < hi) {
-        const int mid = lo + (hi - lo) / 2;
-        if (starts[mid] <= row)
-            lo = mid + 1;
+    const auto kept = wave.kept([&](int lane) {
+        return lane < n_seqs ? (int)(((int64_t)packed_span(starts, lane, tokens).count * per_token + rows - 1) / rows) : 0;
+    });
+    // exact below 2^24: tokens * heads is at most 2^25
+    auto before = [&](int j) { return (int64_t)wave.sum([&](int lane) { return (float)(kept.at(lane) > j ? kept.at(lane) - j : 0); }); };
+    Tile t { -1, 0, { 0, 0 } };
+    if (number >= before(0))
+        return t;
+    int lo = 0, hi = (int)wave.most([&](int lane) { return (float)kept.at(lane); }); // before(lo) > number >= before(hi)
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (before(mid) > number)
+            lo = mid;
         else
             hi = mid;
     }
-    if (lo == 0)
+    uint64_t of = wave.mask([&](int lane) { return kept.at(lane) > lo; });
+    for (int skip = (int)(number - before(lo + 1)); skip > 0 && of; --skip)
+        of &= of - 1;
+    if (of == 0) // sequences that overlap: more tiles than there are rows, too many to count
+        return t;
+    t.seq = __builtin_ctzll(of);
+    t.index = lo;
+    t.span = packed_span(starts, t.seq, tokens);
+    return t;
+}
+
+// the sequence that row `row` belongs to, -1 if none
+template <class Wave>
+FDX_HD int find_row(const Wave& wave, const int32_t* starts, int n_seqs, int tokens, int row)
+{
+    const int i = not_above(wave, n_seqs, [&](int at) { return starts[at] <= row; }) - 1;
+    if (i < 0)
         return -1;
-    const Span s = packed_span(starts, lo - 1, tokens);
-    return row >= s.first && row - s.first < s.count ? lo - 1 : -1;
+    const Span s = packed_span(starts, i, tokens);
+    return row >= s.first && row - s.first < s.count ? i : -1;
 }
 
 // row of position `pos` among the rows of all pages, -1 if the table does not reach it or names no page of the cache

@@ -141,8 +141,8 @@ __device__ __forceinline__ void tile_body(const RaggedParams& p, const Place& pl
     // keys; later tiles of a sequence, which see more keys, first
     const int kv_head = place_in.x % p.kv_heads;
     const int64_t number = place_in.x / p.kv_heads;
-    const Tile tile = p.causal && p.n_seqs <= 64 ? late_tile_wave(p.starts, p.n_seqs, p.tokens, p.group, 128, number)
-                                                 : find_tile_wave(p.starts, p.n_seqs, p.tokens, p.group, 128, place_in.nx / p.kv_heads - 1 - number);
+    const Tile tile = p.causal && p.n_seqs <= 64 ? late_tile(SearchWave(), p.starts, p.n_seqs, p.tokens, p.group, 128, number)
+                                                 : find_tile(SearchWave(), p.starts, p.n_seqs, p.tokens, p.group, 128, place_in.nx / p.kv_heads - 1 - number);
     if (tile.seq < 0)
         return;
     const Sequence s = sequence_of<KIND>(p, tile.seq, tile.span);
@@ -531,7 +531,7 @@ __global__ __launch_bounds__(256) void ragged_ready_kernel(RaggedParams p)
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int kv_head = blockIdx.x % p.kv_heads;
     const int64_t number = blockIdx.x / p.kv_heads;
-    const Tile tile = find_tile_wave(p.starts, p.n_seqs, p.tokens, 1, KT, number);
+    const Tile tile = find_tile(SearchWave(), p.starts, p.n_seqs, p.tokens, 1, KT, number);
     if (tile.seq < 0)
         return;
     const int krow = tid / N, kl = tid % N, vblk = tid / (D / 2), vd = tid % (D / 2) * 2;
@@ -627,8 +627,8 @@ __global__ __launch_bounds__(256, 2) void ragged_packed_kernel(RaggedParams p)
             raise_flag(p, !packed_start_ok(p.starts, i, p.tokens));
     const int kv_head = blockIdx.x % p.kv_heads; // the order of ragged_tile_kernel
     const int64_t number = blockIdx.x / p.kv_heads;
-    const Tile tile = p.causal && p.n_seqs <= 64 ? late_tile_wave(p.starts, p.n_seqs, p.tokens, p.group, 128, number)
-                                                 : find_tile_wave(p.starts, p.n_seqs, p.tokens, p.group, 128, gridDim.x / p.kv_heads - 1 - number);
+    const Tile tile = p.causal && p.n_seqs <= 64 ? late_tile(SearchWave(), p.starts, p.n_seqs, p.tokens, p.group, 128, number)
+                                                 : find_tile(SearchWave(), p.starts, p.n_seqs, p.tokens, p.group, 128, gridDim.x / p.kv_heads - 1 - number);
     if (tile.seq < 0)
         return;
     const Sequence s = sequence_of<kPackedF32>(p, tile.seq, tile.span);
@@ -1183,7 +1183,7 @@ __global__ __launch_bounds__(256) void ragged_join_kernel(RaggedParams p)
     const int row = (int)((uint64_t)item / (uint32_t)p.heads), head = (int)(item - (int64_t)row * p.heads);
     if (row >= p.tokens)
         return;
-    const int index = find_row_wave(p.starts, p.n_seqs, p.tokens, row);
+    const int index = find_row(SearchWave(), p.starts, p.n_seqs, p.tokens, row);
     if (index < 0)
         return;
     const Sequence s = sequence_of<KIND>(p, index, packed_span(p.starts, index, p.tokens));

@@ -118,91 +118,24 @@ __device__ __forceinline__ int visible_keys(const RaggedParams& p, const Sequenc
     return n < 0 ? 0 : n;
 }
 
-// find_tile by a whole wave: sixty-four sequences are looked at together, where a binary search waits for memory once a step
-__device__ __forceinline__ Tile find_tile_wave(const int32_t* starts, int n_seqs, int tokens, int per_token, int rows, int64_t number)
-{
-    const int lane = threadIdx.x & 63;
-    int lo = 0, hi = n_seqs;
-    while (lo < hi) {
-        const int step = (hi - lo + 63) >> 6, i = lo + lane * step;
-        bool not_above = false;
-        if (i < hi) {
-            const int a = starts[i];
-            not_above = first_tile(a < 0 ? 0 : (a > tokens ? tokens : a), i, per_token, rows) <= number;
-        }
-        const int count = __builtin_popcountll(__ballot(not_above));
-        const int next = lo + count * step;
-        if (step == 1) {
-            lo = hi = next;
-        } else {
-            hi = next < hi ? next : hi;
-            lo = count > 0 ? next - step + 1 : hi;
-        }
-    }
-    Tile t { lo - 1, 0, { 0, 0 } };
-    if (t.seq < 0)
-        return t;
-    t.span = packed_span(starts, t.seq, tokens);
-    const int64_t index = number - first_tile(t.span.first, t.seq, per_token, rows);
-    if (index < 0 || index * rows >= (int64_t)t.span.count * per_token)
-        t.seq = -1;
-    t.index = (int)index;
-    return t;
-}
-
-// find_row the same way
-__device__ __forceinline__ int find_row_wave(const int32_t* starts, int n_seqs, int tokens, int row)
-{
-    const int lane = threadIdx.x & 63;
-    int lo = 0, hi = n_seqs;
-    while (lo < hi) {
-        const int step = (hi - lo + 63) >> 6, i = lo + lane * step;
-        const int count = __builtin_popcountll(__ballot(i < hi && starts[i < hi ? i : lo] <= row));
-        const int next = lo + count * step;
-        if (step == 1) {
-            lo = hi = next;
-        } else {
-            hi = next < hi ? next : hi;
-            lo = count > 0 ? next - step + 1 : hi;
-        }
-    }
-    if (lo == 0)
-        return -1;
-    const Span s = packed_span(starts, lo - 1, tokens);
-    return row >= s.first && row - s.first < s.count ? lo - 1 : -1;
-}
-
-// find_tile for up to sixty-four sequences, numbered the other way: tiles furthest inside their sequences first, which see most keys.
-// before(j) = tiles of index j and more; the tile with `number` tiles in front of it has the index j with before(j + 1) <= number < before(j).
-__device__ __forceinline__ Tile late_tile_wave(const int32_t* starts, int n_seqs, int tokens, int per_token, int rows, int64_t number)
-{
-    const int lane = threadIdx.x & 63;
-    Span span { 0, 0 };
-    if (lane < n_seqs)
-        span = packed_span(starts, lane, tokens);
-    const int tiles = (int)(((int64_t)span.count * per_token + rows - 1) / rows);
-    auto before = [&](int j) { return (int64_t)wave_all<false>((float)(tiles > j ? tiles - j : 0)); }; // exact below 2^24: tokens * heads is at most 2^25
-    Tile t { -1, 0, { 0, 0 } };
-    if (number >= before(0))
-        return t;
-    int lo = 0, hi = (int)wave_all<true>((float)tiles); // before(lo) > number >= before(hi)
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (before(mid) > number)
-            lo = mid;
-        else
-            hi = mid;
-    }
-    uint64_t of = __ballot(tiles > lo);
-    for (int skip = (int)(number - before(lo + 1)); skip > 0 && of; --skip)
-        of &= of - 1;
-    if (of == 0) // sequences that overlap: more tiles than there are rows, too many to count
-        return t;
-    t.seq = __builtin_ctzll(of);
-    t.index = lo;
-    t.span = packed_span(starts, t.seq, tokens);
-    return t;
-}
+// the wave that searches, for the functions of kv_pages.hpp
+struct SearchWave {
+    struct Kept {
+        int mine;
+        __device__ __forceinline__ int at(int) const { return mine; }
+    };
+    int lane = threadIdx.x & 63;
+    template <class F>
+    __device__ __forceinline__ Kept kept(const F& f) const { return { f(lane) }; }
+    template <class F>
+    __device__ __forceinline__ uint64_t mask(const F& f) const { return __ballot(f(lane)); }
+    template <class F>
+    __device__ __forceinline__ int count(const F& f) const { return __builtin_popcountll(mask(f)); }
+    template <class F>
+    __device__ __forceinline__ float sum(const F& f) const { return wave_all<false>(f(lane)); }
+    template <class F>
+    __device__ __forceinline__ float most(const F& f) const { return wave_all<true>(f(lane)); }
+};
 
 // exponentials are taken to base two on scores that carry log2(e)
 constexpr float kLog2e = 1.44269504088896340736f;
