@@ -1290,14 +1290,32 @@ static RaggedPlan paged_plan(int tokens, int max_new, int heads, const fdx_kv_pa
 static RaggedPlan packed_plan(int tokens, int n_seqs, int heads, int kv_heads, int dk, int dv, int causal)
 {
     RaggedPlan r {};
-    const int keys_a_tile = dk <= 64 && dv <= 64 ? 64 : 32;
+    const int keys_a_tile = dk <= 64 && dv <= 64 ? 64 : 32, length = tokens / n_seqs;
+    r.tiles = tile_numbers(tokens, n_seqs, heads / kv_heads, 128) * kv_heads;
+    r.tile_ranges = 1;
+    r.tile_keys = 0x7fffffff;
+    // A few long prompts: ranges of 256 keys or more while there are tiles for half the CUs or fewer (three quarters with a mask, which leaves
+    // half of the ranges to nobody); the join is a launch and reads what they wrote.  us without ranges / with: no mask, 4 heads of 64, one prompt
+    // of 600 26.5 / 20.0, 1000 39.0 / 22.8, 4000 (128 tiles) 116 / 79.4, two of 1000 38.6 / 31.2; causal, 12 heads, one of 600 27.7 / 23.6, 1000
+    // 40.0 / 33.3, 2000 (192 tiles) 72.0 / 54.6.  They lose with prompts of 300 to 500 (12 heads, four of 500 causal 24.2 / 38.3) and with
+    // more tiles (12 heads, two of 2000 causal, 384 tiles, 76.2 / 88.5; one of 2000 without a mask, 192 tiles, 72.1 / 75.1).
+    const int64_t full = ((int64_t)tokens * (heads / kv_heads) + 127) / 128 * kv_heads;
+    if (length >= 512 && full <= (causal ? 192 : 128)) {
+        int64_t keys = length / (512 / full);
+        keys = keys < 256 ? 256 : keys;
+        keys = keys < tokens / 16 ? tokens / 16 : keys; // at most 16 ranges, whose sums take scratch memory
+        if (keys < length) {
+            r.tile_ranges = ranges_of(tokens, keys, &r.tile_keys);
+            r.tile_part = (int64_t)tokens * heads;
+            return r;
+        }
+    }
     // The pass of its own moves a tile's 32 KB twice more (of 8192 tokens, 16 heads of 64: 18 us), every 128 rows that use the tile then take a
     // fifth less time.  8192 tokens in sequences of one length, one pass against two in us: no mask, 512 / 1024 / 2048 rows a sequence
     // and key head, 76.7 / 87.4, 133 / 134, 248 / 230 at depth 64 and 144 / 165, 252 / 255, 476 / 439 at 128; causal, 1024 / 2048 / 4096 rows,
     // 81.7 / 94.7, 143 / 144, 266 / 249 and 157 / 182, 274 / 274, 519 / 466.
     if ((int64_t)tokens * (heads / kv_heads) >= (int64_t)n_seqs * (causal ? 2048 : 1024) && tokens >= (int64_t)n_seqs * keys_a_tile)
         r.ready = tile_numbers(tokens, n_seqs, 1, keys_a_tile) * kv_heads;
-    r.tiles = tile_numbers(tokens, n_seqs, heads / kv_heads, 128) * kv_heads;
     return r;
 }
 
@@ -1346,9 +1364,8 @@ static void ragged_launch(RaggedParams p, const RaggedPlan& plan)
         else
             hipLaunchKernelGGL((ragged_tile_kernel<D, KIND, false>), grid, block, 0, stream(), p);
     }
-    if constexpr (KIND != kPackedF32)
-        if (plan.few_ranges > 1 || plan.tile_ranges > 1)
-            hipLaunchKernelGGL(ragged_join_kernel<KIND>, dim3((unsigned)(((int64_t)p.tokens * p.heads + 3) / 4)), block, 0, stream(), p);
+    if (plan.few_ranges > 1 || plan.tile_ranges > 1)
+        hipLaunchKernelGGL(ragged_join_kernel<KIND>, dim3((unsigned)(((int64_t)p.tokens * p.heads + 3) / 4)), block, 0, stream(), p);
 }
 
 template <int KIND>
@@ -1394,7 +1411,13 @@ extern "C" size_t fdx_mha_packed_scratch_bytes(int tokens, int n_seqs, int heads
 {
     if (tokens <= 0 || n_seqs <= 0 || heads <= 0 || kv_heads <= 0 || dk <= 0 || dv <= 0)
         return 0;
-    return packed_plan(tokens, n_seqs, heads, kv_heads, dk, dv, 0).ready_bytes(); // what a call needs with a mask is this or nothing
+    size_t most = 0;
+    for (int causal = 0; causal < 2; ++causal) {
+        const RaggedPlan plan = packed_plan(tokens, n_seqs, heads, kv_heads, dk, dv, causal);
+        const size_t need = plan.ready_bytes() + sizeof(float) * plan.tile_floats(dv);
+        most = need > most ? need : most;
+    }
+    return most;
 }
 
 extern "C" fdx_status fdx_mha_packed_f32(const float* q, int64_t ldq, const float* k, int64_t ldk, const float* v, int64_t ldv,
@@ -1416,6 +1439,7 @@ extern "C" fdx_status fdx_mha_packed_f32(const float* q, int64_t ldq, const floa
     const RaggedPlan plan = packed_plan(tokens, n_seqs, heads, kv_heads, dk, dv, causal);
     p.ready = static_cast<unsigned char*>(scratch_dev);
     p.powers = reinterpret_cast<f32x2_pow*>(p.ready + plan.ready * 32768);
+    p.tile = { static_cast<float*>(scratch_dev), plan.tile_part, plan.tile_ranges, plan.tile_keys, 0 };
     ragged_dispatch<kPackedF32>(p, plan);
     profile_end("mha_packed_f32", 0.0, 4.0 * tokens * ((double)heads + kv_heads) * (dk + dv));
     FDX_LAUNCH_CHECK();

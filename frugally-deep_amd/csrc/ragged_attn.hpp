@@ -81,11 +81,11 @@ __device__ __forceinline__ Sequence sequence_of(const RaggedParams& p, int index
         if (span.count > p.max_new)
             s.span.count = p.max_new;
         s.few = s.span.count * p.group <= p.few_rows;
-        const int most = s.few ? p.few.keys : p.tile.keys;
-        if (s.keys > most) {
-            const int parts = (s.keys + most - 1) / most;
-            s.range = ((s.keys + parts - 1) / parts + 63) & ~63;
-        }
+    }
+    const int most = s.few ? p.few.keys : p.tile.keys;
+    if (s.keys > most) {
+        const int parts = (s.keys + most - 1) / most;
+        s.range = ((s.keys + parts - 1) / parts + 63) & ~63;
     }
     return s;
 }

@@ -75,6 +75,41 @@ def test_packed_of_many_tokens(fdx, lengths, heads, kv_heads, dk, dv, causal):
     test_packed(fdx, lengths, heads, kv_heads, dk, dv, causal)
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lengths,heads,kv_heads,dk,dv", [
+    ([1500], 4, 4, 64, 64), ([513], 1, 1, 64, 64), ([512, 512], 3, 3, 64, 64), ([2100, 0, 700], 4, 2, 64, 64), ([1024], 5, 1, 128, 128),
+    ([700, 1, 1200], 2, 2, 33, 127), ([769, 770, 767], 6, 6, 32, 32), ([1, 0, 3000], 2, 1, 80, 96), ([1025], 12, 12, 64, 64), ([2047], 12, 12, 64, 64)])
+def test_packed_few_long(fdx, lengths, heads, kv_heads, dk, dv, causal):
+    """Fewer tiles than the GPU takes: keys in ranges."""
+    print("packed few", lengths, heads, kv_heads, dk, dv, causal, flush=True)
+    test_packed(fdx, lengths, heads, kv_heads, dk, dv, causal)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lengths,heads,kv_heads,dk,dv", [
+    ([400], 6, 1, 64, 64), ([511, 300, 0, 1], 16, 1, 64, 64), ([257, 128, 129], 16, 1, 128, 128), ([500, 31], 20, 2, 80, 80), ([450], 7, 1, 33, 127),
+    ([1300, 900], 16, 16, 64, 64)])
+def test_packed_split_once(fdx, lengths, heads, kv_heads, dk, dv, causal):
+    """Many query rows a key head: a pass of its own splits keys and values."""
+    print("packed once", lengths, heads, kv_heads, dk, dv, causal, flush=True)
+    test_packed(fdx, lengths, heads, kv_heads, dk, dv, causal)
+
+
+@pytest.mark.parametrize("what", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("name,row", [("v", 333), ("k", 333), ("k", 64), ("v", 399)])
+def test_packed_split_once_infinities_and_nan(fdx, what, name, row):
+    r, n, heads, kv = np.random.default_rng(9), 400, 8, 1
+    q, k, v = (r.standard_normal((n, h * 64)).astype(np.float32) for h in (heads, kv, kv))
+    base = packed_reference(q, k, v, [n], heads, kv, True)
+    print("packed once odd", what, name, row, flush=True)
+    dict(k=k, v=v)[name][row, 7] = what
+    got = fdx.mha_packed(q, k, v, [n], heads, kv, 64, 64)
+    close(got[:row], base[:row])
+    with np.errstate(all="ignore"):
+        want = packed_reference(q, k, v, [n], heads, kv, True)[row:]
+    assert np.array_equal(np.isnan(got[row:]), np.isnan(want)) and np.array_equal(np.isinf(got[row:]), np.isinf(want))
+
+
 @pytest.mark.parametrize("lengths,heads", [([90, 150, 40], 4), ([640, 200], 4), ([260, 150], 64)])
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("power", [12, 18, 30, 70, 124])
