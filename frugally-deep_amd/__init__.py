@@ -636,7 +636,7 @@ def mha_packed(q, k, v, lengths, heads, kv_heads, dk, dv, causal=True):
 
 class PagedCache:
     """Keys and values of several sequences in pages of device memory, for kv_append and mha_paged.  A sequence takes pages as it
-    grows and gives them back with release(); the page table lives on the host and goes to the device when it has changed."""
+    grows and gives them back with release(); the page table lives on the host and goes to the device with every call."""
 
     def __init__(self, n_pages, page_size, kv_heads, dk, dv, n_seqs, max_len, kind="f32"):
         self.n_pages, self.page_size, self.kv_heads, self.dk, self.dv = n_pages, page_size, kv_heads, dk, dv
@@ -648,9 +648,15 @@ class PagedCache:
         self.lens = np.zeros(n_seqs, np.int32)
         self.free = list(range(n_pages - 1, -1, -1))
 
+    def lengths_of(self, lengths):
+        lengths = np.asarray(lengths, np.int64)
+        if lengths.shape != (self.n_seqs,) or lengths.min() < 0:
+            raise FdxError("%d sequences need as many numbers of new rows, not %s" % (self.n_seqs, lengths.tolist()))
+        return lengths
+
     def grow(self, lengths):
         """Makes room for lengths[i] more positions of sequence i."""
-        want = self.lens + np.asarray(lengths, np.int32)
+        want = self.lens + self.lengths_of(lengths)
         if want.max() > self.max_len:
             raise FdxError("a sequence of %d positions in a cache of at most %d" % (want.max(), self.max_len))
         need = [max(0, -(-int(w) // self.page_size) - int((row >= 0).sum())) for w, row in zip(want, self.table)]
@@ -660,7 +666,7 @@ class PagedCache:
             used = int((row >= 0).sum())
             for j in range(used, used + count):
                 row[j] = self.free.pop()
-        self.lens = want
+        self.lens = want.astype(np.int32)
 
     def release(self, seq):
         self.free += [int(page) for page in self.table[seq] if page >= 0]
@@ -676,7 +682,7 @@ class PagedCache:
 def kv_append(cache, k, v, lengths):
     """Adds lengths[i] rows of k [tokens,kv_heads*dk] and v [tokens,kv_heads*dv] to sequence i of a PagedCache."""
     k, v = np.ascontiguousarray(k, np.float32), np.ascontiguousarray(v, np.float32)
-    rows = int(np.sum(lengths))
+    rows = int(cache.lengths_of(lengths).sum())
     _rows_of(rows, k=(k, cache.kv_heads * cache.dk), v=(v, cache.kv_heads * cache.dv))
     cache.grow(lengths)
     if rows == 0:
@@ -691,8 +697,9 @@ def kv_append(cache, k, v, lengths):
 def mha_paged(cache, q, lengths, heads):
     """Attention of the last lengths[i] positions of sequence i, whose queries are rows of q [tokens,heads*dk], over its pages."""
     q = np.ascontiguousarray(q, np.float32)
-    tokens, most = q.shape[0], int(max(lengths))
-    _rows_of(int(np.sum(lengths)), q=(q, heads * cache.dk))
+    lengths = cache.lengths_of(lengths)
+    tokens, most = q.shape[0], int(lengths.max())
+    _rows_of(int(lengths.sum()), q=(q, heads * cache.dk))
     dq, starts, pages = DevBuf.from_host(q), _row_starts(lengths), cache.pages()
     scratch = DevBuf(lib.fdx_mha_paged_scratch_bytes(tokens, most, heads, ctypes.byref(pages)))
     out = DevBuf.from_host(np.zeros((tokens, heads * cache.dv), np.float32))

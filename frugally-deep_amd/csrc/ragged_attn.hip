@@ -1,4 +1,9 @@
 // Attention over packed prompts and over paged caches (gfx950), query heads in groups that share a key / value head.
+//
+//   O = softmax(Q K^T / sqrt(dk)) V a sequence, in one pass over the keys with the running maximum m and sum l of each row:
+//   m' = max(m, max s), l' = l 2^(m - m') + sum 2^(s - m'), o' = o 2^(m - m') + sum 2^(s - m') v; out = o / l, s in units of log2.
+// Three forms: tiles of 128 rows, split as they are fetched (any batch); the same on tiles that a pass of its own has split (long
+// packed prompts); up to 32 rows straight from memory (decode steps).
 #include <cfloat>
 #include <climits>
 
@@ -60,6 +65,9 @@ __device__ __forceinline__ void store_plain_row(const RaggedParams& p, const Seq
 //    (spread_fits; a row of 10^30 behind the mask) is left to plain sums.
 //  * The maximum that a row's exponentials refer to moves only when a score passes it by 2^4, so sums are rescaled a few times a row
 //    instead of every tile; exponentials carry 2^10 to stay clear of fp16's small end, at most 2^14.
+//  * Bound by the vector units, which split, beside the matrix units: 64 keys take a workgroup 1.9 us alone on its CU at depth 64; four
+//    sequences that bring 1000 tokens to 3000 keys in fp32 pages, 32 / 8 heads of 128, 887 us or 258 TFLOP/s, where three products for one come
+//    to 364 at the rate of a large fp16 product.
 //  * Rows whose sums are not finite (infinite or NaN operands, whether the row sees them or not, and tiles left out above) are taken again by
 //    plain_row.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -515,11 +523,13 @@ __global__ __launch_bounds__(256, 2) void ragged_tile_kernel(RaggedParams p)
 
 // ---- packed prompts: keys and values split once, in tiles as the products read them ----
 //
-// In ragged_tile_kernel the vector units are busier than the matrix units: of some 430 issue slots a wave spends on a tile of 64 keys and 32 rows
-// at depth 64, 150 go into splitting keys and values, which every workgroup does again for its 128 rows.  Where sequences are long enough to
+// In ragged_tile_kernel the vector units are busier than the matrix units: a third of a wave's issue slots go into splitting keys and
+// values, which every workgroup does again for its 128 rows.  Where sequences are long enough to
 // fill tiles, ragged_ready_kernel splits them once, into the order that LDS holds: [tile][key head][keys, then values][plane][block][key or
 // depth][16 bytes], 16 KB each (as many bytes as fp32), with the powers of two beside them.  ragged_packed_kernel's loads then go from memory to
 // LDS past the registers, and the registers hold two tiles' scores: the first product of tile t + 1 runs beside the softmax of tile t.
+// Prompts of 8192 and 4001 rows, 32 / 8 heads of 128, causal: 2.02 ms (382 TFLOP/s) on one card and 2.17 (355) on another, bound by the
+// matrix units at the clock that the power limit leaves; the pass that splits is 0.04 of it.
 __device__ __forceinline__ int64_t ready_tile(const RaggedParams& p, int seq, int first, int keys_a_tile) { return first_tile(first, seq, 1, keys_a_tile); }
 
 template <int D, bool EXACT>
@@ -821,13 +831,15 @@ __global__ __launch_bounds__(256, 2) void ragged_packed_kernel(RaggedParams p)
     }
 }
 
-// ---- few query rows: keys and values pass once, straight from memory to the fp32 matrix instructions ----
+// ---- few query rows: keys and values pass once, straight from memory to the matrix instructions ----
 //
 // A workgroup takes the rows that a sequence brings to one key head, over one range of its keys.  Up to sixteen rows: its four waves take every
 // fourth block of 16 keys; up to thirty-two: two waves for either half of the rows take every second block, and the later one of two that load
-// the same keys finds them in the CU's cache (20 rows each of 32 sequences of 3000 keys,
-// 32 / 8 heads of 128, 231 us with fp32 pages; a workgroup for either half 291).  Waves have sums of their own, which meet at the end.  Bound by memory: a lane's loads are the operands of
-// the 16x16x4 fp32 products, nothing is staged, and a block's loads are on their way while the block before is worked on.
+// the same keys finds them in the CU's cache (20 rows each of 32 sequences of 3000 keys, 32 / 8 heads of 128, 231 us with fp32 pages; a
+// workgroup for either half 291).  Waves have sums of their own, which meet at the end.  Bound by memory: a lane's loads are the operands of the
+// products, nothing is staged, and a block's loads are on their way while the block before is worked on.  A token each for 64 sequences of
+// 4000, 32 / 8 heads of 128: 368 us with fp32 pages (5.7 TB/s), 226 with bf16 pages (4.6 TB/s); 12 heads of 64, 64 sequences of 2000: 165 and
+// 87 us (4.8 and 4.5 TB/s).  One of 201 keys, 12 heads of 64: 8.5 us, a chain of dependent trips to memory.
 //  * S^T = K Q^T: lane (c, g) of 16 x 4 loads chunks of key c, chunk i at depth 4 W i + W g (W elements are 16 bytes), and has scores of keys
 //    4 g .. 4 g + 3 of row c.
 //  * O^T = V^T P^T: lane (c, g) loads depths V c .. V c + V - 1 of keys 4 g .. + 3, so the probabilities it has are the operand, and gets
@@ -1160,6 +1172,8 @@ __global__ __launch_bounds__(256, WIDE ? 2 : 1) void ragged_few_kernel(RaggedPar
 }
 
 // Both in one launch: what is bound by memory runs beside what is bound by the matrix and vector units.  Tiles, which take longest, come first.
+// Twelve sequences of 400 to 12 000 keys that bring 1 to 1024 tokens, 32 / 8 heads of 128, fp32 pages: 350 us, one launch behind the other 417,
+// few-row workgroups spread among the tiles 483.
 template <int D, int KIND>
 __global__ __launch_bounds__(256, 2) void ragged_mixed_kernel(RaggedParams p, unsigned tile_x, unsigned tile_wgs, unsigned few_x)
 {
@@ -1409,7 +1423,7 @@ using namespace fdx;
 
 extern "C" size_t fdx_mha_packed_scratch_bytes(int tokens, int n_seqs, int heads, int kv_heads, int dk, int dv)
 {
-    if (tokens <= 0 || n_seqs <= 0 || heads <= 0 || kv_heads <= 0 || dk <= 0 || dv <= 0)
+    if (tokens <= 0 || n_seqs <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || dk <= 0 || dv <= 0)
         return 0;
     size_t most = 0;
     for (int causal = 0; causal < 2; ++causal) {

@@ -628,6 +628,13 @@ def test_shapes_that_do_not_fit(fdx):
     fdx.kv_append(c, x, x, [5])
     with pytest.raises(fdx.FdxError, match="q of shape"):
         fdx.mha_paged(c, x[:3], [5], 2)
+    for lengths in ([5, 0], [], [-5], [[5]], 5):
+        with pytest.raises(fdx.FdxError, match="1 sequences need"):
+            fdx.mha_paged(c, x, lengths, 2)
+        with pytest.raises(fdx.FdxError, match="1 sequences need"):
+            fdx.kv_append(c, x, x, lengths)
+    with pytest.raises(fdx.FdxError, match="lengths of the packed"):
+        fdx.mha_packed(x, x, x, [7, -2], 2, 2, 64, 64)
     with pytest.raises(fdx.FdxError, match="free pages"):
         d = fdx.PagedCache(1, 16, 2, 64, 64, 2, 40)
         d.grow([16, 1])

@@ -78,6 +78,15 @@ def test_paged_scratch(fdx):
         refused(fdx, fdx.lib.fdx_mha_paged_f32(P, I64(256), P, 5, 2, 4, c, P, I64(256), scratch, None), INVALID, "scratch")
 
 
+@pytest.mark.parametrize("tokens,heads,kv_heads", [(1000, 4, 4), (4000, 16, 16), (300, 16, 1)])
+def test_packed_scratch(fdx, tokens, heads, kv_heads):
+    """Key ranges of a few long prompts and prompts that are split once take memory of the caller's."""
+    assert fdx.lib.fdx_mha_packed_scratch_bytes(tokens, 1, heads, kv_heads, 64, 64) > 0
+    for scratch in (None, ctypes.c_void_p((1 << 20) + 4)):
+        refused(fdx, fdx.lib.fdx_mha_packed_f32(P, I64(64 * heads), P, I64(64 * kv_heads), P, I64(64 * kv_heads), P, 1, tokens, heads, kv_heads, 64, 64, 0,
+                                                P, I64(64 * heads), scratch, None), INVALID, "scratch")
+
+
 def test_packed(fdx):
     def call(q=P, ldq=256, k=P, ldk=128, v=P, ldv=128, starts=P, n_seqs=3, tokens=5, heads=4, kv_heads=2, dk=64, dv=64, out=P, ldo=256):
         return fdx.lib.fdx_mha_packed_f32(q, I64(ldq), k, I64(ldk), v, I64(ldv), starts, n_seqs, tokens, heads, kv_heads, dk, dv, 1, out,
@@ -108,6 +117,11 @@ def test_scores(fdx):
 def test_scratch_sizes_of_refused_calls_are_zero(fdx):
     """A size for arguments that the call itself refuses: an answer, not a crash."""
     assert fdx.lib.fdx_mha_packed_scratch_bytes(0, 1, 1, 1, 64, 64) == 0
+    for heads, kv_heads in ((1, 2), (3, 2), (5, 7)):
+        for tokens in (5, 600, 5000):
+            assert fdx.lib.fdx_mha_packed_scratch_bytes(tokens, 1, heads, kv_heads, 64, 64) == 0
+            refused(fdx, fdx.lib.fdx_mha_packed_f32(P, I64(512), P, I64(512), P, I64(512), P, 1, tokens, heads, kv_heads, 64, 64, 1, P, I64(512), P, None),
+                    INVALID, "share")
     assert fdx.lib.fdx_mha_packed_scratch_bytes(5, 1, 4, 0, 64, 64) == 0
     assert fdx.lib.fdx_mha_paged_scratch_bytes(5, 1, 4, None) == 0
     for change in (dict(kv_heads=0), dict(max_len=0), dict(n_seqs=-3), dict(dk=0), dict(dv=0)):
