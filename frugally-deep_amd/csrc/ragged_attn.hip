@@ -1280,8 +1280,10 @@ static RaggedPlan paged_plan(int tokens, int max_new, int heads, const fdx_kv_pa
         // gaps; 256 keys or more, and 64 ranges or fewer, which one pass of ragged_join_kernel takes.  us with at least 128 / 192 / 256 / 384 / 512
         // keys, fp32: one sequence of 8000, 32 / 8 heads of 128, 28.4 / 29.9 / 26.0 / 28.0 / 31.7; 16 of 1000, 12 heads of 64, 28.1 / 29.2 / 26.4 / 28.9 /
         // 28.9; one of 2000, 12.9 / 13.0 / 13.9 / 16.4 / 18.8; four of 32 000, 8 / 1 heads of 128, 60.9 / 56.3 / 46.7 / 48.0 / 41.0.
-        int64_t keys = c->max_len * items / 4096;
-        keys = keys < 256 ? 256 : keys;
+        // Where 512 keys make 768 workgroups or more, 512: with 256 / 512, 32 / 8 heads of 128, 64 sequences of 1000 112 / 105 (bf16 pages 58.8 / 52.7),
+        // of 100 to 2000 92.3 / 86.7 (50.8 / 43.3), 32 of 3000 with 5 tokens each 237 / 220 (134 / 114); below, eight of 200 to 4000 43.2 / 44.6.
+        const int64_t all = c->max_len * items, least = all >= 512 * 768 ? 512 : 256;
+        const int64_t keys = all / 4096 < least ? least : all / 4096;
         r.few_ranges = ranges_of(c->max_len, keys < c->max_len / 64 ? c->max_len / 64 : keys, &r.few_keys);
         r.few_part = items * (most < r.few_rows ? most : r.few_rows);
     }
