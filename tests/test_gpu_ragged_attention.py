@@ -135,7 +135,7 @@ def test_packed_sizes_behind_the_mask(fdx, lengths, heads, d, power):
 
 
 def test_packed_many_tokens_infinities_and_nan(fdx):
-    """As above where keys and values are split in a pass of their own."""
+    """A NaN or infinity in one of several ranges of keys."""
     r, n, heads, kv = np.random.default_rng(8), 700, 6, 1
     q, k, v = (r.standard_normal((n, h * 64)).astype(np.float32) for h in (heads, kv, kv))
     base = packed_reference(q, k, v, [n], heads, kv, True)
@@ -616,6 +616,55 @@ def test_two_threads(fdx):
         assert all(np.array_equal(got[i][0], x) for x in got[i])
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_offsets_beyond_32_bits(fdx, kind):
+    """Pages whose rows start beyond 2^32 elements of the cache."""
+    heads, kv, d, page, context, new = 16, 8, 128, 16, [90, 40], [1, 33]
+    n_pages = (1 << 32) // (page * kv * d) + 20
+    size = n_pages * page * kv * d * (4 if kind == "f32" else 2)
+    c = fdx.PagedCache(1, page, kv, d, d, 2, 100, kind)
+    c.n_pages, c.k, c.v, c.free = n_pages, fdx.DevBuf(size), fdx.DevBuf(size), [*range(n_pages - 8, n_pages), 3, n_pages // 2 + 1]
+    r = np.random.default_rng(12)
+    keys, values = ([r.standard_normal((n, kv * d)).astype(np.float32) for n in context] for _ in range(2))
+    print("far pages", kind, flush=True)
+    fdx.kv_append(c, np.concatenate(keys), np.concatenate(values), context)
+    if kind == "bf16":
+        keys, values = [bf16(x) for x in keys], [bf16(x) for x in values]
+    q = r.standard_normal((sum(new), heads * d)).astype(np.float32)
+    got = fdx.mha_paged(c, q, new, heads)
+    c.k.free()
+    c.v.free()
+    close(got[:1], attend(q[:1], keys[0], values[0], heads, kv, np.array([90])))
+    close(got[1:], attend(q[1:], keys[1], values[1], heads, kv, np.arange(40 - 33, 40) + 1))
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("new", [1, 70])
+def test_a_long_sequence(fdx, new, kind):
+    """Three million positions, all of them in five pages: the row at position p is row p % 80, so the softmax over all positions is that
+    over 80 rows, each with its number of times.  A range has 3e6 / 16 keys or fewer, a wave's accumulators take 2930 tiles of 64 of them in
+    12 additions each, the sums of weights 16: at most (12 + 16) 2930 roundings of 2^-24 to sums of terms of one sign and size, 5e-3
+    of the largest value."""
+    length, heads, d, page = 3000000, 2, 64, 16
+    r = np.random.default_rng(13)
+    rows = [r.standard_normal((80, d)).astype(np.float32) for _ in range(2)]
+    c = fdx.PagedCache(5, page, 1, d, d, 1, length, kind)
+    fdx.kv_append(c, rows[0], rows[1], [80])
+    first = c.table[0][:5].copy()
+    c.table[0][:] = first[np.arange(c.table.shape[1]) % 5]
+    c.lens[0] = length
+    k, v = (x.astype(np.float64) if kind == "f32" else bf16(x).astype(np.float64) for x in rows)
+    q = r.standard_normal((new, heads * d)).astype(np.float32)
+    print("long", new, kind, flush=True)
+    got = fdx.mha_paged(c, q, [new], heads).reshape(new, heads, d)
+    sees = np.arange(length - new, length) + 1
+    times = sees[:, None] // 80 + (np.arange(80)[None] < sees[:, None] % 80)
+    s = q.reshape(new, heads, d).astype(np.float64) @ k.T / np.sqrt(d)
+    p = np.exp(s - s.max(-1, keepdims=True)) * times[:, None]
+    want = p @ v / p.sum(-1, keepdims=True)
+    assert np.abs(got - want).max() <= 5e-3 * np.abs(v).max()
+
+
 def test_shapes_that_do_not_fit(fdx):
     x = np.zeros((5, 128), np.float32)
     with pytest.raises(fdx.FdxError, match="k of shape"):
@@ -640,3 +689,25 @@ def test_shapes_that_do_not_fit(fdx):
         d.grow([16, 1])
     with pytest.raises(fdx.FdxError, match="overlap"):
         fdx.check(fdx.lib.fdx_kv_append_f32(c.k.ptr, ctypes.c_int64(3), c.v.ptr, ctypes.c_int64(128), c.k.ptr, 1, ctypes.byref(c.pages()), None))
+
+
+def test_packed_rows_beyond_32_bits(fdx):
+    """Rows of q, k, v and out so far apart that the last ones start beyond 2^32 floats."""
+    n, heads, kv, d, ld = 150, 4, 2, 64, (1 << 32) // 140
+    r = np.random.default_rng(14)
+    q, k, v = (r.standard_normal((n, h * d)).astype(np.float32) for h in (heads, kv, kv))
+    buf = fdx.DevBuf(4 * (ld * (n - 1) + 1024))   # columns: q, k, v, out
+    at = [0, heads * d, (heads + kv) * d, (heads + 2 * kv) * d]
+    print("packed far rows", flush=True)
+    for i in range(n):
+        row = np.concatenate([q[i], k[i], v[i]])
+        fdx.check(fdx.lib.fdx_h2d(ctypes.c_void_p(buf.ptr.value + 4 * ld * i), row.ctypes.data_as(ctypes.c_void_p), ctypes.c_size_t(row.nbytes)))
+    p = [ctypes.c_void_p(buf.ptr.value + 4 * x) for x in at]
+    for lengths in ([150], [10, 140]):
+        starts = [0, *np.cumsum(lengths).tolist()]
+        assert call_packed(fdx, p[0], ld, p[1], ld, p[2], ld, starts, n, heads, kv, d, d, p[3], ld) == 0
+        got = np.zeros((n, heads * d), np.float32)
+        for i in range(n):
+            fdx.check(fdx.lib.fdx_d2h(got[i].ctypes.data_as(ctypes.c_void_p), ctypes.c_void_p(p[3].value + 4 * ld * i), ctypes.c_size_t(got[i].nbytes)))
+        close(got, packed_reference(q, k, v, lengths, heads, kv, True))
+    buf.free()

@@ -159,3 +159,25 @@ def test_runs_are_equal(fdx):
     for _ in range(3):
         again = fdx.token_logprobs(x, np.arange(9), 32)
         assert all(np.array_equal(first[name], again[name]) for name in first)
+
+
+@pytest.mark.parametrize("rows,vocab", [(5, 50257), (600, 1021)])   # a row in parts and in one; rows that start beyond 2^32 floats
+def test_rows_beyond_32_bits(fdx, rows, vocab):
+    r, top = np.random.default_rng(7), 5
+    ld = (1 << 32) // (rows - 2) + 3
+    x = r.standard_normal((rows, vocab)).astype(np.float32)
+    buf = fdx.DevBuf(4 * (ld * (rows - 1) + vocab))
+    print("token logprobs far rows", rows, vocab, ld, flush=True)
+    for i in range(rows):
+        fdx.check(fdx.lib.fdx_h2d(ctypes.c_void_p(buf.ptr.value + 4 * ld * i), x[i].ctypes.data_as(ctypes.c_void_p), ctypes.c_size_t(4 * vocab)))
+    ids = r.integers(0, vocab, rows).astype(np.int32)
+    di, dl, dt, dtl = fdx.DevBuf.from_host(ids, np.int32), fdx.DevBuf(4 * rows), fdx.DevBuf(4 * rows * top), fdx.DevBuf(4 * rows * top)
+    scratch = fdx.DevBuf(fdx.lib.fdx_token_logprobs_scratch_bytes(ctypes.c_int64(rows), vocab, top))
+    fdx.check(fdx.lib.fdx_token_logprobs_f32(buf.ptr, ctypes.c_int64(ld), ctypes.c_int64(rows), vocab, di.ptr, top, dl.ptr, None, dt.ptr, dtl.ptr,
+                                             scratch.ptr, None))
+    lp, _ = reference(x)
+    got, best = dl.to_host((rows,)), dt.to_host((rows, top), np.int32)
+    buf.free()
+    want = lp[np.arange(rows), ids]
+    assert (np.abs(got - want) <= 4e-6 + 2.0 ** -22 * np.abs(want)).all()
+    assert np.array_equal(best, np.stack([order(row, top) for row in x]))
