@@ -1253,7 +1253,7 @@ __global__ __launch_bounds__(256) void ragged_join_kernel(RaggedParams p)
 // ragged_tile_kernel in ranges of up to tile_keys.
 struct RaggedPlan {
     int few_rows, few_ranges, few_keys; // few_ranges 0: no such launch
-    int tile_ranges, tile_keys;
+    int tile_ranges, tile_keys, tile_whole;
     int64_t few_part, tile_part; // rows whose sums may be kept
     int64_t tiles;
     int64_t ready; // tiles of split keys and values, for all key heads; 0: none are laid out
@@ -1292,11 +1292,18 @@ static RaggedPlan paged_plan(int tokens, int max_new, int heads, const fdx_kv_pa
     if (most > r.few_rows) {
         r.tiles = tile_numbers(tokens, c->n_seqs, group, 128) * c->kv_heads;
         const int64_t full = ((int64_t)tokens * group + 127) / 128 * c->kv_heads;
-        // Ranges while there are fewer tiles than the 512 workgroups that the GPU takes at once, of 512 to 4096 keys.  us with at most 512 / 1024 /
-        // 2048 / 4096 keys, fp32 pages: 128 new tokens at the end of 8000, 32 / 8 heads of 128 (32 tiles), 91 / 128 / 174 / 316; 512 (128 tiles) 310 / 289 /
-        // 279 / 398; twice 2000 of 3000, 16 / 4 heads of 64 (500 tiles) 206 / 197 / 190 / 166; four times 1000 of 4000 (1000 tiles) 1087 / 982 / 957 / 887.
+        // Ranges while there are fewer tiles than the 512 workgroups that the GPU takes at once, of 192 (deep heads: 128) to 4096 keys.  us with at
+        // least 128 / 192 / 256 / 512 keys, fp32 pages: 128 new tokens of 1000, 12 heads of 64 (12 tiles), 19.6 / 20.9 / 22.5 / 30.9; 512 of 1000 (48 tiles)
+        // 30.0 / 28.8 / 27.7 / 34.3; 471 of 1211, 8 / 1 heads of 128 (30 tiles), 35.4 / 37.6 / 40.0 / 52.1; 32 / 8 heads of 128, 128 of 2000 (32 tiles)
+        // 44.7 / 45.8 / 49.2 / 55.8, 128 of 8000 93.8 / 91.3 / 89.8 / 88.4, four times 128 of 1000 (128 tiles) 62.8 / 62.8 / 62.8 / 75.4.  With at most 512 /
+        // 1024 / 2048 / 4096: twice 2000 of 3000, 16 / 4 heads of 64 (500 tiles) 206 / 197 / 190 / 166; four times 1000 of 4000 (1000 tiles) 1087 / 982 /
+        // 957 / 887.  A sequence of up to eight turns of a tile stays whole, the join costs what ranges save: ten of 386 keys, 16 / 4 heads of 64 (124
+        // tiles), 25.9 whole and 28.8 in two; 16 decode steps of 1000 keys beside a prompt of 256, 12 heads of 64, 37.7 and 38.9 (35.3 with a grid for ranges of 512, of which fewer are empty).
+        const bool deep = c->dk > 64 || c->dv > 64;
+        const int64_t least = deep ? 128 : 192;
+        r.tile_whole = deep ? 256 : 512;
         int64_t keys = full < 512 ? c->max_len / (512 / full) : c->max_len;
-        keys = keys < 512 ? 512 : (keys > 4096 ? 4096 : keys);
+        keys = keys < least ? least : (keys > 4096 ? 4096 : keys);
         r.tile_ranges = ranges_of(c->max_len, keys < c->max_len / 16 ? c->max_len / 16 : keys, &r.tile_keys);
         r.tile_part = (int64_t)tokens * heads;
     }
@@ -1455,7 +1462,7 @@ extern "C" fdx_status fdx_mha_packed_f32(const float* q, int64_t ldq, const floa
     const RaggedPlan plan = packed_plan(tokens, n_seqs, heads, kv_heads, dk, dv, causal);
     p.ready = static_cast<unsigned char*>(scratch_dev);
     p.powers = reinterpret_cast<f32x2_pow*>(p.ready + plan.ready * 32768);
-    p.tile = { static_cast<float*>(scratch_dev), plan.tile_part, plan.tile_ranges, plan.tile_keys, 0 };
+    p.tile = { static_cast<float*>(scratch_dev), plan.tile_part, plan.tile_ranges, plan.tile_keys, plan.tile_whole, 0 };
     ragged_dispatch<kPackedF32>(p, plan);
     profile_end("mha_packed_f32", 0.0, 4.0 * tokens * ((double)heads + kv_heads) * (dk + dv));
     FDX_LAUNCH_CHECK();
@@ -1495,8 +1502,8 @@ extern "C" fdx_status fdx_mha_paged_f32(const float* q, int64_t ldq, const int32
     float* part = static_cast<float*>(scratch_dev);
     p.by_group = make_divisor(p.group);
     p.few_rows = plan.few_rows;
-    p.few = { part, plan.few_part, plan.few_ranges, plan.few_keys, (int)(plan.few_part / ((int64_t)p.n_seqs * p.kv_heads)) };
-    p.tile = { part + plan.few_floats(p.dv), plan.tile_part, plan.tile_ranges, plan.tile_keys, 0 };
+    p.few = { part, plan.few_part, plan.few_ranges, plan.few_keys, 0, (int)(plan.few_part / ((int64_t)p.n_seqs * p.kv_heads)) };
+    p.tile = { part + plan.few_floats(p.dv), plan.tile_part, plan.tile_ranges, plan.tile_keys, plan.tile_whole, 0 };
     profile_begin();
     if (cache->type == FDX_KV_F32)
         ragged_dispatch<kPagedF32>(p, plan);

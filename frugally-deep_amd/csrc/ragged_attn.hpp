@@ -19,6 +19,7 @@ struct PartSums {
     float* at;
     int64_t rows;
     int ranges, keys; // of the longest sequence; keys: what a range has at most
+    int whole;        // sequences of up to so many keys have one range
     int a_head;       // few rows: rows of a sequence and key head
 
     __device__ __forceinline__ float* out(int range, int64_t row, int dv) const { return at + (range * rows + row) * dv; }
@@ -83,7 +84,7 @@ __device__ __forceinline__ Sequence sequence_of(const RaggedParams& p, int index
         s.few = s.span.count * p.group <= p.few_rows;
     }
     const int most = s.few ? p.few.keys : p.tile.keys;
-    if (s.keys > most) {
+    if (s.keys > most && s.keys > (s.few ? p.few.whole : p.tile.whole)) {
         const int parts = (s.keys + most - 1) / most;
         s.range = ((s.keys + parts - 1) / parts + 63) & ~63;
     }
