@@ -68,8 +68,8 @@ __device__ __forceinline__ void store_plain_row(const RaggedParams& p, const Seq
 //  * Bound by the vector units, which split, beside the matrix units: 64 keys take a workgroup 1.9 us alone on its CU at depth 64; four
 //    sequences that bring 1000 tokens to 3000 keys in fp32 pages, 32 / 8 heads of 128, 887 us or 258 TFLOP/s, where three products for one come
 //    to 364 at the rate of a large fp16 product.
-//  * Rows whose sums are not finite (infinite or NaN operands, whether the row sees them or not, and tiles left out above) are taken again by
-//    plain_row.
+//  * Rows whose sums are not finite (infinite or NaN operands, whether the row sees them or not, and tiles left out above) or empty though they
+//    see keys are taken again by plain_row.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 // W elements of a row from depth d on, zeros behind `depth`; EXACT: all are there and lie on vectors
@@ -383,9 +383,9 @@ __device__ __forceinline__ void tile_body(const RaggedParams& p, const Place& pl
                 for (int e = 0; e < 16; e += 2)
                     mx = max3(mx, sacc[kb][e], sacc[kb][e + 1]);
             mx = max_halves(mx);
-            const float to_log2 = fmaxf(q_down * sk.down, 1.17549435e-38f); // above zero: -infinity stays what it is
+            const float step = q_down * sk.down, to_log2 = fmaxf(step, 1.17549435e-38f); // above zero: -infinity stays what it is
             mx *= to_log2;
-            l_run = fits ? l_run : NAN;
+            l_run = fits && step < INFINITY ? l_run : NAN; // an infinite step makes every negative score -infinity
             if (__any(mx > m_run + 4.f) || f != 1.f) {
                 const float m_new = mx > m_run + 4.f ? mx : m_run;
                 const float corr = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
@@ -471,8 +471,9 @@ __device__ __forceinline__ void tile_body(const RaggedParams& p, const Place& pl
 #pragma unroll
         for (int e = 0; e < 16; ++e)
             size += fabsf(oacc[d][e]);
-    // a row's two lanes hold half of its depths each
-    const uint64_t odd_lanes = __ballot(q_ok && !(size < INFINITY));
+    // a row's two lanes hold half of its depths each; a row that sees keys and has no sum (scores of -infinity, or pages that are not there)
+    // is plain_row's to tell apart
+    const uint64_t odd_lanes = __ballot(q_ok && (!(size < INFINITY) || (l_run == 0.f && k_first < visible)));
     uint32_t odd = (uint32_t)odd_lanes | (uint32_t)(odd_lanes >> 32);
     const bool in_parts = visible > s.range;
     if (q_ok && !(odd >> c & 1) && (in_parts ? k_first < visible : place_in.y == 0)) {
@@ -733,9 +734,9 @@ __global__ __launch_bounds__(256, 2) void ragged_packed_kernel(RaggedParams p)
 #pragma unroll
                 for (int e = 0; e < 16; e += 2)
                     mx = max3(mx, sc[kb][e], sc[kb][e + 1]);
-            const float to_log2 = fmaxf(q_down * down.k_down, 1.17549435e-38f); // above zero: -infinity stays what it is
+            const float step = q_down * down.k_down, to_log2 = fmaxf(step, 1.17549435e-38f); // above zero: -infinity stays what it is
             mx = max_halves(mx) * to_log2;
-            l_run = down.k_down == down.k_down ? l_run : NAN; // a tile that is left to plain sums
+            l_run = step < INFINITY ? l_run : NAN; // NaN: a tile that is left to plain sums; an infinite step makes every negative score -infinity
             if (__any(mx > m_run + 4.f) || down.v_down != v_down) {
                 const float m_new = mx > m_run + 4.f ? mx : m_run;
                 const float corr = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
@@ -799,7 +800,7 @@ __global__ __launch_bounds__(256, 2) void ragged_packed_kernel(RaggedParams p)
         for (int e = 0; e < 16; ++e)
             size += fabsf(oacc[d][e]);
     // a row's two lanes hold half of its depths each
-    const uint64_t odd_lanes = __ballot(q_ok && !(size < INFINITY));
+    const uint64_t odd_lanes = __ballot(q_ok && (!(size < INFINITY) || l_run == 0.f));
     uint32_t odd = (uint32_t)odd_lanes | (uint32_t)(odd_lanes >> 32);
     if (q_ok && !(odd >> c & 1)) {
         const float f = v_down / l_run;

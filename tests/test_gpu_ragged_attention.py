@@ -711,3 +711,78 @@ def test_packed_rows_beyond_32_bits(fdx):
             fdx.check(fdx.lib.fdx_d2h(got[i].ctypes.data_as(ctypes.c_void_p), ctypes.c_void_p(p[3].value + 4 * ld * i), ctypes.c_size_t(got[i].nbytes)))
         close(got, packed_reference(q, k, v, lengths, heads, kv, True))
     buf.free()
+
+
+def far_scores(r, n, heads, kv, d, e=80):
+    """Queries and keys whose largest elements, 2^80, meet zeros, so that a product's scale passes fp32's range (the sum of the exponents is more
+    than 156) while its scores, products of 2^60 and -2^60, all equal and about -2^117, do not: with equal scores a row's result is the mean of the
+    values it sees.  Powers of two, so that nothing is rounded."""
+    q, k = np.zeros((n, heads, d), np.float32), np.zeros((n, kv, d), np.float32)
+    q[:, :, 0], k[:, :, 1] = 2.0 ** e, 2.0 ** e
+    q[:, :, 2], k[:, :, 2] = -2.0 ** 60, 2.0 ** 60
+    return q.reshape(n, -1), k.reshape(n, -1), r.standard_normal((n, kv * d)).astype(np.float32)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lengths,heads,kv_heads", [([40, 1, 150], 4, 2), ([300], 7, 1), ([1500], 4, 4), ([400], 6, 1), ([511, 300, 0, 1], 16, 1), ([2100], 1, 1)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_packed_scores_far_below_zero(fdx, lengths, heads, kv_heads, d, causal):
+    """No score is near zero: a row's sums are those of its largest scores, however small these are.  Sequences in tiles, in ranges of keys, and
+    with keys that are split once.  The mean of n values that are added in a chain: 0.42 * 2^-24 of the partial sum, some sqrt(i), a step, so
+    0.3 * 2^-24 sqrt(n) of the result, 8e-7 for 2100; twice the usual bound."""
+    print("packed far below zero", lengths, heads, kv_heads, d, causal, flush=True)
+    q, k, v = far_scores(np.random.default_rng(15), sum(lengths), heads, kv_heads, d)
+    close(fdx.mha_packed(q, k, v, lengths, heads, kv_heads, d, d, causal), packed_reference(q, k, v, lengths, heads, kv_heads, causal), 2e-6)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("context,new", [([90], [1]), ([300, 17], [5, 1]), ([150], [60]), ([150, 700], [1, 140]), ([2500, 64], [70, 64])])
+def test_paged_scores_far_below_zero(fdx, context, new, kind):
+    heads, kv, d, page = 4, 2, 64, 16
+    r, total = np.random.default_rng(16), sum(context)
+    q, k, v = far_scores(r, total, heads, kv, d)
+    q = q[:sum(new)]
+    print("paged far below zero", context, new, kind, flush=True)
+    cache = fdx.PagedCache(sum(-(-n // page) for n in context), page, kv, d, d, len(context), max(context), kind)
+    fdx.kv_append(cache, k, v, context)
+    if kind == "bf16":
+        v = bf16(v)
+    want, at, row = [], 0, 0
+    for length, n in zip(context, new):
+        want.append(attend(q[row:row + n], k[at:at + length], v[at:at + length], heads, kv, np.arange(length - n, length) + 1))
+        at, row = at + length, row + n
+    close(fdx.mha_paged(cache, q, new, heads), np.concatenate(want), 2e-6)
+
+
+@pytest.mark.parametrize("new", [1, 4, 60])
+def test_scores_far_below_zero_beside_others(fdx, new):
+    """Scores of -2^110 / 8, and one of -2^102 / 8 in a tile whose keys' scale passes fp32's range: the row sees that one alone.  (2^42 beside
+    2^80 is the last bit that a tile of keys holds.)"""
+    heads, kv, d, n = 4, 2, 64, 192
+    q, k, v = far_scores(np.random.default_rng(17), n, heads, kv, d)
+    k = k.reshape(n, kv, d)
+    k[:, :, 1], k[:, :, 2] = 2.0 ** 60, 2.0 ** 50
+    k[64:128, :, 1] = 2.0 ** 68   # near enough to 2^80 for one scale
+    k[70, :, 1], k[70, :, 2] = 2.0 ** 80, 2.0 ** 42
+    k = k.reshape(n, -1)
+    for lengths in ([n], [100, 92]):
+        print("far below zero beside others", lengths, flush=True)
+        close(fdx.mha_packed(q, k, v, lengths, heads, kv, d, d), packed_reference(q, k, v, lengths, heads, kv, True))
+    cache = fdx.PagedCache(12, 16, kv, d, d, 1, n)
+    fdx.kv_append(cache, k, v, [n])
+    close(fdx.mha_paged(cache, q[-new:], [new], heads), attend(q[-new:], k, v, heads, kv, np.arange(n - new, n) + 1))
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_past_the_range_of_fp32(fdx, sign):
+    """Scores of +-2^160: infinite in fp32, all of them, so no row has a softmax; NaN whatever path takes it."""
+    heads, kv, d = 4, 2, 64
+    for lengths, h, g in (([40, 30], heads, kv), ([400], 6, 1), ([1500], 4, 4)):
+        n = sum(lengths)
+        q, k, v = np.full((n, h * d), sign * 2.0 ** 80, np.float32), np.full((n, g * d), 2.0 ** 80, np.float32), np.ones((n, g * d), np.float32)
+        print("scores past fp32", sign, lengths, flush=True)
+        assert np.isnan(fdx.mha_packed(q, k, v, lengths, h, g, d, d)).all()
+    cache = fdx.PagedCache(10, 16, kv, d, d, 1, 160)
+    fdx.kv_append(cache, np.full((150, kv * d), 2.0 ** 80, np.float32), np.ones((150, kv * d), np.float32), [150])
+    for new in (1, 5, 60, 140):
+        assert np.isnan(fdx.mha_paged(cache, np.full((new, heads * d), sign * 2.0 ** 80, np.float32), [new], heads)).all()
