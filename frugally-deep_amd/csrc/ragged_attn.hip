@@ -1305,7 +1305,11 @@ static RaggedPlan paged_plan(int tokens, int max_new, int heads, const fdx_kv_pa
         r.tile_whole = deep ? 256 : 512;
         int64_t keys = full < 512 ? c->max_len / (512 / full) : c->max_len;
         keys = keys < least ? least : (keys > 4096 ? 4096 : keys);
-        r.tile_ranges = ranges_of(c->max_len, keys < c->max_len / 16 ? c->max_len / 16 : keys, &r.tile_keys);
+        // At most 16 ranges, and 16 384 workgroups of tiles and ranges: every range keeps sums of all rows, so scratch memory ends at 2^21 rows of
+        // them, 1.02 GiB at depth 128.  Without and with that limit, 32 / 8 heads of 128: twice 4096 new tokens of 131 072 55.4 / 55.2 ms (2.2 / 1.1 GB); 128
+        // of 131 072 beside 16 prompts of 512, whose sums nobody needs, 1.77 / 2.24 ms (2.3 / 1.0 GB).
+        const int64_t ranges = 16384 / full < 1 ? 1 : (16384 / full < 16 ? 16384 / full : 16), share = (c->max_len + ranges - 1) / ranges;
+        r.tile_ranges = ranges_of(c->max_len, keys < share ? share : keys, &r.tile_keys);
         r.tile_part = (int64_t)tokens * heads;
     }
     return r;

@@ -403,7 +403,7 @@ fdx_status fdx_kv_append_f32(const float* k, int64_t ldk, const float* v, int64_
  * A token that sees no position (lens[i] < n) gets zeros; rows that belong to no sequence stay as they are.  Positions whose page
  * number is not one of the cache are left out of the sums, lens beyond max_len and tokens beyond max_new are cut, and
  * error_flag_dev (may be NULL) is set to 1 on the device.  Depths up to 128.  scratch_dev as for fdx_mha_packed_f32, of
- * fdx_mha_paged_scratch_bytes bytes; `out` must not overlap an input.
+ * fdx_mha_paged_scratch_bytes bytes, which grow with tokens * heads and max_len up to 1.2 GiB; `out` must not overlap an input.
  */
 size_t fdx_mha_paged_scratch_bytes(int tokens, int max_new, int heads, const fdx_kv_pages* cache);
 fdx_status fdx_mha_paged_f32(const float* q, int64_t ldq, const int32_t* starts, int tokens, int max_new, int heads,

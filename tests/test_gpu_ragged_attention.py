@@ -786,3 +786,21 @@ def test_scores_past_the_range_of_fp32(fdx, sign):
     fdx.kv_append(cache, np.full((150, kv * d), 2.0 ** 80, np.float32), np.ones((150, kv * d), np.float32), [150])
     for new in (1, 5, 60, 140):
         assert np.isnan(fdx.mha_paged(cache, np.full((new, heads * d), sign * 2.0 ** 80, np.float32), [new], heads)).all()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_paged_ranges_of_many_tokens(fdx, kind):
+    """2000 tiles in a cache of up to 131 072 positions: eight ranges of 16 384 keys, no more than scratch memory of 1 GiB holds; a few rows of
+    each sequence are looked at.  Bound: 5e-7 of the operands as above; an accumulator adds three products for 16 keys, 1880 in a range of 10 000 keys,
+    each rounded by 0.29 of the last bit, some 0.42 * 2^-24 of a partial sum that grows with their root: 0.42 * 2^-24 sqrt(1880 / 2) = 8e-7 of the
+    result; sqrt(5^2 + 8^2) e-7 = 9.4e-7 are to be expected, twice that allowed."""
+    context, new, heads, kv, d = [20000, 16500, 300], [3900, 60, 40], 64, 8, 64
+    print("paged ranges of many tokens", kind, flush=True)
+    f = Filled(fdx, context, kv, d, d, 64, kind, seed=18, steps=1, max_len=131072)
+    q = np.random.default_rng(19).standard_normal((sum(new), heads * d)).astype(np.float32)
+    got, at = fdx.mha_paged(f.cache, q, new, heads), 0
+    for s, n in enumerate(new):
+        rows = np.unique([0, n // 3, n - 1])
+        sees = context[s] - n + 1 + rows
+        close(got[at + rows], attend(q[at + rows], f.keys[s], f.values[s], heads, kv, sees), 2e-6)
+        at += n

@@ -78,6 +78,23 @@ def test_paged_scratch(fdx):
         refused(fdx, fdx.lib.fdx_mha_paged_f32(P, I64(256), P, 5, 2, 4, c, P, I64(256), scratch, None), INVALID, "scratch")
 
 
+@pytest.mark.parametrize("max_len", [257, 4097, 32769, 131072, 1 << 30])
+@pytest.mark.parametrize("heads,kv_heads", [(32, 8), (12, 12), (8, 1), (64, 1)])
+def test_paged_scratch_is_bounded(fdx, max_len, heads, kv_heads):
+    """Sums of key ranges: of 2^21 rows for tiles, and of some 2^18 for few rows (4096 workgroups and one more for each sequence and key head, of which
+    there are fewer than that, 32 rows each), however many tokens and sequences a call has and however long they may get."""
+    most = 0
+    for dv in (1, 64, 128):
+        for n_seqs in (1, 3, 64, 500, 4000, 1 << 18):
+            c = ctypes.byref(pages(fdx, page_size=1 << 20, n_pages=1 << 10, table_width=1 << 10, kv_heads=kv_heads, dv=dv, n_seqs=n_seqs, max_len=max_len))
+            for tokens in (1, 100, 1000, 2000, 4000, 8192, 16384, 1 << 16, (1 << 25) // heads):
+                for max_new in (1, 5, tokens):
+                    need = fdx.lib.fdx_mha_paged_scratch_bytes(tokens, max_new, heads, c)
+                    assert need <= 4 * (dv + 2) * ((1 << 21) + (1 << 18) + (1 << 14)), (n_seqs, tokens, max_new, need)
+                    most = max(most, need)
+    assert max_len == 257 or most > 0
+
+
 @pytest.mark.parametrize("tokens,heads,kv_heads", [(1000, 4, 4), (4000, 16, 16), (300, 16, 1)])
 def test_packed_scratch(fdx, tokens, heads, kv_heads):
     """Key ranges of a few long prompts and prompts that are split once take memory of the caller's."""
