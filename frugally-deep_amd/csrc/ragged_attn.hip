@@ -1285,7 +1285,8 @@ static RaggedPlan paged_plan(int tokens, int max_new, int heads, const fdx_kv_pa
         // of 100 to 2000 92.3 / 86.7 (50.8 / 43.3), 32 of 3000 with 5 tokens each 237 / 220 (134 / 114); below, eight of 200 to 4000 43.2 / 44.6.
         const int64_t all = c->max_len * items, least = all >= 512 * 768 ? 512 : 256;
         const int64_t keys = all / 4096 < least ? least : all / 4096;
-        r.few_ranges = ranges_of(c->max_len, keys < c->max_len / 64 ? c->max_len / 64 : keys, &r.few_keys);
+        const int64_t share = ((int64_t)c->max_len + 63) / 64;
+        r.few_ranges = ranges_of(c->max_len, keys < share ? share : keys, &r.few_keys);
         r.few_part = items * (most < r.few_rows ? most : r.few_rows);
     }
     if (r.few_ranges == 0)
@@ -1331,7 +1332,8 @@ static RaggedPlan packed_plan(int tokens, int n_seqs, int heads, int kv_heads, i
     if (length >= 512 && full <= (causal ? 192 : 128)) {
         int64_t keys = length / (512 / full);
         keys = keys < 256 ? 256 : keys;
-        keys = keys < tokens / 16 ? tokens / 16 : keys; // at most 16 ranges, whose sums take scratch memory
+        const int64_t share = ((int64_t)tokens + 15) / 16; // at most 16 ranges, whose sums take scratch memory
+        keys = keys < share ? share : keys;
         if (keys < length) {
             r.tile_ranges = ranges_of(tokens, keys, &r.tile_keys);
             r.tile_part = (int64_t)tokens * heads;

@@ -95,6 +95,16 @@ def test_paged_scratch_is_bounded(fdx, max_len, heads, kv_heads):
     assert max_len == 257 or most > 0
 
 
+def test_numbers_of_ranges(fdx):
+    """Up to 64 for few rows and 16 for tiles, where the length leaves a remainder too; sums of a row and range are m, l and `depth` values."""
+    for max_len in [16385, 32768, 32769, 40000, 65535, 65537, (1 << 20) + 1] + list(range(33000, 36000, 7)):
+        c = ctypes.byref(pages(fdx, page_size=1 << 20, n_pages=1 << 10, table_width=1 << 10, kv_heads=1, dv=62, n_seqs=1, max_len=max_len))
+        assert 0 < fdx.lib.fdx_mha_paged_scratch_bytes(1, 1, 1, c) <= 64 * 4 * 64, max_len
+        assert 0 < fdx.lib.fdx_mha_paged_scratch_bytes(1000, 1000, 1, c) - fdx.lib.fdx_mha_paged_scratch_bytes(32, 32, 1, c) <= 16 * 4 * 64 * 1000
+    for tokens in range(4096, 9000):
+        assert fdx.lib.fdx_mha_packed_scratch_bytes(tokens, tokens // 512, 1, 1, 62, 62) <= 16 * 4 * 64 * tokens, tokens
+
+
 @pytest.mark.parametrize("tokens,heads,kv_heads", [(1000, 4, 4), (4000, 16, 16), (300, 16, 1)])
 def test_packed_scratch(fdx, tokens, heads, kv_heads):
     """Key ranges of a few long prompts and prompts that are split once take memory of the caller's."""
