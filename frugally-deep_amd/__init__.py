@@ -680,18 +680,26 @@ class PagedCache:
 
 
 def kv_append(cache, k, v, lengths):
-    """Adds lengths[i] rows of k [tokens,kv_heads*dk] and v [tokens,kv_heads*dv] to sequence i of a PagedCache."""
+    """Adds lengths[i] rows of k [tokens,kv_heads*dk] and v [tokens,kv_heads*dv] to sequence i of a PagedCache, all of them or none."""
     k, v = np.ascontiguousarray(k, np.float32), np.ascontiguousarray(v, np.float32)
     rows = int(cache.lengths_of(lengths).sum())
     _rows_of(rows, k=(k, cache.kv_heads * cache.dk), v=(v, cache.kv_heads * cache.dv))
+    before, used = cache.lens, (cache.table >= 0).sum(1)
     cache.grow(lengths)
     if rows == 0:
         return
-    dk_, dv_, starts, pages = DevBuf.from_host(k), DevBuf.from_host(v), _row_starts(lengths), cache.pages()
-    flag = DevBuf.from_host(np.zeros(1, np.int32), np.int32)
-    check(lib.fdx_kv_append_f32(_dp(dk_), ctypes.c_int64(k.shape[1]), _dp(dv_), ctypes.c_int64(v.shape[1]), starts.ptr, k.shape[0],
-                                ctypes.byref(pages), flag.ptr))
-    _raise_if_set(flag, "rows outside the cache")
+    try:
+        dk_, dv_, starts, pages = DevBuf.from_host(k), DevBuf.from_host(v), _row_starts(lengths), cache.pages()
+        flag = DevBuf.from_host(np.zeros(1, np.int32), np.int32)
+        check(lib.fdx_kv_append_f32(_dp(dk_), ctypes.c_int64(k.shape[1]), _dp(dv_), ctypes.c_int64(v.shape[1]), starts.ptr, k.shape[0],
+                                    ctypes.byref(pages), flag.ptr))
+        _raise_if_set(flag, "rows outside the cache")
+    except BaseException:   # no length counts rows that may not have been written
+        cache.lens = before
+        for row, count in reversed(list(zip(cache.table, used))):
+            cache.free += [int(page) for page in row[count:][::-1] if page >= 0]
+            row[count:] = -1
+        raise
 
 
 def mha_paged(cache, q, lengths, heads):

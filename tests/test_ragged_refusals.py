@@ -4,6 +4,7 @@ import ctypes
 import os
 import subprocess
 
+import numpy as np
 import pytest
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -166,3 +167,50 @@ def test_rows_and_pages_on_the_host(tmp_path):
                            "-o", exe])
     out = subprocess.run([exe], capture_output=True, text=True, timeout=300, env=dict(os.environ, ASAN_OPTIONS="detect_leaks=0"))
     assert out.returncode == 0 and "kv_pages done" in out.stdout, (out.stdout, out.stderr[-3000:])
+
+
+class HostBuf:
+    """Memory that no call looks into."""
+
+    def __init__(self, nbytes=0):
+        self.ptr = P
+
+    @classmethod
+    def from_host(cls, arr, dtype=None):
+        return cls()
+
+
+def cache_on_host(fdx, monkeypatch, **change):
+    args = dict(n_pages=9, page_size=4, kv_heads=2, dk=8, dv=6, n_seqs=3, max_len=20)
+    args.update(change)
+    monkeypatch.setattr(fdx, "DevBuf", HostBuf)
+    return fdx.PagedCache(**args)
+
+
+@pytest.mark.parametrize("how", ["memory", "call", "flag"])
+def test_append_that_fails_leaves_the_cache(fdx, monkeypatch, how):
+    """Lengths, page table and free pages (their order too) are those in front of the call, and the next call takes the same pages."""
+    cache = cache_on_host(fdx, monkeypatch)
+    cache.grow([5, 0, 4])
+    table, lens, free = cache.table.copy(), cache.lens.copy(), list(cache.free)
+    k, v = np.zeros((12, 16), np.float32), np.zeros((12, 12), np.float32)
+
+    def fail(*args):
+        raise fdx.FdxError("failed on purpose")
+    with monkeypatch.context() as m:
+        m.setattr(fdx, "check", fail if how == "call" else lambda status: None)
+        m.setattr(fdx, "_raise_if_set", fail if how == "flag" else lambda flag, message: None)
+        m.setattr(fdx.lib, "fdx_kv_append_f32", lambda *args: 0)
+        if how == "memory":
+            m.setattr(HostBuf, "from_host", classmethod(lambda cls, arr, dtype=None: fail()))
+        with pytest.raises(fdx.FdxError, match="on purpose"):
+            fdx.kv_append(cache, k, v, [2, 9, 1])
+    assert np.array_equal(cache.table, table) and np.array_equal(cache.lens, lens) and cache.free == free
+    with pytest.raises(fdx.FdxError, match="free pages"):
+        fdx.kv_append(cache, np.zeros((34, 16), np.float32), np.zeros((34, 12), np.float32), [8, 17, 9])
+    assert np.array_equal(cache.table, table) and np.array_equal(cache.lens, lens) and cache.free == free
+    with monkeypatch.context() as m:
+        m.setattr(fdx, "_raise_if_set", lambda flag, message: None)
+        m.setattr(fdx.lib, "fdx_kv_append_f32", lambda *args: 0)
+        fdx.kv_append(cache, k, v, [2, 9, 1])
+    assert cache.lens.tolist() == [7, 9, 5] and sorted(cache.free + [int(x) for x in cache.table.ravel() if x >= 0]) == list(range(9))
