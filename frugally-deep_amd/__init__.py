@@ -624,6 +624,8 @@ def mha_packed(q, k, v, lengths, heads, kv_heads, dk, dv, causal=True):
     q, k, v = (np.ascontiguousarray(a, np.float32) for a in (q, k, v))
     tokens = q.shape[0]
     _rows_of(tokens, q=(q, heads * dk), k=(k, kv_heads * dk), v=(v, kv_heads * dv))
+    if tokens == 0 and not np.any(lengths):
+        return np.zeros((0, heads * dv), np.float32)
     dq, dk_, dv_, starts = DevBuf.from_host(q), DevBuf.from_host(k), DevBuf.from_host(v), _row_starts(lengths)
     scratch = DevBuf(lib.fdx_mha_packed_scratch_bytes(tokens, len(lengths), heads, kv_heads, dk, dv))
     out, flag = DevBuf.from_host(np.zeros((tokens, heads * dv), np.float32)), DevBuf.from_host(np.zeros(1, np.int32), np.int32)
@@ -708,6 +710,8 @@ def mha_paged(cache, q, lengths, heads):
     lengths = cache.lengths_of(lengths)
     tokens, most = q.shape[0], int(lengths.max())
     _rows_of(int(lengths.sum()), q=(q, heads * cache.dk))
+    if tokens == 0:
+        return np.zeros((0, heads * cache.dv), np.float32)
     dq, starts, pages = DevBuf.from_host(q), _row_starts(lengths), cache.pages()
     scratch = DevBuf(lib.fdx_mha_paged_scratch_bytes(tokens, most, heads, ctypes.byref(pages)))
     out = DevBuf.from_host(np.zeros((tokens, heads * cache.dv), np.float32))

@@ -214,3 +214,21 @@ def test_append_that_fails_leaves_the_cache(fdx, monkeypatch, how):
         m.setattr(fdx.lib, "fdx_kv_append_f32", lambda *args: 0)
         fdx.kv_append(cache, k, v, [2, 9, 1])
     assert cache.lens.tolist() == [7, 9, 5] and sorted(cache.free + [int(x) for x in cache.table.ravel() if x >= 0]) == list(range(9))
+
+
+def test_nothing_new(fdx, monkeypatch):
+    """Batches without a row: nothing to write, no rows of attention; shapes are checked all the same."""
+    cache = cache_on_host(fdx, monkeypatch)
+    cache.grow([5, 0, 4])
+    none = lambda width: np.zeros((0, width), np.float32)
+    fdx.kv_append(cache, none(16), none(12), [0, 0, 0])
+    assert cache.lens.tolist() == [5, 0, 4]
+    assert fdx.mha_paged(cache, none(32), [0, 0, 0], 4).shape == (0, 24)
+    for lengths in ([0, 0], []):
+        assert fdx.mha_packed(none(32), none(16), none(12), lengths, 4, 2, 8, 6).shape == (0, 24)
+    with pytest.raises(fdx.FdxError, match="q of shape"):
+        fdx.mha_paged(cache, none(32), [0, 1, 0], 4)
+    with pytest.raises(fdx.FdxError, match="q of shape"):
+        fdx.mha_paged(cache, none(16), [0, 0, 0], 4)
+    with pytest.raises(fdx.FdxError, match="v of shape"):
+        fdx.mha_packed(none(32), none(16), none(16), [0], 4, 2, 8, 6)
