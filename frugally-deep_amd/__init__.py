@@ -604,6 +604,14 @@ def mha_decode(q, k_cache, v_cache, heads, dk, dv, length):
     return out.to_host((b, heads * dv))
 
 
+def _whole(name, numbers):
+    """numbers as int64, none of them changed on the way"""
+    a = np.asarray(numbers)
+    if a.dtype.kind not in "biuf" or not ((a == np.floor(a)) & (a >= -2.0 ** 63) & (a < 2.0 ** 63)).all():
+        raise FdxError("%s must be whole numbers of up to 63 bits" % name)
+    return a.astype(np.int64)
+
+
 def _row_starts(lengths):
     return DevBuf.from_host(np.concatenate([[0], np.cumsum(lengths)]).astype(np.int32), np.int32)
 
@@ -622,9 +630,11 @@ def _raise_if_set(flag, message):
 def mha_packed(q, k, v, lengths, heads, kv_heads, dk, dv, causal=True):
     """q [tokens,heads*dk], k [tokens,kv_heads*dk], v [tokens,kv_heads*dv]: sequences of `lengths` rows, one behind the other."""
     q, k, v = (np.ascontiguousarray(a, np.float32) for a in (q, k, v))
-    tokens = q.shape[0]
+    tokens, lengths = q.shape[0], _whole("lengths", lengths).reshape(-1)
+    if (lengths < 0).any() or (lengths > tokens).any() or lengths.sum() > tokens:
+        raise FdxError("lengths of the packed sequences exceed the rows")
     _rows_of(tokens, q=(q, heads * dk), k=(k, kv_heads * dk), v=(v, kv_heads * dv))
-    if tokens == 0 and not np.any(lengths):
+    if tokens == 0:
         return np.zeros((0, heads * dv), np.float32)
     dq, dk_, dv_, starts = DevBuf.from_host(q), DevBuf.from_host(k), DevBuf.from_host(v), _row_starts(lengths)
     scratch = DevBuf(lib.fdx_mha_packed_scratch_bytes(tokens, len(lengths), heads, kv_heads, dk, dv))
@@ -651,7 +661,7 @@ class PagedCache:
         self.free = list(range(n_pages - 1, -1, -1))
 
     def lengths_of(self, lengths):
-        lengths = np.asarray(lengths, np.int64)
+        lengths = _whole("lengths", lengths)
         if lengths.shape != (self.n_seqs,) or lengths.min() < 0:
             raise FdxError("%d sequences need as many numbers of new rows, not %s" % (self.n_seqs, lengths.tolist()))
         return lengths
@@ -727,8 +737,13 @@ def token_logprobs(logits, ids=None, top=0):
     top_ids and top_logprobs [rows,top] (if top > 0)."""
     logits = np.ascontiguousarray(logits, np.float32)
     rows, vocab = logits.shape
-    if ids is not None and np.shape(ids) != (rows,):
-        raise FdxError("ids of shape %s for %d rows" % (np.shape(ids), rows))
+    if ids is not None:
+        if np.shape(ids) != (rows,):
+            raise FdxError("ids of shape %s for %d rows" % (np.shape(ids), rows))
+        ids = _whole("ids", ids)
+        if (ids >= vocab).any():
+            raise FdxError("token ids must be less than the number of logits")
+        ids = np.maximum(ids, -1)
     dx = DevBuf.from_host(logits)
     di = None if ids is None else DevBuf.from_host(ids, np.int32)
     dl, de = (None if ids is None else DevBuf(4 * rows)), DevBuf(4 * rows)

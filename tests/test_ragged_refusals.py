@@ -232,3 +232,33 @@ def test_nothing_new(fdx, monkeypatch):
         fdx.mha_paged(cache, none(16), [0, 0, 0], 4)
     with pytest.raises(fdx.FdxError, match="v of shape"):
         fdx.mha_packed(none(32), none(16), none(16), [0], 4, 2, 8, 6)
+
+
+@pytest.mark.parametrize("lengths", [[2.5, 2.5], [float("nan"), 5], [1e30, 5], [2**32, 5], [2**32 - 3, 8], [2**63 - 1, 2**63 - 1], [2**64 - 1, 6], [5, 1],
+                                     [7, -2], ["5"], [None]])
+def test_lengths_that_are_none(fdx, monkeypatch, lengths):
+    """Numbers that 32 bits or whole numbers would make others of are refused before anything is cut or kept."""
+    cache = cache_on_host(fdx, monkeypatch, n_seqs=2)
+    q, k, v = np.zeros((5, 32), np.float32), np.zeros((5, 16), np.float32), np.zeros((5, 12), np.float32)
+    with pytest.raises(fdx.FdxError, match="lengths"):
+        fdx.mha_packed(q, k, v, lengths, 4, 2, 8, 6)
+    with pytest.raises(fdx.FdxError):
+        fdx.kv_append(cache, k, v, lengths)
+    with pytest.raises(fdx.FdxError):
+        fdx.mha_paged(cache, q, lengths, 4)
+    assert cache.lens.tolist() == [0, 0]
+
+
+@pytest.mark.parametrize("ids", [[0, 10], [0, 2**31], [2**32, 1], [2**32 + 3, 1], [0, 2**63], [2**64 - 1, 1], [0.5, 1], [1e30, 0], [float("nan"), 0], ["0", "1"]])
+def test_ids_that_are_none(fdx, monkeypatch, ids):
+    monkeypatch.setattr(fdx, "DevBuf", HostBuf)
+    with pytest.raises(fdx.FdxError, match="less than the number of logits|whole numbers"):
+        fdx.token_logprobs(np.zeros((2, 10), np.float32), ids)
+
+
+def test_numbers_in_any_type(fdx):
+    """Whole numbers of every type are taken as they are."""
+    for dtype in (np.int8, np.uint8, np.int32, np.int64, np.uint64, np.float32, np.float64):
+        assert fdx._whole("ids", np.array([0, 7, 100], dtype)).tolist() == [0, 7, 100]
+    assert fdx._whole("ids", [-2**63, 2**62 + 1, True]).tolist() == [-2**63, 2**62 + 1, 1]
+    assert fdx._whole("lengths", []).shape == (0,) and fdx._whole("lengths", 5).shape == ()
