@@ -143,8 +143,8 @@ __device__ __forceinline__ void tile_body(const RaggedParams& p, const Place& pl
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 31, half = lane >> 5;
     if (p.error_flag && place_in.x == 0 && place_in.y == 0)
-        for (int i = tid; i < p.n_seqs; i += 256)
-            raise_flag(p, !packed_start_ok(p.starts, i, p.tokens));
+        for (int i = tid; i < p.n_seqs; i += 256) // lengths too: a sequence without new tokens has no tile
+            raise_flag(p, !packed_start_ok(p.starts, i, p.tokens) || (kPaged && (p.lens[i] < 0 || p.lens[i] > p.max_len)));
     // key heads next to each other: consecutive workgroups go to the eight XCDs in turn, so that an XCD's cache holds few heads'
     // keys; later tiles of a sequence, which see more keys, first
     const int kv_head = place_in.x % p.kv_heads;

@@ -804,3 +804,20 @@ def test_paged_ranges_of_many_tokens(fdx, kind):
         sees = context[s] - n + 1 + rows
         close(got[at + rows], attend(q[at + rows], f.keys[s], f.values[s], heads, kv, sees), 2e-6)
         at += n
+
+
+@pytest.mark.parametrize("heads", [4, 40])
+def test_paged_lengths_of_sequences_without_new_tokens(fdx, heads):
+    """A length that is none is reported whether its sequence brings rows or not, also where many heads share a key head; the others' rows are right."""
+    kv, d = 1, 64
+    f = Filled(fdx, [90, 131, 20], kv, d, d, 16, "f32")
+    for new in ([1, 0, 1], [50, 0, 1]):
+        tokens = sum(new)
+        q = np.random.default_rng(20).standard_normal((tokens, heads * d)).astype(np.float32)
+        dq, out = fdx.DevBuf.from_host(q), fdx.DevBuf(q.nbytes)
+        for length, flag in ((131, 0), (132, 1), (-1, 1), (0, 0), (2**31 - 1, 1), (-2**31, 1)):
+            print("paged lengths without tokens", heads, new, length, flush=True)
+            assert call_paged(fdx, f.cache, dq.ptr, heads * d, np.concatenate([[0], np.cumsum(new)]), tokens, max(new), heads, out.ptr, heads * d,
+                              lens=[90, length, 20]) == flag
+            close(out.to_host(q.shape), np.concatenate([attend(q[:new[0]], f.keys[0], f.values[0], heads, kv, np.arange(90 - new[0], 90) + 1),
+                                                        attend(q[new[0]:], f.keys[2], f.values[2], heads, kv, np.array([20]))]))
