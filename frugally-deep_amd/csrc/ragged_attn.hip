@@ -61,8 +61,8 @@ __device__ __forceinline__ void store_plain_row(const RaggedParams& p, const Seq
 //    which lane l of the N has.  Keys lie as [plane][depth block][key][16 bytes], which the first product reads as it is; values as
 //    [plane][key][depth], and the transposing LDS read gives the second product four keys of a depth at a time.
 //  * A query row, a tile's keys and its values are each brought to fp16's range by a power of two.  The sums have the power of the last
-//    tile's values, which changes with one that is another multiple of four.  A tile whose rows are too far apart in size for one power
-//    (spread_fits; a row of 10^30 behind the mask) is left to plain sums.
+//    tile's values that are not all zeros, which changes with one that is another multiple of four.  A tile whose rows are too far apart in
+//    size for one power (spread_fits; a row of 10^30 behind the mask) is left to plain sums.
 //  * The maximum that a row's exponentials refer to moves only when a score passes it by 2^4, so sums are rescaled a few times a row
 //    instead of every tile; exponentials carry 2^10 to stay clear of fp16's small end, at most 2^14.
 //  * Bound by the vector units, which split, beside the matrix units: 64 keys take a workgroup 1.9 us alone on its CU at depth 64; four
@@ -283,8 +283,9 @@ __device__ __forceinline__ void tile_body(const RaggedParams& p, const Place& pl
     for (int d = 0; d < DB; ++d)
         oacc[d] = kZero;
     float m_run = -INFINITY, l_run = 0.f;
-    // of the tile at work (sv: of the sums) and of the one behind it
-    Pow2 sk = pow2_for<1>(0), sv = pow2_for<4>(0), sk_next = sk, sv_next = sv;
+    // of the tile at work and of the one behind it
+    Pow2 sk = pow2_for<1>(0), sk_next = sk, sv_next = pow2_for<4>(0);
+    float v_down = 0.f; // of the sums; 0 while all values were zeros
     bool fits = true, fits_next = true;
     auto scale_next = [&](int t) {
         const Spread* r = spread[t & 1];
@@ -292,6 +293,7 @@ __device__ __forceinline__ void tile_body(const RaggedParams& p, const Place& pl
         fits_next = spread_fits(top, low);
         sk_next = pow2_for<1>(top[0]);
         sv_next = pow2_for<4>(top[1]);
+        sv_next.down = low[1] == 0 ? 0.f : sv_next.down; // values that are all zeros take any power
     };
     auto stage = [&](unsigned char* ks, unsigned char* vs) {
 #pragma unroll
@@ -323,11 +325,8 @@ __device__ __forceinline__ void tile_body(const RaggedParams& p, const Place& pl
     auto turn = [&](int t, const unsigned char* ks, const unsigned char* vs, unsigned char* ks_next, unsigned char* vs_next) {
         const int j0 = k_first + t * KT;
         const bool work = j0 < wave_any; // some row of this wave sees some key of the tile
-        float f = sv_next.up * sv.down;
-        f = t == 0 || (f > 1e-18f && f < 1e18f) ? f : NAN; // sums that would leave fp32's range
+        const float f = sv_next.up * v_down, down = sv_next.down;
         sk = sk_next;
-        if (work)
-            sv = sv_next; // a wave that is through keeps its sums as they are
         fits = fits_next;
         if (t + 1 < tiles)
             scale_next(t + 1);
@@ -389,13 +388,16 @@ __device__ __forceinline__ void tile_body(const RaggedParams& p, const Place& pl
             if (__any(mx > m_run + 4.f) || f != 1.f) {
                 const float m_new = mx > m_run + 4.f ? mx : m_run;
                 const float corr = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
+                // NAN: sums that would leave fp32's range
+                const float by = down == 0.f || v_down == 0.f ? corr : (f > 1e-18f && f < 1e18f ? corr * f : NAN);
+                v_down = down == 0.f ? v_down : down;
                 m_run = m_new;
                 l_run *= corr;
 #pragma unroll
                 for (int d = 0; d < DB; ++d)
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
-                        oacc[d][e] *= corr * f;
+                        oacc[d][e] *= by;
             }
             const float base = kShift - (m_run == -INFINITY ? 0.f : m_run); // a row that has seen no key yet adds zeros
             float rs = 0.f;
@@ -450,7 +452,6 @@ __device__ __forceinline__ void tile_body(const RaggedParams& p, const Place& pl
             measure(1);
         }
         __syncthreads();
-        sv = sv_next;
     }
     for (int t = 0; t < tiles; t += 2) {
         turn(t, ks0, vs0, ks1, vs1);
@@ -477,7 +478,7 @@ __device__ __forceinline__ void tile_body(const RaggedParams& p, const Place& pl
     uint32_t odd = (uint32_t)odd_lanes | (uint32_t)(odd_lanes >> 32);
     const bool in_parts = visible > s.range;
     if (q_ok && !(odd >> c & 1) && (in_parts ? k_first < visible : place_in.y == 0)) {
-        const float f = l_run > 0.f ? sv.down / l_run : 0.f; // no key: zeros
+        const float f = l_run > 0.f ? v_down / l_run : 0.f; // no key: zeros
         float* to = p.out + q_row * p.ldo + (int64_t)head * p.dv;
         if (in_parts) {
             const int64_t id = part_row(p, s, at_row.token, head);
@@ -608,7 +609,7 @@ __global__ __launch_bounds__(256) void ragged_ready_kernel(RaggedParams p)
         *reinterpret_cast<f16x8*>(&out[16384 + ((VB + vblk) * D + vd + g) * 16]) = l;
     }
     if (tid == 0)
-        p.powers[blockIdx.x] = { spread_fits(top, low) ? sk.down : NAN, sv.down };
+        p.powers[blockIdx.x] = { spread_fits(top, low) ? sk.down : NAN, low[1] == 0 ? 0.f : sv.down };
     __syncthreads();
     unsigned char* to = p.ready + (int64_t)blockIdx.x * 32768;
 #pragma unroll
@@ -692,7 +693,7 @@ __global__ __launch_bounds__(256, 2) void ragged_packed_kernel(RaggedParams p)
     for (int d = 0; d < DB; ++d)
         oacc[d] = kZero;
     float m_run = -INFINITY, l_run = 0.f;
-    float v_down = 0.f; // what takes the sums' power back: that of the last tile's values
+    float v_down = 0.f; // what takes the sums' power back: that of the last tile with a value that is not zero
 
     auto scores = [&](f32x16 (&sc)[HALVES], const unsigned char* ks) {
 #pragma unroll
@@ -741,14 +742,16 @@ __global__ __launch_bounds__(256, 2) void ragged_packed_kernel(RaggedParams p)
                 const float m_new = mx > m_run + 4.f ? mx : m_run;
                 const float corr = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
                 const float f = v_down / down.v_down;
+                // NAN: sums that would leave fp32's range
+                const float by = down.v_down == 0.f || v_down == 0.f ? corr : (f > 1e-18f && f < 1e18f ? corr * f : NAN);
                 m_run = m_new;
-                v_down = down.v_down;
+                v_down = down.v_down == 0.f ? v_down : down.v_down;
                 l_run *= corr;
 #pragma unroll
                 for (int d = 0; d < DB; ++d)
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
-                        oacc[d][e] *= t == 0 || (f > 1e-18f && f < 1e18f) ? corr * f : NAN; // NAN: sums that would leave fp32's range
+                        oacc[d][e] *= by;
             }
             const float base = kShift - (m_run == -INFINITY ? 0.f : m_run);
             float rs = 0.f;

@@ -27,7 +27,7 @@ struct PartSums {
 };
 
 struct f32x2_pow {
-    float k_down, v_down; // what takes a tile's power of two back
+    float k_down, v_down; // what takes a tile's powers of two back; k_down NaN: a tile for plain sums, v_down 0: values of zeros
 };
 
 struct RaggedParams {

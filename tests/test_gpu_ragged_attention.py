@@ -821,3 +821,85 @@ def test_paged_lengths_of_sequences_without_new_tokens(fdx, heads):
                               lens=[90, length, 20]) == flag
             close(out.to_host(q.shape), np.concatenate([attend(q[:new[0]], f.keys[0], f.values[0], heads, kv, np.arange(90 - new[0], 90) + 1),
                                                         attend(q[new[0]:], f.keys[2], f.values[2], heads, kv, np.array([20]))]))
+
+
+def fastest(fdx, call):
+    """Seconds of a call, the best of four."""
+    import time
+    best = 1e9
+    for _ in range(4):
+        fdx.sync()
+        start = time.perf_counter()
+        call()
+        fdx.sync()
+        best = min(best, time.perf_counter() - start)
+    return best
+
+
+ZEROS = [(0, 128), (64, 192), (256, 320), (0, 64), (300, 500), (0, 500), (37, 300)]
+
+
+@pytest.mark.parametrize("first,last", ZEROS)
+@pytest.mark.parametrize("lengths,heads,kv_heads,d", [([520, 30], 4, 2, 64), ([520, 30], 4, 2, 128), ([600], 6, 1, 64), ([600], 16, 1, 128), ([1500], 4, 4, 64)])
+def test_packed_values_of_zeros(fdx, lengths, heads, kv_heads, d, first, last):
+    """Whole tiles of values that are zeros, in front of, between and behind values of sizes that differ by 2^40."""
+    for causal in (True, False):
+        print("packed zeros", lengths, heads, kv_heads, d, first, last, causal, flush=True)
+        r, n = np.random.default_rng(21), sum(lengths)
+        q, k, v = (r.standard_normal((n, h * d)).astype(np.float32) for h in (heads, kv_heads, kv_heads))
+        v[first:last] = 0
+        close(fdx.mha_packed(q, k, v, lengths, heads, kv_heads, d, d, causal), packed_reference(q, k, v, lengths, heads, kv_heads, causal))
+        v[last:] *= np.float32(2.0 ** -40)
+        got, want = fdx.mha_packed(q, k, v, lengths, heads, kv_heads, d, d, causal), packed_reference(q, k, v, lengths, heads, kv_heads, causal)
+        close(got, want)
+        v[:] = 0
+        assert (fdx.mha_packed(q, k, v, lengths, heads, kv_heads, d, d, causal) == 0).all()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("new", [1, 9, 60, 300])
+def test_paged_values_of_zeros(fdx, new, kind):
+    heads, kv, d, page, length = 4, 2, 64, 16, 1200
+    for first, last in ZEROS + [(0, length)]:
+        f = Filled(fdx, [length], kv, d, d, page, kind, steps=1)
+        f.values[0][first:last] = 0
+        f.cache.release(0)
+        fdx.kv_append(f.cache, f.keys[0], f.values[0], [length])
+        q = np.random.default_rng(22).standard_normal((new, heads * d)).astype(np.float32)
+        print("paged zeros", new, kind, first, last, flush=True)
+        close(fdx.mha_paged(f.cache, q, [new], heads), f.reference(q, [new], heads))
+
+
+@pytest.mark.parametrize("n,heads,kv_heads", [(2048, 12, 12), (2048, 16, 4)])
+def test_packed_values_of_zeros_take_no_longer(fdx, n, heads, kv_heads):
+    """No row by row sums because of them, which take a hundred times as long; ten leaves room for a disturbed call."""
+    d, r = 64, np.random.default_rng(23)
+    q, k, v = (r.standard_normal((n, h * d)).astype(np.float32) for h in (heads, kv_heads, kv_heads))
+    dq, dk, out, times = fdx.DevBuf.from_host(q), fdx.DevBuf.from_host(k), fdx.DevBuf(q.nbytes), []
+    scratch, starts = fdx.DevBuf(fdx.lib.fdx_mha_packed_scratch_bytes(n, 1, heads, kv_heads, d, d)), fdx.DevBuf.from_host(np.array([0, n], np.int32), np.int32)
+    i64 = ctypes.c_int64
+    for first, last in ((0, 0), (0, 128), (1024, 1152)):
+        v[first:last] = 0
+        dv = fdx.DevBuf.from_host(v)
+        times.append(fastest(fdx, lambda: fdx.check(fdx.lib.fdx_mha_packed_f32(dq.ptr, i64(heads * d), dk.ptr, i64(kv_heads * d), dv.ptr, i64(kv_heads * d),
+                                                                              starts.ptr, 1, n, heads, kv_heads, d, d, 1, out.ptr, i64(heads * d),
+                                                                              scratch.ptr, None))))
+    print("times in us", [round(1e6 * t) for t in times], flush=True)
+    assert max(times[1:]) < 10 * times[0]
+
+
+def test_paged_values_of_zeros_take_no_longer(fdx):
+    heads, kv, d, page, length, new = 12, 12, 64, 64, 2000, 300
+    f, times = Filled(fdx, [length], kv, d, d, page, "f32", steps=1), []
+    q = fdx.DevBuf.from_host(np.random.default_rng(24).standard_normal((new, heads * d)).astype(np.float32))
+    out, starts = fdx.DevBuf(4 * new * heads * d), fdx.DevBuf.from_host(np.array([0, new], np.int32), np.int32)
+    for first, last in ((0, 0), (1024, 1280)):
+        f.values[0][first:last] = 0
+        f.cache.release(0)
+        fdx.kv_append(f.cache, f.keys[0], f.values[0], [length])
+        c = f.cache.pages()
+        scratch = fdx.DevBuf(fdx.lib.fdx_mha_paged_scratch_bytes(new, new, heads, ctypes.byref(c)))
+        times.append(fastest(fdx, lambda: fdx.check(fdx.lib.fdx_mha_paged_f32(q.ptr, ctypes.c_int64(heads * d), starts.ptr, new, new, heads, ctypes.byref(c),
+                                                                             out.ptr, ctypes.c_int64(heads * d), scratch.ptr, None))))
+    print("times in us", [round(1e6 * t) for t in times], flush=True)
+    assert times[1] < 10 * times[0]
