@@ -903,3 +903,52 @@ def test_paged_values_of_zeros_take_no_longer(fdx):
                                                                              out.ptr, ctypes.c_int64(heads * d), scratch.ptr, None))))
     print("times in us", [round(1e6 * t) for t in times], flush=True)
     assert times[1] < 10 * times[0]
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("new", [1, 70])
+def test_every_part_of_a_long_sequence_counts_once(fdx, new, kind):
+    """Three million positions of which two pages decide: their keys score 40 above the rest, their values are their own.  A range of keys that were
+    left out, summed twice or read from elsewhere would change the share of its page, wherever that lies, by a sixth or more of the values.
+    Scores of 320 / 8 are chains of 64 sums (three products each in tiles) of up to 320, each off by up to 2^-24 * 320: at most 192 * 2.4e-6 = 5e-4 of a
+    probability; 1e-3 of the largest value for that and the sums of the rest (e^-40 * 3e6 of the whole)."""
+    length, heads, d, page = 3000000, 2, 64, 16
+    r, n_pages = np.random.default_rng(25), 3000000 // 16
+    keys, values = (r.standard_normal((7 * page, d)).astype(np.float32) for _ in range(2))   # pages 0 to 4 everywhere, 5 and 6 once each
+    keys[:, 0] = 0
+    keys[5 * page:, 0] = 40
+    c = fdx.PagedCache(7, page, 1, d, d, 1, length, kind)
+    fdx.kv_append(c, keys, values, [7 * page])
+    first = c.table[0][:7].copy()
+    c.lens[0] = length
+    q = r.standard_normal((new, heads * d)).astype(np.float32)
+    q[:, ::d] = 8
+    k, v = (x[5 * page:].astype(np.float64) if kind == "f32" else bf16(x)[5 * page:].astype(np.float64) for x in (keys, values))
+    s = q.reshape(new, heads, d).astype(np.float64) @ k.T / np.sqrt(d)
+    p = np.exp(s - s.max(-1, keepdims=True))
+    want = p @ v / p.sum(-1, keepdims=True)
+    # the last pages hold keys that not every row sees
+    last = n_pages - 6
+    places = sorted({0, 1, last} | {last * i // 71 for i in range(72)} | {int(x) for x in r.integers(0, last, 20)})
+    for at in places:
+        other = (at + last // 2 + 1) % last
+        c.table[0][:] = first[np.arange(n_pages) % 5]
+        c.table[0][at], c.table[0][other] = first[5], first[6]
+        got = fdx.mha_paged(c, q, [new], heads).reshape(new, heads, d)
+        assert np.abs(got - want).max() <= 1e-3 * np.abs(v).max(), (at, np.abs(got - want).max())
+
+
+@pytest.mark.parametrize("what", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("name,row", [("v", 333), ("v", 399), ("v", 0), ("k", 333)])
+def test_packed_split_once_values_beside_infinities_and_nan(fdx, what, name, row):
+    """The other depths of rows that see a NaN or an infinity among the values, and every depth behind a key of -infinity's score."""
+    r, n, heads, kv = np.random.default_rng(9), 400, 8, 1
+    q, k, v = (r.standard_normal((n, h * 64)).astype(np.float32) for h in (heads, kv, kv))
+    print("packed once beside", what, name, row, flush=True)
+    dict(k=k, v=v)[name][row, 7] = what
+    got = fdx.mha_packed(q, k, v, [n], heads, kv, 64, 64)
+    with np.errstate(all="ignore"):
+        want = packed_reference(q, k, v, [n], heads, kv, True)
+    ok = np.isfinite(want)
+    assert np.array_equal(np.isfinite(got), ok)
+    close(got[ok], want[ok])
