@@ -23,7 +23,7 @@ template <int STEP>
 __device__ __forceinline__ Pow2 pow2_for(int e)
 {
     int field = (268 - e) / STEP * STEP;
-    field = field > 253 ? 253 / STEP * STEP : (field < 1 ? STEP : field);
+    field = field > 253 ? 253 / STEP * STEP : field; // 12 or more: e is at most 255
     return { __builtin_bit_cast(float, (uint32_t)field << 23), __builtin_bit_cast(float, (uint32_t)(254 - field) << 23) };
 }
 __device__ __forceinline__ int exponent(float x) { return (int)(__builtin_bit_cast(uint32_t, x) >> 23 & 255u); }

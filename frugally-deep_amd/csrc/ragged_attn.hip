@@ -65,9 +65,10 @@ __device__ __forceinline__ void store_plain_row(const RaggedParams& p, const Seq
 //    size for one power (spread_fits; a row of 10^30 behind the mask) is left to plain sums.
 //  * The maximum that a row's exponentials refer to moves only when a score passes it by 2^4, so sums are rescaled a few times a row
 //    instead of every tile; exponentials carry 2^10 to stay clear of fp16's small end, at most 2^14.
-//  * Bound by the vector units, which split, beside the matrix units: 64 keys take a workgroup 1.9 us alone on its CU at depth 64; four
-//    sequences that bring 1000 tokens to 3000 keys in fp32 pages, 32 / 8 heads of 128, 887 us or 258 TFLOP/s, where three products for one come
-//    to 364 at the rate of a large fp16 product.
+//  * Bound by the vector units, which split, and the matrix units, whose times still add up for the most part: four sequences that bring 1000
+//    tokens to 3000 keys in fp32 pages, 32 / 8 heads of 128, 887 us or 258 TFLOP/s, where three products for one come to 364 at the rate of a
+//    large fp16 product; vector instructions 55 % of a busy CU's time, matrix instructions 40 %, LDS 10 %, two waves a SIMD.  64 keys take a
+//    workgroup 1.9 us alone on its CU at depth 64.
 //  * Rows whose sums are not finite (infinite or NaN operands, whether the row sees them or not, and tiles left out above) or empty though they
 //    see keys are taken again by plain_row.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -1280,8 +1281,9 @@ static RaggedPlan paged_plan(int tokens, int max_new, int heads, const fdx_kv_pa
     r.few_rows = most <= 16 ? 16 : 32;
     if (group <= r.few_rows) {
         const int64_t items = (int64_t)c->n_seqs * c->kv_heads;
-        // Ranges enough for some 4096 workgroups when every sequence is as long as the longest, which leaves those of shorter ones to fill
-        // gaps; 256 keys or more, and 64 ranges or fewer, which one pass of ragged_join_kernel takes.  us with at least 128 / 192 / 256 / 384 / 512
+        // Ranges enough for some 4096 workgroups when every sequence is as long as the longest (max_len in all figures here: what a longer
+        // max_len costs stands at fdx_kv_pages), which leaves those of shorter ones to fill gaps; 256 keys or more, and 64 ranges or fewer, which one
+        // pass of ragged_join_kernel takes.  us with at least 128 / 192 / 256 / 384 / 512
         // keys, fp32: one sequence of 8000, 32 / 8 heads of 128, 28.4 / 29.9 / 26.0 / 28.0 / 31.7; 16 of 1000, 12 heads of 64, 28.1 / 29.2 / 26.4 / 28.9 /
         // 28.9; one of 2000, 12.9 / 13.0 / 13.9 / 16.4 / 18.8; four of 32 000, 8 / 1 heads of 128, 60.9 / 56.3 / 46.7 / 48.0 / 41.0.
         // Where 512 keys make 768 workgroups or more, 512: with 256 / 512, 32 / 8 heads of 128, 64 sequences of 1000 112 / 105 (bf16 pages 58.8 / 52.7),

@@ -324,7 +324,8 @@ __global__ __launch_bounds__(256) void token_scores_join_kernel(ScoreParams p)
     score_results(p, row, s, list);
 }
 
-// Rows are cut in parts of 4096 logits or more while that makes no more workgroups than two for each CU.
+// Rows are cut in one part for 4096 logits, or fewer parts, all but the last of whole thousands and 3072 or more, while that makes no more
+// workgroups than two for each CU.
 struct ScorePlan {
     int parts, part_len, chunk;
     size_t keys, sums; // bytes
