@@ -324,8 +324,8 @@ __global__ __launch_bounds__(256) void token_scores_join_kernel(ScoreParams p)
     score_results(p, row, s, list);
 }
 
-// Rows are cut in one part for 4096 logits, or fewer parts, all but the last of whole thousands and 3072 or more, while that makes no more
-// workgroups than two for each CU.
+// Rows are cut in one part for 4096 logits, or fewer parts, while that makes no more workgroups than two for each CU; all but the last part are
+// whole thousands (of 1024), three at least.
 struct ScorePlan {
     int parts, part_len, chunk;
     size_t keys, sums; // bytes
