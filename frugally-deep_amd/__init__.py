@@ -54,6 +54,21 @@ class KvPages(ctypes.Structure):
         self._kept = (k, v, table, lens)
 
 
+KV8_TYPES = {"i8": 2, "e4m3": 3}
+
+
+class KvPages8(ctypes.Structure):
+    """fdx_kv_pages8: a key / value cache in pages of 8-bit codes, kind "i8" or "e4m3", with a scale for each block of positions and head.
+    Takes what KvPages takes, then k_scale and v_scale (like its other tensors) and block."""
+    _fields_ = [("pages", KvPages), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p), ("block", ctypes.c_int)]
+
+    def __init__(self, k, v, kind, n_pages, page_size, kv_heads, dk, dv, table, table_width, lens, n_seqs, max_len, k_scale, v_scale, block):
+        super().__init__(k_scale=k_scale.ptr, v_scale=v_scale.ptr, block=block)
+        self.pages.__init__(k, v, "f32", n_pages, page_size, kv_heads, dk, dv, table, table_width, lens, n_seqs, max_len)
+        self.pages.type = KV8_TYPES[kind]
+        self._kept = (k, v, table, lens, k_scale, v_scale)
+
+
 class FdxError(RuntimeError):
     pass
 
@@ -73,7 +88,8 @@ def _load():
 lib = _load()
 lib.fdx_last_error.restype = ctypes.c_char_p
 lib.fdx_set_last_error.restype = None
-for _name in ("fdx_mha_scratch_bytes", "fdx_mha_packed_scratch_bytes", "fdx_mha_paged_scratch_bytes", "fdx_token_logprobs_scratch_bytes"):
+for _name in ("fdx_mha_scratch_bytes", "fdx_mha_packed_scratch_bytes", "fdx_mha_paged_scratch_bytes", "fdx_token_logprobs_scratch_bytes",
+              "fdx_mha_paged8_scratch_bytes", "fdx_kv_fork_scratch_bytes", "fdx_kv8_fork_scratch_bytes", "fdx_beam_select_scratch_bytes"):
     getattr(lib, _name).restype = ctypes.c_size_t
 
 
@@ -647,14 +663,24 @@ def mha_packed(q, k, v, lengths, heads, kv_heads, dk, dv, causal=True):
 
 
 class PagedCache:
-    """Keys and values of several sequences in pages of device memory, for kv_append and mha_paged.  A sequence takes pages as it
-    grows and gives them back with release(); the page table lives on the host and goes to the device with every call."""
+    """Keys and values of several sequences in pages of device memory, for kv_append, mha_paged and kv_fork.  A sequence takes pages as
+    it grows and gives them back with release(); the page table lives on the host and goes to the device with every call.  kind "f32",
+    "bf16", or in 8 bits "i8" or "e4m3", with a scale for each `block` positions of a page (None: the whole page) and key head."""
 
-    def __init__(self, n_pages, page_size, kv_heads, dk, dv, n_seqs, max_len, kind="f32"):
+    def __init__(self, n_pages, page_size, kv_heads, dk, dv, n_seqs, max_len, kind="f32", block=None):
         self.n_pages, self.page_size, self.kv_heads, self.dk, self.dv = n_pages, page_size, kv_heads, dk, dv
         self.n_seqs, self.max_len, self.kind = n_seqs, max_len, kind
-        size = 4 if kind == "f32" else 2
+        if kind not in KV_TYPES and kind not in KV8_TYPES:
+            raise FdxError("a cache of kind %r" % (kind,))
+        size = 4 if kind == "f32" else 2 if kind == "bf16" else 1
         rows = n_pages * page_size * kv_heads
+        if kind in KV8_TYPES:
+            self.block = page_size if block is None else block
+            if self.block <= 0 or page_size % self.block:
+                raise FdxError("blocks of %d positions do not divide pages of %d" % (self.block, page_size))
+            self.k_scale, self.v_scale = (DevBuf.from_host(np.zeros(rows // self.block, np.float32)) for _ in range(2))
+        elif block is not None:
+            raise FdxError("blocks belong to caches in 8 bits")
         self.k, self.v = (DevBuf.from_host(np.zeros(rows * d * size, np.uint8), np.uint8) for d in (dk, dv))
         self.table = np.full((n_seqs, -(-max_len // page_size)), -1, np.int32)
         self.lens = np.zeros(n_seqs, np.int32)
@@ -685,10 +711,10 @@ class PagedCache:
         self.table[seq], self.lens[seq] = -1, 0
 
     def pages(self):
-        """The cache as the entry points take it (fdx_kv_pages)."""
-        return KvPages(self.k, self.v, self.kind, self.n_pages, self.page_size, self.kv_heads, self.dk, self.dv,
-                       DevBuf.from_host(self.table, np.int32), self.table.shape[1], DevBuf.from_host(self.lens, np.int32), self.n_seqs,
-                       self.max_len)
+        """The cache as the entry points take it (fdx_kv_pages, fdx_kv_pages8)."""
+        args = (self.k, self.v, self.kind, self.n_pages, self.page_size, self.kv_heads, self.dk, self.dv,
+                DevBuf.from_host(self.table, np.int32), self.table.shape[1], DevBuf.from_host(self.lens, np.int32), self.n_seqs, self.max_len)
+        return KvPages8(*args, self.k_scale, self.v_scale, self.block) if self.kind in KV8_TYPES else KvPages(*args)
 
 
 def kv_append(cache, k, v, lengths):
@@ -703,8 +729,9 @@ def kv_append(cache, k, v, lengths):
     try:
         dk_, dv_, starts, pages = DevBuf.from_host(k), DevBuf.from_host(v), _row_starts(lengths), cache.pages()
         flag = DevBuf.from_host(np.zeros(1, np.int32), np.int32)
-        check(lib.fdx_kv_append_f32(_dp(dk_), ctypes.c_int64(k.shape[1]), _dp(dv_), ctypes.c_int64(v.shape[1]), starts.ptr, k.shape[0],
-                                    ctypes.byref(pages), flag.ptr))
+        append = lib.fdx_kv8_append_f32 if cache.kind in KV8_TYPES else lib.fdx_kv_append_f32
+        check(append(_dp(dk_), ctypes.c_int64(k.shape[1]), _dp(dv_), ctypes.c_int64(v.shape[1]), starts.ptr, k.shape[0],
+                     ctypes.byref(pages), flag.ptr))
         _raise_if_set(flag, "rows outside the cache")
     except BaseException:   # no length counts rows that may not have been written
         cache.lens = before
@@ -723,13 +750,60 @@ def mha_paged(cache, q, lengths, heads):
     if tokens == 0:
         return np.zeros((0, heads * cache.dv), np.float32)
     dq, starts, pages = DevBuf.from_host(q), _row_starts(lengths), cache.pages()
-    scratch = DevBuf(lib.fdx_mha_paged_scratch_bytes(tokens, most, heads, ctypes.byref(pages)))
+    attend, need = lib.fdx_mha_paged_f32, lib.fdx_mha_paged_scratch_bytes
+    if cache.kind in KV8_TYPES:
+        attend, need = lib.fdx_mha_paged8_f32, lib.fdx_mha_paged8_scratch_bytes
+    scratch = DevBuf(need(tokens, most, heads, ctypes.byref(pages)))
     out = DevBuf.from_host(np.zeros((tokens, heads * cache.dv), np.float32))
     flag = DevBuf.from_host(np.zeros(1, np.int32), np.int32)
-    check(lib.fdx_mha_paged_f32(_dp(dq), ctypes.c_int64(q.shape[1]), starts.ptr, tokens, most, heads, ctypes.byref(pages), _dp(out),
-                                ctypes.c_int64(heads * cache.dv), scratch.ptr, flag.ptr))
+    check(attend(_dp(dq), ctypes.c_int64(q.shape[1]), starts.ptr, tokens, most, heads, ctypes.byref(pages), _dp(out),
+                 ctypes.c_int64(heads * cache.dv), scratch.ptr, flag.ptr))
     _raise_if_set(flag, "positions outside the cache")
     return out.to_host((tokens, heads * cache.dv))
+
+
+def kv_fork(cache, parents):
+    """Sequence i of a PagedCache goes on as a copy of what sequence parents[i] was, or ends if that is negative; all of them or none."""
+    parents = _whole("parents", parents)
+    if parents.shape != (cache.n_seqs,) or parents.max() >= cache.n_seqs:
+        raise FdxError("%d sequences need as many parents among them, not %s" % (cache.n_seqs, parents.tolist()))
+    pages, dparents = cache.pages(), DevBuf.from_host(np.maximum(parents, -1), np.int32)
+    fork, need = (lib.fdx_kv8_fork, lib.fdx_kv8_fork_scratch_bytes) if cache.kind in KV8_TYPES else (lib.fdx_kv_fork, lib.fdx_kv_fork_scratch_bytes)
+    scratch, table, lens = DevBuf(need(ctypes.byref(pages))), DevBuf(4 * cache.table.size), DevBuf(4 * cache.n_seqs)
+    flag = DevBuf.from_host(np.zeros(1, np.int32), np.int32)
+    check(fork(ctypes.byref(pages), dparents.ptr, None, table.ptr, lens.ptr, None, scratch.ptr, flag.ptr))
+    _raise_if_set(flag, "the cache has too few free pages for the copies")
+    table, lens = table.to_host(cache.table.shape, np.int32), lens.to_host((cache.n_seqs,), np.int32)
+    used = set(table.ravel().tolist())
+    cache.table, cache.lens = table.copy(), lens.copy()
+    cache.free = [page for page in range(cache.n_pages - 1, -1, -1) if page not in used]
+
+
+def beam_select(logits, scores, keep, done=None, end_id=-1):
+    """logits [n,beams,vocab], scores [n,beams]; the `keep` best continuations of each of the n sequences: a dict of parents (rows
+    s * beams + b), tokens, scores and, if there is an end_id, done, all [n,keep].  done [n,beams]: beams that have ended."""
+    logits, scores = np.ascontiguousarray(logits, np.float32), np.ascontiguousarray(scores, np.float32)
+    if logits.ndim != 3 or scores.shape != logits.shape[:2]:
+        raise FdxError("scores of shape %s for logits of shape %s" % (scores.shape, logits.shape))
+    n, beams, vocab = logits.shape
+    if done is not None and np.shape(done) != (n, beams):
+        raise FdxError("done of shape %s for %d sequences of %d beams" % (np.shape(done), n, beams))
+    if n == 0:
+        return dict({key: np.zeros((0, keep), np.int32) for key in ("parents", "tokens", "done")[:3 if end_id >= 0 else 2]},
+                    scores=np.zeros((0, keep), np.float32))
+    dx, ds = DevBuf.from_host(logits), DevBuf.from_host(scores)
+    dd = None if done is None else DevBuf.from_host(np.asarray(done) != 0, np.int32)
+    parents, tokens, new_scores = (DevBuf(4 * n * max(keep, 1)) for _ in range(3))
+    new_done = DevBuf(4 * n * max(keep, 1)) if end_id >= 0 else None
+    scratch = DevBuf(lib.fdx_beam_select_scratch_bytes(n, beams, vocab, keep))
+    flag = DevBuf.from_host(np.zeros(1, np.int32), np.int32)
+    check(lib.fdx_beam_select_f32(_dp(dx), ctypes.c_int64(vocab), n, beams, vocab, _dp(ds), dd and dd.ptr, end_id, keep, parents.ptr, tokens.ptr,
+                                  _dp(new_scores), new_done and new_done.ptr, scratch.ptr, flag.ptr))
+    _raise_if_set(flag, "logits or scores that are NaN or infinite")
+    out = dict(parents=parents.to_host((n, keep), np.int32), tokens=tokens.to_host((n, keep), np.int32), scores=new_scores.to_host((n, keep)))
+    if new_done is not None:
+        out["done"] = new_done.to_host((n, keep), np.int32)
+    return out
 
 
 def token_logprobs(logits, ids=None, top=0):

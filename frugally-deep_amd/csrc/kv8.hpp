@@ -1,0 +1,49 @@
+// Elements of a cache in 8 bits: a code times the fp32 scale of its block (fdx_kv_pages8).
+#pragma once
+#include "ragged_attn.hpp"
+
+namespace fdx {
+
+enum { kI8 = 0, kE4M3 = 1 };
+constexpr float kMostI8 = 127.f, kMostE4M3 = 448.f;
+constexpr float kLeastScale = 0x1p-126f; // of a block of zeros too: its reciprocal is finite
+
+template <int KIND>
+__device__ __forceinline__ constexpr float most_code() { return KIND == kI8 ? kMostI8 : kMostE4M3; }
+
+// four values, in units of codes, as four codes
+template <int KIND>
+__device__ __forceinline__ uint32_t to_codes(const float (&x)[4])
+{
+    if constexpr (KIND == kI8) {
+        uint32_t r = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            r |= ((uint32_t)(int)__builtin_amdgcn_fmed3f(__builtin_rintf(x[e]), -kMostI8, kMostI8) & 255u) << (8 * e);
+        return r;
+    } else {
+        float y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            y[e] = __builtin_amdgcn_fmed3f(x[e], -kMostE4M3, kMostE4M3);
+        int r = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+        return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], r, true);
+    }
+}
+// and back
+template <int KIND>
+__device__ __forceinline__ void from_codes(uint32_t c, float (&x)[4])
+{
+    if constexpr (KIND == kI8) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            x[e] = (float)(int8_t)(c >> (8 * e));
+    } else {
+        x[0] = __builtin_amdgcn_cvt_f32_fp8((int)c, 0);
+        x[1] = __builtin_amdgcn_cvt_f32_fp8((int)c, 1);
+        x[2] = __builtin_amdgcn_cvt_f32_fp8((int)c, 2);
+        x[3] = __builtin_amdgcn_cvt_f32_fp8((int)c, 3);
+    }
+}
+
+} // namespace fdx

@@ -63,11 +63,11 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendParams p)
         append_row<T, W>(p.k + (int64_t)row * p.ldk, static_cast<T*>(p.c.k) + (int64_t)at * nk, nk, lane);
 }
 
-// what fdx_kv_append_f32 and fdx_mha_paged_f32 ask of a cache
-fdx_status check_kv_pages(const char* who, const fdx_kv_pages* c)
+// what every call asks of a cache whose elements have `size` bytes
+static fdx_status check_kv_shape(const char* who, const fdx_kv_pages* c, bool type_ok, uintptr_t size)
 {
     FDX_REQUIRE(c && c->k && c->v && c->table && c->lens, "%s: null pointer", who);
-    FDX_REQUIRE(c->type == FDX_KV_F32 || c->type == FDX_KV_BF16, "%s: unknown element type %d of the cache", who, c->type);
+    FDX_REQUIRE(type_ok, "%s: unknown element type %d of the cache", who, c->type);
     FDX_REQUIRE(c->n_pages > 0 && c->page_size > 0 && c->kv_heads > 0 && c->dk > 0 && c->dv > 0 && c->n_seqs > 0 && c->table_width > 0
             && c->max_len > 0,
         "%s: bad shape of the cache", who);
@@ -76,9 +76,23 @@ fdx_status check_kv_pages(const char* who, const fdx_kv_pages* c)
         "%s: rows of the cache too long", who);
     FDX_REQUIRE(c->max_len <= (1 << 30), "%s: sequences of more than 2^30 positions", who);
     FDX_REQUIRE((int64_t)c->table_width * c->page_size >= c->max_len, "%s: the table does not reach max_len", who);
-    const uintptr_t size = c->type == FDX_KV_BF16 ? 2 : 4;
     FDX_REQUIRE(((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & (size - 1)) == 0,
         "%s: pages that are not aligned to their elements", who);
+    return FDX_OK;
+}
+fdx_status check_kv_pages(const char* who, const fdx_kv_pages* c)
+{
+    return check_kv_shape(who, c, c && (c->type == FDX_KV_F32 || c->type == FDX_KV_BF16), c && c->type == FDX_KV_BF16 ? 2 : 4);
+}
+fdx_status check_kv_pages8(const char* who, const fdx_kv_pages8* c)
+{
+    const fdx_kv_pages* pages = c ? &c->pages : nullptr;
+    const fdx_status st = check_kv_shape(who, pages, pages && (pages->type == FDX_KV_I8 || pages->type == FDX_KV_E4M3), 1);
+    if (st != FDX_OK)
+        return st;
+    FDX_REQUIRE(c->k_scale && c->v_scale, "%s: null pointer", who);
+    FDX_REQUIRE(((reinterpret_cast<uintptr_t>(c->k_scale) | reinterpret_cast<uintptr_t>(c->v_scale)) & 3) == 0, "%s: scales that are not aligned", who);
+    FDX_REQUIRE(c->block > 0 && pages->page_size % c->block == 0, "%s: blocks of %d positions do not divide pages of %d", who, c->block, pages->page_size);
     return FDX_OK;
 }
 

@@ -1,0 +1,316 @@
+// The page table after a selection: sequences go on as copies of others, full pages are shared, partly filled ones get copies.
+//
+// Which pages are kept is a bit each; the free ones are then the zeros, taken from the lowest on by ranks: of the sequences' needs (a prefix
+// sum) and of the zeros (prefix sums over the words' counts), so nothing depends on the order in which threads arrive.
+#include <cfloat>
+#include <climits>
+
+#include "kv8.hpp"
+
+namespace fdx {
+
+struct ForkParams {
+    const int32_t *table, *lens, *parents, *grow;
+    int32_t *new_table, *new_lens, *free_pages;
+    int n_seqs, width, n_pages, max_len;
+    Divisor page_size, by_width;
+    uint32_t* used;   // a bit a page
+    int32_t* owner;   // of a partly filled page: the first sequence that goes on in it
+    int32_t* list;    // free pages that are taken
+    int4* plan;       // a sequence: its partly filled page (-1: none), its copy's page (-1: none), filled rows, entries of the new table
+    int* error_flag;
+};
+
+struct Fork {
+    int parent, length, want; // positions that it goes on from, and has room for
+};
+__device__ __forceinline__ Fork fork_of(const ForkParams& p, int i, bool& odd)
+{
+    Fork f { p.parents[i], 0, 0 };
+    odd = false;
+    if (f.parent >= p.n_seqs) {
+        odd = true;
+        f.parent = -1;
+    }
+    if (f.parent < 0)
+        return { -1, 0, 0 };
+    const int len = p.lens[f.parent], more = p.grow ? p.grow[i] : 0;
+    f.length = len < 0 ? 0 : (len > p.max_len ? p.max_len : len);
+    f.want = more < 0 || more > p.max_len - f.length ? f.length : f.length + more;
+    odd = f.length != len || f.want - f.length != more;
+    return f;
+}
+
+// sum over the workgroup's threads in front of this one, and over all
+__device__ __forceinline__ int before_me(int v, int* lds, int& total)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int sum = v;
+    for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(sum, d, 64);
+        sum += lane >= d ? o : 0;
+    }
+    __syncthreads();
+    if (lane == 63)
+        lds[wave] = sum;
+    __syncthreads();
+    int front = 0;
+    total = 0;
+    for (int w = 0; w < (int)(blockDim.x >> 6); ++w) {
+        front += w < wave ? lds[w] : 0;
+        total += lds[w];
+    }
+    return front + sum - v;
+}
+
+__device__ __forceinline__ int agent_load(const int32_t* at) { return __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ void agent_store(int32_t* at, int v) { __hip_atomic_store(at, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+constexpr int kForkThreads = 1024;
+
+__global__ __launch_bounds__(kForkThreads) void kv_fork_kernel(ForkParams p)
+{
+    __shared__ int sums[kForkThreads / 64];
+    const int tid = threadIdx.x, words = (p.n_pages + 31) / 32, page = (int)p.page_size.by;
+    for (int w = tid; w < words; w += kForkThreads)
+        agent_store(reinterpret_cast<int32_t*>(p.used) + w, 0);
+    __syncthreads();
+    // shared pages
+    const int64_t entries = (int64_t)p.n_seqs * p.width;
+    bool odd = false;
+    for (int64_t e = tid; e < entries; e += kForkThreads) {
+        const int i = quotient((int)e, p.by_width), j = (int)(e - (int64_t)i * p.width);
+        bool bad;
+        const Fork f = fork_of(p, i, bad);
+        int at = -1;
+        if (j < quotient(f.length, p.page_size)) {
+            at = p.table[(int64_t)f.parent * p.width + j];
+            if (at < 0 || at >= p.n_pages) {
+                at = -1;
+                odd = true;
+            } else {
+                atomicOr(p.used + (at >> 5), 1u << (at & 31));
+            }
+        }
+        p.new_table[e] = at;
+    }
+    // partly filled ones
+    for (int i = tid; i < p.n_seqs; i += kForkThreads) {
+        bool bad;
+        const Fork f = fork_of(p, i, bad);
+        odd = odd || bad;
+        const int full = quotient(f.length, p.page_size);
+        int at = -1;
+        if (f.length - full * page > 0) {
+            at = p.table[(int64_t)f.parent * p.width + full];
+            if (at < 0 || at >= p.n_pages) {
+                at = -1;
+                odd = true;
+            } else {
+                agent_store(p.owner + at, INT_MAX);
+            }
+        }
+        p.plan[i].x = at;
+        p.new_lens[i] = f.want;
+    }
+    __syncthreads();
+    for (int i = tid; i < p.n_seqs; i += kForkThreads)
+        if (p.plan[i].x >= 0)
+            atomicMin(p.owner + p.plan[i].x, i);
+    __syncthreads();
+    // who keeps one: no full page of another's, and the first; their bits are set when all have looked
+    for (int i = tid; i < p.n_seqs; i += kForkThreads) {
+        const int at = p.plan[i].x;
+        const bool kept = at >= 0 && agent_load(p.owner + at) == i && !(agent_load(reinterpret_cast<int32_t*>(p.used) + (at >> 5)) >> (at & 31) & 1);
+        p.plan[i].w = kept;
+    }
+    __syncthreads();
+    for (int i = tid; i < p.n_seqs; i += kForkThreads)
+        if (p.plan[i].w)
+            atomicOr(p.used + (p.plan[i].x >> 5), 1u << (p.plan[i].x & 31));
+    __syncthreads();
+    // needs, in the order of the sequences
+    int needed = 0;
+    for (int i0 = 0; i0 < p.n_seqs; i0 += kForkThreads) {
+        const int i = i0 + tid;
+        int need = 0;
+        if (i < p.n_seqs) {
+            bool bad;
+            const Fork f = fork_of(p, i, bad);
+            const int full = quotient(f.length, p.page_size), part = f.length - full * page;
+            const int end = quotient(f.want, p.page_size) + (f.want % page != 0);
+            // a partly filled page that is none of the cache has no copy
+            const int begin = full + (part > 0 && (p.plan[i].w || p.plan[i].x < 0));
+            need = end - begin;
+        }
+        int total;
+        const int front = before_me(need, sums, total);
+        if (i < p.n_seqs)
+            p.plan[i].z = needed + front;
+        needed += total;
+    }
+    // the free pages, by rank
+    int ranked = 0;
+    for (int w0 = 0; w0 < words; w0 += kForkThreads) {
+        const int w = w0 + tid;
+        uint32_t zeros = 0;
+        if (w < words) {
+            zeros = ~(uint32_t)agent_load(reinterpret_cast<int32_t*>(p.used) + w);
+            if (w == words - 1 && p.n_pages % 32)
+                zeros &= (1u << (p.n_pages % 32)) - 1;
+        }
+        int total;
+        int rank = ranked + before_me(__builtin_popcount(zeros), sums, total);
+        ranked += total;
+        for (; zeros && rank < needed; zeros &= zeros - 1)
+            p.list[rank++] = w * 32 + __builtin_ctz(zeros);
+    }
+    __syncthreads();
+    const int there = needed < ranked ? needed : ranked;
+    odd = odd || needed > ranked;
+    for (int i = tid; i < p.n_seqs; i += kForkThreads) {
+        bool bad;
+        const Fork f = fork_of(p, i, bad);
+        const int full = quotient(f.length, p.page_size), part = f.length - full * page;
+        const int end = quotient(f.want, p.page_size) + (f.want % page != 0);
+        const int at = p.plan[i].x;
+        const bool kept = p.plan[i].w;
+        int32_t* row = p.new_table + (int64_t)i * p.width;
+        int rank = p.plan[i].z, j = full;
+        if (part > 0 && (kept || at < 0))
+            row[j++] = at;
+        const int copy = part > 0 && !kept && at >= 0 && rank < there ? p.list[rank] : -1;
+        for (; j < end; ++j, ++rank)
+            row[j] = rank < there ? p.list[rank] : -1;
+        p.plan[i] = int4 { at, copy, part, 0 };
+    }
+    if (odd && p.error_flag)
+        *p.error_flag = 1;
+    if (tid == 0 && p.free_pages)
+        *p.free_pages = ranked - there;
+}
+
+struct ForkCopyParams {
+    const int4* plan;
+    char *k, *v, *k_scale, *v_scale;
+    int64_t k_row, v_row;      // bytes
+    int page_size, block, kv_heads; // block 0: no scales
+    int wide;                  // rows are whole 16-byte vectors
+};
+
+constexpr int kCopyThreads = 256, kCopyBytes = 16384;
+
+template <typename T>
+__device__ __forceinline__ void copy_bytes(const char* from, char* to, int64_t first, int64_t last)
+{
+    for (int64_t i = first + threadIdx.x * (int64_t)sizeof(T); i < last; i += kCopyThreads * (int64_t)sizeof(T))
+        *reinterpret_cast<T*>(to + i) = *reinterpret_cast<const T*>(from + i);
+}
+
+// A workgroup takes 16 KB of the filled rows of one sequence's page, keys and values one behind the other.
+__global__ __launch_bounds__(kCopyThreads) void kv_fork_copy_kernel(ForkCopyParams p)
+{
+    const int4 plan = p.plan[blockIdx.x];
+    if (plan.y < 0 || plan.x < 0 || plan.z <= 0)
+        return;
+    const int64_t from = (int64_t)plan.x * p.page_size, to = (int64_t)plan.y * p.page_size;
+    auto part = [&](char* base, int64_t row, int64_t first) {
+        const int64_t all = plan.z * row, last = first + kCopyBytes < all ? first + kCopyBytes : all;
+        if (p.wide)
+            copy_bytes<f32x4>(base + from * row, base + to * row, first, last);
+        else
+            copy_bytes<char>(base + from * row, base + to * row, first, last);
+    };
+    for (int64_t first = (int64_t)blockIdx.y * kCopyBytes; first < plan.z * p.k_row; first += (int64_t)gridDim.y * kCopyBytes)
+        part(p.k, p.k_row, first);
+    for (int64_t first = (int64_t)blockIdx.y * kCopyBytes; first < plan.z * p.v_row; first += (int64_t)gridDim.y * kCopyBytes)
+        part(p.v, p.v_row, first);
+    if (p.block > 0 && blockIdx.y == 0) {
+        const int64_t row = 4 * (int64_t)p.kv_heads, bytes = (plan.z + p.block - 1) / p.block * row;
+        const int64_t a = (int64_t)plan.x * (p.page_size / p.block) * row, b = (int64_t)plan.y * (p.page_size / p.block) * row;
+        copy_bytes<float>(p.k_scale + a, p.k_scale + b, 0, bytes);
+        copy_bytes<float>(p.v_scale + a, p.v_scale + b, 0, bytes);
+    }
+}
+
+struct ForkScratch {
+    size_t used, owner, list, plan, all;
+};
+static ForkScratch fork_scratch(const fdx_kv_pages* c)
+{
+    auto round = [](size_t n) { return (n + 15) & ~(size_t)15; };
+    ForkScratch r;
+    r.used = 0;
+    r.owner = round(((size_t)c->n_pages + 31) / 32 * 4);
+    r.list = r.owner + round((size_t)c->n_pages * 4);
+    r.plan = r.list + round((size_t)c->n_pages * 4);
+    r.all = r.plan + (size_t)c->n_seqs * sizeof(int4);
+    return r;
+}
+
+static bool overlap(const void* a, size_t na, const void* b, size_t nb)
+{
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y + nb && y < x + na;
+}
+
+static fdx_status fork_launch(const char* who, const fdx_kv_pages* c, size_t size, const fdx_kv_pages8* eight, const int32_t* parents,
+    const int32_t* grow, int32_t* new_table, int32_t* new_lens, int32_t* free_pages, void* scratch_dev, int* error_flag_dev)
+{
+    FDX_REQUIRE(parents && new_table && new_lens, "%s: null pointer", who);
+    FDX_REQUIRE((int64_t)c->n_seqs * c->table_width < ((int64_t)1 << 31), "%s: a table of more than 2^31 entries", who);
+    FDX_REQUIRE(scratch_dev && (reinterpret_cast<uintptr_t>(scratch_dev) & 15) == 0, "%s: scratch missing or not 16-byte aligned", who);
+    const size_t table_bytes = (size_t)c->n_seqs * c->table_width * 4, lens_bytes = (size_t)c->n_seqs * 4;
+    const struct {
+        const void* at;
+        size_t bytes;
+    } tensors[] = { { new_table, table_bytes }, { new_lens, lens_bytes }, { free_pages, free_pages ? 4u : 0u }, { c->table, table_bytes },
+        { c->lens, lens_bytes }, { parents, lens_bytes }, { grow, grow ? lens_bytes : 0 } };
+    for (int i = 0; i < 3; ++i)
+        for (int j = i + 1; j < 7; ++j)
+            FDX_REQUIRE(!overlap(tensors[i].at, tensors[i].bytes, tensors[j].at, tensors[j].bytes),
+                "%s: the new table, the new lengths or free_pages overlap an input or each other", who);
+    const ForkScratch at = fork_scratch(c);
+    char* scratch = static_cast<char*>(scratch_dev);
+    const ForkParams p { c->table, c->lens, parents, grow, new_table, new_lens, free_pages, c->n_seqs, c->table_width, c->n_pages, c->max_len,
+        make_divisor(c->page_size), make_divisor(c->table_width), reinterpret_cast<uint32_t*>(scratch + at.used),
+        reinterpret_cast<int32_t*>(scratch + at.owner), reinterpret_cast<int32_t*>(scratch + at.list), reinterpret_cast<int4*>(scratch + at.plan),
+        error_flag_dev };
+    const int64_t k_row = (int64_t)c->kv_heads * c->dk * (int64_t)size, v_row = (int64_t)c->kv_heads * c->dv * (int64_t)size;
+    const bool wide = ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v) | (uintptr_t)k_row | (uintptr_t)v_row) & 15) == 0;
+    const ForkCopyParams copy { p.plan, static_cast<char*>(c->k), static_cast<char*>(c->v), eight ? reinterpret_cast<char*>(eight->k_scale) : nullptr,
+        eight ? reinterpret_cast<char*>(eight->v_scale) : nullptr, k_row, v_row, c->page_size, eight ? eight->block : 0, c->kv_heads, wide };
+    const int64_t parts = ((k_row > v_row ? k_row : v_row) * c->page_size + kCopyBytes - 1) / kCopyBytes;
+    profile_begin();
+    hipLaunchKernelGGL(kv_fork_kernel, dim3(1), dim3(kForkThreads), 0, stream(), p);
+    hipLaunchKernelGGL(kv_fork_copy_kernel, dim3((unsigned)c->n_seqs, (unsigned)(parts < 64 ? parts : 64)), dim3(kCopyThreads), 0, stream(), copy);
+    profile_end("kv_fork", 0.0, 2.0 * table_bytes);
+    FDX_LAUNCH_CHECK();
+    return FDX_OK;
+}
+
+} // namespace fdx
+
+using namespace fdx;
+
+extern "C" size_t fdx_kv_fork_scratch_bytes(const fdx_kv_pages* cache)
+{
+    return cache && cache->n_pages > 0 && cache->n_seqs > 0 ? fork_scratch(cache).all : 0;
+}
+extern "C" size_t fdx_kv8_fork_scratch_bytes(const fdx_kv_pages8* cache) { return cache ? fdx_kv_fork_scratch_bytes(&cache->pages) : 0; }
+
+extern "C" fdx_status fdx_kv_fork(const fdx_kv_pages* cache, const int32_t* parents, const int32_t* grow, int32_t* new_table, int32_t* new_lens,
+    int32_t* free_pages, void* scratch_dev, int* error_flag_dev)
+{
+    const fdx_status st = check_kv_pages("kv_fork", cache);
+    return st != FDX_OK ? st : fork_launch("kv_fork", cache, cache->type == FDX_KV_BF16 ? 2 : 4, nullptr, parents, grow, new_table, new_lens,
+        free_pages, scratch_dev, error_flag_dev);
+}
+
+extern "C" fdx_status fdx_kv8_fork(const fdx_kv_pages8* cache, const int32_t* parents, const int32_t* grow, int32_t* new_table, int32_t* new_lens,
+    int32_t* free_pages, void* scratch_dev, int* error_flag_dev)
+{
+    const fdx_status st = check_kv_pages8("kv8_fork", cache);
+    return st != FDX_OK ? st : fork_launch("kv8_fork", &cache->pages, 1, cache, parents, grow, new_table, new_lens, free_pages, scratch_dev,
+        error_flag_dev);
+}

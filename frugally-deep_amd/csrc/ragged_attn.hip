@@ -13,8 +13,6 @@
 
 namespace fdx {
 
-fdx_status check_kv_pages(const char* who, const fdx_kv_pages* c); // kv_append.hip
-
 // a row by plain sums, into its place
 template <int KIND>
 __device__ __forceinline__ void store_plain_row(const RaggedParams& p, const Sequence& s, int token, int head, int kv_head, int range, int lane)
@@ -1254,26 +1252,13 @@ __global__ __launch_bounds__(256) void ragged_join_kernel(RaggedParams p)
         to[64 + lane] = finish(o1, l, top != -INFINITY);
 }
 
-// How a call is cut: sequences of few rows (up to `few_rows`) go to ragged_few_kernel in ranges of up to few_keys keys, the others to
-// ragged_tile_kernel in ranges of up to tile_keys.
-struct RaggedPlan {
-    int few_rows, few_ranges, few_keys; // few_ranges 0: no such launch
-    int tile_ranges, tile_keys, tile_whole;
-    int64_t few_part, tile_part; // rows whose sums may be kept
-    int64_t tiles;
-    int64_t ready; // tiles of split keys and values, for all key heads; 0: none are laid out
-    size_t ready_bytes() const { return (size_t)ready * (32768 + sizeof(f32x2_pow)); }
-    size_t few_floats(int dv) const { return few_ranges > 1 ? ((size_t)few_ranges * few_part * (2 + (size_t)dv) + 3) & ~(size_t)3 : 0; }
-    size_t tile_floats(int dv) const { return tile_ranges > 1 ? (size_t)tile_ranges * tile_part * (2 + (size_t)dv) : 0; }
-};
-
 static int ranges_of(int keys, int64_t most, int* range_keys)
 {
     *range_keys = (int)(most > keys ? keys : (most + 63) & ~(int64_t)63);
     return (keys + *range_keys - 1) / *range_keys;
 }
 
-static RaggedPlan paged_plan(int tokens, int max_new, int heads, const fdx_kv_pages* c)
+RaggedPlan paged_plan(int tokens, int max_new, int heads, const fdx_kv_pages* c)
 {
     RaggedPlan r {};
     const int group = heads / c->kv_heads;
@@ -1438,6 +1423,32 @@ static fdx_status check_ragged(const char* who, const RaggedParams& p, const voi
     return FDX_OK;
 }
 
+// checks the arguments of a call on a paged cache and makes a launch's parameters of them
+fdx_status paged_params(const char* who, const float* q, int64_t ldq, const int32_t* starts, int tokens, int max_new, int heads,
+    const fdx_kv_pages* cache, float* out, int64_t ldo, void* scratch_dev, int* error_flag_dev, RaggedParams& p, RaggedPlan& plan)
+{
+    FDX_REQUIRE(max_new > 0, "%s: bad shape", who);
+    p.q = q; p.ldq = ldq; p.out = out; p.ldo = ldo;
+    p.k = cache->k; p.ldk = (int64_t)cache->kv_heads * cache->dk; p.v = cache->v; p.ldv = (int64_t)cache->kv_heads * cache->dv;
+    p.starts = starts; p.n_seqs = cache->n_seqs; p.tokens = tokens;
+    p.heads = heads; p.kv_heads = cache->kv_heads; p.group = heads / cache->kv_heads;
+    p.dk = cache->dk; p.dv = cache->dv; p.causal = 1;
+    p.table = cache->table; p.lens = cache->lens; p.table_width = cache->table_width; p.n_pages = cache->n_pages;
+    p.page_size = make_divisor(cache->page_size); p.max_len = cache->max_len; p.max_new = max_new < tokens ? max_new : tokens;
+    p.error_flag = error_flag_dev;
+    const fdx_status st = check_ragged(who, p, scratch_dev, fdx_mha_paged_scratch_bytes(tokens, max_new, heads, cache));
+    if (st != FDX_OK)
+        return st;
+    p.scale = (float)(1.0 / std::sqrt((double)p.dk));
+    plan = paged_plan(tokens, max_new, heads, cache);
+    float* part = static_cast<float*>(scratch_dev);
+    p.by_group = make_divisor(p.group);
+    p.few_rows = plan.few_rows;
+    p.few = { part, plan.few_part, plan.few_ranges, plan.few_keys, 0, (int)(plan.few_part / ((int64_t)p.n_seqs * p.kv_heads)) };
+    p.tile = { part + plan.few_floats(p.dv), plan.tile_part, plan.tile_ranges, plan.tile_keys, plan.tile_whole, 0 };
+    return FDX_OK;
+}
+
 } // namespace fdx
 
 using namespace fdx;
@@ -1496,26 +1507,11 @@ extern "C" fdx_status fdx_mha_paged_f32(const float* q, int64_t ldq, const int32
     fdx_status st = check_kv_pages("mha_paged", cache);
     if (st != FDX_OK)
         return st;
-    FDX_REQUIRE(max_new > 0, "mha_paged: bad shape");
     RaggedParams p {};
-    p.q = q; p.ldq = ldq; p.out = out; p.ldo = ldo;
-    p.k = cache->k; p.ldk = (int64_t)cache->kv_heads * cache->dk; p.v = cache->v; p.ldv = (int64_t)cache->kv_heads * cache->dv;
-    p.starts = starts; p.n_seqs = cache->n_seqs; p.tokens = tokens;
-    p.heads = heads; p.kv_heads = cache->kv_heads; p.group = heads / cache->kv_heads;
-    p.dk = cache->dk; p.dv = cache->dv; p.causal = 1;
-    p.table = cache->table; p.lens = cache->lens; p.table_width = cache->table_width; p.n_pages = cache->n_pages;
-    p.page_size = make_divisor(cache->page_size); p.max_len = cache->max_len; p.max_new = max_new < tokens ? max_new : tokens;
-    p.error_flag = error_flag_dev;
-    st = check_ragged("mha_paged", p, scratch_dev, fdx_mha_paged_scratch_bytes(tokens, max_new, heads, cache));
+    RaggedPlan plan;
+    st = paged_params("mha_paged", q, ldq, starts, tokens, max_new, heads, cache, out, ldo, scratch_dev, error_flag_dev, p, plan);
     if (st != FDX_OK)
         return st;
-    p.scale = (float)(1.0 / std::sqrt((double)p.dk));
-    const RaggedPlan plan = paged_plan(tokens, max_new, heads, cache);
-    float* part = static_cast<float*>(scratch_dev);
-    p.by_group = make_divisor(p.group);
-    p.few_rows = plan.few_rows;
-    p.few = { part, plan.few_part, plan.few_ranges, plan.few_keys, 0, (int)(plan.few_part / ((int64_t)p.n_seqs * p.kv_heads)) };
-    p.tile = { part + plan.few_floats(p.dv), plan.tile_part, plan.tile_ranges, plan.tile_keys, plan.tile_whole, 0 };
     profile_begin();
     if (cache->type == FDX_KV_F32)
         ragged_dispatch<kPagedF32>(p, plan);

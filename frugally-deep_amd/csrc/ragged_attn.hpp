@@ -8,6 +8,10 @@
 
 namespace fdx {
 
+// what calls ask of their caches (kv_append.hip)
+fdx_status check_kv_pages(const char* who, const fdx_kv_pages* c);
+fdx_status check_kv_pages8(const char* who, const fdx_kv_pages8* c);
+
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // where keys and values come from
@@ -49,6 +53,24 @@ struct RaggedParams {
     unsigned char* ready; // packed prompts: tiles of split keys and values, [tile][key head][32 KB], and their powers [tile][key head]
     f32x2_pow* powers;
 };
+
+// How a call is cut: sequences of few rows (up to `few_rows`) go to ragged_few_kernel in ranges of up to few_keys keys, the others to
+// ragged_tile_kernel in ranges of up to tile_keys.
+struct RaggedPlan {
+    int few_rows, few_ranges, few_keys; // few_ranges 0: no such launch
+    int tile_ranges, tile_keys, tile_whole;
+    int64_t few_part, tile_part; // rows whose sums may be kept
+    int64_t tiles;
+    int64_t ready; // tiles of split keys and values, for all key heads; 0: none are laid out
+    size_t ready_bytes() const { return (size_t)ready * (32768 + sizeof(f32x2_pow)); }
+    size_t few_floats(int dv) const { return few_ranges > 1 ? ((size_t)few_ranges * few_part * (2 + (size_t)dv) + 3) & ~(size_t)3 : 0; }
+    size_t tile_floats(int dv) const { return tile_ranges > 1 ? (size_t)tile_ranges * tile_part * (2 + (size_t)dv) : 0; }
+};
+
+// of a call on a paged cache: how it is cut, and its parameters after its arguments have been checked (ragged_attn.hip)
+RaggedPlan paged_plan(int tokens, int max_new, int heads, const fdx_kv_pages* c);
+fdx_status paged_params(const char* who, const float* q, int64_t ldq, const int32_t* starts, int tokens, int max_new, int heads,
+    const fdx_kv_pages* cache, float* out, int64_t ldo, void* scratch_dev, int* error_flag_dev, RaggedParams& p, RaggedPlan& plan);
 
 template <int KIND>
 struct KvElement {

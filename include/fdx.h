@@ -423,6 +423,82 @@ fdx_status fdx_mha_paged_f32(const float* q, int64_t ldq, const int32_t* starts,
     const fdx_kv_pages* cache, float* out, int64_t ldo, void* scratch_dev, int* error_flag_dev);
 
 /*
+ * A paged cache in 8 bits: a quarter of fp32's memory and traffic.  `pages` is a cache as above with `type` FDX_KV_I8 (whole numbers
+ * -127 .. 127) or FDX_KV_E4M3 (8-bit floating point with 4 bits of exponent and 3 of mantissa, up to 448); an element is its code times
+ * the fp32 scale of its block.  A block is `block` positions of one page and one key head, keys and values apart: the scale of row r of
+ * page p, head h lies at k_scale (v_scale) [p * (page_size / block) + r / block][h].  `block` divides page_size; 1 is a scale for each
+ * token.  The entry points that take fdx_kv_pages refuse these types, those that take fdx_kv_pages8 the others.
+ */
+enum { FDX_KV_I8 = 2, FDX_KV_E4M3 = 3 };
+typedef struct fdx_kv_pages8 {
+    fdx_kv_pages pages;
+    float* k_scale;                   /* [n_pages * page_size / block][kv_heads]     */
+    float* v_scale;
+    int block;
+} fdx_kv_pages8;
+/*
+ * fdx_kv_append_f32 for such a cache.  With Q = 127 (448 for FDX_KV_E4M3) and a the largest |x| that the call brings to a block, the
+ * block's scale becomes s = max(a / Q, 2^-126), or stays what it was if that is more and the block has tokens of earlier calls (those in
+ * front of the call's first position); the code of x is x * (1 / s) rounded to the nearest code, ties to even.  Where the scale grows
+ * from s0, codes c of earlier tokens become c * (s0 / s), rounded the same way.  All in fp32.  So a value is off by at most half a step of
+ * its block's largest value, and by half a step more for every time that the scale has grown since.  An infinity or a NaN makes its
+ * block's scale NaN, and its codes 0: the block's keys (values) of that head are NaN until a call starts the block anew.
+ * No two sequences of one call may write to the same block (fdx_kv8_fork gives each its own).  error_flag_dev as there.
+ */
+fdx_status fdx_kv8_append_f32(const float* k, int64_t ldk, const float* v, int64_t ldv, const int32_t* starts, int tokens,
+    const fdx_kv_pages8* cache, int* error_flag_dev);
+/*
+ * fdx_mha_paged_f32 for such a cache: the same sums over code * scale, the same arguments, refusals and error_flag_dev.
+ * Precision: fp32 sums, exact codes; queries are held as two fp16 values: 22 bits of an element not below 2^-17 of the largest of its
+ * row and head, 2^-40 of that largest below.  A row that sees a block whose scale is NaN, or whose query holds an infinity or a NaN, gets NaN;
+ * rows that do not see it keep their sums.
+ */
+size_t fdx_mha_paged8_scratch_bytes(int tokens, int max_new, int heads, const fdx_kv_pages8* cache);
+fdx_status fdx_mha_paged8_f32(const float* q, int64_t ldq, const int32_t* starts, int tokens, int max_new, int heads,
+    const fdx_kv_pages8* cache, float* out, int64_t ldo, void* scratch_dev, int* error_flag_dev);
+
+/*
+ * The page table after a selection, for fdx_kv_pages of either type and for fdx_kv_pages8 (fdx_kv8_fork): sequence i goes on as a copy of
+ * what sequence parents[i] was, with grow[i] more positions (grow may be NULL: none), or ends if parents[i] is negative.
+ *   new_lens[i]   = lens[parents[i]] + grow[i], 0 for one that ends
+ *   new_table[i]  = the pages of its positions, -1 behind them
+ * Pages that are full are shared.  A partly filled one is kept by the first sequence that goes on in it (unless another holds it as a
+ * full page); every other one gets a page of its own with a copy of the filled rows, and of their blocks' scales.  Pages for those
+ * copies and for more positions are the ones that no sequence keeps, lowest numbers first, in the order of the sequences; so pages of
+ * sequences that nobody goes on from are free by that, and the pages of all users of the cache have to stand in its table.
+ * free_pages (may be NULL) receives how many are left.  The cache's own table and lens are not changed, its pages only where they were free:
+ * new_table and new_lens take their place afterwards; they overlap no input.
+ * A parent of n_seqs or more, a length out of 0 .. max_len, a negative grow or one beyond max_len (both count as 0), a kept page number that
+ * is none of the cache, and a lack of free pages (-1 in new_table) set error_flag_dev (may be NULL) to 1 on the device.
+ * scratch_dev: fdx_kv_fork_scratch_bytes bytes, 16-byte aligned, as for fdx_mha_packed_f32.  n_seqs * table_width < 2^31.
+ */
+size_t fdx_kv_fork_scratch_bytes(const fdx_kv_pages* cache);
+fdx_status fdx_kv_fork(const fdx_kv_pages* cache, const int32_t* parents, const int32_t* grow, int32_t* new_table, int32_t* new_lens,
+    int32_t* free_pages, void* scratch_dev, int* error_flag_dev);
+size_t fdx_kv8_fork_scratch_bytes(const fdx_kv_pages8* cache);
+fdx_status fdx_kv8_fork(const fdx_kv_pages8* cache, const int32_t* parents, const int32_t* grow, int32_t* new_table, int32_t* new_lens,
+    int32_t* free_pages, void* scratch_dev, int* error_flag_dev);
+
+/*
+ * The step of a beam search: of all continuations of a sequence's beams the `keep` best.  Row s * beams + b of logits [n_seqs * beams]
+ * [vocab] (rows ld floats apart) is beam b of sequence s, scores[s][b] its log probability so far; going on with token t comes to
+ *   total(b, t) = scores[s][b] + log softmax(row)[t],
+ * compared in 64 bits; equal totals by ascending beam, then descending logit, then ascending token.  A beam with done[s][b] != 0 (done may
+ * be NULL) has ended: its row is not read, and it has one continuation, end_id with the score it has.
+ *   parents[s][j]     = the row that the j-th best goes on from, s * beams + b (what fdx_kv_fork takes where keep is beams)
+ *   tokens[s][j]      = its token
+ *   new_scores[s][j]  = its total
+ *   new_done[s][j]    = 1 if its token is end_id or its beam had ended, else 0 (new_done may be NULL)
+ * end_id: 0 .. vocab - 1, or negative if no token ends a beam (done and new_done are NULL then).
+ * Logits and scores of -infinity are no continuations; places that are left over get row -1, token -1, score -infinity, done 0.  Rows that
+ * hold a NaN or +infinity, and scores that are one, give no continuations either, and set error_flag_dev (may be NULL) to 1 on the device.
+ * 1 <= keep <= 32, keep <= beams * vocab, beams <= 32.  scratch_dev: fdx_beam_select_scratch_bytes bytes, as for fdx_mha_packed_f32.
+ */
+size_t fdx_beam_select_scratch_bytes(int n_seqs, int beams, int vocab, int keep);
+fdx_status fdx_beam_select_f32(const float* logits, int64_t ld, int n_seqs, int beams, int vocab, const float* scores, const int32_t* done,
+    int end_id, int keep, int32_t* parents, int32_t* tokens, float* new_scores, int32_t* new_done, void* scratch_dev, int* error_flag_dev);
+
+/*
  * What a program reports or decides with besides the greedy token: per row of logits, with p = softmax(row),
  *   logprobs[r]          = log p[ids[r]]        (0 for a negative id, "no token here": a padded place of a batch)
  *   entropy[r]           = -sum_i p[i] log p[i]
