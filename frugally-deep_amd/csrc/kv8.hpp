@@ -46,4 +46,35 @@ __device__ __forceinline__ void from_codes(uint32_t c, float (&x)[4])
     }
 }
 
+// Four codes as four bf16 values, exactly (both kinds have up to eight significant bits): two pairs
+template <int KIND>
+__device__ __forceinline__ void bf16_of_codes(uint32_t c, uint32_t& lo, uint32_t& hi)
+{
+    if constexpr (KIND == kI8) {
+        float x[4];
+        from_codes<KIND>(c, x);
+        lo = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, x[1]), __builtin_bit_cast(uint32_t, x[0]), 0x07060302u);
+        hi = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, x[3]), __builtin_bit_cast(uint32_t, x[2]), 0x07060302u);
+    } else {
+        lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, 1.f, false));
+        hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, 1.f, true));
+    }
+}
+// four rows of four codes, transposed
+__device__ __forceinline__ void transpose_codes(const uint32_t (&r)[4], uint32_t (&t)[4])
+{
+    const uint32_t a = __builtin_amdgcn_perm(r[1], r[0], 0x05010400u), b = __builtin_amdgcn_perm(r[3], r[2], 0x05010400u);
+    const uint32_t c = __builtin_amdgcn_perm(r[1], r[0], 0x07030602u), d = __builtin_amdgcn_perm(r[3], r[2], 0x07030602u);
+    t[0] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+    t[1] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+    t[2] = __builtin_amdgcn_perm(d, c, 0x05040100u);
+    t[3] = __builtin_amdgcn_perm(d, c, 0x07060302u);
+}
+
+// where the scales of a cache are
+struct Scales8 {
+    const float *k, *v;
+    Divisor block;
+};
+
 } // namespace fdx

@@ -1252,6 +1252,11 @@ __global__ __launch_bounds__(256) void ragged_join_kernel(RaggedParams p)
         to[64 + lane] = finish(o1, l, top != -INFINITY);
 }
 
+void ragged_join_launch(const RaggedParams& p)
+{
+    hipLaunchKernelGGL(ragged_join_kernel<kPagedF32>, dim3((unsigned)(((int64_t)p.tokens * p.heads + 3) / 4)), dim3(256), 0, stream(), p);
+}
+
 static int ranges_of(int keys, int64_t most, int* range_keys)
 {
     *range_keys = (int)(most > keys ? keys : (most + 63) & ~(int64_t)63);

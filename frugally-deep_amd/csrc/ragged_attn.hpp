@@ -72,6 +72,8 @@ RaggedPlan paged_plan(int tokens, int max_new, int heads, const fdx_kv_pages* c)
 fdx_status paged_params(const char* who, const float* q, int64_t ldq, const int32_t* starts, int tokens, int max_new, int heads,
     const fdx_kv_pages* cache, float* out, int64_t ldo, void* scratch_dev, int* error_flag_dev, RaggedParams& p, RaggedPlan& plan);
 
+void ragged_join_launch(const RaggedParams& p); // sums of key ranges, whatever the pages hold
+
 template <int KIND>
 struct KvElement {
     typedef float type;
