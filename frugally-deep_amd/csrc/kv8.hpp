@@ -60,6 +60,22 @@ __device__ __forceinline__ void bf16_of_codes(uint32_t c, uint32_t& lo, uint32_t
         hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, 1.f, true));
     }
 }
+// and as four fp16 values
+template <int KIND>
+__device__ __forceinline__ void f16_of_codes(uint32_t c, uint32_t& lo, uint32_t& hi)
+{
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    if constexpr (KIND == kI8) {
+        // 1024 + n has n as its last bits for n = code + 128
+        const uint32_t n = c ^ 0x80808080u;
+        const f16x2 off = { (_Float16)1152.f, (_Float16)1152.f };
+        lo = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(n, 0x64646464u, 0x00050004u)) - off);
+        hi = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(n, 0x64646464u, 0x00070006u)) - off);
+    } else {
+        lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c, 1.f, false));
+        hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c, 1.f, true));
+    }
+}
 // four rows of four codes, transposed
 __device__ __forceinline__ void transpose_codes(const uint32_t (&r)[4], uint32_t (&t)[4])
 {

@@ -2,6 +2,7 @@
 #include <cfloat>
 
 #include "bf16_split.hpp"
+#include "f16_split.hpp"
 #include "kv8.hpp"
 
 namespace fdx {
@@ -57,17 +58,21 @@ __device__ __forceinline__ void load_codes<1, true>(const uint8_t* row, int d, i
     c[0] = d < depth ? *reinterpret_cast<const uint32_t*>(row + d) : 0;
 }
 
+// LDS where the waves' sums meet: a wave's 16 (D + 4) floats each, and 2 * 4 * 16 of m and l
+struct Meet8 {
+    float *of_0, *of_1, *of_2, *of_3, *ml;
+};
+
 template <int D, int KIND, bool WIDE>
-__global__ __launch_bounds__(256, WIDE ? 2 : 1) void paged8_few_kernel(RaggedParams p, Scales8 scales)
+__device__ __forceinline__ void few8_body(const RaggedParams& p, const Scales8& scales, const Place& place, const Meet8& meet)
 {
     typedef Block8<D, WIDE> Block;
     constexpr int NK = Block::NK, DL = Block::DL;
-    __shared__ float meet[4 * 16 * (D + 4)], meet_m[4][16], meet_l[4][16];
-    auto meet_o = [&](int w, int row) { return meet + (w * 16 + row) * (D + 4); };
+    float (*meet_m)[16] = reinterpret_cast<float (*)[16]>(meet.ml), (*meet_l)[16] = meet_m + 4;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 15, g = lane >> 4;
-    const int seq = blockIdx.x / p.kv_heads, kv_head = blockIdx.x % p.kv_heads;
-    if (p.error_flag && blockIdx.x == 0 && blockIdx.y == 0)
+    const int seq = place.x / p.kv_heads, kv_head = place.x % p.kv_heads;
+    if (p.error_flag && place.x == 0 && place.y == 0)
         for (int i = tid; i < p.n_seqs; i += 256)
             raise_flag(p, !packed_start_ok(p.starts, i, p.tokens));
     const Sequence s = sequence_of<kPagedF32>(p, seq, packed_span(p.starts, seq, p.tokens));
@@ -79,8 +84,8 @@ __global__ __launch_bounds__(256, WIDE ? 2 : 1) void paged8_few_kernel(RaggedPar
     const bool halves = count > 16;
     const int step = halves ? 2 : 4, slot = halves ? wave & 1 : wave, r_first = halves ? (wave >> 1) * 16 : 0; // of this wave
     int k_end = visible_keys(p, s, s.span.count - 1);
-    const int64_t k_from = (int64_t)blockIdx.y * s.range;
-    if (blockIdx.y > 0 && k_from >= k_end)
+    const int64_t k_from = (int64_t)place.y * s.range;
+    if (place.y > 0 && k_from >= k_end)
         return;
     const int k_first = (int)k_from;
     if (k_end - k_first > s.range)
@@ -302,11 +307,21 @@ __global__ __launch_bounds__(256, WIDE ? 2 : 1) void paged8_few_kernel(RaggedPar
         meet_m[wave][c] = some && m_run == -INFINITY ? -FLT_MAX : m_run;
         meet_l[wave][c] = l_run;
     }
+    auto leave = [&](float* of) {
 #pragma unroll
-    for (int e = 0; e < DL; ++e)
+        for (int e = 0; e < DL; ++e)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            meet_o(wave, c)[DL * (4 * g + i) + e] = oacc[e][i];
+            for (int i = 0; i < 4; ++i)
+                of[c * (D + 4) + DL * (4 * g + i) + e] = oacc[e][i];
+    };
+    if (wave == 0) // no pointer is chosen by a number: that would be a table in scratch memory
+        leave(meet.of_0);
+    else if (wave == 1)
+        leave(meet.of_1);
+    else if (wave == 2)
+        leave(meet.of_2);
+    else
+        leave(meet.of_3);
     __syncthreads();
     const int row_at = tid >> 4, d0 = (tid & 15) * DL;
     for (int half = 0; half <= (halves ? 1 : 0); ++half) {
@@ -319,12 +334,20 @@ __global__ __launch_bounds__(256, WIDE ? 2 : 1) void paged8_few_kernel(RaggedPar
 #pragma unroll
         for (int e = 0; e < DL; ++e)
             o[e] = 0.f;
-        for (int w = w_first; w <= w_last; ++w) {
+        auto add = [&](int w, const float* of) {
             const float f = __builtin_amdgcn_exp2f(meet_m[w][row_at] - m);
             l += f * meet_l[w][row_at];
 #pragma unroll
             for (int e = 0; e < DL; ++e)
-                o[e] += f * meet_o(w, row_at)[d0 + e];
+                o[e] += f * of[row_at * (D + 4) + d0 + e];
+        };
+        if (w_first == 0) {
+            add(0, meet.of_0);
+            add(1, meet.of_1);
+        }
+        if (w_last == 3) {
+            add(2, meet.of_2);
+            add(3, meet.of_3);
         }
         const int r = 16 * half + row_at;
         if (r >= count)
@@ -332,13 +355,13 @@ __global__ __launch_bounds__(256, WIDE ? 2 : 1) void paged8_few_kernel(RaggedPar
         const int token = quotient(r, p.by_group), head = kv_head * p.group + r - token * p.group;
         const int sees = visible_keys(p, s, token);
         const bool in_parts = sees > s.range;
-        if (in_parts ? k_first >= sees : blockIdx.y > 0)
+        if (in_parts ? k_first >= sees : place.y > 0)
             continue;
         float* to = p.out + (int64_t)(s.span.first + token) * p.ldo + (int64_t)head * p.dv;
         if (in_parts) {
             const int64_t id = part_row(p, s, token, head);
-            to = p.few.out(blockIdx.y, id, p.dv);
-            float* size_at = p.few.size(blockIdx.y, id, p.dv);
+            to = p.few.out(place.y, id, p.dv);
+            float* size_at = p.few.size(place.y, id, p.dv);
             if ((tid & 15) == 0) {
                 size_at[0] = top;
                 size_at[1] = l;
@@ -362,75 +385,420 @@ __global__ __launch_bounds__(256, WIDE ? 2 : 1) void paged8_few_kernel(RaggedPar
     }
 }
 
-// A wave takes a row: a lane has a key's score, then depths lane and 64 + lane of the output.
-template <int KIND>
-__global__ __launch_bounds__(256) void paged8_kernel(RaggedParams p, Scales8 scales)
+template <int D, int KIND, bool WIDE>
+__global__ __launch_bounds__(256, WIDE ? 2 : 1) void paged8_few_kernel(RaggedParams p, Scales8 scales)
 {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t item = (int64_t)blockIdx.x * 4 + wave;
-    if (blockIdx.x == 0)
-        for (int i = threadIdx.x; i < p.n_seqs; i += 256)
+    __shared__ float meet[4][16 * (D + 4)], ml[2 * 4 * 16];
+    few8_body<D, KIND, WIDE>(p, scales, Place { blockIdx.x, blockIdx.y, gridDim.x }, Meet8 { meet[0], meet[1], meet[2], meet[3], ml });
+}
+
+// ---- many query rows: tiles on the fp16 matrix instructions ----
+//
+// A workgroup takes 128 rows of one key head of one sequence, rows counting through the query heads of the group first (row = token *
+// group + head), a wave 32 of them; keys and values pass through LDS in tiles of 4096 / D keys, codes as the fp16 values that they are.  Products
+// are taken transposed, S^T = K Q^T and O^T = V^T P^T: a query is a lane's column and keys are the accumulator's registers.
+//  * A query row is brought to fp16's range by a power of two and held as two fp16 values (f16_split.hpp).  So are its probabilities times
+//    the values' scales, by a power that keeps the largest of them so far between 2^6 and 2^15: a row has sums of its own power, and none
+//    depends on keys that it does not see.  A key's scale meets its score.
+//  * LDS holds two tiles.  While the probabilities of tile t meet its values, the scores of tile t + 1 are multiplied; tile t + 2's keys and tile
+//    t + 1's values go to LDS, what comes behind them to registers; one barrier a tile.
+template <int D>
+struct Tile8 {
+    static constexpr int KT = 4096 / D, N = 256 / KT; // keys of a tile; threads that fetch a key, 16 codes each
+    static constexpr int KBLK = KT * 16 + 128 / N, VROW = D * 2 + 32; // bytes of a block of 8 depths, of a row of values, offset against each other
+    static constexpr int kKeys = D / 8 * KBLK, kValues = KT * VROW; // bytes of a tile
+    static constexpr int kAhead = 512; // places of two halves of as many positions are looked up ahead, all threads at once
+};
+struct TileLds8 {
+    unsigned char *ks0, *ks1, *vs0, *vs1;
+    float *scale0, *scale1; // of a tile's keys, then of its values
+    int *rows_of, *some_absent;
+};
+#define FDX_TILE8_LDS(D, lds)                                                                                               \
+    __shared__ __attribute__((aligned(16))) unsigned char lds##_ks0[Tile8<D>::kKeys], lds##_ks1[Tile8<D>::kKeys];           \
+    __shared__ __attribute__((aligned(16))) unsigned char lds##_vs0[Tile8<D>::kValues], lds##_vs1[Tile8<D>::kValues];       \
+    __shared__ __attribute__((aligned(16))) float lds##_scale0[2 * Tile8<D>::KT], lds##_scale1[2 * Tile8<D>::KT];           \
+    __shared__ int lds##_rows_of[2 * Tile8<D>::kAhead];                                                                     \
+    __shared__ int lds##_absent;                                                                                            \
+    const TileLds8 lds { lds##_ks0, lds##_ks1, lds##_vs0, lds##_vs1, lds##_scale0, lds##_scale1, lds##_rows_of, &lds##_absent }
+
+template <int D, int KIND, bool WIDE>
+__device__ __forceinline__ void tile8_body(const RaggedParams& p, const Scales8& scales, const Place& place_in, const TileLds8& lds)
+{
+    typedef Tile8<D> S;
+    typedef float f32x16 __attribute__((ext_vector_type(16)));
+    constexpr int KT = S::KT, HALVES = KT / 32, N = S::N, STEPS = D / 16, DB = D / 32, KBLK = S::KBLK, VROW = S::VROW, kAhead = S::kAhead;
+    int* rows_of = lds.rows_of;
+    int& some_absent = *lds.some_absent;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c = lane & 31, half = lane >> 5;
+    if (p.error_flag && place_in.x == 0 && place_in.y == 0)
+        for (int i = tid; i < p.n_seqs; i += 256) // lengths too: a sequence without new tokens has no tile
             raise_flag(p, !packed_start_ok(p.starts, i, p.tokens) || p.lens[i] < 0 || p.lens[i] > p.max_len);
-    const int row = (int)(item / p.heads), head = (int)(item - (int64_t)row * p.heads);
-    if (row >= p.tokens)
+    // key heads next to each other, later tiles of a sequence, which see more keys, first
+    const int kv_head = place_in.x % p.kv_heads;
+    const int64_t number = place_in.x / p.kv_heads;
+    const Tile tile = p.n_seqs <= 64 ? late_tile(SearchWave(), p.starts, p.n_seqs, p.tokens, p.group, 128, number)
+                                     : find_tile(SearchWave(), p.starts, p.n_seqs, p.tokens, p.group, 128, place_in.nx / p.kv_heads - 1 - number);
+    if (tile.seq < 0)
         return;
-    const int index = find_row(SearchWave(), p.starts, p.n_seqs, p.tokens, row);
-    if (index < 0)
+    const Sequence s = sequence_of<kPagedF32>(p, tile.seq, tile.span);
+    if (tid == 0)
+        raise_flag(p, s.cut);
+    const int count = s.span.count * p.group; // rows
+    const int r_first = tile.index * 128;
+    if (r_first >= count || s.few)
         return;
-    const Sequence s = sequence_of<kPagedF32>(p, index, packed_span(p.starts, index, p.tokens));
-    raise_flag(p, s.cut);
-    const int token = row - s.span.first;
-    if (token >= s.span.count || s.few)
+    const int mine = r_first + wave * 32 + c;
+    const bool q_ok = mine < count;
+    const int token = quotient(q_ok ? mine : count - 1, p.by_group), head = kv_head * p.group + (q_ok ? mine : count - 1) - token * p.group;
+    const int64_t q_row = s.span.first + token;
+    const int visible = visible_keys(p, s, token);
+    const int r_last = r_first + 128 < count ? r_first + 127 : count - 1;
+    int k_end = visible_keys(p, s, quotient(r_last, p.by_group)); // of the workgroup's last row
+    const int64_t k_from = (int64_t)place_in.y * s.range;
+    if (place_in.y > 0 && k_from >= k_end)
         return;
-    const int kv_head = quotient(head, p.by_group), last = visible_keys(p, s, token);
-    const float* q = p.q + (int64_t)row * p.ldq + (int64_t)head * p.dk;
-    const uint8_t* kb = static_cast<const uint8_t*>(p.k) + (int64_t)kv_head * p.dk;
-    const uint8_t* vb = static_cast<const uint8_t*>(p.v) + (int64_t)kv_head * p.dv;
-    float m = -INFINITY, l = 0.f, o[2] = { 0.f, 0.f };
-    bool seen = false;
-    for (int j0 = 0; j0 < last; j0 += 64) {
-        const int at = j0 + lane < last ? key_row<kPagedF32>(p, s, j0 + lane) : -1;
-        seen = seen || __any(at >= 0);
-        raise_flag(p, j0 + lane < last && at < 0);
-        float sc = -INFINITY, vs = 0.f;
-        if (at >= 0) {
-            const int64_t scale = (int64_t)quotient(at, scales.block) * p.kv_heads + kv_head;
-            float dot = 0.f;
-            for (int d = 0; d < p.dk; ++d) {
-                float x[4];
-                from_codes<KIND>(kb[(int64_t)at * p.ldk + d], x);
-                dot = fmaf(q[d], x[0], dot);
+    const int k_first = (int)k_from;
+    if (k_end - k_first > s.range)
+        k_end = k_first + s.range;
+    const int tiles = k_end > k_first ? (k_end - k_first + KT - 1) / KT : 0;
+    // what the wave's rows see: all of them the first `wave_all_see`, some the first `wave_any`
+    const int w_first = r_first + wave * 32, w_last = w_first + 31 < count ? w_first + 31 : count - 1;
+    const int wave_all_see = visible_keys(p, s, quotient(w_first < count ? w_first : count - 1, p.by_group));
+    const int wave_any = visible_keys(p, s, quotient(w_last, p.by_group));
+
+    const uint8_t* kbase = static_cast<const uint8_t*>(p.k) + (int64_t)kv_head * p.dk;
+    const uint8_t* vbase = static_cast<const uint8_t*>(p.v) + (int64_t)kv_head * p.dv;
+    const int krow = tid / N, kl = tid % N;
+    // 2 KT threads, whole waves or halves of one, fetch a scale each: of a key, or of its values
+    const bool scaled = tid < 2 * KT;
+    const float* scale_base = (tid < KT ? scales.k : scales.v) + kv_head;
+    uint32_t kst[4], vst[4];
+    float sst = 0.f;
+    auto place = [&](int t, int key) { return rows_of[(t * KT + key) & (2 * kAhead - 1)]; };
+    auto look_up = [&](int first) { // places of positions first .. first + kAhead - 1 of the range; those behind it repeat its last one
+#pragma unroll
+        for (int i = 0; i < kAhead; i += 256) {
+            const int at = k_first + first + i + tid;
+            const int row = key_row<kPagedF32>(p, s, at < k_end ? at : k_end - 1);
+            rows_of[(first + i + tid) & (2 * kAhead - 1)] = row;
+            if (row < 0) {
+                some_absent = 1;
+                raise_flag(p, true);
             }
-            sc = dot * (p.scale * kLog2e) * scales.k[scale];
-            vs = scales.v[scale];
         }
-        const bool nan = __any(sc != sc);
-        const float m_new = nan ? NAN : fmaxf(m, wave_all<true>(sc)), m_use = m_new == -INFINITY ? 0.f : m_new;
-        const float corr = __builtin_amdgcn_exp2f(m - m_use), pr = at >= 0 ? __builtin_amdgcn_exp2f(sc - m_use) : 0.f;
-        l = l * corr + wave_all<false>(pr);
-        m = m_new;
-        float part[2] = { 0.f, 0.f }; // of these keys: one chain over all of them would round a thousand times
-        const float w = at >= 0 ? pr * vs : 0.f;
-        for (int j = 0; j < 64; ++j) {
-            const int r = __shfl(at, j, 64);
-            const float wj = __shfl(w, j, 64);
-            if (r < 0)
-                continue;
+    };
+    auto zero_codes = [](uint32_t (&x)[4]) { x[0] = x[1] = x[2] = x[3] = 0; };
+    auto fetch_keys = [&](int t) {
+        const int row = place(t, krow);
+        load_codes<4, WIDE>(kbase + (int64_t)(row < 0 ? 0 : row) * p.ldk, 16 * kl, p.dk, kst);
+        if (row < 0)
+            zero_codes(kst);
+    };
+    auto fetch_values = [&](int t) {
+        const int row = place(t, krow);
+        load_codes<4, WIDE>(vbase + (int64_t)(row < 0 ? 0 : row) * p.ldv, 16 * kl, p.dv, vst);
+        if (row < 0)
+            zero_codes(vst);
+        if (scaled) {
+            const int at = place(t, tid & (KT - 1));
+            sst = at < 0 ? 0.f : scale_base[(int64_t)quotient(at, scales.block) * p.kv_heads];
+        }
+    };
+    auto stage_keys = [&](unsigned char* ks) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-                if (64 * i + lane < p.dv) {
-                    float x[4];
-                    from_codes<KIND>(vb[(int64_t)r * p.ldv + 64 * i + lane], x);
-                    part[i] = fmaf(wj, x[0], part[i]);
-                }
+        for (int h = 0; h < 2; ++h) {
+            u32x4 w;
+            uint32_t lo, hi;
+            f16_of_codes<KIND>(kst[2 * h], lo, hi);
+            w[0] = lo;
+            w[1] = hi;
+            f16_of_codes<KIND>(kst[2 * h + 1], lo, hi);
+            w[2] = lo;
+            w[3] = hi;
+            *reinterpret_cast<u32x4*>(&ks[(2 * kl + h) * KBLK + krow * 16]) = w;
         }
-        o[0] = fmaf(o[0], corr, part[0]);
-        o[1] = fmaf(o[1], corr, part[1]);
+    };
+    auto stage_values = [&](unsigned char* vs, float* scale) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            u32x4 w;
+            uint32_t lo, hi;
+            f16_of_codes<KIND>(vst[2 * h], lo, hi);
+            w[0] = lo;
+            w[1] = hi;
+            f16_of_codes<KIND>(vst[2 * h + 1], lo, hi);
+            w[2] = lo;
+            w[3] = hi;
+            *reinterpret_cast<u32x4*>(&vs[krow * VROW + 32 * kl + 16 * h]) = w;
+        }
+        if (scaled)
+            scale[tid] = sst;
+    };
+
+    if (tiles > 0) {
+        if (tid == 0)
+            some_absent = 0;
+        __syncthreads();
+        look_up(0);
+        if (tiles > kAhead / KT)
+            look_up(kAhead);
+        __syncthreads();
+        fetch_keys(0);
+        fetch_values(0);
     }
+
+    f16x8 qh[STEPS], ql[STEPS]; // depths 16 u + 8 half ..
+    float to_log2;
+    {
+        float x[STEPS][8], top = 0.f;
+        const float* from = p.q + q_row * p.ldq + (int64_t)head * p.dk;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-        if (64 * i + lane < p.dv)
-            p.out[(int64_t)row * p.ldo + (int64_t)head * p.dv + 64 * i + lane] = finish(o[i], l, seen);
+        for (int u = 0; u < STEPS; ++u)
+#pragma unroll
+            for (int e = 0; e < 8; e += 4) {
+                const int d = 16 * u + 8 * half + e;
+                f32x4 y = { 0.f, 0.f, 0.f, 0.f };
+                if (WIDE) {
+                    if (d < p.dk)
+                        y = *reinterpret_cast<const f32x4*>(from + d);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (d + i < p.dk)
+                            y[i] = from[d + i];
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    x[u][e + i] = y[i];
+                    top = fmaxf(top, fabsf(y[i]));
+                }
+            }
+        const Pow2 sq = pow2_for<1>(exponent(max_halves(top)));
+        to_log2 = sq.down * (p.scale * kLog2e);
+#pragma unroll
+        for (int u = 0; u < STEPS; ++u)
+            split2x8(x[u], sq.up, qh[u], ql[u]);
+    }
+
+    auto mfma = [](f16x8 a, f16x8 b, const f32x16& acc) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, acc, 0, 0, 0); };
+    constexpr f32x16 kZero = { 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f };
+    f32x16 oacc[DB], sa[HALVES], sb[HALVES];
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+        oacc[d] = kZero;
+    float m_run = -INFINITY, l_run = 0.f;
+    float w_most = 0.f; // the largest probability times scale so far, to within 2^4
+    Pow2 power = pow2_for<1>(0); // of the sums
+    bool seen = false;
+
+    auto scores = [&](f32x16 (&sc)[HALVES], const unsigned char* ks) {
+#pragma unroll
+        for (int kb = 0; kb < HALVES; ++kb) {
+            sc[kb] = kZero;
+#pragma unroll
+            for (int u = 0; u < STEPS; ++u) {
+                const f16x8 k = *reinterpret_cast<const f16x8*>(&ks[(2 * u + half) * KBLK + (kb * 32 + c) * 16]);
+                sc[kb] = mfma(k, ql[u], sc[kb]);
+                sc[kb] = mfma(k, qh[u], sc[kb]);
+            }
+        }
+    };
+    // values of four keys for this lane's depth: sixteen lanes address four rows of sixteen depths
+    const int v_at = (4 * half + ((c & 15) >> 2)) * VROW + (16 * (c >> 4) + 4 * (c & 3)) * 2;
+    auto values = [&](const unsigned char* vs, int key, int d) {
+        typedef short s16x4 __attribute__((ext_vector_type(4)));
+        struct {
+            s16x4 a, b;
+        } r;
+        r.a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(vs + v_at + key * VROW + d * 64));
+        r.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(vs + v_at + (key + 8) * VROW + d * 64));
+        return __builtin_bit_cast(f16x8, r);
+    };
+    // tile t: its scores are in sc, its values and scales in vs and scale, the keys of tile t + 1 in ks; registers hold the codes of tile t + 2's
+    // keys and of tile t + 1's values
+    auto turn = [&](int t, f32x16 (&sc)[HALVES], f32x16 (&next)[HALVES], const unsigned char* ks, const unsigned char* vs, const float* scale,
+                    unsigned char* ks_to, unsigned char* vs_to, float* scale_to) {
+        const int j0 = k_first + t * KT;
+        if (t + 1 < tiles) {
+            stage_values(vs_to, scale_to);
+            if (t + 2 < tiles) {
+                stage_keys(ks_to);
+                fetch_values(t + 2);
+                if (t + 3 < tiles)
+                    fetch_keys(t + 3);
+            }
+        }
+        const int absent = some_absent;
+        if ((t * KT & (kAhead - 1)) == 0 && t > 0 && (t + kAhead / KT) < tiles)
+            look_up(t * KT + kAhead); // into the half that is done with
+        if (j0 < wave_any) { // some row of this wave sees some key of the tile
+            const int limit = (visible < k_end ? visible : k_end) - j0; // keys of the tile that this lane's row sees
+            const bool some_hidden = j0 + KT > wave_all_see || j0 + KT > k_end, some_gone = __builtin_amdgcn_readfirstlane(absent) != 0;
+            auto hidden = [&](int key) { return key >= limit || (some_gone && rows_of[(t * KT + key) & (2 * kAhead - 1)] < 0); };
+            float mx = -INFINITY;
+#pragma unroll
+            for (int kb = 0; kb < HALVES; ++kb)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const f32x4 by = *reinterpret_cast<const f32x4*>(scale + kb * 32 + 8 * g + 4 * half);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        sc[kb][4 * g + i] = sc[kb][4 * g + i] * to_log2 * by[i];
+                }
+            if (some_hidden || some_gone) {
+#pragma unroll
+                for (int kb = 0; kb < HALVES; ++kb)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const bool h = hidden(kb * 32 + 8 * (e >> 2) + 4 * half + (e & 3));
+                        sc[kb][e] = h ? -INFINITY : sc[kb][e];
+                        seen = seen || !h;
+                    }
+            } else {
+                seen = true;
+            }
+#pragma unroll
+            for (int kb = 0; kb < HALVES; ++kb)
+#pragma unroll
+                for (int e = 0; e < 16; e += 2)
+                    mx = fmaxf(fmaxf(mx, sc[kb][e]), sc[kb][e + 1]);
+            mx = max_halves(mx);
+            float corr = 1.f;
+            if (__any(mx > m_run + 4.f)) {
+                const float m_new = mx > m_run + 4.f ? mx : m_run;
+                corr = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
+                m_run = m_new;
+                l_run *= corr;
+                w_most *= corr;
+            }
+            const float base = m_run == -INFINITY ? 0.f : m_run; // a row that has seen no key yet adds zeros
+            float rs = 0.f, most = 0.f;
+#pragma unroll
+            for (int kb = 0; kb < HALVES; ++kb)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    sc[kb][e] = __builtin_amdgcn_exp2f(sc[kb][e] - base);
+                    rs += sc[kb][e];
+                }
+            l_run += rs; // the other half of the tile's keys lies in lane + 32: they meet at the end
+#pragma unroll
+            for (int kb = 0; kb < HALVES; ++kb)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const f32x4 by = *reinterpret_cast<const f32x4*>(scale + KT + kb * 32 + 8 * g + 4 * half);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        sc[kb][4 * g + i] *= by[i];
+                }
+            if (some_hidden || some_gone) { // a scale of NaN is for the rows that see it
+#pragma unroll
+                for (int kb = 0; kb < HALVES; ++kb)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        sc[kb][e] = hidden(kb * 32 + 8 * (e >> 2) + 4 * half + (e & 3)) ? 0.f : sc[kb][e];
+            }
+#pragma unroll
+            for (int kb = 0; kb < HALVES; ++kb)
+#pragma unroll
+                for (int e = 0; e < 16; e += 2)
+                    most = fmaxf(fmaxf(most, sc[kb][e]), sc[kb][e + 1]);
+            most = max_halves(most);
+            if (__any(most > w_most * 16.f || corr != 1.f)) {
+                w_most = fmaxf(w_most, most);
+                const Pow2 now = pow2_for<1>(exponent(w_most) + 5); // at most 2^10
+                const float by = corr * (now.up * power.down);
+                power = now;
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        oacc[d][e] *= by;
+            }
+            scores(next, ks);
+            // O^T += V^T P^T
+#pragma unroll
+            for (int u = 0; u < KT / 16; ++u) { // keys of block 2 u + half: registers 8 (u % 2) .. + 7 of accumulator u / 2
+                float x[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    x[j] = sc[u >> 1][8 * (u & 1) + j];
+                f16x8 ph, pl;
+                split2x8(x, power.up, ph, pl);
+#pragma unroll
+                for (int d = 0; d < DB; ++d) {
+                    const f16x8 v = values(vs, 16 * u, d);
+                    oacc[d] = mfma(v, pl, oacc[d]);
+                    oacc[d] = mfma(v, ph, oacc[d]);
+                }
+            }
+        }
+        __syncthreads();
+    };
+    if (tiles > 0) {
+        stage_keys(lds.ks0);
+        stage_values(lds.vs0, lds.scale0);
+        if (tiles > 1) {
+            fetch_keys(1);
+            fetch_values(1);
+            stage_keys(lds.ks1);
+            if (tiles > 2)
+                fetch_keys(2);
+        }
+        __syncthreads();
+        scores(sa, lds.ks0);
+        __syncthreads(); // ks0 is done with
+    }
+    for (int t = 0; t < tiles; t += 2) {
+        turn(t, sa, sb, lds.ks1, lds.vs0, lds.scale0, lds.ks0, lds.vs1, lds.scale1);
+        if (t + 1 < tiles)
+            turn(t + 1, sb, sa, lds.ks0, lds.vs1, lds.scale1, lds.ks1, lds.vs0, lds.scale0);
+    }
+
+    l_run += __shfl_xor(l_run, 32, 64);
+    const uint64_t seen_by = __ballot(seen);
+    const bool some = ((seen_by | seen_by >> 32) >> c & 1) != 0;
+    const bool in_parts = visible > s.range;
+    if (!q_ok || !(in_parts ? k_first < visible : place_in.y == 0))
+        return;
+    float* to = p.out + q_row * p.ldo + (int64_t)head * p.dv;
+    if (in_parts) {
+        const int64_t id = part_row(p, s, token, head);
+        to = p.tile.out(place_in.y, id, p.dv);
+        float* at = p.tile.size(place_in.y, id, p.dv);
+        if (half == 0) {
+            at[0] = some && m_run == -INFINITY ? -FLT_MAX : m_run;
+            at[1] = l_run;
+        }
+    }
+    const float none = some && !in_parts ? NAN : 0.f; // no key: zeros; scores of -infinity only: no softmax
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int depth = 32 * d + 8 * g + 4 * half;
+            f32x4 o;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                o[i] = l_run == 0.f ? none : oacc[d][4 * g + i] / l_run * power.down;
+            if (WIDE) {
+                if (depth < p.dv)
+                    *reinterpret_cast<f32x4*>(to + depth) = o;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (depth + i < p.dv)
+                        to[depth + i] = o[i];
+            }
+        }
+}
+
+template <int D, int KIND, bool WIDE>
+__global__ __launch_bounds__(256, 2) void paged8_tile_kernel(RaggedParams p, Scales8 scales)
+{
+    FDX_TILE8_LDS(D, lds);
+    tile8_body<D, KIND, WIDE>(p, scales, Place { blockIdx.x, blockIdx.y, gridDim.x }, lds);
 }
 
 template <int D, int KIND>
@@ -447,8 +815,13 @@ static void paged8_launch(const RaggedParams& p, const RaggedPlan& plan, const S
         else
             hipLaunchKernelGGL((paged8_few_kernel<D, KIND, false>), few, dim3(256), 0, stream(), p, scales);
     }
-    if (plan.tiles > 0)
-        hipLaunchKernelGGL(paged8_kernel<KIND>, dim3((unsigned)(((int64_t)p.tokens * p.heads + 3) / 4)), dim3(256), 0, stream(), p, scales);
+    if (plan.tiles > 0) {
+        const dim3 grid((unsigned)plan.tiles, (unsigned)plan.tile_ranges);
+        if (wide)
+            hipLaunchKernelGGL((paged8_tile_kernel<D, KIND, true>), grid, dim3(256), 0, stream(), p, scales);
+        else
+            hipLaunchKernelGGL((paged8_tile_kernel<D, KIND, false>), grid, dim3(256), 0, stream(), p, scales);
+    }
     if (plan.few_ranges > 1 || plan.tile_ranges > 1)
         ragged_join_launch(p);
 }
@@ -473,8 +846,6 @@ extern "C" fdx_status fdx_mha_paged8_f32(const float* q, int64_t ldq, const int3
     st = paged_params("mha_paged8", q, ldq, starts, tokens, max_new, heads, &cache->pages, out, ldo, scratch_dev, error_flag_dev, p, plan);
     if (st != FDX_OK)
         return st;
-    p.tile.keys = 0x7fffffff;
-    plan.tile_ranges = 1;
     const Scales8 scales { cache->k_scale, cache->v_scale, make_divisor(cache->block) };
     const bool small = p.dk <= 64 && p.dv <= 64;
     profile_begin();

@@ -101,11 +101,6 @@ __device__ __forceinline__ QueryRow row_of(const RaggedParams& p, const Sequence
 
 constexpr float kShift = 10.f; // exponentials are 2^kShift times the probability's numerator
 
-// where a workgroup stands in its launch
-struct Place {
-    unsigned x, y, nx;
-};
-
 template <int D, int KIND>
 struct TileSizes {
     static constexpr int KT = 4096 / D, N = D / 16; // keys of a tile; threads that fetch a key

@@ -74,6 +74,11 @@ fdx_status paged_params(const char* who, const float* q, int64_t ldq, const int3
 
 void ragged_join_launch(const RaggedParams& p); // sums of key ranges, whatever the pages hold
 
+// where a workgroup stands in its launch
+struct Place {
+    unsigned x, y, nx;
+};
+
 template <int KIND>
 struct KvElement {
     typedef float type;
