@@ -46,21 +46,7 @@ __device__ __forceinline__ void from_codes(uint32_t c, float (&x)[4])
     }
 }
 
-// Four codes as four bf16 values, exactly (both kinds have up to eight significant bits): two pairs
-template <int KIND>
-__device__ __forceinline__ void bf16_of_codes(uint32_t c, uint32_t& lo, uint32_t& hi)
-{
-    if constexpr (KIND == kI8) {
-        float x[4];
-        from_codes<KIND>(c, x);
-        lo = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, x[1]), __builtin_bit_cast(uint32_t, x[0]), 0x07060302u);
-        hi = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, x[3]), __builtin_bit_cast(uint32_t, x[2]), 0x07060302u);
-    } else {
-        lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, 1.f, false));
-        hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, 1.f, true));
-    }
-}
-// and as four fp16 values
+// Four codes as four fp16 values, exactly: two pairs
 template <int KIND>
 __device__ __forceinline__ void f16_of_codes(uint32_t c, uint32_t& lo, uint32_t& hi)
 {

@@ -15,8 +15,9 @@ namespace fdx {
 //    16 + 4 g .. of row c.
 //  * O^T = V^T P^T over the turn's 32 keys: lane (c, g) loads D / 16 codes of those eight keys at depth D / 16 c, so the probabilities it has are
 //    the operand, and gets depths D / 16 (4 g + i) + e of row c.
-//  * Codes are bf16 values exactly; queries, and probabilities times their values' scales, are the exact sums of three bf16 values.  A key's scale
-//    meets its score, so neither takes a step of its own: lane (c, g) has looked up one scale, and a lane's number in its row of sixteen names it.
+//  * Codes are fp16 values exactly; a query is held as two fp16 values (f16_split.hpp), and so are its probabilities times their values' scales, by a
+//    power that keeps the largest of them so far in fp16's range: a row has sums of its own power, and none depends on keys that it does not see.
+//  * A key's scale meets its score; lane (c, g) has looked up one scale, and a lane's number in its row of sixteen names it for all of them.
 template <int D, bool WIDE>
 struct Block8 {
     static constexpr int NK = D / 64, DL = D / 16;
@@ -26,21 +27,24 @@ struct Block8 {
     int row;              // place of key lane % 32
 };
 
-// 4 N codes of a row from depth d on, zeros behind `depth`
+// 4 N codes of a row from depth d on; WIDE: from its first on where d is behind `depth`, any codes: queries are zeros there, and nobody stores that depth
 template <int N, bool WIDE>
-__device__ __forceinline__ void load_codes(const uint8_t* row, int d, int depth, uint32_t* c)
+__device__ __forceinline__ void load_codes(const uint8_t* row, int d, int depth, uint32_t (&c)[N])
 {
-    typedef uint32_t cv __attribute__((ext_vector_type(N)));
     if constexpr (WIDE) {
-        cv x;
+        const uint8_t* from = row + (d < depth ? d : 0);
+        if constexpr (N == 4) {
+            const u32x4 x = *reinterpret_cast<const u32x4*>(from);
 #pragma unroll
-        for (int e = 0; e < N; ++e)
-            x[e] = 0;
-        if (d < depth)
-            x = *reinterpret_cast<const cv*>(row + d);
-#pragma unroll
-        for (int e = 0; e < N; ++e)
-            c[e] = x[e];
+            for (int e = 0; e < 4; ++e)
+                c[e] = x[e];
+        } else if constexpr (N == 2) {
+            const uint2 x = *reinterpret_cast<const uint2*>(from);
+            c[0] = x.x;
+            c[1] = x.y;
+        } else {
+            c[0] = *reinterpret_cast<const uint32_t*>(from);
+        }
     } else {
 #pragma unroll
         for (int e = 0; e < N; ++e) {
@@ -51,11 +55,6 @@ __device__ __forceinline__ void load_codes(const uint8_t* row, int d, int depth,
                     c[e] |= (uint32_t)row[d + 4 * e + i] << (8 * i);
         }
     }
-}
-template <>
-__device__ __forceinline__ void load_codes<1, true>(const uint8_t* row, int d, int depth, uint32_t* c)
-{
-    c[0] = d < depth ? *reinterpret_cast<const uint32_t*>(row + d) : 0;
 }
 
 // LDS where the waves' sums meet: a wave's 16 (D + 4) floats each, and 2 * 4 * 16 of m and l
@@ -100,19 +99,25 @@ __device__ __forceinline__ void few8_body(const RaggedParams& p, const Scales8& 
         const int at = k_first + blk * 32 + (lane & 31);
         return key_row<kPagedF32>(p, s, at < k_end ? at : k_end - 1);
     };
+    // where rows start is 32 bits in units of 16 bytes (see `wide` of paged8_launch), which saves the products of 64 bits
+    const uint32_t k_units = (uint32_t)(p.ldk >> 4), v_units = (uint32_t)(p.ldv >> 4);
     auto fetch = [&](Block& b, int row) {
         b.row = row;
         row = row < 0 ? 0 : row;
+        const uint32_t k_at = (uint32_t)row * k_units, v_at = (uint32_t)row * v_units;
 #pragma unroll
         for (int z = 0; z < 2; ++z) {
-            const uint8_t* kr = kbase + (int64_t)__shfl(row, 16 * z + c, 64) * p.ldk;
+            const uint8_t* kr = WIDE ? kbase + ((uint64_t)(uint32_t)__shfl((int)k_at, 16 * z + c, 64) << 4) : kbase + (int64_t)__shfl(row, 16 * z + c, 64) * p.ldk;
 #pragma unroll
             for (int i = 0; i < NK; ++i)
                 load_codes<4, WIDE>(kr, 64 * i + 16 * g, p.dk, b.k[z][i]);
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            load_codes<DL / 4, WIDE>(vbase + (int64_t)__shfl(row, 16 * (i >> 2) + 4 * g + (i & 3), 64) * p.ldv, DL * c, p.dv, b.v[i]);
+        for (int i = 0; i < 8; ++i) {
+            const int key = 16 * (i >> 2) + 4 * g + (i & 3);
+            const uint8_t* vr = WIDE ? vbase + ((uint64_t)(uint32_t)__shfl((int)v_at, key, 64) << 4) : vbase + (int64_t)__shfl(row, key, 64) * p.ldv;
+            load_codes<DL / 4, WIDE>(vr, DL * c, p.dv, b.v[i]);
+        }
         b.scale = scale_base[(int64_t)quotient(__shfl(row, scale_key, 64), scales.block) * p.kv_heads];
     };
     Block a, b;
@@ -124,43 +129,46 @@ __device__ __forceinline__ void few8_body(const RaggedParams& p, const Scales8& 
     }
 
     // the query: step (i, h) has depths 64 i + 16 g + 8 h ..
-    bf16x8 q[2 * NK][3];
+    f16x8 qh[2 * NK], ql[2 * NK];
+    float to_log2;
     const bool q_ok = r_first + c < count;
     const int q_token = quotient(q_ok ? r_first + c : 0, p.by_group);
     const int visible = q_ok ? visible_keys(p, s, q_token) : 0;
     {
         const float* from = p.q + (int64_t)(s.span.first + q_token) * p.ldq
             + (int64_t)(kv_head * p.group + (q_ok ? r_first + c : 0) - q_token * p.group) * p.dk;
+        float x[2 * NK][8], top = 0.f;
 #pragma unroll
-        for (int u = 0; u < 2 * NK; ++u) {
-            const int d = 64 * (u >> 1) + 16 * g + 8 * (u & 1);
-            float x[8];
+        for (int u = 0; u < 2 * NK; ++u)
 #pragma unroll
             for (int e = 0; e < 8; e += 4) {
+                const int d = 64 * (u >> 1) + 16 * g + 8 * (u & 1) + e;
                 f32x4 y = { 0.f, 0.f, 0.f, 0.f };
                 if (WIDE) {
-                    if (d + e < p.dk)
-                        y = *reinterpret_cast<const f32x4*>(from + d + e);
+                    if (d < p.dk)
+                        y = *reinterpret_cast<const f32x4*>(from + d);
                 } else {
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        if (d + e + i < p.dk)
-                            y[i] = from[d + e + i];
+                        if (d + i < p.dk)
+                            y[i] = from[d + i];
                 }
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    x[e + i] = y[i] * (p.scale * kLog2e);
+                for (int i = 0; i < 4; ++i) {
+                    x[u][e + i] = y[i];
+                    top = fmaxf(top, fabsf(y[i]));
+                }
             }
-            uint32_t w[3][4];
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        const Pow2 sq = pow2_for<1>(exponent(max_halves(top)));
+        to_log2 = sq.down * (p.scale * kLog2e);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                split3(x[2 * i], x[2 * i + 1], w[0][i], w[1][i], w[2][i]);
-#pragma unroll
-            for (int z = 0; z < 3; ++z)
-                q[u][z] = __builtin_bit_cast(bf16x8, (u32x4 { w[z][0], w[z][1], w[z][2], w[z][3] }));
-        }
+        for (int u = 0; u < 2 * NK; ++u)
+            split2x8(x[u], sq.up, qh[u], ql[u]);
     }
     float m_run = -INFINITY, l_run = 0.f;
+    float w_most = 0.f; // the largest probability times scale so far, to within 2^4
+    Pow2 power = pow2_for<1>(0); // of the sums
     f32x4 oacc[DL];
 #pragma unroll
     for (int e = 0; e < DL; ++e)
@@ -168,36 +176,43 @@ __device__ __forceinline__ void few8_body(const RaggedParams& p, const Scales8& 
     // keys that the first row sees are seen by all
     const int first_sees = visible_keys(p, s, quotient(r_first, p.by_group)), all_see = first_sees < k_end ? first_sees : k_end;
     bool missing = false, seen = false;
-    auto mfma = [](bf16x8 x, bf16x8 y, const f32x4& acc) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, acc, 0, 0, 0); };
+    auto mfma = [](f16x8 x, f16x8 y, const f32x4& acc) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, acc, 0, 0, 0); };
+    auto most_of_row = [](float x) { return max_halves(fmaxf(x, __shfl_xor(x, 16, 64))); }; // lanes c, 16 + c, 32 + c and 48 + c
     auto work = [&](Block& x, int blk) {
+        auto operand = [](uint32_t a, uint32_t b) {
+            u32x4 w;
+            uint32_t lo, hi;
+            f16_of_codes<KIND>(a, lo, hi);
+            w[0] = lo;
+            w[1] = hi;
+            f16_of_codes<KIND>(b, lo, hi);
+            w[2] = lo;
+            w[3] = hi;
+            return __builtin_bit_cast(f16x8, w);
+        };
         f32x4 acc[2];
 #pragma unroll
         for (int z = 0; z < 2; ++z) {
             acc[z] = f32x4 { 0.f, 0.f, 0.f, 0.f };
 #pragma unroll
             for (int u = 0; u < 2 * NK; ++u) {
-                u32x4 w;
-                uint32_t lo, hi;
-                bf16_of_codes<KIND>(x.k[z][u >> 1][2 * (u & 1)], lo, hi);
-                w[0] = lo;
-                w[1] = hi;
-                bf16_of_codes<KIND>(x.k[z][u >> 1][2 * (u & 1) + 1], lo, hi);
-                w[2] = lo;
-                w[3] = hi;
-#pragma unroll
-                for (int n = 2; n >= 0; --n) // small ones first
-                    acc[z] = mfma(__builtin_bit_cast(bf16x8, w), q[u][n], acc[z]);
+                const f16x8 k = operand(x.k[z][u >> 1][2 * (u & 1)], x.k[z][u >> 1][2 * (u & 1) + 1]);
+                acc[z] = mfma(k, ql[u], acc[z]);
+                acc[z] = mfma(k, qh[u], acc[z]);
             }
         }
         float sc[8], vs[8]; // keys 4 g + i, then 16 + 4 g + i
-        sc[0] = acc[0][0] * dpp_move<0x150>(x.scale); // row_newbcast: lane n of a row of sixteen, for all of them
-        sc[1] = acc[0][1] * dpp_move<0x151>(x.scale);
-        sc[2] = acc[0][2] * dpp_move<0x152>(x.scale);
-        sc[3] = acc[0][3] * dpp_move<0x153>(x.scale);
-        sc[4] = acc[1][0] * dpp_move<0x154>(x.scale);
-        sc[5] = acc[1][1] * dpp_move<0x155>(x.scale);
-        sc[6] = acc[1][2] * dpp_move<0x156>(x.scale);
-        sc[7] = acc[1][3] * dpp_move<0x157>(x.scale);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            sc[i] = acc[i >> 2][i & 3] * to_log2;
+        sc[0] *= dpp_move<0x150>(x.scale); // row_newbcast: lane n of a row of sixteen, for all of them
+        sc[1] *= dpp_move<0x151>(x.scale);
+        sc[2] *= dpp_move<0x152>(x.scale);
+        sc[3] *= dpp_move<0x153>(x.scale);
+        sc[4] *= dpp_move<0x154>(x.scale);
+        sc[5] *= dpp_move<0x155>(x.scale);
+        sc[6] *= dpp_move<0x156>(x.scale);
+        sc[7] *= dpp_move<0x157>(x.scale);
         vs[0] = dpp_move<0x158>(x.scale);
         vs[1] = dpp_move<0x159>(x.scale);
         vs[2] = dpp_move<0x15A>(x.scale);
@@ -208,7 +223,8 @@ __device__ __forceinline__ void few8_body(const RaggedParams& p, const Scales8& 
         vs[7] = dpp_move<0x15F>(x.scale);
         const int at = k_first + blk * 32;
         const bool absent = __any(x.row < 0);
-        if (at + 32 > all_see || absent) {
+        if (__builtin_expect(at + 32 > all_see || absent, 0)) {
+            asm volatile(""); // a branch: what is in it costs a fifth of a turn
             missing = missing || absent;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -226,36 +242,37 @@ __device__ __forceinline__ void few8_body(const RaggedParams& p, const Scales8& 
             seen = true;
         }
         float mx = fmaxf(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])), fmaxf(fmaxf(sc[4], sc[5]), fmaxf(sc[6], sc[7])));
+        float corr = 1.f;
         if (__any(mx > m_run + 8.f)) { // the maximum moves when a score passes it by 2^8
-            mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-            const float m_new = fmaxf(m_run, mx);
-            const float corr = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
+            const float m_new = fmaxf(m_run, most_of_row(mx));
+            corr = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
             m_run = m_new;
             l_run *= corr;
-#pragma unroll
-            for (int e = 0; e < DL; ++e)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    oacc[e][i] *= corr;
+            w_most *= corr;
         }
         const float base = m_run == -INFINITY ? 0.f : m_run;
-        float sum = 0.f;
+        float sum = 0.f, most = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             sc[i] = __builtin_amdgcn_exp2f(sc[i] - base);
             sum += sc[i];
             sc[i] *= vs[i];
+            most = fmaxf(most, sc[i]);
         }
         l_run += sum;
-        uint32_t w[3][4];
+        if (__any(most > w_most * 16.f || corr != 1.f)) {
+            w_most = fmaxf(w_most, most_of_row(most));
+            const Pow2 now = pow2_for<1>(exponent(w_most) + 5); // at most 2^10
+            const float by = corr * (now.up * power.down);
+            power = now;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            split3(sc[2 * i], sc[2 * i + 1], w[0][i], w[1][i], w[2][i]);
-        bf16x8 pr[3];
+            for (int e = 0; e < DL; ++e)
 #pragma unroll
-        for (int z = 0; z < 3; ++z)
-            pr[z] = __builtin_bit_cast(bf16x8, (u32x4 { w[z][0], w[z][1], w[z][2], w[z][3] }));
+                for (int i = 0; i < 4; ++i)
+                    oacc[e][i] *= by;
+        }
+        f16x8 ph, pl;
+        split2x8(sc, power.up, ph, pl);
 #pragma unroll
         for (int e = 0; e < DL; e += 4) {
             uint32_t t[2][4];
@@ -266,17 +283,9 @@ __device__ __forceinline__ void few8_body(const RaggedParams& p, const Scales8& 
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                u32x4 v;
-                uint32_t lo, hi;
-                bf16_of_codes<KIND>(t[0][i], lo, hi);
-                v[0] = lo;
-                v[1] = hi;
-                bf16_of_codes<KIND>(t[1][i], lo, hi);
-                v[2] = lo;
-                v[3] = hi;
-#pragma unroll
-                for (int z = 2; z >= 0; --z)
-                    oacc[e + i] = mfma(__builtin_bit_cast(bf16x8, v), pr[z], oacc[e + i]);
+                const f16x8 v = operand(t[0][i], t[1][i]);
+                oacc[e + i] = mfma(v, pl, oacc[e + i]);
+                oacc[e + i] = mfma(v, ph, oacc[e + i]);
             }
         }
     };
@@ -312,7 +321,7 @@ __device__ __forceinline__ void few8_body(const RaggedParams& p, const Scales8& 
         for (int e = 0; e < DL; ++e)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                of[c * (D + 4) + DL * (4 * g + i) + e] = oacc[e][i];
+                of[c * (D + 4) + DL * (4 * g + i) + e] = oacc[e][i] * power.down;
     };
     if (wave == 0) // no pointer is chosen by a number: that would be a table in scratch memory
         leave(meet.of_0);
@@ -804,10 +813,11 @@ __global__ __launch_bounds__(256, 2) void paged8_tile_kernel(RaggedParams p, Sca
 template <int D, int KIND>
 static void paged8_launch(const RaggedParams& p, const RaggedPlan& plan, const Scales8& scales)
 {
-    // rows of codes are whole 16-byte vectors (values: of a lane's codes), those of q and out whole float4
+    // codes of a row and head are whole 16-byte vectors, those of q and out whole float4; rows start below 2^32 times 16 bytes
     const uintptr_t all = reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.k)
         | reinterpret_cast<uintptr_t>(p.v);
-    const bool wide = (all & 15) == 0 && ((p.ldq | p.ldo) & 3) == 0 && p.dk % 16 == 0 && p.dv % (D / 16) == 0;
+    const int64_t rows = (int64_t)p.n_pages * p.page_size.by, ld = p.ldk > p.ldv ? p.ldk : p.ldv;
+    const bool wide = (all & 15) == 0 && ((p.ldq | p.ldo) & 3) == 0 && ((p.dk | p.dv) & 15) == 0 && rows * (ld >> 4) < ((int64_t)1 << 32);
     const dim3 few((unsigned)(p.n_seqs * p.kv_heads), (unsigned)plan.few_ranges);
     if (plan.few_ranges > 0) {
         if (wide)
