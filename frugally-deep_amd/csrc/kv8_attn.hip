@@ -1,5 +1,6 @@
 // Attention over paged caches in 8 bits, query heads in groups that share a key / value head.
 #include <cfloat>
+#include <climits>
 
 #include "bf16_split.hpp"
 #include "f16_split.hpp"
@@ -9,8 +10,11 @@ namespace fdx {
 
 // ---- few query rows: keys and values pass once, straight from memory to the matrix instructions ----
 //
-// A workgroup takes the rows that a sequence brings to one key head, over one range of its keys; its waves take 32 keys a turn.  Up to sixteen
-// rows: every fourth turn is a wave's; up to thirty-two: two waves for either half of the rows take every second one.
+// A key head's blocks of 32 keys, those of all sequences one behind the other, are dealt to its workgroups in equal shares, from the lengths that
+// are there: none waits for a longer one, there are as many as the GPU takes at once, and those of all heads walk through the same rows of the
+// cache side by side.  Where a share ends inside a sequence, its rows' sums are kept for paged8_join_kernel.  A workgroup takes the rows that a
+// sequence brings to its key head over the blocks that are its, 32 keys a turn of a wave.  Up to sixteen rows: every fourth block is a wave's;
+// up to thirty-two: two waves for either half of the rows take every second one.
 //  * S^T = K Q^T: lane (c, g) of 16 x 4 loads 16 codes of keys c and 16 + c at depths 64 i + 16 g, and has the scores of keys 4 g .. 4 g + 3 and
 //    16 + 4 g .. of row c.
 //  * O^T = V^T P^T over the turn's 32 keys: lane (c, g) loads D / 16 codes of those eight keys at depth D / 16 c, so the probabilities it has are
@@ -57,39 +61,89 @@ __device__ __forceinline__ void load_codes(const uint8_t* row, int d, int depth,
     }
 }
 
-// LDS where the waves' sums meet: a wave's 16 (D + 4) floats each, and 2 * 4 * 16 of m and l
+// LDS where the waves' sums meet: a wave's 16 (D + 4) floats each, and 2 * 4 * 16 of m and l; and of 64 sequences their ends among the blocks, first
+// rows, new tokens, keys, positions of their first new tokens
 struct Meet8 {
     float *of_0, *of_1, *of_2, *of_3, *ml;
+    int (*seqs)[64];
 };
 
+// the shares of sequences with few rows
+struct Few8 {
+    float* parts;    // [share][key head][2][row][dv] of o / l, then as much of [m, l]: of its first sequence (0) if that began before, of its last (1)
+    int shares;      // of a key head
+    int rows;        // of a sequence and key head at most
+    int unit;        // blocks that shares are counted in: one, or so many that there are fewer than 2^31
+    int kv_heads;
+
+    __device__ __forceinline__ int64_t row_of(int share, int head, int slot, int row) const
+    {
+        return ((int64_t)(share * kv_heads + head) * 2 + slot) * rows + row;
+    }
+    __device__ __forceinline__ float* out(int64_t row, int dv) const { return parts + row * dv; }
+    __device__ __forceinline__ float* size(int64_t row, int dv) const { return parts + (int64_t)shares * kv_heads * 2 * rows * dv + row * 2; }
+};
+constexpr int kLeastShare = 8; // blocks: two turns of each wave
+
+// one of the sequences with few rows: its new rows, its keys, its units of blocks.  One that sees no key has a unit all the same: its rows get zeros.
+struct FewSequence {
+    int first, count, keys, ahead, units;
+};
+__device__ __forceinline__ FewSequence few_sequence(const RaggedParams& p, const Few8& few, int i, bool& cut)
+{
+    cut = false;
+    if (i >= p.n_seqs)
+        return { 0, 0, 0, 0, 0 };
+    const Sequence s = sequence_of<kPagedF32>(p, i, packed_span(p.starts, i, p.tokens));
+    cut = s.cut;
+    if (s.span.count == 0 || !s.few)
+        return { 0, 0, 0, 0, 0 };
+    const int blocks = (s.keys + 31) / 32;
+    return { s.span.first, s.span.count, s.keys, s.ahead, blocks > 0 ? (blocks - 1) / few.unit + 1 : 1 };
+}
+// sum over the lanes up to this one
+__device__ __forceinline__ int up_to_me(int v)
+{
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true); // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, true); // the last lane of a row to the row behind it
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, true); // lane 31 to lanes 32 ..
+    return v;
+}
+// units of the sequences in front of `before`
+__device__ __forceinline__ int units_before(const RaggedParams& p, const Few8& few, int before)
+{
+    const int lane = threadIdx.x & 63;
+    int sum = 0;
+    bool cut;
+    for (int i = lane; i < before; i += 64)
+        sum += few_sequence(p, few, i, cut).units;
+    return __builtin_amdgcn_readlane(up_to_me(sum), 63);
+}
+__device__ __forceinline__ int share_of(const Few8& few, int all)
+{
+    const int share = (all + few.shares - 1) / few.shares, least = (kLeastShare + few.unit - 1) / few.unit;
+    return share < least ? least : share;
+}
+
 template <int D, int KIND, bool WIDE>
-__device__ __forceinline__ void few8_body(const RaggedParams& p, const Scales8& scales, const Place& place, const Meet8& meet)
+__device__ __forceinline__ void few8_segment(const RaggedParams& p, const Scales8& scales, const Few8& few, const Meet8& meet, const Sequence& s,
+    int kv_head, int first_block, int last_block, int share, int part)
 {
     typedef Block8<D, WIDE> Block;
     constexpr int NK = Block::NK, DL = Block::DL;
     float (*meet_m)[16] = reinterpret_cast<float (*)[16]>(meet.ml), (*meet_l)[16] = meet_m + 4;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid)); // what follows from it is found out for each segment, no register keeps it
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 15, g = lane >> 4;
-    const int seq = place.x / p.kv_heads, kv_head = place.x % p.kv_heads;
-    if (p.error_flag && place.x == 0 && place.y == 0)
-        for (int i = tid; i < p.n_seqs; i += 256)
-            raise_flag(p, !packed_start_ok(p.starts, i, p.tokens));
-    const Sequence s = sequence_of<kPagedF32>(p, seq, packed_span(p.starts, seq, p.tokens));
-    if (tid == 0)
-        raise_flag(p, s.cut);
     const int count = s.span.count * p.group;
-    if (count == 0 || !s.few)
-        return;
     const bool halves = count > 16;
     const int step = halves ? 2 : 4, slot = halves ? wave & 1 : wave, r_first = halves ? (wave >> 1) * 16 : 0; // of this wave
-    int k_end = visible_keys(p, s, s.span.count - 1);
-    const int64_t k_from = (int64_t)place.y * s.range;
-    if (place.y > 0 && k_from >= k_end)
-        return;
-    const int k_first = (int)k_from;
-    if (k_end - k_first > s.range)
-        k_end = k_first + s.range;
-    const int blocks = k_end > k_first ? (k_end - k_first + 31) / 32 : 0;
+    const int k_first = first_block * 32, k_end = last_block * 32 < s.keys ? last_block * 32 : s.keys;
+    const int blocks = (k_end - k_first + 31) / 32;
 
     const uint8_t* kbase = static_cast<const uint8_t*>(p.k) + (int64_t)kv_head * p.dk;
     const uint8_t* vbase = static_cast<const uint8_t*>(p.v) + (int64_t)kv_head * p.dv;
@@ -362,15 +416,11 @@ __device__ __forceinline__ void few8_body(const RaggedParams& p, const Scales8& 
         if (r >= count)
             continue;
         const int token = quotient(r, p.by_group), head = kv_head * p.group + r - token * p.group;
-        const int sees = visible_keys(p, s, token);
-        const bool in_parts = sees > s.range;
-        if (in_parts ? k_first >= sees : place.y > 0)
-            continue;
         float* to = p.out + (int64_t)(s.span.first + token) * p.ldo + (int64_t)head * p.dv;
-        if (in_parts) {
-            const int64_t id = part_row(p, s, token, head);
-            to = p.few.out(place.y, id, p.dv);
-            float* size_at = p.few.size(place.y, id, p.dv);
+        if (part >= 0) {
+            const int64_t id = few.row_of(share, kv_head, part, r);
+            to = few.out(id, p.dv);
+            float* size_at = few.size(id, p.dv);
             if ((tid & 15) == 0) {
                 size_at[0] = top;
                 size_at[1] = l;
@@ -378,7 +428,7 @@ __device__ __forceinline__ void few8_body(const RaggedParams& p, const Scales8& 
         }
 #pragma unroll
         for (int e = 0; e < DL; ++e)
-            o[e] = finish(o[e], l, top != -INFINITY && !in_parts);
+            o[e] = finish(o[e], l, top != -INFINITY && part < 0);
 #pragma unroll
         for (int e = 0; e < DL; e += 4) {
             if (WIDE) {
@@ -395,10 +445,88 @@ __device__ __forceinline__ void few8_body(const RaggedParams& p, const Scales8& 
 }
 
 template <int D, int KIND, bool WIDE>
-__global__ __launch_bounds__(256, WIDE ? 2 : 1) void paged8_few_kernel(RaggedParams p, Scales8 scales)
+__device__ __forceinline__ void few8_body(const RaggedParams& p, const Scales8& scales, const Few8& few, int wg, const Meet8& meet)
+{
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int kv_head = wg % p.kv_heads, mine = wg / p.kv_heads;
+    if (p.error_flag && wg == 0)
+        for (int i = tid; i < p.n_seqs; i += 256)
+            raise_flag(p, !packed_start_ok(p.starts, i, p.tokens));
+    int at = 0, end = 0, front = 0; // units; those in front of sequences i0 ..
+    for (int i0 = 0; i0 < p.n_seqs; i0 += 64) {
+        bool cut;
+        const FewSequence of_lane = few_sequence(p, few, i0 + lane, cut);
+        const int up_to = front + up_to_me(of_lane.units), before = front;
+        front = __builtin_amdgcn_readlane(up_to, 63);
+        if (wg == 0)
+            raise_flag(p, cut);
+        if (i0 == 0) {
+            const int all = p.n_seqs <= 64 ? front : units_before(p, few, p.n_seqs), share = share_of(few, all);
+            if ((int64_t)mine * share >= all)
+                return;
+            at = mine * share;
+            end = all - at < share ? all : at + share;
+        }
+        if (at >= front)
+            continue;
+        if (tid < 64) { // no register keeps it through the segments
+            meet.seqs[0][lane] = up_to;
+            meet.seqs[1][lane] = of_lane.first;
+            meet.seqs[2][lane] = of_lane.count;
+            meet.seqs[3][lane] = of_lane.keys;
+            meet.seqs[4][lane] = of_lane.ahead;
+        }
+        __syncthreads();
+        while (at < end && at < front) {
+            int me = lane;
+            asm volatile("" : "+v"(me));
+            const int of = __builtin_popcountll(__ballot(meet.seqs[0][me] <= at));
+            auto number = [&](int which, int i) { return __builtin_amdgcn_readfirstlane(meet.seqs[which][i]); };
+            const int first = of > 0 ? number(0, of - 1) : before, last = number(0, of);
+            const Sequence s { { number(1, of), number(2, of) }, number(3, of), number(4, of), i0 + of, true, INT_MAX, false };
+            const int stop = end < last ? end : last;
+            few8_segment<D, KIND, WIDE>(p, scales, few, meet, s, kv_head, (at - first) * few.unit, (stop - first) * few.unit, mine,
+                at == first && stop == last ? -1 : (at > first ? 0 : 1));
+            at = stop;
+            __syncthreads(); // the waves' sums have been read
+        }
+        if (at >= end)
+            return;
+        __syncthreads();
+    }
+}
+
+template <int D, int KIND, bool WIDE>
+__global__ __launch_bounds__(256, WIDE ? 2 : 1) void paged8_few_kernel(RaggedParams p, Scales8 scales, Few8 few)
 {
     __shared__ float meet[4][16 * (D + 4)], ml[2 * 4 * 16];
-    few8_body<D, KIND, WIDE>(p, scales, Place { blockIdx.x, blockIdx.y, gridDim.x }, Meet8 { meet[0], meet[1], meet[2], meet[3], ml });
+    __shared__ int seqs[5][64];
+    few8_body<D, KIND, WIDE>(p, scales, few, blockIdx.x, Meet8 { meet[0], meet[1], meet[2], meet[3], ml, seqs });
+}
+
+// Rows whose keys more than one share has: sum of 2^(m - M) l o over the shares, divided by that of 2^(m - M) l.
+__global__ __launch_bounds__(256) void paged8_join_kernel(RaggedParams p, Few8 few)
+{
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t item = (int64_t)blockIdx.x * 4 + wave;
+    const int row = (int)((uint64_t)item / (uint32_t)p.heads), head = (int)(item - (int64_t)row * p.heads);
+    if (row >= p.tokens)
+        return;
+    const int index = find_row(SearchWave(), p.starts, p.n_seqs, p.tokens, row);
+    if (index < 0)
+        return;
+    bool cut;
+    const FewSequence s = few_sequence(p, few, index, cut);
+    const int token = row - s.first;
+    if (token >= s.count)
+        return;
+    const int kv_head = quotient(head, p.by_group), r = token * p.group + head - kv_head * p.group;
+    const int share = share_of(few, units_before(p, few, p.n_seqs)), first = units_before(p, few, index);
+    const int from = first / share, parts = (first + s.units - 1) / share - from + 1;
+    if (parts == 1)
+        return;
+    auto id = [&](int i) { return few.row_of(from + i, kv_head, i > 0 ? 0 : 1, r); };
+    join_parts(p, row, head, parts, [&](int i) { return few.out(id(i), p.dv); }, [&](int i) { return few.size(id(i), p.dv); });
 }
 
 // ---- many query rows: tiles on the fp16 matrix instructions ----
@@ -810,29 +938,57 @@ __global__ __launch_bounds__(256, 2) void paged8_tile_kernel(RaggedParams p, Sca
     tile8_body<D, KIND, WIDE>(p, scales, Place { blockIdx.x, blockIdx.y, gridDim.x }, lds);
 }
 
+// How a call is cut: paged_plan's tiles; sequences with few rows in as many shares as workgroups fit on the GPU, or as the longest lengths make.
+struct Plan8 {
+    RaggedPlan tiles;
+    Few8 few;
+    unsigned few_wgs;
+    size_t few_floats;
+};
+static Plan8 plan8(int tokens, int max_new, int heads, const fdx_kv_pages* c)
+{
+    Plan8 r {};
+    r.tiles = paged_plan(tokens, max_new, heads, c);
+    if (r.tiles.few_ranges > 0) {
+        const int64_t most = (int64_t)c->n_seqs * (((int64_t)c->max_len + 31) / 32), shares = (most + kLeastShare - 1) / kLeastShare;
+        const int fit = (c->dk <= 64 && c->dv <= 64 ? 768 : 512) / c->kv_heads;
+        r.few.shares = fit < 1 ? 1 : (shares < fit ? (int)shares : fit);
+        r.few.rows = (int)(r.tiles.few_part / ((int64_t)c->n_seqs * c->kv_heads));
+        r.few.unit = 1;
+        while (most / r.few.unit + c->n_seqs >= ((int64_t)1 << 30))
+            r.few.unit *= 2;
+        r.few.kv_heads = c->kv_heads;
+        r.few_wgs = (unsigned)(r.few.shares * c->kv_heads);
+        if (r.few.shares > 1)
+            r.few_floats = ((size_t)r.few_wgs * 2 * r.few.rows * (2 + (size_t)c->dv) + 3) & ~(size_t)3;
+    }
+    return r;
+}
+
 template <int D, int KIND>
-static void paged8_launch(const RaggedParams& p, const RaggedPlan& plan, const Scales8& scales)
+static void paged8_launch(const RaggedParams& p, const Plan8& plan, const Scales8& scales)
 {
     // codes of a row and head are whole 16-byte vectors, those of q and out whole float4; rows start below 2^32 times 16 bytes
     const uintptr_t all = reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.k)
         | reinterpret_cast<uintptr_t>(p.v);
     const int64_t rows = (int64_t)p.n_pages * p.page_size.by, ld = p.ldk > p.ldv ? p.ldk : p.ldv;
     const bool wide = (all & 15) == 0 && ((p.ldq | p.ldo) & 3) == 0 && ((p.dk | p.dv) & 15) == 0 && rows * (ld >> 4) < ((int64_t)1 << 32);
-    const dim3 few((unsigned)(p.n_seqs * p.kv_heads), (unsigned)plan.few_ranges);
-    if (plan.few_ranges > 0) {
+    if (plan.few_wgs > 0) {
         if (wide)
-            hipLaunchKernelGGL((paged8_few_kernel<D, KIND, true>), few, dim3(256), 0, stream(), p, scales);
+            hipLaunchKernelGGL((paged8_few_kernel<D, KIND, true>), dim3(plan.few_wgs), dim3(256), 0, stream(), p, scales, plan.few);
         else
-            hipLaunchKernelGGL((paged8_few_kernel<D, KIND, false>), few, dim3(256), 0, stream(), p, scales);
+            hipLaunchKernelGGL((paged8_few_kernel<D, KIND, false>), dim3(plan.few_wgs), dim3(256), 0, stream(), p, scales, plan.few);
     }
-    if (plan.tiles > 0) {
-        const dim3 grid((unsigned)plan.tiles, (unsigned)plan.tile_ranges);
+    if (plan.tiles.tiles > 0) {
+        const dim3 grid((unsigned)plan.tiles.tiles, (unsigned)plan.tiles.tile_ranges);
         if (wide)
             hipLaunchKernelGGL((paged8_tile_kernel<D, KIND, true>), grid, dim3(256), 0, stream(), p, scales);
         else
             hipLaunchKernelGGL((paged8_tile_kernel<D, KIND, false>), grid, dim3(256), 0, stream(), p, scales);
     }
-    if (plan.few_ranges > 1 || plan.tile_ranges > 1)
+    if (plan.few.shares > 1)
+        hipLaunchKernelGGL(paged8_join_kernel, dim3((unsigned)(((int64_t)p.tokens * p.heads + 3) / 4)), dim3(256), 0, stream(), p, plan.few);
+    if (plan.tiles.tile_ranges > 1)
         ragged_join_launch(p);
 }
 
@@ -842,7 +998,12 @@ using namespace fdx;
 
 extern "C" size_t fdx_mha_paged8_scratch_bytes(int tokens, int max_new, int heads, const fdx_kv_pages8* cache)
 {
-    return cache ? fdx_mha_paged_scratch_bytes(tokens, max_new, heads, &cache->pages) : 0;
+    const fdx_kv_pages* c = cache ? &cache->pages : nullptr;
+    if (!c || tokens <= 0 || max_new <= 0 || heads <= 0 || c->kv_heads <= 0 || heads % c->kv_heads != 0 || c->dk <= 0 || c->dv <= 0 || c->n_seqs <= 0
+        || c->max_len <= 0)
+        return 0;
+    const Plan8 plan = plan8(tokens, max_new, heads, c);
+    return sizeof(float) * (plan.few_floats + plan.tiles.tile_floats(c->dv));
 }
 
 extern "C" fdx_status fdx_mha_paged8_f32(const float* q, int64_t ldq, const int32_t* starts, int tokens, int max_new, int heads,
@@ -851,15 +1012,21 @@ extern "C" fdx_status fdx_mha_paged8_f32(const float* q, int64_t ldq, const int3
     fdx_status st = check_kv_pages8("mha_paged8", cache);
     if (st != FDX_OK)
         return st;
+    const fdx_kv_pages& c = cache->pages;
     RaggedParams p {};
-    RaggedPlan plan;
-    st = paged_params("mha_paged8", q, ldq, starts, tokens, max_new, heads, &cache->pages, out, ldo, scratch_dev, error_flag_dev, p, plan);
+    st = paged_params("mha_paged8", q, ldq, starts, tokens, max_new, heads, &c, out, ldo, scratch_dev,
+        fdx_mha_paged8_scratch_bytes(tokens, max_new, heads, cache), error_flag_dev, p);
     if (st != FDX_OK)
         return st;
+    Plan8 plan = plan8(tokens, max_new, heads, &c);
+    plan.few.parts = static_cast<float*>(scratch_dev);
+    p.few_rows = plan.tiles.few_rows;
+    p.few = { nullptr, 0, 1, INT_MAX, 0, 0 }; // no ranges: sequences with few rows are cut in shares, and ragged_join_kernel leaves them alone
+    p.tile = { plan.few.parts + plan.few_floats, plan.tiles.tile_part, plan.tiles.tile_ranges, plan.tiles.tile_keys, plan.tiles.tile_whole, 0 };
     const Scales8 scales { cache->k_scale, cache->v_scale, make_divisor(cache->block) };
     const bool small = p.dk <= 64 && p.dv <= 64;
     profile_begin();
-    if (cache->pages.type == FDX_KV_I8)
+    if (c.type == FDX_KV_I8)
         small ? paged8_launch<64, kI8>(p, plan, scales) : paged8_launch<128, kI8>(p, plan, scales);
     else
         small ? paged8_launch<64, kE4M3>(p, plan, scales) : paged8_launch<128, kE4M3>(p, plan, scales);

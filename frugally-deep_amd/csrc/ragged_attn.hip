@@ -1186,11 +1186,11 @@ __global__ __launch_bounds__(256, 2) void ragged_mixed_kernel(RaggedParams p, un
     }
 }
 
-// Rows that more than one range of keys was summed for: sum of 2^(m - M) l o over the ranges, divided by that of 2^(m - M) l.
+// Rows that more than one range of keys was summed for.
 template <int KIND>
 __global__ __launch_bounds__(256) void ragged_join_kernel(RaggedParams p)
 {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t item = (int64_t)blockIdx.x * 4 + wave;
     const int row = (int)((uint64_t)item / (uint32_t)p.heads), head = (int)(item - (int64_t)row * p.heads);
     if (row >= p.tokens)
@@ -1208,43 +1208,7 @@ __global__ __launch_bounds__(256) void ragged_join_kernel(RaggedParams p)
     const int parts = (visible + s.range - 1) / s.range;
     const PartSums& part = s.few ? p.few : p.tile;
     const int64_t id = part_row(p, s, token, head);
-    // a lane a range for the sizes, then all lanes a range at a time for the rows, four of them on their way together
-    float top = -INFINITY;
-    for (int i0 = 0; i0 < parts; i0 += 64)
-        if (i0 + lane < parts)
-            top = fmaxf(top, part.size(i0 + lane, id, p.dv)[0]);
-    top = wave_all<true>(top);
-    const float m = top == -INFINITY ? 0.f : top;
-    float l = 0.f, o0 = 0.f, o1 = 0.f;
-    for (int i0 = 0; i0 < parts; i0 += 64) {
-        float w = 0.f;
-        if (i0 + lane < parts) {
-            const float* at = part.size(i0 + lane, id, p.dv);
-            w = at[1] * __builtin_amdgcn_exp2f(at[0] - m);
-        }
-        l += wave_all<false>(w);
-        const int count = parts - i0 < 64 ? parts - i0 : 64;
-        for (int i = 0; i < count; i += 4) {
-            float x0[4], x1[4];
-#pragma unroll
-            for (int z = 0; z < 4; ++z) {
-                const float* from = part.out(i0 + (i + z < count ? i + z : i), id, p.dv);
-                x0[z] = from[lane < p.dv ? lane : 0];
-                x1[z] = from[64 + lane < p.dv ? 64 + lane : 0];
-            }
-#pragma unroll
-            for (int z = 0; z < 4; ++z) {
-                const float wi = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), i + z < count ? i + z : i));
-                o0 = fmaf(i + z < count ? wi : 0.f, x0[z], o0);
-                o1 = fmaf(i + z < count ? wi : 0.f, x1[z], o1);
-            }
-        }
-    }
-    float* to = p.out + (int64_t)row * p.ldo + (int64_t)head * p.dv;
-    if (lane < p.dv)
-        to[lane] = finish(o0, l, top != -INFINITY);
-    if (64 + lane < p.dv)
-        to[64 + lane] = finish(o1, l, top != -INFINITY);
+    join_parts(p, row, head, parts, [&](int i) { return part.out(i, id, p.dv); }, [&](int i) { return part.size(i, id, p.dv); });
 }
 
 void ragged_join_launch(const RaggedParams& p)
@@ -1425,7 +1389,7 @@ static fdx_status check_ragged(const char* who, const RaggedParams& p, const voi
 
 // checks the arguments of a call on a paged cache and makes a launch's parameters of them
 fdx_status paged_params(const char* who, const float* q, int64_t ldq, const int32_t* starts, int tokens, int max_new, int heads,
-    const fdx_kv_pages* cache, float* out, int64_t ldo, void* scratch_dev, int* error_flag_dev, RaggedParams& p, RaggedPlan& plan)
+    const fdx_kv_pages* cache, float* out, int64_t ldo, const void* scratch_dev, size_t scratch_bytes, int* error_flag_dev, RaggedParams& p)
 {
     FDX_REQUIRE(max_new > 0, "%s: bad shape", who);
     p.q = q; p.ldq = ldq; p.out = out; p.ldo = ldo;
@@ -1436,16 +1400,11 @@ fdx_status paged_params(const char* who, const float* q, int64_t ldq, const int3
     p.table = cache->table; p.lens = cache->lens; p.table_width = cache->table_width; p.n_pages = cache->n_pages;
     p.page_size = make_divisor(cache->page_size); p.max_len = cache->max_len; p.max_new = max_new < tokens ? max_new : tokens;
     p.error_flag = error_flag_dev;
-    const fdx_status st = check_ragged(who, p, scratch_dev, fdx_mha_paged_scratch_bytes(tokens, max_new, heads, cache));
+    const fdx_status st = check_ragged(who, p, scratch_dev, scratch_bytes);
     if (st != FDX_OK)
         return st;
     p.scale = (float)(1.0 / std::sqrt((double)p.dk));
-    plan = paged_plan(tokens, max_new, heads, cache);
-    float* part = static_cast<float*>(scratch_dev);
     p.by_group = make_divisor(p.group);
-    p.few_rows = plan.few_rows;
-    p.few = { part, plan.few_part, plan.few_ranges, plan.few_keys, 0, (int)(plan.few_part / ((int64_t)p.n_seqs * p.kv_heads)) };
-    p.tile = { part + plan.few_floats(p.dv), plan.tile_part, plan.tile_ranges, plan.tile_keys, plan.tile_whole, 0 };
     return FDX_OK;
 }
 
@@ -1508,10 +1467,15 @@ extern "C" fdx_status fdx_mha_paged_f32(const float* q, int64_t ldq, const int32
     if (st != FDX_OK)
         return st;
     RaggedParams p {};
-    RaggedPlan plan;
-    st = paged_params("mha_paged", q, ldq, starts, tokens, max_new, heads, cache, out, ldo, scratch_dev, error_flag_dev, p, plan);
+    st = paged_params("mha_paged", q, ldq, starts, tokens, max_new, heads, cache, out, ldo, scratch_dev,
+        fdx_mha_paged_scratch_bytes(tokens, max_new, heads, cache), error_flag_dev, p);
     if (st != FDX_OK)
         return st;
+    const RaggedPlan plan = paged_plan(tokens, max_new, heads, cache);
+    float* part = static_cast<float*>(scratch_dev);
+    p.few_rows = plan.few_rows;
+    p.few = { part, plan.few_part, plan.few_ranges, plan.few_keys, 0, (int)(plan.few_part / ((int64_t)p.n_seqs * p.kv_heads)) };
+    p.tile = { part + plan.few_floats(p.dv), plan.tile_part, plan.tile_ranges, plan.tile_keys, plan.tile_whole, 0 };
     profile_begin();
     if (cache->type == FDX_KV_F32)
         ragged_dispatch<kPagedF32>(p, plan);

@@ -348,6 +348,31 @@ def test_paged_pages_that_are_none(fdx, new):
     assert (out.to_host((sum(new) + 50, heads * d))[sum(new):] == 0).all()
 
 
+@pytest.mark.parametrize("heads", [4, 40])
+def test_lengths_of_sequences_without_new_tokens(fdx, heads):
+    """A length out of range is reported though nobody reads it."""
+    f = Filled(fdx, [20, 30, 9], 2, 64, 64, 16, "i8", 8)
+    q = np.random.default_rng(1).standard_normal((2, heads * 64)).astype(np.float32)
+    dq, out = fdx.DevBuf.from_host(q), fdx.DevBuf.from_host(np.zeros((2, heads * 64), np.float32))
+    for lens, flag in (([20, 30, 9], 0), ([20, -1, 9], 1), ([20, 31, 9], 1), ([20, 2**31 - 1, 9], 1)):
+        assert call_paged(fdx, f.cache, dq.ptr, heads * 64, [0, 1, 1, 2], 2, 1, heads, out.ptr, heads * 64, lens=lens) == flag
+        f.cache.lens = np.array([20, 30, 9], np.int32)
+        close(out.to_host((2, heads * 64)), f.reference(q, [1, 0, 1], heads))
+
+
+@pytest.mark.parametrize("n_seqs", [65, 200])
+@pytest.mark.parametrize("heads,kv", [(4, 2), (6, 6)])
+def test_shares_over_many_sequences(fdx, n_seqs, heads, kv):
+    """Long sequences beside short ones and ones without tokens, more than a wave has lanes: every key counts once, whoever has it."""
+    r = np.random.default_rng(n_seqs)
+    context = np.where(r.random(n_seqs) < 0.05, r.integers(500, 2500, n_seqs), r.integers(0, 30, n_seqs))
+    f = Filled(fdx, context.tolist(), kv, 32, 32, 16, "i8", 8)
+    new = np.where(context > 0, r.integers(0, 3, n_seqs), 0)
+    new = np.minimum(new, context)
+    q = r.standard_normal((int(new.sum()), heads * 32)).astype(np.float32)
+    close(fdx.mha_paged(f.cache, q, new, heads), f.reference(q, new, heads))
+
+
 def test_paged_more_new_tokens_than_said(fdx):
     f, heads = Filled(fdx, [90, 131], 2, 64, 64, 16, "i8"), 4
     q = np.random.default_rng(4).standard_normal((45, heads * 64)).astype(np.float32)
