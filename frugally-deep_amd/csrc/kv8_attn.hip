@@ -66,6 +66,7 @@ __device__ __forceinline__ void load_codes(const uint8_t* row, int d, int depth,
 struct Meet8 {
     float *of_0, *of_1, *of_2, *of_3, *ml;
     int (*seqs)[64];
+    unsigned char* q; // queries of either half of the rows, as the products read them: [half][step][plane][lane][16 bytes]
 };
 
 // the shares of sequences with few rows
@@ -155,24 +156,26 @@ __device__ __forceinline__ void few8_segment(const RaggedParams& p, const Scales
     };
     // where rows start is 32 bits in units of 16 bytes (see `wide` of paged8_launch), which saves the products of 64 bits
     const uint32_t k_units = (uint32_t)(p.ldk >> 4), v_units = (uint32_t)(p.ldv >> 4);
+    const int lane_c = 4 * c, lane_g = 16 * g, lane_scale = 4 * scale_key; // bytes, as the lane that a number comes from is told
+    auto of_lane = [](int v, int lane, int more) { return __builtin_amdgcn_ds_bpermute(lane + 4 * more, v); };
     auto fetch = [&](Block& b, int row) {
         b.row = row;
         row = row < 0 ? 0 : row;
         const uint32_t k_at = (uint32_t)row * k_units, v_at = (uint32_t)row * v_units;
 #pragma unroll
         for (int z = 0; z < 2; ++z) {
-            const uint8_t* kr = WIDE ? kbase + ((uint64_t)(uint32_t)__shfl((int)k_at, 16 * z + c, 64) << 4) : kbase + (int64_t)__shfl(row, 16 * z + c, 64) * p.ldk;
+            const uint8_t* kr = WIDE ? kbase + ((uint64_t)(uint32_t)of_lane((int)k_at, lane_c, 16 * z) << 4) : kbase + (int64_t)of_lane(row, lane_c, 16 * z) * p.ldk;
 #pragma unroll
             for (int i = 0; i < NK; ++i)
                 load_codes<4, WIDE>(kr, 64 * i + 16 * g, p.dk, b.k[z][i]);
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const int key = 16 * (i >> 2) + 4 * g + (i & 3);
-            const uint8_t* vr = WIDE ? vbase + ((uint64_t)(uint32_t)__shfl((int)v_at, key, 64) << 4) : vbase + (int64_t)__shfl(row, key, 64) * p.ldv;
+            const int key = 16 * (i >> 2) + (i & 3);
+            const uint8_t* vr = WIDE ? vbase + ((uint64_t)(uint32_t)of_lane((int)v_at, lane_g, key) << 4) : vbase + (int64_t)of_lane(row, lane_g, key) * p.ldv;
             load_codes<DL / 4, WIDE>(vr, DL * c, p.dv, b.v[i]);
         }
-        b.scale = scale_base[(int64_t)quotient(__shfl(row, scale_key, 64), scales.block) * p.kv_heads];
+        b.scale = scale_base[(int64_t)quotient(of_lane(row, lane_scale, 0), scales.block) * p.kv_heads];
     };
     Block a, b;
     int row_b = 0;
@@ -183,7 +186,8 @@ __device__ __forceinline__ void few8_segment(const RaggedParams& p, const Scales
     }
 
     // the query: step (i, h) has depths 64 i + 16 g + 8 h ..
-    f16x8 qh[2 * NK], ql[2 * NK];
+    // In LDS, which leaves registers to the blocks on their way; waves that share rows write the same.
+    f16x8* q_at = reinterpret_cast<f16x8*>(meet.q) + (r_first > 0 ? 4 * NK * 64 : 0) + lane;
     float to_log2;
     const bool q_ok = r_first + c < count;
     const int q_token = quotient(q_ok ? r_first + c : 0, p.by_group);
@@ -218,7 +222,12 @@ __device__ __forceinline__ void few8_segment(const RaggedParams& p, const Scales
         to_log2 = sq.down * (p.scale * kLog2e);
 #pragma unroll
         for (int u = 0; u < 2 * NK; ++u)
-            split2x8(x[u], sq.up, qh[u], ql[u]);
+        {
+            f16x8 h, l;
+            split2x8(x[u], sq.up, h, l);
+            q_at[(2 * u) * 64] = l;
+            q_at[(2 * u + 1) * 64] = h;
+        }
     }
     float m_run = -INFINITY, l_run = 0.f;
     float w_most = 0.f; // the largest probability times scale so far, to within 2^4
@@ -244,15 +253,15 @@ __device__ __forceinline__ void few8_segment(const RaggedParams& p, const Scales
             w[3] = hi;
             return __builtin_bit_cast(f16x8, w);
         };
-        f32x4 acc[2];
+        f32x4 acc[2] = { { 0.f, 0.f, 0.f, 0.f }, { 0.f, 0.f, 0.f, 0.f } };
 #pragma unroll
-        for (int z = 0; z < 2; ++z) {
-            acc[z] = f32x4 { 0.f, 0.f, 0.f, 0.f };
+        for (int u = 0; u < 2 * NK; ++u) {
+            const f16x8 ql = q_at[(2 * u) * 64], qh = q_at[(2 * u + 1) * 64];
 #pragma unroll
-            for (int u = 0; u < 2 * NK; ++u) {
+            for (int z = 0; z < 2; ++z) {
                 const f16x8 k = operand(x.k[z][u >> 1][2 * (u & 1)], x.k[z][u >> 1][2 * (u & 1) + 1]);
-                acc[z] = mfma(k, ql[u], acc[z]);
-                acc[z] = mfma(k, qh[u], acc[z]);
+                acc[z] = mfma(k, ql, acc[z]);
+                acc[z] = mfma(k, qh, acc[z]);
             }
         }
         float sc[8], vs[8]; // keys 4 g + i, then 16 + 4 g + i
@@ -278,12 +287,13 @@ __device__ __forceinline__ void few8_segment(const RaggedParams& p, const Scales
         const int at = k_first + blk * 32;
         const bool absent = __any(x.row < 0);
         if (__builtin_expect(at + 32 > all_see || absent, 0)) {
-            asm volatile(""); // a branch: what is in it costs a fifth of a turn
             missing = missing || absent;
+            int g4 = 4 * g;
+            asm volatile("" : "+v"(g4)); // no register keeps the keys' numbers for the next time
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int key = 16 * (i >> 2) + 4 * g + (i & 3);
-                const bool there = __shfl(x.row, key, 64) >= 0;
+                const int key = 16 * (i >> 2) + g4 + (i & 3);
+                const bool there = of_lane(x.row, lane_g, 16 * (i >> 2) + (i & 3)) >= 0;
                 const bool sees = there && at + key < (visible < k_end ? visible : k_end);
                 sc[i] = sees ? sc[i] : -INFINITY;
                 vs[i] = sees ? vs[i] : 0.f; // a scale of NaN is for the rows that see it
@@ -447,13 +457,15 @@ __device__ __forceinline__ void few8_segment(const RaggedParams& p, const Scales
 template <int D, int KIND, bool WIDE>
 __device__ __forceinline__ void few8_body(const RaggedParams& p, const Scales8& scales, const Few8& few, int wg, const Meet8& meet)
 {
-    const int tid = threadIdx.x, lane = tid & 63;
     const int kv_head = wg % p.kv_heads, mine = wg / p.kv_heads;
     if (p.error_flag && wg == 0)
-        for (int i = tid; i < p.n_seqs; i += 256)
+        for (int i = threadIdx.x; i < p.n_seqs; i += 256)
             raise_flag(p, !packed_start_ok(p.starts, i, p.tokens));
     int at = 0, end = 0, front = 0; // units; those in front of sequences i0 ..
     for (int i0 = 0; i0 < p.n_seqs; i0 += 64) {
+        int tid = threadIdx.x;
+        asm volatile("" : "+v"(tid));
+        const int lane = tid & 63;
         bool cut;
         const FewSequence of_lane = few_sequence(p, few, i0 + lane, cut);
         const int up_to = front + up_to_me(of_lane.units), before = front;
@@ -478,9 +490,9 @@ __device__ __forceinline__ void few8_body(const RaggedParams& p, const Scales8& 
         }
         __syncthreads();
         while (at < end && at < front) {
-            int me = lane;
+            int me = threadIdx.x;
             asm volatile("" : "+v"(me));
-            const int of = __builtin_popcountll(__ballot(meet.seqs[0][me] <= at));
+            const int of = __builtin_popcountll(__ballot(meet.seqs[0][me & 63] <= at));
             auto number = [&](int which, int i) { return __builtin_amdgcn_readfirstlane(meet.seqs[which][i]); };
             const int first = of > 0 ? number(0, of - 1) : before, last = number(0, of);
             const Sequence s { { number(1, of), number(2, of) }, number(3, of), number(4, of), i0 + of, true, INT_MAX, false };
@@ -501,7 +513,8 @@ __global__ __launch_bounds__(256, WIDE ? 2 : 1) void paged8_few_kernel(RaggedPar
 {
     __shared__ float meet[4][16 * (D + 4)], ml[2 * 4 * 16];
     __shared__ int seqs[5][64];
-    few8_body<D, KIND, WIDE>(p, scales, few, blockIdx.x, Meet8 { meet[0], meet[1], meet[2], meet[3], ml, seqs });
+    __shared__ __attribute__((aligned(16))) unsigned char q[2 * D / 32 * 2 * 1024];
+    few8_body<D, KIND, WIDE>(p, scales, few, blockIdx.x, Meet8 { meet[0], meet[1], meet[2], meet[3], ml, seqs, q });
 }
 
 // Rows whose keys more than one share has: sum of 2^(m - M) l o over the shares, divided by that of 2^(m - M) l.

@@ -2,6 +2,7 @@
 #pragma once
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include "common.hpp"
 #include "kv_pages.hpp"
@@ -242,7 +243,7 @@ template <class Out, class Size>
 __device__ __forceinline__ void join_parts(const RaggedParams& p, int row, int head, int parts, const Out& out, const Size& size)
 {
     const int lane = threadIdx.x & 63;
-    // a lane a range for the sizes, then all lanes a range at a time for the rows, four of them on their way together
+    // a lane a range for the sizes, then all lanes a range at a time for the rows, up to sixteen of them on their way together
     float top = -INFINITY;
     for (int i0 = 0; i0 < parts; i0 += 64)
         if (i0 + lane < parts)
@@ -258,21 +259,27 @@ __device__ __forceinline__ void join_parts(const RaggedParams& p, int row, int h
         }
         l += wave_all<false>(w);
         const int count = parts - i0 < 64 ? parts - i0 : 64;
-        for (int i = 0; i < count; i += 4) {
-            float x0[4], x1[4];
+        auto add = [&](int i, auto width) { // ranges i .. i + width - 1
+            constexpr int W = decltype(width)::value;
+            float x0[W], x1[W];
 #pragma unroll
-            for (int z = 0; z < 4; ++z) {
+            for (int z = 0; z < W; ++z) {
                 const float* from = out(i0 + (i + z < count ? i + z : i));
                 x0[z] = from[lane < p.dv ? lane : 0];
                 x1[z] = from[64 + lane < p.dv ? 64 + lane : 0];
             }
 #pragma unroll
-            for (int z = 0; z < 4; ++z) {
+            for (int z = 0; z < W; ++z) {
                 const float wi = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), i + z < count ? i + z : i));
                 o0 = fmaf(i + z < count ? wi : 0.f, x0[z], o0);
                 o1 = fmaf(i + z < count ? wi : 0.f, x1[z], o1);
             }
-        }
+        };
+        int i = 0;
+        for (; count - i > 4; i += 16)
+            add(i, std::integral_constant<int, 16>());
+        if (i < count)
+            add(i, std::integral_constant<int, 4>());
     }
     float* to = p.out + (int64_t)row * p.ldo + (int64_t)head * p.dv;
     if (lane < p.dv)
