@@ -517,31 +517,6 @@ __global__ __launch_bounds__(256, WIDE ? 2 : 1) void paged8_few_kernel(RaggedPar
     few8_body<D, KIND, WIDE>(p, scales, few, blockIdx.x, Meet8 { meet[0], meet[1], meet[2], meet[3], ml, seqs, q });
 }
 
-// Rows whose keys more than one share has: sum of 2^(m - M) l o over the shares, divided by that of 2^(m - M) l.
-__global__ __launch_bounds__(256) void paged8_join_kernel(RaggedParams p, Few8 few)
-{
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t item = (int64_t)blockIdx.x * 4 + wave;
-    const int row = (int)((uint64_t)item / (uint32_t)p.heads), head = (int)(item - (int64_t)row * p.heads);
-    if (row >= p.tokens)
-        return;
-    const int index = find_row(SearchWave(), p.starts, p.n_seqs, p.tokens, row);
-    if (index < 0)
-        return;
-    bool cut;
-    const FewSequence s = few_sequence(p, few, index, cut);
-    const int token = row - s.first;
-    if (token >= s.count)
-        return;
-    const int kv_head = quotient(head, p.by_group), r = token * p.group + head - kv_head * p.group;
-    const int share = share_of(few, units_before(p, few, p.n_seqs)), first = units_before(p, few, index);
-    const int from = first / share, parts = (first + s.units - 1) / share - from + 1;
-    if (parts == 1)
-        return;
-    auto id = [&](int i) { return few.row_of(from + i, kv_head, i > 0 ? 0 : 1, r); };
-    join_parts(p, row, head, parts, [&](int i) { return few.out(id(i), p.dv); }, [&](int i) { return few.size(id(i), p.dv); });
-}
-
 // ---- many query rows: tiles on the fp16 matrix instructions ----
 //
 // A workgroup takes 128 rows of one key head of one sequence, rows counting through the query heads of the group first (row = token *
@@ -725,8 +700,8 @@ __device__ __forceinline__ void tile8_body(const RaggedParams& p, const Scales8&
                     top = fmaxf(top, fabsf(y[i]));
                 }
             }
-        const Pow2 sq = pow2_for<1>(exponent(max_halves(top)));
-        to_log2 = sq.down * (p.scale * kLog2e);
+        const Pow2 sq = pow2_for<1>(exponent(max_halves(top)) + 6); // at most 2^9: scores before to_log2 stay in fp32's range for keys up to 2^100
+        to_log2 = fmaxf(sq.down * (p.scale * kLog2e), 1.17549435e-38f); // above zero: -infinity stays what it is
 #pragma unroll
         for (int u = 0; u < STEPS; ++u)
             split2x8(x[u], sq.up, qh[u], ql[u]);
@@ -766,6 +741,25 @@ __device__ __forceinline__ void tile8_body(const RaggedParams& p, const Scales8&
         r.b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(vs + v_at + (key + 8) * VROW + d * 64));
         return __builtin_bit_cast(f16x8, r);
     };
+    // the products' operands are read from LDS two pairs of products ahead
+    auto in_order = [] {
+        constexpr int kProducts = 0x8, kReads = 0x100;
+        __builtin_amdgcn_sched_group_barrier(kReads, 2, 0);
+#pragma unroll
+        for (int i = 0; i < HALVES * STEPS; ++i) {
+            __builtin_amdgcn_sched_group_barrier(kProducts, 2, 0);
+            if (i + 2 < HALVES * STEPS)
+                __builtin_amdgcn_sched_group_barrier(kReads, 1, 0);
+            else
+                __builtin_amdgcn_sched_group_barrier(kReads, 2, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < KT / 16 * DB; ++i) {
+            __builtin_amdgcn_sched_group_barrier(kProducts, 2, 0);
+            if (i + 2 < KT / 16 * DB)
+                __builtin_amdgcn_sched_group_barrier(kReads, 2, 0);
+        }
+    };
     // tile t: its scores are in sc, its values and scales in vs and scale, the keys of tile t + 1 in ks; registers hold the codes of tile t + 2's
     // keys and of tile t + 1's values
     auto turn = [&](int t, f32x16 (&sc)[HALVES], f32x16 (&next)[HALVES], const unsigned char* ks, const unsigned char* vs, const float* scale,
@@ -795,7 +789,7 @@ __device__ __forceinline__ void tile8_body(const RaggedParams& p, const Scales8&
                     const f32x4 by = *reinterpret_cast<const f32x4*>(scale + kb * 32 + 8 * g + 4 * half);
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        sc[kb][4 * g + i] = sc[kb][4 * g + i] * to_log2 * by[i];
+                        sc[kb][4 * g + i] *= by[i];
                 }
             if (some_hidden || some_gone) {
 #pragma unroll
@@ -814,7 +808,7 @@ __device__ __forceinline__ void tile8_body(const RaggedParams& p, const Scales8&
 #pragma unroll
                 for (int e = 0; e < 16; e += 2)
                     mx = fmaxf(fmaxf(mx, sc[kb][e]), sc[kb][e + 1]);
-            mx = max_halves(mx);
+            mx = max_halves(mx) * to_log2;
             float corr = 1.f;
             if (__any(mx > m_run + 4.f)) {
                 const float m_new = mx > m_run + 4.f ? mx : m_run;
@@ -823,13 +817,13 @@ __device__ __forceinline__ void tile8_body(const RaggedParams& p, const Scales8&
                 l_run *= corr;
                 w_most *= corr;
             }
-            const float base = m_run == -INFINITY ? 0.f : m_run; // a row that has seen no key yet adds zeros
+            const float base = m_run == -INFINITY ? 0.f : -m_run; // a row that has seen no key yet adds zeros
             float rs = 0.f, most = 0.f;
 #pragma unroll
             for (int kb = 0; kb < HALVES; ++kb)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    sc[kb][e] = __builtin_amdgcn_exp2f(sc[kb][e] - base);
+                    sc[kb][e] = __builtin_amdgcn_exp2f(fmaf(sc[kb][e], to_log2, base));
                     rs += sc[kb][e];
                 }
             l_run += rs; // the other half of the tile's keys lies in lane + 32: they meet at the end
@@ -866,6 +860,7 @@ __device__ __forceinline__ void tile8_body(const RaggedParams& p, const Scales8&
                     for (int e = 0; e < 16; ++e)
                         oacc[d][e] *= by;
             }
+            __builtin_amdgcn_s_setprio(1); // beside another workgroup's wave that is not at its products (416 -> 406 us)
             scores(next, ks);
             // O^T += V^T P^T
 #pragma unroll
@@ -883,6 +878,8 @@ __device__ __forceinline__ void tile8_body(const RaggedParams& p, const Scales8&
                     oacc[d] = mfma(v, ph, oacc[d]);
                 }
             }
+            in_order();
+            __builtin_amdgcn_s_setprio(0);
         }
         __syncthreads();
     };
@@ -951,6 +948,65 @@ __global__ __launch_bounds__(256, 2) void paged8_tile_kernel(RaggedParams p, Sca
     tile8_body<D, KIND, WIDE>(p, scales, Place { blockIdx.x, blockIdx.y, gridDim.x }, lds);
 }
 
+// Both in one launch: what is bound by memory runs beside what is bound by the matrix and vector units.  Tiles, which take longest, come first.
+template <int D, int KIND>
+__global__ __launch_bounds__(256, 2) void paged8_mixed_kernel(RaggedParams p, Scales8 scales, Few8 few, unsigned tile_x, unsigned tile_wgs)
+{
+    FDX_TILE8_LDS(D, lds);
+    __shared__ __attribute__((aligned(16))) unsigned char q[2 * D / 32 * 2 * 1024];
+    if (blockIdx.x < tile_wgs) {
+        tile8_body<D, KIND, true>(p, scales, Place { blockIdx.x % tile_x, blockIdx.x / tile_x, tile_x }, lds);
+    } else {
+        static_assert(16 * (D + 4) * sizeof(float) <= sizeof(lds_ks0) && 16 * (D + 4) * sizeof(float) <= sizeof(lds_vs0)
+                && (2 * 4 * 16 + 5 * 64) * sizeof(float) <= sizeof(lds_rows_of), "fits into the tiles' LDS");
+        int* rest = lds.rows_of;
+        few8_body<D, KIND, true>(p, scales, few, blockIdx.x - tile_wgs,
+            Meet8 { reinterpret_cast<float*>(lds.ks0), reinterpret_cast<float*>(lds.ks1), reinterpret_cast<float*>(lds.vs0), reinterpret_cast<float*>(lds.vs1),
+                reinterpret_cast<float*>(rest), reinterpret_cast<int (*)[64]>(rest + 2 * 4 * 16), q });
+    }
+}
+
+// Rows whose keys more than one share, or range, has: sum of 2^(m - M) l o over them, divided by that of 2^(m - M) l.  A wave takes eight heads of a
+// row, for which it finds the row's sequence once.
+constexpr int kJoinHeads = 8;
+__global__ __launch_bounds__(256) void paged8_join_kernel(RaggedParams p, Few8 few)
+{
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const unsigned groups = (unsigned)(p.heads + kJoinHeads - 1) / kJoinHeads, item = blockIdx.x * 4 + wave;
+    const int row = (int)(item / groups), head0 = (int)(item % groups) * kJoinHeads, head1 = head0 + kJoinHeads < p.heads ? head0 + kJoinHeads : p.heads;
+    if (row >= p.tokens)
+        return;
+    const int index = find_row(SearchWave(), p.starts, p.n_seqs, p.tokens, row);
+    if (index < 0)
+        return;
+    const Sequence s = sequence_of<kPagedF32>(p, index, packed_span(p.starts, index, p.tokens));
+    const int token = row - s.span.first;
+    if (token >= s.span.count)
+        return;
+    if (!s.few) {
+        const int visible = visible_keys(p, s, token);
+        if (visible <= s.range)
+            return;
+        const int parts = (visible + s.range - 1) / s.range;
+        for (int head = head0; head < head1; ++head) {
+            const int64_t id = part_row(p, s, token, head);
+            join_parts(p, row, head, parts, [&](int i) { return p.tile.out(i, id, p.dv); }, [&](int i) { return p.tile.size(i, id, p.dv); });
+        }
+        return;
+    }
+    bool cut;
+    const int units = few_sequence(p, few, index, cut).units;
+    const int share = share_of(few, units_before(p, few, p.n_seqs)), first = units_before(p, few, index);
+    const int from = first / share, parts = (first + units - 1) / share - from + 1;
+    if (parts == 1)
+        return;
+    for (int head = head0; head < head1; ++head) {
+        const int kv_head = quotient(head, p.by_group), r = token * p.group + head - kv_head * p.group;
+        auto id = [&](int i) { return few.row_of(from + i, kv_head, i > 0 ? 0 : 1, r); };
+        join_parts(p, row, head, parts, [&](int i) { return few.out(id(i), p.dv); }, [&](int i) { return few.size(id(i), p.dv); });
+    }
+}
+
 // How a call is cut: paged_plan's tiles; sequences with few rows in as many shares as workgroups fit on the GPU, or as the longest lengths make.
 struct Plan8 {
     RaggedPlan tiles;
@@ -986,23 +1042,28 @@ static void paged8_launch(const RaggedParams& p, const Plan8& plan, const Scales
         | reinterpret_cast<uintptr_t>(p.v);
     const int64_t rows = (int64_t)p.n_pages * p.page_size.by, ld = p.ldk > p.ldv ? p.ldk : p.ldv;
     const bool wide = (all & 15) == 0 && ((p.ldq | p.ldo) & 3) == 0 && ((p.dk | p.dv) & 15) == 0 && rows * (ld >> 4) < ((int64_t)1 << 32);
-    if (plan.few_wgs > 0) {
-        if (wide)
-            hipLaunchKernelGGL((paged8_few_kernel<D, KIND, true>), dim3(plan.few_wgs), dim3(256), 0, stream(), p, scales, plan.few);
-        else
-            hipLaunchKernelGGL((paged8_few_kernel<D, KIND, false>), dim3(plan.few_wgs), dim3(256), 0, stream(), p, scales, plan.few);
+    const unsigned tile_x = (unsigned)plan.tiles.tiles, tile_y = (unsigned)(plan.tiles.tile_ranges > 0 ? plan.tiles.tile_ranges : 1);
+    const uint64_t tile_wgs = (uint64_t)tile_x * tile_y, all_wgs = tile_wgs + plan.few_wgs;
+    if (wide && tile_wgs > 0 && plan.few_wgs > 0 && all_wgs < (1u << 23)) {
+        hipLaunchKernelGGL((paged8_mixed_kernel<D, KIND>), dim3((unsigned)all_wgs), dim3(256), 0, stream(), p, scales, plan.few, tile_x, (unsigned)tile_wgs);
+    } else {
+        if (plan.few_wgs > 0) {
+            if (wide)
+                hipLaunchKernelGGL((paged8_few_kernel<D, KIND, true>), dim3(plan.few_wgs), dim3(256), 0, stream(), p, scales, plan.few);
+            else
+                hipLaunchKernelGGL((paged8_few_kernel<D, KIND, false>), dim3(plan.few_wgs), dim3(256), 0, stream(), p, scales, plan.few);
+        }
+        if (tile_wgs > 0) {
+            if (wide)
+                hipLaunchKernelGGL((paged8_tile_kernel<D, KIND, true>), dim3(tile_x, tile_y), dim3(256), 0, stream(), p, scales);
+            else
+                hipLaunchKernelGGL((paged8_tile_kernel<D, KIND, false>), dim3(tile_x, tile_y), dim3(256), 0, stream(), p, scales);
+        }
     }
-    if (plan.tiles.tiles > 0) {
-        const dim3 grid((unsigned)plan.tiles.tiles, (unsigned)plan.tiles.tile_ranges);
-        if (wide)
-            hipLaunchKernelGGL((paged8_tile_kernel<D, KIND, true>), grid, dim3(256), 0, stream(), p, scales);
-        else
-            hipLaunchKernelGGL((paged8_tile_kernel<D, KIND, false>), grid, dim3(256), 0, stream(), p, scales);
+    if (plan.few.shares > 1 || tile_y > 1) {
+        const int64_t items = (int64_t)p.tokens * ((p.heads + kJoinHeads - 1) / kJoinHeads);
+        hipLaunchKernelGGL(paged8_join_kernel, dim3((unsigned)((items + 3) / 4)), dim3(256), 0, stream(), p, plan.few);
     }
-    if (plan.few.shares > 1)
-        hipLaunchKernelGGL(paged8_join_kernel, dim3((unsigned)(((int64_t)p.tokens * p.heads + 3) / 4)), dim3(256), 0, stream(), p, plan.few);
-    if (plan.tiles.tile_ranges > 1)
-        ragged_join_launch(p);
 }
 
 } // namespace fdx
@@ -1034,7 +1095,7 @@ extern "C" fdx_status fdx_mha_paged8_f32(const float* q, int64_t ldq, const int3
     Plan8 plan = plan8(tokens, max_new, heads, &c);
     plan.few.parts = static_cast<float*>(scratch_dev);
     p.few_rows = plan.tiles.few_rows;
-    p.few = { nullptr, 0, 1, INT_MAX, 0, 0 }; // no ranges: sequences with few rows are cut in shares, and ragged_join_kernel leaves them alone
+    p.few = { nullptr, 0, 1, INT_MAX, 0, 0 }; // no ranges: sequences with few rows are cut in shares
     p.tile = { plan.few.parts + plan.few_floats, plan.tiles.tile_part, plan.tiles.tile_ranges, plan.tiles.tile_keys, plan.tiles.tile_whole, 0 };
     const Scales8 scales { cache->k_scale, cache->v_scale, make_divisor(cache->block) };
     const bool small = p.dk <= 64 && p.dv <= 64;

@@ -1211,11 +1211,6 @@ __global__ __launch_bounds__(256) void ragged_join_kernel(RaggedParams p)
     join_parts(p, row, head, parts, [&](int i) { return part.out(i, id, p.dv); }, [&](int i) { return part.size(i, id, p.dv); });
 }
 
-void ragged_join_launch(const RaggedParams& p)
-{
-    hipLaunchKernelGGL(ragged_join_kernel<kPagedF32>, dim3((unsigned)(((int64_t)p.tokens * p.heads + 3) / 4)), dim3(256), 0, stream(), p);
-}
-
 static int ranges_of(int keys, int64_t most, int* range_keys)
 {
     *range_keys = (int)(most > keys ? keys : (most + 63) & ~(int64_t)63);

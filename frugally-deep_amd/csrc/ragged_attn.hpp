@@ -73,8 +73,6 @@ RaggedPlan paged_plan(int tokens, int max_new, int heads, const fdx_kv_pages* c)
 fdx_status paged_params(const char* who, const float* q, int64_t ldq, const int32_t* starts, int tokens, int max_new, int heads,
     const fdx_kv_pages* cache, float* out, int64_t ldo, const void* scratch_dev, size_t scratch_bytes, int* error_flag_dev, RaggedParams& p);
 
-void ragged_join_launch(const RaggedParams& p); // sums of key ranges, whatever the pages hold
-
 // where a workgroup stands in its launch
 struct Place {
     unsigned x, y, nx;

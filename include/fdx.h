@@ -449,8 +449,9 @@ fdx_status fdx_kv8_append_f32(const float* k, int64_t ldk, const float* v, int64
     const fdx_kv_pages8* cache, int* error_flag_dev);
 /*
  * fdx_mha_paged_f32 for such a cache: the same sums over code * scale, the same arguments, refusals and error_flag_dev.
- * Precision: fp32 sums, exact codes; queries are held as two fp16 values: 22 bits of an element not below 2^-17 of the largest of its
- * row and head, 2^-40 of that largest below.  A row that sees a block whose scale is NaN, or whose query holds an infinity or a NaN, gets NaN;
+ * Precision: fp32 sums, exact codes; queries are held as two fp16 values: 22 bits of an element not below 2^-11 of the largest of its
+ * row and head, 2^-34 of that largest below.  So is a row's probability times the scale of the value, of the largest such product.  Keys up to
+ * 2^100.  A row that sees a block whose scale is NaN, or whose query holds an infinity or a NaN, gets NaN;
  * rows that do not see it keep their sums.
  */
 size_t fdx_mha_paged8_scratch_bytes(int tokens, int max_new, int heads, const fdx_kv_pages8* cache);
