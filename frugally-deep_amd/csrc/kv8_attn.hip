@@ -966,14 +966,82 @@ __global__ __launch_bounds__(256, 2) void paged8_mixed_kernel(RaggedParams p, Sc
     }
 }
 
-// Rows whose keys more than one share, or range, has: sum of 2^(m - M) l o over them, divided by that of 2^(m - M) l.  A wave takes eight heads of a
-// row, for which it finds the row's sequence once.
-constexpr int kJoinHeads = 8;
+// Rows whose keys more than one share, or range, has: sum of 2^(m - M) l o over them, divided by that of 2^(m - M) l.  A wave takes four heads of a
+// row, for which it finds the row's sequence once; eight parts of each are on their way together.
+constexpr int kJoinHeads = 4;
+template <class Out, class Size>
+__device__ __forceinline__ void join_heads(const RaggedParams& p, int row, int head0, int parts, const Out& out, const Size& size)
+{
+    constexpr int H = kJoinHeads, W = 8;
+    const int lane = threadIdx.x & 63;
+    float top[H], m[H], l[H], o0[H], o1[H];
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+        top[h] = -INFINITY;
+        l[h] = o0[h] = o1[h] = 0.f;
+    }
+    for (int i0 = 0; i0 < parts; i0 += 64)
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+            if (i0 + lane < parts)
+                top[h] = fmaxf(top[h], size(i0 + lane, h)[0]);
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+        top[h] = wave_all<true>(top[h]);
+        m[h] = top[h] == -INFINITY ? 0.f : top[h];
+    }
+    const int d0 = lane < p.dv ? lane : 0, d1 = 64 + lane < p.dv ? 64 + lane : 0;
+    for (int i0 = 0; i0 < parts; i0 += 64) {
+        float w[H];
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            w[h] = 0.f;
+            if (i0 + lane < parts) {
+                const float* at = size(i0 + lane, h);
+                w[h] = at[1] * __builtin_amdgcn_exp2f(at[0] - m[h]);
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+            l[h] += wave_all<false>(w[h]);
+        const int count = parts - i0 < 64 ? parts - i0 : 64;
+        for (int i = 0; i < count; i += W) {
+            float x0[H][W], x1[H][W];
+#pragma unroll
+            for (int z = 0; z < W; ++z)
+#pragma unroll
+                for (int h = 0; h < H; ++h) {
+                    const float* from = out(i0 + (i + z < count ? i + z : i), h);
+                    x0[h][z] = from[d0];
+                    x1[h][z] = from[d1];
+                }
+#pragma unroll
+            for (int z = 0; z < W; ++z)
+#pragma unroll
+                for (int h = 0; h < H; ++h) {
+                    const float wi = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w[h]), i + z < count ? i + z : i));
+                    o0[h] = fmaf(i + z < count ? wi : 0.f, x0[h][z], o0[h]);
+                    o1[h] = fmaf(i + z < count ? wi : 0.f, x1[h][z], o1[h]);
+                }
+        }
+    }
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+        if (head0 + h >= p.heads)
+            break;
+        float* to = p.out + (int64_t)row * p.ldo + (int64_t)(head0 + h) * p.dv;
+        if (lane < p.dv)
+            to[lane] = finish(o0[h], l[h], top[h] != -INFINITY);
+        if (64 + lane < p.dv)
+            to[64 + lane] = finish(o1[h], l[h], top[h] != -INFINITY);
+    }
+}
+
 __global__ __launch_bounds__(256) void paged8_join_kernel(RaggedParams p, Few8 few)
 {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const unsigned groups = (unsigned)(p.heads + kJoinHeads - 1) / kJoinHeads, item = blockIdx.x * 4 + wave;
-    const int row = (int)(item / groups), head0 = (int)(item % groups) * kJoinHeads, head1 = head0 + kJoinHeads < p.heads ? head0 + kJoinHeads : p.heads;
+    const int row = (int)(item / groups), head0 = (int)(item % groups) * kJoinHeads;
     if (row >= p.tokens)
         return;
     const int index = find_row(SearchWave(), p.starts, p.n_seqs, p.tokens, row);
@@ -983,15 +1051,14 @@ __global__ __launch_bounds__(256) void paged8_join_kernel(RaggedParams p, Few8 f
     const int token = row - s.span.first;
     if (token >= s.span.count)
         return;
+    auto head_of = [&](int h) { return head0 + h < p.heads ? head0 + h : p.heads - 1; };
     if (!s.few) {
         const int visible = visible_keys(p, s, token);
         if (visible <= s.range)
             return;
-        const int parts = (visible + s.range - 1) / s.range;
-        for (int head = head0; head < head1; ++head) {
-            const int64_t id = part_row(p, s, token, head);
-            join_parts(p, row, head, parts, [&](int i) { return p.tile.out(i, id, p.dv); }, [&](int i) { return p.tile.size(i, id, p.dv); });
-        }
+        const int64_t first = (int64_t)row * p.heads; // part_row
+        join_heads(p, row, head0, (visible + s.range - 1) / s.range, [&](int i, int h) { return p.tile.out(i, first + head_of(h), p.dv); },
+            [&](int i, int h) { return p.tile.size(i, first + head_of(h), p.dv); });
         return;
     }
     bool cut;
@@ -1000,11 +1067,11 @@ __global__ __launch_bounds__(256) void paged8_join_kernel(RaggedParams p, Few8 f
     const int from = first / share, parts = (first + units - 1) / share - from + 1;
     if (parts == 1)
         return;
-    for (int head = head0; head < head1; ++head) {
-        const int kv_head = quotient(head, p.by_group), r = token * p.group + head - kv_head * p.group;
-        auto id = [&](int i) { return few.row_of(from + i, kv_head, i > 0 ? 0 : 1, r); };
-        join_parts(p, row, head, parts, [&](int i) { return few.out(id(i), p.dv); }, [&](int i) { return few.size(id(i), p.dv); });
-    }
+    auto id = [&](int i, int h) {
+        const int head = head_of(h), kv_head = quotient(head, p.by_group);
+        return few.row_of(from + i, kv_head, i > 0 ? 0 : 1, token * p.group + head - kv_head * p.group);
+    };
+    join_heads(p, row, head0, parts, [&](int i, int h) { return few.out(id(i, h), p.dv); }, [&](int i, int h) { return few.size(id(i, h), p.dv); });
 }
 
 // How a call is cut: paged_plan's tiles; sequences with few rows in as many shares as workgroups fit on the GPU, or as the longest lengths make.
