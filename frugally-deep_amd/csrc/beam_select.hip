@@ -1,12 +1,19 @@
 // The best continuations of a sequence's beams over the vocabulary.
-#include <cmath>
-#include <cstdint>
-
-#include "common.hpp"
+//
+//   total(b, t) = score_b + x[b, t] - (m_b + log sum exp(x[b, :] - m_b)), the best `keep` of beams * vocab
+// A row's order is its logits', so its `keep` likeliest are all that can be among the best.  Two launches: a workgroup reads a row, or a part of one,
+// once, and leaves its sum and its list (score_lists.hpp); then a workgroup a sequence brings the lists together.
+//  * Totals of different beams decide an order, so sums are held in 64 bits (a thread's chunk in 32: some 20 terms of one size) and totals are taken in
+//    64 bits: two rows' sums are off by some 5e-8, not by the 5e-7 of fp32 totals of ten or so.  What a term costs more is one multiply-add for
+//    log2(e)'s second half.
+//  * Of all lists' heads the `keep`-th best is a threshold: no fewer continuations reach it, and of a list behind it none does, so they are at most
+//    keep * keep.  Those that reach it, twice as many as are kept on random logits, are ordered by counting the better ones of each.
+#include "score_lists.hpp"
+#include "kv_pages.hpp"
 
 namespace fdx {
 
-constexpr int kMostKeep = 32, kMostBeams = 32;
+constexpr int kMostBeams = 32, kBeamLists = 128, kBeamE = 8; // lists of a sequence
 
 struct BeamParams {
     const float* x;
@@ -18,143 +25,253 @@ struct BeamParams {
     int32_t *parents, *tokens, *new_done;
     float* new_scores;
     int* error_flag;
-    double* sums;   // [row]: log of the sum of exponentials
-    uint64_t* keys; // [row][keep]
+    uint64_t* part_keys; // [row][part][keep]
+    double* part_sums;   // [row][part][m, z]
+    int parts, part_len, chunk;
+    int width; // a power of two, not less than parts
+    Divisor by_parts, by_keep;
 };
 
-// Order of a row's tokens: descending logit, then ascending id.  Larger keys come first, 0 is no token.
-__device__ __forceinline__ uint32_t logit_bits(float x)
+// beams that have ended, or have no score, are not read
+__device__ __forceinline__ bool beam_reads(const BeamParams& p, int64_t row)
 {
-    const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.f); // -0 and +0 are equal logits
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
+    const float score = p.scores[row];
+    return !(p.done && p.done[row]) && score > -INFINITY && score < INFINITY;
 }
-__device__ __forceinline__ float bits_logit(uint32_t b) { return __builtin_bit_cast(float, b & 0x80000000u ? b & 0x7fffffffu : ~b); }
 
-// A workgroup takes a row: its sum, then its best tokens one after another.
+template <int E>
 __global__ __launch_bounds__(256) void beam_rows_kernel(BeamParams p)
 {
-    __shared__ double sum_of[256];
-    __shared__ uint64_t best_of[256];
-    const int64_t row = blockIdx.x;
-    const int tid = threadIdx.x;
-    const float* x = p.x + row * p.ld;
-    if (p.done && p.done[row])
+    __shared__ __attribute__((aligned(16))) uint64_t lists[8 * kMostTop]; // a wave: its list and a spare one
+    __shared__ __attribute__((aligned(16))) uint64_t found_by[4][kFound];
+    __shared__ double met[4][2];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int64_t row = blockIdx.x / p.parts;
+    const int part = blockIdx.x % p.parts;
+    if (!beam_reads(p, row))
         return;
+    const int first = part * p.part_len, last = p.vocab - first < p.part_len ? p.vocab : first + p.part_len;
+    const float* x = p.x + row * p.ld;
+    TopList t { lists + wave * 2 * kMostTop, lists + wave * 2 * kMostTop + kMostTop, found_by[wave], 0 };
+    if (lane < p.keep)
+        t.list[lane] = 0;
     float m = -INFINITY;
-    bool odd = false;
-    for (int i = tid; i < p.vocab; i += 256) {
-        m = fmaxf(m, x[i]);
-        odd = odd || !(x[i] < INFINITY);
-    }
-    odd = __syncthreads_or(odd);
-    sum_of[tid] = m;
-    __syncthreads();
-    for (int w = 128; w > 0; w >>= 1) {
-        if (tid < w)
-            sum_of[tid] = fmax(sum_of[tid], sum_of[tid + w]);
-        __syncthreads();
-    }
-    m = (float)sum_of[0];
-    __syncthreads();
     double z = 0.0;
-    for (int i = tid; i < p.vocab; i += 256)
-        z += exp((double)x[i] - (double)m);
-    sum_of[tid] = z;
+    for (int c0 = first; c0 < last; c0 += p.chunk) {
+        const int end = last - c0 < p.chunk ? last : c0 + p.chunk;
+        f32x4 v[E];
+        load_chunk(x, c0, end, v);
+        const float best = most_of_chunk(v, c0, end);
+        const float top = fmaxf(m, wave_all<true>(best)), use = top == -INFINITY ? 0.f : top;
+        constexpr float kHigh = 0x1.715476p+0f, kLow = 0x1.4ae0cp-26f; // log2(e) = kHigh + kLow
+        float sum[2] = { 0.f, 0.f };
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+            if (c0 + j * 256 * 4 < end) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float d = __builtin_elementwise_maximum(v[j][e] - use, -1e30f); // finite, so that the halves do not cancel; NaN stays NaN
+                    sum[e & 1] += __builtin_amdgcn_exp2f(fmaf(d, kHigh, d * kLow));
+                }
+            }
+        if (top > m && m > -INFINITY) // a few times a row
+            z *= exp((double)m - (double)top);
+        z += (double)(sum[0] + sum[1]);
+        m = top;
+        add_chunk(t, p.keep, v, c0, end, best);
+    }
+    for (int w = 32; w > 0; w >>= 1)
+        z += __shfl_xor(z, w, 64);
+    if (lane == 0) {
+        met[wave][0] = m;
+        met[wave][1] = z;
+    }
+    uint64_t* flat = found_by[0]; // candidates are done with
     __syncthreads();
-    for (int w = 128; w > 0; w >>= 1) {
-        if (tid < w)
-            sum_of[tid] += sum_of[tid + w];
-        __syncthreads();
-    }
-    if (tid == 0) {
-        p.sums[row] = (double)m + log(sum_of[0]);
-        if (odd && p.error_flag)
-            *p.error_flag = 1;
-    }
-    uint64_t before = ~(uint64_t)0;
-    for (int j = 0; j < p.keep; ++j) {
-        uint64_t best = 0;
-        for (int i = tid; i < p.vocab; i += 256) {
-            const uint64_t key = (uint64_t)logit_bits(x[i]) << 32 | (uint32_t)~i;
-            best = x[i] > -INFINITY && !odd && key < before && key > best ? key : best;
-        }
-        __syncthreads();
-        best_of[tid] = best;
-        __syncthreads();
-        for (int w = 128; w > 0; w >>= 1) {
-            if (tid < w && best_of[tid + w] > best_of[tid])
-                best_of[tid] = best_of[tid + w];
-            __syncthreads();
-        }
-        before = best_of[0];
-        if (tid == 0)
-            p.keys[row * p.keep + j] = before;
+    if (lane < p.keep)
+        flat[wave * p.keep + lane] = t.list[lane];
+    const uint64_t* all = join_lists(flat, flat + 4 * p.keep, 4, p.keep);
+    if (tid < p.keep)
+        p.part_keys[(int64_t)blockIdx.x * p.keep + tid] = all[tid];
+    if (tid == 64) {
+        const double most = fmax(fmax(met[0][0], met[1][0]), fmax(met[2][0], met[3][0]));
+        double sum = 0.0;
+        for (int i = 0; i < 4; ++i)
+            sum += met[i][0] == -INFINITY ? met[i][1] : met[i][1] * exp(met[i][0] - most);
+        p.part_sums[(int64_t)blockIdx.x * 2] = most;
+        p.part_sums[(int64_t)blockIdx.x * 2 + 1] = sum;
     }
 }
 
-// A wave takes a sequence: the best of its beams' next ones, one after another.
-__global__ __launch_bounds__(64) void beam_select_kernel(BeamParams p)
+// continuations in their order: the larger key of a beam is the larger logit, or the lower token of equal ones
+struct Continuation {
+    double total;
+    uint64_t key;
+    int beam;
+};
+__device__ __forceinline__ bool better(const Continuation& a, const Continuation& b)
 {
-    const int s = blockIdx.x, lane = threadIdx.x;
-    const int64_t row = (int64_t)s * p.beams + lane;
-    bool ended = false, live = lane < p.beams;
-    double before = 0.0, log_sum = 0.0;
-    if (live) {
-        before = p.scores[row];
-        ended = p.done && p.done[row];
-        const bool odd = !(before < INFINITY);
-        if (odd && p.error_flag)
-            *p.error_flag = 1;
-        live = before > -INFINITY && !odd;
-        log_sum = ended ? 0.0 : p.sums[row];
+    return a.total > b.total || (a.total == b.total && (a.beam < b.beam || (a.beam == b.beam && a.key > b.key)));
+}
+// a set of them in LDS
+template <int N>
+struct Continuations {
+    double total[N];
+    uint64_t key[N];
+    int beam[N];
+
+    __device__ __forceinline__ Continuation at(int i) const { return { total[i], key[i], beam[i] }; }
+    __device__ __forceinline__ void put(int i, const Continuation& c)
+    {
+        total[i] = c.total;
+        key[i] = c.key;
+        beam[i] = c.beam;
     }
-    int next = 0;
-    for (int j = 0; j < p.keep; ++j) {
-        double total = -INFINITY;
-        int token = -1;
-        if (live && ended) {
-            token = p.end_id;
-            total = next == 0 ? before : -INFINITY;
-        } else if (live && next < p.keep) {
-            const uint64_t key = p.keys[row * p.keep + next];
-            token = (int)~(uint32_t)key;
-            total = key ? before + ((double)bits_logit((uint32_t)(key >> 32)) - log_sum) : -INFINITY;
+    // how many of the first n are better than c, the me-th; those that are the same (empty) by their places
+    __device__ __forceinline__ int in_front(int n, const Continuation& c, int me) const
+    {
+        int count = 0;
+#pragma unroll 4
+        for (int k = 0; k < n; ++k) {
+            const double t = total[k];
+            count += t > c.total;
+            if (__builtin_expect(t == c.total && k != me, 0)) // of one total
+                count += better(at(k), c) || (beam[k] == c.beam && key[k] == c.key && k < me);
         }
-        double best = total;
-        int who = lane;
-        for (int w = 32; w > 0; w >>= 1) {
-            const double o = __shfl_xor(best, w, 64);
-            const int ow = __shfl_xor(who, w, 64);
-            if (o > best || (o == best && ow < who)) {
-                best = o;
-                who = ow;
-            }
+        return count;
+    }
+};
+
+__global__ __launch_bounds__(256) void beam_select_kernel(BeamParams p)
+{
+    __shared__ Continuations<kMostTop * kMostTop> items;
+    __shared__ Continuations<kBeamLists> heads;
+    __shared__ double before_of[kMostBeams], log_sum_of[kMostBeams];
+    __shared__ int ended_of[kMostBeams], count;
+    __shared__ Continuation threshold;
+    const int tid = threadIdx.x;
+    const int64_t s = blockIdx.x, row0 = s * p.beams;
+    const int lists = p.beams * p.parts;
+    const uint64_t* keys = p.part_keys + row0 * p.parts * p.keep;
+    if (tid == 0) {
+        count = 0;
+        threshold = { -INFINITY, 0, kMostBeams };
+    }
+    const uint64_t first_key = tid < lists ? keys[tid * p.keep] : 0; // on its way beside the sums (rows that are not read have left anything)
+    // the rows' sums: p.width threads a beam, one a part
+    for (int b = tid / p.width; b < p.beams; b += 256 / p.width) {
+        const int64_t row = row0 + b;
+        const int part = tid & (p.width - 1);
+        const float score = p.scores[row];
+        const bool done = p.done && p.done[row], finite = score > -INFINITY && score < INFINITY, reads = finite && !done;
+        double m = -INFINITY, z = 0.0;
+        if (part < p.parts) {
+            m = p.part_sums[(row * p.parts + part) * 2];
+            z = p.part_sums[(row * p.parts + part) * 2 + 1];
         }
-        const bool there = best > -INFINITY;
-        if (lane == who) {
-            const int64_t at = (int64_t)s * p.keep + j;
-            p.parents[at] = there ? (int)row : -1;
-            p.tokens[at] = there ? token : -1;
-            p.new_scores[at] = (float)best;
+        double most = m;
+        for (int w = p.width / 2; w > 0; w >>= 1)
+            most = fmax(most, __shfl_xor(most, w, 64));
+        z = m == -INFINITY || m == most ? z : z * exp(m - most);
+        for (int w = p.width / 2; w > 0; w >>= 1)
+            z += __shfl_xor(z, w, 64);
+        if (part == 0) {
+            const bool bad = !(score < INFINITY) || (reads && !(z < INFINITY)); // a NaN or an infinity: no continuation
+            before_of[b] = bad || !finite || (reads && z == 0.0) ? -INFINITY : (double)score;
+            log_sum_of[b] = reads && z > 0.0 ? most + log(z) : 0.0;
+            ended_of[b] = finite && done;
+            if (bad && p.error_flag)
+                *p.error_flag = 1;
+        }
+    }
+    __syncthreads();
+    auto listed = [&](int list, int j, uint64_t key) -> Continuation { // an ended beam has one continuation, in its first list
+        const int b = quotient(list, p.by_parts);
+        const double before = before_of[b];
+        if (ended_of[b])
+            return list == b * p.parts && j == 0 ? Continuation { before, 1, b } : Continuation { -INFINITY, 0, b };
+        if (key == 0 || before == -INFINITY)
+            return { -INFINITY, 0, b };
+        return { before + ((double)bits_score((uint32_t)(key >> 32)) - log_sum_of[b]), key, b };
+    };
+    const bool cut = lists > p.keep;
+    if (cut) {
+        if (tid < lists)
+            heads.put(tid, listed(tid, 0, first_key));
+        __syncthreads();
+        if (tid < lists) {
+            const Continuation mine = heads.at(tid);
+            if (heads.in_front(lists, mine, tid) == p.keep - 1)
+                threshold = mine;
+        }
+        __syncthreads();
+    }
+    const Continuation least = threshold;
+    for (int i = tid; i < lists * p.keep; i += 256) {
+        const int list = quotient(i, p.by_keep);
+        if (cut && better(least, heads.at(list)))
+            continue;
+        const Continuation c = listed(list, i - list * p.keep, keys[i]);
+        if (c.total > -INFINITY && !better(least, c))
+            items.put(atomicAdd(&count, 1), c);
+    }
+    __syncthreads();
+    const int found = count;
+    for (int i = tid; i < found; i += 256) {
+        const Continuation mine = items.at(i);
+        const int place = items.in_front(found, mine, i);
+        if (place < p.keep) {
+            const int64_t at = s * p.keep + place;
+            const bool ended = ended_of[mine.beam];
+            const int token = ended ? p.end_id : (int)~(uint32_t)mine.key;
+            p.parents[at] = (int)(row0 + mine.beam);
+            p.tokens[at] = token;
+            p.new_scores[at] = (float)mine.total;
             if (p.new_done)
-                p.new_done[at] = there && (ended || token == p.end_id);
-            ++next;
+                p.new_done[at] = ended || token == p.end_id;
         }
     }
+    if (tid < p.keep && tid >= found) { // places that are left over
+        const int64_t at = s * p.keep + tid;
+        p.parents[at] = p.tokens[at] = -1;
+        p.new_scores[at] = -INFINITY;
+        if (p.new_done)
+            p.new_done[at] = 0;
+    }
+}
+
+// Rows are cut in one part for 4096 logits, or fewer parts, while that makes no more workgroups than kBeamGroups and no more lists of a sequence than
+// kBeamLists; all but the last part are whole thousands (of 1024).
+constexpr int kBeamGroups = 1024;
+struct BeamPlan {
+    int parts, part_len, chunk;
+    size_t keys, all; // bytes
+};
+static BeamPlan beam_plan(int64_t rows, int beams, int vocab, int keep)
+{
+    BeamPlan r {};
+    auto thousands = [&](int64_t n, int64_t into) { return (int)((n + into * 1024 - 1) / (into * 1024) * 1024); };
+    const int64_t most = ((int64_t)vocab + 4095) / 4096;
+    int64_t parts = kBeamGroups / rows < most ? kBeamGroups / rows : most;
+    parts = parts < kBeamLists / beams ? parts : kBeamLists / beams;
+    parts = parts < 1 ? 1 : (parts > 64 ? 64 : parts);
+    r.part_len = thousands(vocab, parts);
+    r.parts = (vocab + r.part_len - 1) / r.part_len;
+    r.chunk = thousands(r.part_len, (r.part_len + 1024 * kBeamE - 1) / (1024 * kBeamE)); // chunks of a part are of one length
+    r.keys = ((size_t)rows * r.parts * keep * sizeof(uint64_t) + 15) & ~(size_t)15;
+    r.all = r.keys + (size_t)rows * r.parts * 2 * sizeof(double);
+    return r;
 }
 
 } // namespace fdx
 
 using namespace fdx;
 
-static size_t beam_sums(int64_t rows) { return ((size_t)rows * sizeof(double) + 15) & ~(size_t)15; }
-
 extern "C" size_t fdx_beam_select_scratch_bytes(int n_seqs, int beams, int vocab, int keep)
 {
     if (n_seqs <= 0 || beams <= 0 || vocab <= 0 || keep <= 0)
         return 0;
-    const int64_t rows = (int64_t)n_seqs * beams;
-    return beam_sums(rows) + (size_t)rows * keep * sizeof(uint64_t);
+    return beams <= kMostBeams ? beam_plan((int64_t)n_seqs * beams, beams, vocab, keep).all : 0;
 }
 
 extern "C" fdx_status fdx_beam_select_f32(const float* logits, int64_t ld, int n_seqs, int beams, int vocab, const float* scores, const int32_t* done,
@@ -164,16 +281,25 @@ extern "C" fdx_status fdx_beam_select_f32(const float* logits, int64_t ld, int n
     FDX_REQUIRE(n_seqs > 0 && beams > 0 && beams <= kMostBeams && (int64_t)n_seqs * beams <= (1 << 23), "beam_select: 1 to 32 beams, up to 2^23 rows");
     FDX_REQUIRE(vocab > 0 && vocab <= (1 << 24), "beam_select: 1 to 2^24 logits a row");
     FDX_REQUIRE(ld >= vocab, "beam_select: rows overlap");
-    FDX_REQUIRE(keep > 0 && keep <= kMostKeep && keep <= (int64_t)beams * vocab, "beam_select: 1 to 32 continuations, no more than there are");
+    FDX_REQUIRE(keep > 0 && keep <= kMostTop && keep <= (int64_t)beams * vocab, "beam_select: 1 to 32 continuations, no more than there are");
     FDX_REQUIRE(end_id < vocab && (end_id >= 0 || (!done && !new_done)), "beam_select: end_id is no token");
     FDX_REQUIRE(scratch_dev && (reinterpret_cast<uintptr_t>(scratch_dev) & 15) == 0, "beam_select: scratch missing or not 16-byte aligned");
     const int64_t rows = (int64_t)n_seqs * beams;
+    const BeamPlan plan = beam_plan(rows, beams, vocab, keep);
+    int width = 1;
+    while (width < plan.parts)
+        width *= 2;
     char* scratch = static_cast<char*>(scratch_dev);
     const BeamParams p { logits, ld, beams, vocab, keep, scores, done, end_id, parents, tokens, new_done, new_scores, error_flag_dev,
-        reinterpret_cast<double*>(scratch), reinterpret_cast<uint64_t*>(scratch + beam_sums(rows)) };
+        reinterpret_cast<uint64_t*>(scratch), reinterpret_cast<double*>(scratch + plan.keys), plan.parts, plan.part_len, plan.chunk, width,
+        make_divisor(plan.parts), make_divisor(keep) };
+    const dim3 grid((unsigned)(rows * plan.parts));
     profile_begin();
-    hipLaunchKernelGGL(beam_rows_kernel, dim3((unsigned)rows), dim3(256), 0, stream(), p);
-    hipLaunchKernelGGL(beam_select_kernel, dim3((unsigned)n_seqs), dim3(64), 0, stream(), p);
+    if (plan.chunk <= 4096)
+        hipLaunchKernelGGL(beam_rows_kernel<4>, grid, dim3(256), 0, stream(), p);
+    else
+        hipLaunchKernelGGL(beam_rows_kernel<kBeamE>, grid, dim3(256), 0, stream(), p);
+    hipLaunchKernelGGL(beam_select_kernel, dim3((unsigned)n_seqs), dim3(256), 0, stream(), p);
     profile_end("beam_select_f32", 4.0 * rows * vocab, 4.0 * rows * (double)vocab);
     FDX_LAUNCH_CHECK();
     return FDX_OK;

@@ -5,23 +5,13 @@
 // that is asked of it (2048 rows of 50 257: 76 us, 5.4 TB/s, without alternatives, 102 us, 4.0 TB/s, with 20, where ordering them takes the
 // vector units; 16 rows with 5: 11 us, two dependent launches).
 //
-// A workgroup takes a row, or a part of one, in chunks of 4 E logits a thread; waves keep sums of their own, which meet at the end.  The likeliest
-// `top` tokens of a wave are a sorted list in LDS.  Of a chunk, `top` lanes' largest logits are a threshold that no fewer than `top` tokens
-// reach: it is found bit by bit with votes on the lanes' largest, and stops as soon as not many more lanes than that pass.  On
-// random logits about as many tokens pass as are asked for; they and the list so far are ordered by counting, for each, the better ones.
-// Where more pass than there is room for (equal logits), the best are taken one at a time.  Only finite logits are listed: places that stay
-// empty are those of ruled-out tokens, the lowest ids that are not listed.  Lists of waves and of parts meet in pairs, an item's place being its
-// place in its own list plus the number of better ones in the other.
-#include <cmath>
-#include <cstdint>
-
-#include "common.hpp"
+// A workgroup takes a row, or a part of one, in chunks of 4 E logits a thread; waves keep sums of their own, which meet at the end, and lists of
+// the likeliest tokens (score_lists.hpp).  Places of a list that stay empty are those of ruled-out tokens, the lowest ids that are not listed.
+#include "score_lists.hpp"
 
 namespace fdx {
 
-constexpr int kMostTop = 32, kMostParts = 64, kFound = 192;
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4))); // rows start at any multiple of four bytes
+constexpr int kMostParts = 64;
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
 
 struct ScoreParams {
@@ -37,14 +27,6 @@ struct ScoreParams {
     int parts, part_len, chunk; // logits of a part, and of a chunk: multiples of what the workgroup's threads load at once
 };
 
-// Order of the likeliest tokens: descending logit, then ascending id.  Larger keys come first, 0 is no token.
-__device__ __forceinline__ uint32_t score_bits(float x)
-{
-    const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.f); // -0 and +0 are equal logits
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
-}
-__device__ __forceinline__ float bits_score(uint32_t b) { return __builtin_bit_cast(float, b & 0x80000000u ? b & 0x7fffffffu : ~b); }
-
 struct Sums {
     float m, z, w; // w in units of log2
 };
@@ -57,54 +39,6 @@ __device__ __forceinline__ void add_sums(Sums& a, float m, float z, float w)
     a.w = fa * (a.w + a.z * da) + fb * (w + z * db);
     a.z = fa * a.z + fb * z;
     a.m = top;
-}
-
-__device__ __forceinline__ void wave_lds_fence()
-{
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-__device__ __forceinline__ uint64_t wave_max_key(uint64_t v)
-{
-    for (int w = 32; w > 0; w >>= 1) {
-        const uint32_t lo = __shfl_xor((int)(uint32_t)v, w, 64), hi = __shfl_xor((int)(v >> 32), w, 64);
-        const uint64_t o = (uint64_t)hi << 32 | lo;
-        v = o > v ? o : v;
-    }
-    return v;
-}
-__device__ __forceinline__ uint64_t uniform_key(uint64_t v)
-{
-    return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)v);
-}
-
-// `lists` sorted lists of `top` keys, one behind the other in `from`, become one at the returned place (`from` or `to`, both in LDS)
-__device__ __forceinline__ uint64_t* join_lists(uint64_t* from, uint64_t* to, int lists, int top)
-{
-    while (lists > 1) {
-        __syncthreads();
-        for (int i = threadIdx.x; i < lists * top; i += 256) {
-            const int list = i / top, place = i - list * top, other = list ^ 1;
-            const uint64_t key = from[i];
-            int better = 0;
-            if (other < lists)
-                for (int step = 32; step > 0; step >>= 1) // how many of the other list are larger
-                    if (better + step <= top && from[other * top + better + step - 1] > key)
-                        better += step;
-            // equal keys are empty places: those of the second list go behind
-            if (other < lists && key == 0 && (list & 1))
-                better = top;
-            if (place + better < top)
-                to[(list >> 1) * top + place + better] = key;
-        }
-        uint64_t* t = from;
-        from = to;
-        to = t;
-        lists = (lists + 1) / 2;
-    }
-    __syncthreads();
-    return from;
 }
 
 // what is asked of a row, from its sums and its list
@@ -162,36 +96,15 @@ __global__ __launch_bounds__(256) void token_scores_kernel(ScoreParams p)
     const int part = blockIdx.x % p.parts;
     const int first = part * p.part_len, last = p.vocab - first < p.part_len ? p.vocab : first + p.part_len;
     const float* x = p.x + row * p.ld;
-    uint64_t* list = lists + wave * 2 * kMostTop;
-    uint64_t* spare = list + kMostTop;
-    uint64_t* found = found_by[TOP ? wave : 0];
-    uint32_t worst = 0; // logit of a full list's last token
+    TopList t { lists + wave * 2 * kMostTop, lists + wave * 2 * kMostTop + kMostTop, found_by[TOP ? wave : 0], 0 };
     if (TOP && lane < p.top)
-        list[lane] = 0;
+        t.list[lane] = 0;
     Sums s { -INFINITY, 0.f, 0.f };
     for (int c0 = first; c0 < last; c0 += p.chunk) {
         const int end = last - c0 < p.chunk ? last : c0 + p.chunk;
         f32x4 v[E];
-#pragma unroll
-        for (int j = 0; j < E; ++j) {
-            const int at = c0 + (j * 256 + tid) * 4;
-            v[j] = f32x4 { -INFINITY, -INFINITY, -INFINITY, -INFINITY };
-            if (c0 + j * 256 * 4 < end) { // the same for the workgroup
-                if (at + 3 < end) {
-                    v[j] = *reinterpret_cast<const f32x4_any*>(x + at);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 3; ++e)
-                        if (at + e < end)
-                            v[j][e] = x[at + e];
-                }
-            }
-        }
-        float best = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < E; ++j)
-            if (c0 + j * 256 * 4 < end)
-                best = fmaxf(fmaxf(fmaxf(best, v[j][0]), fmaxf(v[j][1], v[j][2])), v[j][3]);
+        load_chunk(x, c0, end, v);
+        const float best = most_of_chunk(v, c0, end);
         const float m = wave_all<true>(best), use = m == -INFINITY ? 0.f : m;
         float z[2] = { 0.f, 0.f }, w[2] = { 0.f, 0.f };
 #pragma unroll
@@ -205,80 +118,8 @@ __global__ __launch_bounds__(256) void token_scores_kernel(ScoreParams p)
                 }
             }
         add_sums(s, m, wave_all<false>(z[0] + z[1]), wave_all<false>(w[0] + w[1]));
-        if constexpr (TOP) {
-            const uint32_t mine = best > -INFINITY ? score_bits(best) : 0;
-            if (__ballot(mine > worst)) {
-                uint32_t cut = worst + 1; // equal logits: those of lower ids are in the list already
-                if (worst == 0) {
-                    cut = 0;
-                    for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
-                        const int pass = __builtin_popcountll(__ballot(mine >= (cut | bit)));
-                        cut = pass >= p.top ? cut | bit : cut;
-                        if (pass >= p.top && pass <= p.top + 4)
-                            break;
-                    }
-                }
-                const float cut_score = bits_score(cut > 0x00800000u ? cut : 0x00800000u); // no less than -FLT_MAX
-                int count = 0;
-#pragma unroll
-                for (int j = 0; j < E; ++j)
-                    if (c0 + j * 256 * 4 < end) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const uint64_t in = __ballot(v[j][e] >= cut_score);
-                            if (in) {
-                                const int at = count + __builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in, 0));
-                                if (v[j][e] >= cut_score && at < kFound)
-                                    found[at] = (uint64_t)score_bits(v[j][e]) << 32 | (uint32_t)~(c0 + (j * 256 + tid) * 4 + e);
-                                count += __builtin_popcountll(in);
-                            }
-                        }
-                    }
-                if (count > kFound) { // the best ones, one at a time
-                    uint64_t before = ~(uint64_t)0;
-                    count = 0;
-                    while (count < p.top) {
-                        uint64_t most = 0;
-#pragma unroll
-                        for (int j = 0; j < E; ++j)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const uint64_t key = (uint64_t)score_bits(v[j][e]) << 32 | (uint32_t)~(c0 + (j * 256 + tid) * 4 + e);
-                                most = v[j][e] >= cut_score && key < before && key > most ? key : most;
-                            }
-                        before = uniform_key(wave_max_key(most));
-                        if (before == 0)
-                            break;
-                        if (lane == 0)
-                            found[count] = before;
-                        ++count;
-                    }
-                }
-                if (count > 0) {
-                    wave_lds_fence();
-                    if (lane < p.top)
-                        spare[lane] = 0;
-                    wave_lds_fence();
-                    for (int i = lane; i < p.top + count; i += 64) {
-                        const uint64_t key = i < p.top ? list[i] : found[i - p.top];
-                        int place = 0;
-#pragma unroll 4
-                        for (int k = 0; k < p.top; ++k)
-                            place += list[k] > key;
-#pragma unroll 4
-                        for (int k = 0; k < count; ++k)
-                            place += found[k] > key;
-                        if (key != 0 && place < p.top)
-                            spare[place] = key;
-                    }
-                    wave_lds_fence();
-                    uint64_t* t = list;
-                    list = spare;
-                    spare = t;
-                    worst = (uint32_t)(uniform_key(list[p.top - 1]) >> 32);
-                }
-            }
-        }
+        if constexpr (TOP)
+            add_chunk(t, p.top, v, c0, end, best);
     }
     if (lane == 0)
         met[wave] = s;
@@ -287,7 +128,7 @@ __global__ __launch_bounds__(256) void token_scores_kernel(ScoreParams p)
         uint64_t* flat = found_by[0]; // candidates are done with
         __syncthreads();
         if (lane < p.top)
-            flat[wave * p.top + lane] = list[lane];
+            flat[wave * p.top + lane] = t.list[lane];
         all = join_lists(flat, flat + 4 * p.top, 4, p.top);
     } else {
         __syncthreads();
