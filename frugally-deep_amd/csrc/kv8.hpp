@@ -73,6 +73,17 @@ __device__ __forceinline__ void transpose_codes(const uint32_t (&r)[4], uint32_t
     t[3] = __builtin_amdgcn_perm(d, c, 0x07060302u);
 }
 
+// sum over the lanes up to this one
+__device__ __forceinline__ int wave_prefix(int v)
+{
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true); // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, true); // the last lane of a row to the row behind it
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, true); // lane 31 to lanes 32 ..
+    return v;
+}
 // where the scales of a cache are
 struct Scales8 {
     const float *k, *v;

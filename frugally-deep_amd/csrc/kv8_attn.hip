@@ -102,17 +102,6 @@ __device__ __forceinline__ FewSequence few_sequence(const RaggedParams& p, const
     const int blocks = (s.keys + 31) / 32;
     return { s.span.first, s.span.count, s.keys, s.ahead, blocks > 0 ? (blocks - 1) / few.unit + 1 : 1 };
 }
-// sum over the lanes up to this one
-__device__ __forceinline__ int up_to_me(int v)
-{
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true); // row_shr 1, 2, 4, 8
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, true); // the last lane of a row to the row behind it
-    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, true); // lane 31 to lanes 32 ..
-    return v;
-}
 // units of the sequences in front of `before`
 __device__ __forceinline__ int units_before(const RaggedParams& p, const Few8& few, int before)
 {
@@ -121,7 +110,7 @@ __device__ __forceinline__ int units_before(const RaggedParams& p, const Few8& f
     bool cut;
     for (int i = lane; i < before; i += 64)
         sum += few_sequence(p, few, i, cut).units;
-    return __builtin_amdgcn_readlane(up_to_me(sum), 63);
+    return __builtin_amdgcn_readlane(wave_prefix(sum), 63);
 }
 __device__ __forceinline__ int share_of(const Few8& few, int all)
 {
@@ -468,7 +457,7 @@ __device__ __forceinline__ void few8_body(const RaggedParams& p, const Scales8& 
         const int lane = tid & 63;
         bool cut;
         const FewSequence of_lane = few_sequence(p, few, i0 + lane, cut);
-        const int up_to = front + up_to_me(of_lane.units), before = front;
+        const int up_to = front + wave_prefix(of_lane.units), before = front;
         front = __builtin_amdgcn_readlane(up_to, 63);
         if (wg == 0)
             raise_flag(p, cut);

@@ -1,8 +1,10 @@
 // The page table after a selection: sequences go on as copies of others, full pages are shared, partly filled ones get copies.
 //
 // Which pages are kept is a bit each; the free ones are then the zeros, taken from the lowest on by ranks: of the sequences' needs (a prefix
-// sum) and of the zeros (prefix sums over the words' counts), so nothing depends on the order in which threads arrive.
-#include <cfloat>
+// sum) and of the zeros (prefix sums over the words' counts), so nothing depends on the order in which threads arrive.  A chain of a dozen
+// dependent steps, bound by their latency: one workgroup takes them all where its LDS holds a number for each sequence and a bit for each page
+// (64 groups of eight beams, 24 000 entries of the table: 15 us; through memory 28), so that the steps meet at barriers instead of launches.  Larger
+// tables are marked by a launch of their own.  The copies follow in a launch, at the memory's rate.
 #include <climits>
 
 #include "kv8.hpp"
@@ -14,10 +16,10 @@ struct ForkParams {
     int32_t *new_table, *new_lens, *free_pages;
     int n_seqs, width, n_pages, max_len;
     Divisor page_size, by_width;
-    uint32_t* used;   // a bit a page
+    uint32_t* used;   // a bit a page (these three: of large tables only)
     int32_t* owner;   // of a partly filled page: the first sequence that goes on in it
     int32_t* list;    // free pages that are taken
-    int4* plan;       // a sequence: its partly filled page (-1: none), its copy's page (-1: none), filled rows, entries of the new table
+    int4* plan;       // a sequence: its partly filled page (-1: none), its copy's page (-1: none), filled rows
     int* error_flag;
 };
 
@@ -26,16 +28,12 @@ struct Fork {
 };
 __device__ __forceinline__ Fork fork_of(const ForkParams& p, int i, bool& odd)
 {
-    Fork f { p.parents[i], 0, 0 };
-    odd = false;
-    if (f.parent >= p.n_seqs) {
-        odd = true;
-        f.parent = -1;
-    }
-    if (f.parent < 0)
+    const int parent = p.parents[i], more = p.grow ? p.grow[i] : 0;
+    odd = parent >= p.n_seqs;
+    if (odd || parent < 0)
         return { -1, 0, 0 };
-    const int len = p.lens[f.parent], more = p.grow ? p.grow[i] : 0;
-    f.length = len < 0 ? 0 : (len > p.max_len ? p.max_len : len);
+    const int len = p.lens[parent];
+    Fork f { parent, len < 0 ? 0 : (len > p.max_len ? p.max_len : len), 0 };
     f.want = more < 0 || more > p.max_len - f.length ? f.length : f.length + more;
     odd = f.length != len || f.want - f.length != more;
     return f;
@@ -45,11 +43,7 @@ __device__ __forceinline__ Fork fork_of(const ForkParams& p, int i, bool& odd)
 __device__ __forceinline__ int before_me(int v, int* lds, int& total)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int sum = v;
-    for (int d = 1; d < 64; d <<= 1) {
-        const int o = __shfl_up(sum, d, 64);
-        sum += lane >= d ? o : 0;
-    }
+    const int sum = wave_prefix(v);
     __syncthreads();
     if (lane == 63)
         lds[wave] = sum;
@@ -67,48 +61,184 @@ __device__ __forceinline__ int agent_load(const int32_t* at) { return __hip_atom
 __device__ __forceinline__ void agent_store(int32_t* at, int v) { __hip_atomic_store(at, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
 constexpr int kForkThreads = 1024;
+// what a workgroup's LDS is laid out for: a sequence a thread, and a hash table of twice as many pages
+constexpr int kSmallSeqs = kForkThreads, kSmallWords = 4096, kHash = 2 * kSmallSeqs;
+constexpr int64_t kSmallEntries = 1 << 17;
 
-__global__ __launch_bounds__(kForkThreads) void kv_fork_kernel(ForkParams p)
+// entry j of a sequence in the table: the page that it shares, -1 if none
+__device__ __forceinline__ int checked_page(const ForkParams& p, int at, bool& odd)
+{
+    if (at >= 0 && at < p.n_pages)
+        return at;
+    odd = true;
+    return -1;
+}
+
+// where a sequence's new pages begin and end among its entries
+struct Entries {
+    int full, part, begin, end;
+};
+__device__ __forceinline__ Entries entries_of(const ForkParams& p, const Fork& f, int page, bool kept)
+{
+    Entries e;
+    e.full = quotient(f.length, p.page_size);
+    e.part = f.length - e.full * (int)p.page_size.by;
+    e.end = quotient(f.want, p.page_size);
+    e.end += f.want > e.end * (int)p.page_size.by;
+    e.begin = e.full + (e.part > 0 && (kept || page < 0)); // a partly filled page that is none of the cache has no copy
+    return e;
+}
+__device__ __forceinline__ void write_entries(const ForkParams& p, int i, const Entries& e, int page, bool kept, int rank, int there, const int32_t* list)
+{
+    int32_t* row = p.new_table + (int64_t)i * p.width;
+    if (e.part > 0 && (kept || page < 0))
+        row[e.full] = page;
+    const int copy = e.part > 0 && !kept && page >= 0 && rank < there ? list[rank] : -1;
+    for (int j = e.begin; j < e.end; ++j, ++rank)
+        row[j] = rank < there ? list[rank] : -1;
+    p.plan[i] = int4 { page, copy, e.part, 0 };
+}
+
+// All of it, for up to kSmallSeqs sequences (no more than the workgroup has threads) and 32 kSmallWords pages.
+__global__ __launch_bounds__(kForkThreads) void kv_fork_small_kernel(ForkParams p)
+{
+    __shared__ uint32_t used[kSmallWords];
+    __shared__ int32_t parent_of[kSmallSeqs], length_of[kSmallSeqs], page_of[kSmallSeqs], hashed[2 * kHash];
+    __shared__ int sums[kForkThreads / 64];
+    int32_t *pages = hashed, *first = hashed + kHash; // who is the first to go on in a page
+    const int tid = threadIdx.x, threads = blockDim.x, words = (p.n_pages + 31) / 32;
+    const bool mine = tid < p.n_seqs;
+    bool odd = false;
+    Fork f { -1, 0, 0 };
+    if (mine) {
+        f = fork_of(p, tid, odd);
+        parent_of[tid] = f.parent;
+        length_of[tid] = f.length;
+        page_of[tid] = -1;
+        p.new_lens[tid] = f.want;
+    }
+    for (int w = tid; w < words; w += threads)
+        used[w] = 0;
+    for (int w = tid; w < kHash; w += threads) {
+        pages[w] = -1;
+        first[w] = INT_MAX;
+    }
+    __syncthreads();
+    const int entries = p.n_seqs * p.width;
+    constexpr int W = 8; // loads of a thread that are on their way together
+    for (int e0 = tid; e0 < entries; e0 += W * threads) {
+        int at[W], seq[W], entry[W], filled[W];
+#pragma unroll
+        for (int z = 0; z < W; ++z) {
+            const int e = e0 + z * threads < entries ? e0 + z * threads : e0;
+            seq[z] = quotient(e, p.by_width);
+            entry[z] = e - seq[z] * p.width;
+            filled[z] = length_of[seq[z]] - entry[z] * (int)p.page_size.by; // rows from this entry's first on
+            at[z] = filled[z] > 0 ? p.table[(int64_t)parent_of[seq[z]] * p.width + entry[z]] : -1;
+        }
+#pragma unroll
+        for (int z = 0; z < W; ++z) {
+            if (z > 0 && e0 + z * threads >= entries)
+                break;
+            const int page = filled[z] > 0 ? checked_page(p, at[z], odd) : -1;
+            const bool full = filled[z] >= (int)p.page_size.by;
+            if (full && page >= 0)
+                atomicOr(used + (page >> 5), 1u << (page & 31));
+            if (filled[z] > 0 && !full)
+                page_of[seq[z]] = page;
+            p.new_table[(int64_t)seq[z] * p.width + entry[z]] = full ? page : -1;
+        }
+    }
+    __syncthreads();
+    const int page = mine ? page_of[tid] : -1;
+    int slot = 0;
+    if (page >= 0) {
+        slot = (int)((uint32_t)page * 2654435761u >> 16) & (kHash - 1);
+        for (;;) { // half of the places are free
+            const int was = atomicCAS(pages + slot, -1, page);
+            if (was == -1 || was == page)
+                break;
+            slot = (slot + 1) & (kHash - 1);
+        }
+        atomicMin(first + slot, tid);
+    }
+    __syncthreads();
+    // who keeps one: no full page of another's, and the first; the bits are set when all have looked
+    const bool kept = page >= 0 && first[slot] == tid && !(used[page >> 5] >> (page & 31) & 1);
+    const Entries e = entries_of(p, f, page, kept);
+    int needed;
+    const int rank = before_me(mine ? e.end - e.begin : 0, sums, needed);
+    if (kept)
+        atomicOr(used + (page >> 5), 1u << (page & 31));
+    __syncthreads();
+    // the free pages, by rank, into what the hash table had if they fit
+    int32_t* list = needed <= 2 * kHash ? hashed : p.list;
+    int ranked = 0;
+    for (int w0 = 0; w0 < words; w0 += threads) {
+        const int w = w0 + tid;
+        uint32_t zeros = w < words ? ~used[w] : 0;
+        if (w == words - 1 && p.n_pages % 32)
+            zeros &= (1u << (p.n_pages % 32)) - 1;
+        int total;
+        int r = ranked + before_me(__builtin_popcount(zeros), sums, total);
+        ranked += total;
+        for (; zeros && r < needed; zeros &= zeros - 1)
+            list[r++] = w * 32 + __builtin_ctz(zeros);
+    }
+    __syncthreads();
+    const int there = needed < ranked ? needed : ranked;
+    if (mine)
+        write_entries(p, tid, e, page, kept, rank, there, list);
+    if ((odd || needed > ranked) && p.error_flag)
+        *p.error_flag = 1;
+    if (tid == 0 && p.free_pages)
+        *p.free_pages = ranked - there;
+}
+
+// The same for tables of any size, through memory: the bits are cleared, the shared pages marked by as many workgroups as there are entries for, and one
+// workgroup does the rest.
+__global__ __launch_bounds__(256) void kv_fork_clear_kernel(ForkParams p)
+{
+    const int64_t w = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (w < (p.n_pages + 31) / 32)
+        p.used[w] = 0;
+}
+
+__global__ __launch_bounds__(256) void kv_fork_mark_kernel(ForkParams p)
+{
+    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (e >= (int64_t)p.n_seqs * p.width)
+        return;
+    const int i = quotient((int)e, p.by_width), j = (int)(e - (int64_t)i * p.width);
+    bool odd, bad = false;
+    const Fork f = fork_of(p, i, odd);
+    int at = -1;
+    if (j < quotient(f.length, p.page_size)) {
+        at = checked_page(p, p.table[(int64_t)f.parent * p.width + j], bad);
+        if (at >= 0)
+            atomicOr(p.used + (at >> 5), 1u << (at & 31));
+    }
+    p.new_table[e] = at;
+    if (bad && p.error_flag)
+        *p.error_flag = 1;
+}
+
+__global__ __launch_bounds__(kForkThreads) void kv_fork_rest_kernel(ForkParams p)
 {
     __shared__ int sums[kForkThreads / 64];
-    const int tid = threadIdx.x, words = (p.n_pages + 31) / 32, page = (int)p.page_size.by;
-    for (int w = tid; w < words; w += kForkThreads)
-        agent_store(reinterpret_cast<int32_t*>(p.used) + w, 0);
-    __syncthreads();
-    // shared pages
-    const int64_t entries = (int64_t)p.n_seqs * p.width;
+    const int tid = threadIdx.x, words = (p.n_pages + 31) / 32;
+    int32_t* bits = reinterpret_cast<int32_t*>(p.used);
     bool odd = false;
-    for (int64_t e = tid; e < entries; e += kForkThreads) {
-        const int i = quotient((int)e, p.by_width), j = (int)(e - (int64_t)i * p.width);
-        bool bad;
-        const Fork f = fork_of(p, i, bad);
-        int at = -1;
-        if (j < quotient(f.length, p.page_size)) {
-            at = p.table[(int64_t)f.parent * p.width + j];
-            if (at < 0 || at >= p.n_pages) {
-                at = -1;
-                odd = true;
-            } else {
-                atomicOr(p.used + (at >> 5), 1u << (at & 31));
-            }
-        }
-        p.new_table[e] = at;
-    }
-    // partly filled ones
     for (int i = tid; i < p.n_seqs; i += kForkThreads) {
         bool bad;
         const Fork f = fork_of(p, i, bad);
         odd = odd || bad;
         const int full = quotient(f.length, p.page_size);
         int at = -1;
-        if (f.length - full * page > 0) {
-            at = p.table[(int64_t)f.parent * p.width + full];
-            if (at < 0 || at >= p.n_pages) {
-                at = -1;
-                odd = true;
-            } else {
+        if (f.length > full * (int)p.page_size.by) {
+            at = checked_page(p, p.table[(int64_t)f.parent * p.width + full], odd);
+            if (at >= 0)
                 agent_store(p.owner + at, INT_MAX);
-            }
         }
         p.plan[i].x = at;
         p.new_lens[i] = f.want;
@@ -118,30 +248,21 @@ __global__ __launch_bounds__(kForkThreads) void kv_fork_kernel(ForkParams p)
         if (p.plan[i].x >= 0)
             atomicMin(p.owner + p.plan[i].x, i);
     __syncthreads();
-    // who keeps one: no full page of another's, and the first; their bits are set when all have looked
     for (int i = tid; i < p.n_seqs; i += kForkThreads) {
         const int at = p.plan[i].x;
-        const bool kept = at >= 0 && agent_load(p.owner + at) == i && !(agent_load(reinterpret_cast<int32_t*>(p.used) + (at >> 5)) >> (at & 31) & 1);
-        p.plan[i].w = kept;
+        p.plan[i].w = at >= 0 && agent_load(p.owner + at) == i && !(agent_load(bits + (at >> 5)) >> (at & 31) & 1);
     }
     __syncthreads();
-    for (int i = tid; i < p.n_seqs; i += kForkThreads)
-        if (p.plan[i].w)
-            atomicOr(p.used + (p.plan[i].x >> 5), 1u << (p.plan[i].x & 31));
-    __syncthreads();
-    // needs, in the order of the sequences
     int needed = 0;
     for (int i0 = 0; i0 < p.n_seqs; i0 += kForkThreads) {
         const int i = i0 + tid;
         int need = 0;
         if (i < p.n_seqs) {
             bool bad;
-            const Fork f = fork_of(p, i, bad);
-            const int full = quotient(f.length, p.page_size), part = f.length - full * page;
-            const int end = quotient(f.want, p.page_size) + (f.want % page != 0);
-            // a partly filled page that is none of the cache has no copy
-            const int begin = full + (part > 0 && (p.plan[i].w || p.plan[i].x < 0));
-            need = end - begin;
+            const Entries e = entries_of(p, fork_of(p, i, bad), p.plan[i].x, p.plan[i].w);
+            need = e.end - e.begin;
+            if (p.plan[i].w)
+                atomicOr(p.used + (p.plan[i].x >> 5), 1u << (p.plan[i].x & 31));
         }
         int total;
         const int front = before_me(need, sums, total);
@@ -149,42 +270,27 @@ __global__ __launch_bounds__(kForkThreads) void kv_fork_kernel(ForkParams p)
             p.plan[i].z = needed + front;
         needed += total;
     }
-    // the free pages, by rank
+    __syncthreads();
     int ranked = 0;
     for (int w0 = 0; w0 < words; w0 += kForkThreads) {
         const int w = w0 + tid;
-        uint32_t zeros = 0;
-        if (w < words) {
-            zeros = ~(uint32_t)agent_load(reinterpret_cast<int32_t*>(p.used) + w);
-            if (w == words - 1 && p.n_pages % 32)
-                zeros &= (1u << (p.n_pages % 32)) - 1;
-        }
+        uint32_t zeros = w < words ? ~(uint32_t)agent_load(bits + w) : 0;
+        if (w == words - 1 && p.n_pages % 32)
+            zeros &= (1u << (p.n_pages % 32)) - 1;
         int total;
-        int rank = ranked + before_me(__builtin_popcount(zeros), sums, total);
+        int r = ranked + before_me(__builtin_popcount(zeros), sums, total);
         ranked += total;
-        for (; zeros && rank < needed; zeros &= zeros - 1)
-            p.list[rank++] = w * 32 + __builtin_ctz(zeros);
+        for (; zeros && r < needed; zeros &= zeros - 1)
+            p.list[r++] = w * 32 + __builtin_ctz(zeros);
     }
     __syncthreads();
     const int there = needed < ranked ? needed : ranked;
-    odd = odd || needed > ranked;
     for (int i = tid; i < p.n_seqs; i += kForkThreads) {
         bool bad;
-        const Fork f = fork_of(p, i, bad);
-        const int full = quotient(f.length, p.page_size), part = f.length - full * page;
-        const int end = quotient(f.want, p.page_size) + (f.want % page != 0);
-        const int at = p.plan[i].x;
-        const bool kept = p.plan[i].w;
-        int32_t* row = p.new_table + (int64_t)i * p.width;
-        int rank = p.plan[i].z, j = full;
-        if (part > 0 && (kept || at < 0))
-            row[j++] = at;
-        const int copy = part > 0 && !kept && at >= 0 && rank < there ? p.list[rank] : -1;
-        for (; j < end; ++j, ++rank)
-            row[j] = rank < there ? p.list[rank] : -1;
-        p.plan[i] = int4 { at, copy, part, 0 };
+        const int4 plan = p.plan[i];
+        write_entries(p, i, entries_of(p, fork_of(p, i, bad), plan.x, plan.w), plan.x, plan.w, plan.z, there, p.list);
     }
-    if (odd && p.error_flag)
+    if ((odd || needed > ranked) && p.error_flag)
         *p.error_flag = 1;
     if (tid == 0 && p.free_pages)
         *p.free_pages = ranked - there;
@@ -282,7 +388,15 @@ static fdx_status fork_launch(const char* who, const fdx_kv_pages* c, size_t siz
         eight ? reinterpret_cast<char*>(eight->v_scale) : nullptr, k_row, v_row, c->page_size, eight ? eight->block : 0, c->kv_heads, wide };
     const int64_t parts = ((k_row > v_row ? k_row : v_row) * c->page_size + kCopyBytes - 1) / kCopyBytes;
     profile_begin();
-    hipLaunchKernelGGL(kv_fork_kernel, dim3(1), dim3(kForkThreads), 0, stream(), p);
+    const int64_t entries = (int64_t)c->n_seqs * c->table_width;
+    if (c->n_seqs <= kSmallSeqs && c->n_pages <= 32 * kSmallWords && entries <= kSmallEntries) {
+        const int threads = entries <= 2048 && c->n_seqs <= 256 ? 256 : kForkThreads; // barriers of four waves take less
+        hipLaunchKernelGGL(kv_fork_small_kernel, dim3(1), dim3(threads), 0, stream(), p);
+    } else {
+        hipLaunchKernelGGL(kv_fork_clear_kernel, dim3((unsigned)(((int64_t)c->n_pages + 31) / 32 + 255) / 256), dim3(256), 0, stream(), p);
+        hipLaunchKernelGGL(kv_fork_mark_kernel, dim3((unsigned)((entries + 255) / 256)), dim3(256), 0, stream(), p);
+        hipLaunchKernelGGL(kv_fork_rest_kernel, dim3(1), dim3(kForkThreads), 0, stream(), p);
+    }
     hipLaunchKernelGGL(kv_fork_copy_kernel, dim3((unsigned)c->n_seqs, (unsigned)(parts < 64 ? parts : 64)), dim3(kCopyThreads), 0, stream(), copy);
     profile_end("kv_fork", 0.0, 2.0 * table_bytes);
     FDX_LAUNCH_CHECK();
