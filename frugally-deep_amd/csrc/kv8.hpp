@@ -16,11 +16,12 @@ template <int KIND>
 __device__ __forceinline__ uint32_t to_codes(const float (&x)[4])
 {
     if constexpr (KIND == kI8) {
-        uint32_t r = 0;
+        // beside 1.5 * 2^23 the last bit is one: the sum is rounded to a whole number, ties to even, and its last byte is the code
+        uint32_t r[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            r |= ((uint32_t)(int)__builtin_amdgcn_fmed3f(__builtin_rintf(x[e]), -kMostI8, kMostI8) & 255u) << (8 * e);
-        return r;
+            r[e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_fmed3f(x[e], -kMostI8, kMostI8) + 12582912.f);
+        return __builtin_amdgcn_perm(__builtin_amdgcn_perm(r[3], r[2], 0x0c0c0400u), __builtin_amdgcn_perm(r[1], r[0], 0x0c0c0400u), 0x05040100u);
     } else {
         float y[4];
 #pragma unroll
@@ -84,6 +85,15 @@ __device__ __forceinline__ int wave_prefix(int v)
     v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, true); // lane 31 to lanes 32 ..
     return v;
 }
+// the largest of sixteen lanes' numbers, in all of them
+template <int CTRL>
+__device__ __forceinline__ uint32_t most_dpp(uint32_t v)
+{
+    const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true);
+    return o > v ? o : v;
+}
+__device__ __forceinline__ uint32_t row16_most(uint32_t v) { return most_dpp<0x140>(most_dpp<0x141>(most_dpp<0x4E>(most_dpp<0xB1>(v)))); }
+
 // where the scales of a cache are
 struct Scales8 {
     const float *k, *v;

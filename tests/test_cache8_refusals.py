@@ -84,8 +84,10 @@ def test_append(fdx):
     for change, text in ((dict(k=None), "null"), (dict(v=None), "null"), (dict(starts=None), "null"), (dict(ldk=127), "overlap"), (dict(ldv=0), "overlap"),
                          (dict(tokens=0), "tokens"), (dict(tokens=-4), "tokens"), (dict(tokens=(1 << 24) + 1), "tokens")):
         refused(fdx, append(fdx, ctypes.byref(pages8(fdx)), **change), INVALID, text)
-    c = pages8(fdx, kv_heads=1 << 16, dk=1, dv=1, block=1)
-    refused(fdx, append(fdx, ctypes.byref(c), tokens=1 << 20, ldk=1 << 16, ldv=1 << 16), INVALID, "too many")
+    c = pages8(fdx, kv_heads=1 << 20, dk=1, dv=1, block=1)
+    refused(fdx, append(fdx, ctypes.byref(c), tokens=1 << 20, ldk=1 << 20, ldv=1 << 20), INVALID, "too many")
+    c = pages8(fdx, n_pages=1, page_size=1 << 24, kv_heads=1, dk=64, block=1 << 24)
+    refused(fdx, append(fdx, ctypes.byref(c)), INVALID, "2^30 elements")
 
 
 def test_paged(fdx):

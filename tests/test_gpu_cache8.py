@@ -108,7 +108,8 @@ def same(cache, host):
 # ---------------------------------------------------------------- new tokens
 
 SHAPES = [(2, 64, 64, 16, 16), (3, 128, 128, 20, 5), (1, 80, 80, 64, 32), (2, 13, 7, 3, 3), (2, 96, 64, 8, 1), (1, 32, 128, 200, 40), (2, 61, 45, 12, 4),
-          (1, 300, 260, 6, 2), (12, 64, 64, 16, 16), (1, 4, 4, 128, 128), (1, 128, 128, 96, 96)]
+          (1, 300, 260, 6, 2), (12, 64, 64, 16, 16), (1, 4, 4, 128, 128), (1, 128, 128, 96, 96), (2, 128, 128, 64, 64), (1, 128, 64, 130, 65),
+          (3, 128, 128, 40, 1), (1, 8, 8, 70, 1), (2, 100, 36, 24, 12)]
 
 
 @pytest.mark.parametrize("kind", KINDS)
