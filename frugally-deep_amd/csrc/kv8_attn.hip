@@ -955,52 +955,60 @@ __global__ __launch_bounds__(256, 2) void paged8_mixed_kernel(RaggedParams p, Sc
     }
 }
 
-// Rows whose keys more than one share, or range, has: sum of 2^(m - M) l o over them, divided by that of 2^(m - M) l.  A wave takes four heads of a
-// row, for which it finds the row's sequence once; eight parts of each are on their way together.
-constexpr int kJoinHeads = 4;
-template <class Out, class Size>
-__device__ __forceinline__ void join_heads(const RaggedParams& p, int row, int head0, int parts, const Out& out, const Size& size)
+// Rows whose keys more than one share, or range, has: sum of 2^(m - M) l o over them, divided by that of 2^(m - M) l.  Eight parts of a head are on
+// their way together.  Where there are many rows a wave takes four heads of a row, for which it finds the row's sequence once; where there are few, the four
+// waves of a workgroup every fourth part of one head, and their sums meet.  The whole call in us,
+// a wave for four heads / a workgroup for each: 32 rows of 64 parts 82.9 / 55.9, of 32 parts 31.1 / 16.5, 192 rows of up to 4 25.8 / 21.5, 1536 of tiles 24.6 /
+// 25.8, 2048 of two or three 92.9 / 92.9, 4096 of tiles 35.7 / 41.8.
+template <int H>
+struct RowSums {
+    float top[H], l[H], o0[H], o1[H]; // of depths lane and 64 + lane
+};
+// parts first, first + step, ... of H heads
+template <int H, class Out, class Size>
+__device__ __forceinline__ void sum_parts(const RaggedParams& p, int first, int step, int parts, const Out& out, const Size& size, RowSums<H>& r)
 {
-    constexpr int H = kJoinHeads, W = 8;
-    const int lane = threadIdx.x & 63;
-    float top[H], m[H], l[H], o0[H], o1[H];
+    constexpr int W = 8;
+    const int lane = threadIdx.x & 63, mine = parts > first ? (parts - first + step - 1) / step : 0;
+    auto part = [&](int i) { return first + i * step; };
+    float m[H];
 #pragma unroll
     for (int h = 0; h < H; ++h) {
-        top[h] = -INFINITY;
-        l[h] = o0[h] = o1[h] = 0.f;
+        r.top[h] = -INFINITY;
+        r.l[h] = r.o0[h] = r.o1[h] = 0.f;
     }
-    for (int i0 = 0; i0 < parts; i0 += 64)
+    for (int i0 = 0; i0 < mine; i0 += 64)
 #pragma unroll
         for (int h = 0; h < H; ++h)
-            if (i0 + lane < parts)
-                top[h] = fmaxf(top[h], size(i0 + lane, h)[0]);
+            if (i0 + lane < mine)
+                r.top[h] = fmaxf(r.top[h], size(part(i0 + lane), h)[0]);
 #pragma unroll
     for (int h = 0; h < H; ++h) {
-        top[h] = wave_all<true>(top[h]);
-        m[h] = top[h] == -INFINITY ? 0.f : top[h];
+        r.top[h] = wave_all<true>(r.top[h]);
+        m[h] = r.top[h] == -INFINITY ? 0.f : r.top[h];
     }
     const int d0 = lane < p.dv ? lane : 0, d1 = 64 + lane < p.dv ? 64 + lane : 0;
-    for (int i0 = 0; i0 < parts; i0 += 64) {
+    for (int i0 = 0; i0 < mine; i0 += 64) {
         float w[H];
 #pragma unroll
         for (int h = 0; h < H; ++h) {
             w[h] = 0.f;
-            if (i0 + lane < parts) {
-                const float* at = size(i0 + lane, h);
+            if (i0 + lane < mine) {
+                const float* at = size(part(i0 + lane), h);
                 w[h] = at[1] * __builtin_amdgcn_exp2f(at[0] - m[h]);
             }
         }
 #pragma unroll
         for (int h = 0; h < H; ++h)
-            l[h] += wave_all<false>(w[h]);
-        const int count = parts - i0 < 64 ? parts - i0 : 64;
+            r.l[h] += wave_all<false>(w[h]);
+        const int count = mine - i0 < 64 ? mine - i0 : 64;
         for (int i = 0; i < count; i += W) {
             float x0[H][W], x1[H][W];
 #pragma unroll
             for (int z = 0; z < W; ++z)
 #pragma unroll
                 for (int h = 0; h < H; ++h) {
-                    const float* from = out(i0 + (i + z < count ? i + z : i), h);
+                    const float* from = out(part(i0 + (i + z < count ? i + z : i)), h);
                     x0[h][z] = from[d0];
                     x1[h][z] = from[d1];
                 }
@@ -1009,28 +1017,30 @@ __device__ __forceinline__ void join_heads(const RaggedParams& p, int row, int h
 #pragma unroll
                 for (int h = 0; h < H; ++h) {
                     const float wi = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w[h]), i + z < count ? i + z : i));
-                    o0[h] = fmaf(i + z < count ? wi : 0.f, x0[h][z], o0[h]);
-                    o1[h] = fmaf(i + z < count ? wi : 0.f, x1[h][z], o1[h]);
+                    r.o0[h] = fmaf(i + z < count ? wi : 0.f, x0[h][z], r.o0[h]);
+                    r.o1[h] = fmaf(i + z < count ? wi : 0.f, x1[h][z], r.o1[h]);
                 }
         }
     }
-#pragma unroll
-    for (int h = 0; h < H; ++h) {
-        if (head0 + h >= p.heads)
-            break;
-        float* to = p.out + (int64_t)row * p.ldo + (int64_t)(head0 + h) * p.dv;
-        if (lane < p.dv)
-            to[lane] = finish(o0[h], l[h], top[h] != -INFINITY);
-        if (64 + lane < p.dv)
-            to[64 + lane] = finish(o1[h], l[h], top[h] != -INFINITY);
-    }
+}
+__device__ __forceinline__ void store_row(const RaggedParams& p, int row, int head, float top, float l, float o0, float o1)
+{
+    const int lane = threadIdx.x & 63;
+    float* to = p.out + (int64_t)row * p.ldo + (int64_t)head * p.dv;
+    if (lane < p.dv)
+        to[lane] = finish(o0, l, top != -INFINITY);
+    if (64 + lane < p.dv)
+        to[64 + lane] = finish(o1, l, top != -INFINITY);
 }
 
+template <bool FEW>
 __global__ __launch_bounds__(256) void paged8_join_kernel(RaggedParams p, Few8 few)
 {
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const unsigned groups = (unsigned)(p.heads + kJoinHeads - 1) / kJoinHeads, item = blockIdx.x * 4 + wave;
-    const int row = (int)(item / groups), head0 = (int)(item % groups) * kJoinHeads;
+    constexpr int H = FEW ? 1 : 4;
+    __shared__ float met[FEW ? 4 : 1][4][64];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const unsigned groups = (unsigned)(p.heads + H - 1) / H, item = FEW ? blockIdx.x : blockIdx.x * 4 + wave;
+    const int row = (int)(item / groups), head0 = (int)(item % groups) * H;
     if (row >= p.tokens)
         return;
     const int index = find_row(SearchWave(), p.starts, p.n_seqs, p.tokens, row);
@@ -1041,26 +1051,52 @@ __global__ __launch_bounds__(256) void paged8_join_kernel(RaggedParams p, Few8 f
     if (token >= s.span.count)
         return;
     auto head_of = [&](int h) { return head0 + h < p.heads ? head0 + h : p.heads - 1; };
+    RowSums<H> r;
     if (!s.few) {
         const int visible = visible_keys(p, s, token);
         if (visible <= s.range)
             return;
         const int64_t first = (int64_t)row * p.heads; // part_row
-        join_heads(p, row, head0, (visible + s.range - 1) / s.range, [&](int i, int h) { return p.tile.out(i, first + head_of(h), p.dv); },
-            [&](int i, int h) { return p.tile.size(i, first + head_of(h), p.dv); });
-        return;
+        sum_parts<H>(p, FEW ? wave : 0, FEW ? 4 : 1, (visible + s.range - 1) / s.range, [&](int i, int h) { return p.tile.out(i, first + head_of(h), p.dv); },
+            [&](int i, int h) { return p.tile.size(i, first + head_of(h), p.dv); }, r);
+    } else {
+        bool cut;
+        const int units = few_sequence(p, few, index, cut).units;
+        const int share = share_of(few, units_before(p, few, p.n_seqs)), first = units_before(p, few, index);
+        const int from = first / share, parts = (first + units - 1) / share - from + 1;
+        if (parts == 1)
+            return;
+        auto id = [&](int i, int h) {
+            const int head = head_of(h), kv_head = quotient(head, p.by_group);
+            return few.row_of(from + i, kv_head, i > 0 ? 0 : 1, token * p.group + head - kv_head * p.group);
+        };
+        sum_parts<H>(p, FEW ? wave : 0, FEW ? 4 : 1, parts, [&](int i, int h) { return few.out(id(i, h), p.dv); },
+            [&](int i, int h) { return few.size(id(i, h), p.dv); }, r);
     }
-    bool cut;
-    const int units = few_sequence(p, few, index, cut).units;
-    const int share = share_of(few, units_before(p, few, p.n_seqs)), first = units_before(p, few, index);
-    const int from = first / share, parts = (first + units - 1) / share - from + 1;
-    if (parts == 1)
-        return;
-    auto id = [&](int i, int h) {
-        const int head = head_of(h), kv_head = quotient(head, p.by_group);
-        return few.row_of(from + i, kv_head, i > 0 ? 0 : 1, token * p.group + head - kv_head * p.group);
-    };
-    join_heads(p, row, head0, parts, [&](int i, int h) { return few.out(id(i, h), p.dv); }, [&](int i, int h) { return few.size(id(i, h), p.dv); });
+    if constexpr (FEW) {
+        met[wave][0][lane] = r.top[0];
+        met[wave][1][lane] = r.l[0];
+        met[wave][2][lane] = r.o0[0];
+        met[wave][3][lane] = r.o1[0];
+        __syncthreads();
+        if (wave > 0)
+            return;
+        const float top = fmaxf(fmaxf(met[0][0][lane], met[1][0][lane]), fmaxf(met[2][0][lane], met[3][0][lane])), m = top == -INFINITY ? 0.f : top;
+        float l = 0.f, o0 = 0.f, o1 = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float f = __builtin_amdgcn_exp2f(met[w][0][lane] - m);
+            l = fmaf(f, met[w][1][lane], l);
+            o0 = fmaf(f, met[w][2][lane], o0);
+            o1 = fmaf(f, met[w][3][lane], o1);
+        }
+        store_row(p, row, head0, top, l, o0, o1);
+    } else {
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+            if (head0 + h < p.heads)
+                store_row(p, row, head0 + h, r.top[h], r.l[h], r.o0[h], r.o1[h]);
+    }
 }
 
 // How a call is cut: paged_plan's tiles; sequences with few rows in as many shares as workgroups fit on the GPU, or as the longest lengths make.
@@ -1090,6 +1126,8 @@ static Plan8 plan8(int tokens, int max_new, int heads, const fdx_kv_pages* c)
     return r;
 }
 
+constexpr int64_t kFewJoins = 1024; // rows that are joined by a workgroup each
+
 template <int D, int KIND>
 static void paged8_launch(const RaggedParams& p, const Plan8& plan, const Scales8& scales)
 {
@@ -1117,8 +1155,11 @@ static void paged8_launch(const RaggedParams& p, const Plan8& plan, const Scales
         }
     }
     if (plan.few.shares > 1 || tile_y > 1) {
-        const int64_t items = (int64_t)p.tokens * ((p.heads + kJoinHeads - 1) / kJoinHeads);
-        hipLaunchKernelGGL(paged8_join_kernel, dim3((unsigned)((items + 3) / 4)), dim3(256), 0, stream(), p, plan.few);
+        const int64_t joined = (int64_t)p.tokens * p.heads, groups = (int64_t)p.tokens * ((p.heads + 3) / 4);
+        if (joined <= kFewJoins)
+            hipLaunchKernelGGL(paged8_join_kernel<true>, dim3((unsigned)joined), dim3(256), 0, stream(), p, plan.few);
+        else
+            hipLaunchKernelGGL(paged8_join_kernel<false>, dim3((unsigned)((groups + 3) / 4)), dim3(256), 0, stream(), p, plan.few);
     }
 }
 
