@@ -86,7 +86,7 @@ def test_append(fdx):
         refused(fdx, append(fdx, ctypes.byref(pages8(fdx)), **change), INVALID, text)
     c = pages8(fdx, kv_heads=1 << 20, dk=1, dv=1, block=1)
     refused(fdx, append(fdx, ctypes.byref(c), tokens=1 << 20, ldk=1 << 20, ldv=1 << 20), INVALID, "too many")
-    c = pages8(fdx, n_pages=1, page_size=1 << 24, kv_heads=1, dk=64, block=1 << 24)
+    c = pages8(fdx, n_pages=1, page_size=1 << 24, kv_heads=1, dk=65, dv=65, block=1 << 24)
     refused(fdx, append(fdx, ctypes.byref(c)), INVALID, "2^30 elements")
 
 
