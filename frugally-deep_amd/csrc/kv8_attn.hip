@@ -316,7 +316,7 @@ __device__ __forceinline__ void few8_segment(const RaggedParams& p, const Scales
         if (__any(most > w_most * 16.f || corr != 1.f)) {
             w_most = fmaxf(w_most, most_of_row(most));
             const Pow2 now = pow2_for<1>(exponent(w_most) + 5); // at most 2^10
-            const float by = corr * (now.up * power.down);
+            const float by = corr * now.up * power.down; // from the left: the powers' product alone may pass fp32's range
             power = now;
 #pragma unroll
             for (int e = 0; e < DL; ++e)
@@ -369,12 +369,13 @@ __device__ __forceinline__ void few8_segment(const RaggedParams& p, const Scales
         meet_m[wave][c] = some && m_run == -INFINITY ? -FLT_MAX : m_run;
         meet_l[wave][c] = l_run;
     }
+    const float part_of = l_run > 0.f ? 1.f / l_run : 0.f; // sums meet as means, which stay in fp32's range where the values are; NaN stays NaN below
     auto leave = [&](float* of) {
 #pragma unroll
         for (int e = 0; e < DL; ++e)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                of[c * (D + 4) + DL * (4 * g + i) + e] = oacc[e][i] * power.down;
+                of[c * (D + 4) + DL * (4 * g + i) + e] = oacc[e][i] * part_of * power.down;
     };
     if (wave == 0) // no pointer is chosen by a number: that would be a table in scratch memory
         leave(meet.of_0);
@@ -393,23 +394,31 @@ __device__ __forceinline__ void few8_segment(const RaggedParams& p, const Scales
             top = fmaxf(top, meet_m[w][row_at]);
         const float m = top == -INFINITY ? 0.f : top;
         float l = 0.f, o[DL];
+        for (int w = w_first; w <= w_last; ++w)
+            l += __builtin_amdgcn_exp2f(meet_m[w][row_at] - m) * meet_l[w][row_at];
 #pragma unroll
         for (int e = 0; e < DL; ++e)
             o[e] = 0.f;
+        const float none = top != -INFINITY && part < 0 ? NAN : 0.f; // as finish() has it
         auto add = [&](int w, const float* of) {
-            const float f = __builtin_amdgcn_exp2f(meet_m[w][row_at] - m);
-            l += f * meet_l[w][row_at];
+            const float f = __builtin_amdgcn_exp2f(meet_m[w][row_at] - m) * meet_l[w][row_at] / l;
 #pragma unroll
             for (int e = 0; e < DL; ++e)
-                o[e] += f * of[row_at * (D + 4) + d0 + e];
+                o[e] = fmaf(f, of[row_at * (D + 4) + d0 + e], o[e]);
         };
-        if (w_first == 0) {
-            add(0, meet.of_0);
-            add(1, meet.of_1);
-        }
-        if (w_last == 3) {
-            add(2, meet.of_2);
-            add(3, meet.of_3);
+        if (l != 0.f) {
+            if (w_first == 0) {
+                add(0, meet.of_0);
+                add(1, meet.of_1);
+            }
+            if (w_last == 3) {
+                add(2, meet.of_2);
+                add(3, meet.of_3);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < DL; ++e)
+                o[e] = none;
         }
         const int r = 16 * half + row_at;
         if (r >= count)
@@ -425,9 +434,6 @@ __device__ __forceinline__ void few8_segment(const RaggedParams& p, const Scales
                 size_at[1] = l;
             }
         }
-#pragma unroll
-        for (int e = 0; e < DL; ++e)
-            o[e] = finish(o[e], l, top != -INFINITY && part < 0);
 #pragma unroll
         for (int e = 0; e < DL; e += 4) {
             if (WIDE) {
@@ -690,7 +696,7 @@ __device__ __forceinline__ void tile8_body(const RaggedParams& p, const Scales8&
                 }
             }
         const Pow2 sq = pow2_for<1>(exponent(max_halves(top)) + 6); // at most 2^9: scores before to_log2 stay in fp32's range for keys up to 2^100
-        to_log2 = fmaxf(sq.down * (p.scale * kLog2e), 1.17549435e-38f); // above zero: -infinity stays what it is
+        to_log2 = sq.down * (p.scale * kLog2e); // above zero: -infinity stays what it is
 #pragma unroll
         for (int u = 0; u < STEPS; ++u)
             split2x8(x[u], sq.up, qh[u], ql[u]);
@@ -841,7 +847,7 @@ __device__ __forceinline__ void tile8_body(const RaggedParams& p, const Scales8&
             if (__any(most > w_most * 16.f || corr != 1.f)) {
                 w_most = fmaxf(w_most, most);
                 const Pow2 now = pow2_for<1>(exponent(w_most) + 5); // at most 2^10
-                const float by = corr * (now.up * power.down);
+                const float by = corr * now.up * power.down; // from the left: the powers' product alone may pass fp32's range
                 power = now;
 #pragma unroll
                 for (int d = 0; d < DB; ++d)
@@ -962,7 +968,7 @@ __global__ __launch_bounds__(256, 2) void paged8_mixed_kernel(RaggedParams p, Sc
 // 25.8, 2048 of two or three 92.9 / 92.9, 4096 of tiles 35.7 / 41.8.
 template <int H>
 struct RowSums {
-    float top[H], l[H], o0[H], o1[H]; // of depths lane and 64 + lane
+    float top[H], l[H], o0[H], o1[H]; // means of depths lane and 64 + lane
 };
 // parts first, first + step, ... of H heads
 template <int H, class Out, class Size>
@@ -988,19 +994,19 @@ __device__ __forceinline__ void sum_parts(const RaggedParams& p, int first, int 
         m[h] = r.top[h] == -INFINITY ? 0.f : r.top[h];
     }
     const int d0 = lane < p.dv ? lane : 0, d1 = 64 + lane < p.dv ? 64 + lane : 0;
-    for (int i0 = 0; i0 < mine; i0 += 64) {
-        float w[H];
-#pragma unroll
-        for (int h = 0; h < H; ++h) {
-            w[h] = 0.f;
-            if (i0 + lane < mine) {
-                const float* at = size(part(i0 + lane), h);
-                w[h] = at[1] * __builtin_amdgcn_exp2f(at[0] - m[h]);
-            }
-        }
+    auto weight = [&](int i, int h) {
+        const float* at = size(part(i), h);
+        return at[1] * __builtin_amdgcn_exp2f(at[0] - m[h]);
+    };
+    for (int i0 = 0; i0 < mine; i0 += 64)
 #pragma unroll
         for (int h = 0; h < H; ++h)
-            r.l[h] += wave_all<false>(w[h]);
+            r.l[h] += wave_all<false>(i0 + lane < mine ? weight(i0 + lane, h) : 0.f);
+    for (int i0 = 0; i0 < mine; i0 += 64) {
+        float w[H]; // parts of the whole: what they multiply may be near fp32's end
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+            w[h] = i0 + lane < mine && r.l[h] != 0.f ? weight(i0 + lane, h) / r.l[h] : 0.f;
         const int count = mine - i0 < 64 ? mine - i0 : 64;
         for (int i = 0; i < count; i += W) {
             float x0[H][W], x1[H][W];
@@ -1027,10 +1033,11 @@ __device__ __forceinline__ void store_row(const RaggedParams& p, int row, int he
 {
     const int lane = threadIdx.x & 63;
     float* to = p.out + (int64_t)row * p.ldo + (int64_t)head * p.dv;
+    const float none = top != -INFINITY ? NAN : 0.f; // as finish() has it
     if (lane < p.dv)
-        to[lane] = finish(o0, l, top != -INFINITY);
+        to[lane] = l == 0.f ? none : o0;
     if (64 + lane < p.dv)
-        to[64 + lane] = finish(o1, l, top != -INFINITY);
+        to[64 + lane] = l == 0.f ? none : o1;
 }
 
 template <bool FEW>
@@ -1082,13 +1089,16 @@ __global__ __launch_bounds__(256) void paged8_join_kernel(RaggedParams p, Few8 f
         if (wave > 0)
             return;
         const float top = fmaxf(fmaxf(met[0][0][lane], met[1][0][lane]), fmaxf(met[2][0][lane], met[3][0][lane])), m = top == -INFINITY ? 0.f : top;
-        float l = 0.f, o0 = 0.f, o1 = 0.f;
+        float l = 0.f, f[4], o0 = 0.f, o1 = 0.f;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            const float f = __builtin_amdgcn_exp2f(met[w][0][lane] - m);
-            l = fmaf(f, met[w][1][lane], l);
-            o0 = fmaf(f, met[w][2][lane], o0);
-            o1 = fmaf(f, met[w][3][lane], o1);
+            f[w] = __builtin_amdgcn_exp2f(met[w][0][lane] - m) * met[w][1][lane];
+            l += f[w];
+        }
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            o0 = fmaf(f[w] / l, met[w][2][lane], o0);
+            o1 = fmaf(f[w] / l, met[w][3][lane], o1);
         }
         store_row(p, row, head0, top, l, o0, o1);
     } else {

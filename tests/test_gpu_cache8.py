@@ -426,7 +426,7 @@ def test_paged_queries_of_nan(fdx, new, what):
 
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("new", [[1, 1], [3, 40], [140, 1]])
-@pytest.mark.parametrize("eq,ek,ev", [(60, -60, 0), (-60, 60, 0), (-100, 100, 0), (0, 0, 100), (0, 0, -100), (-40, -80, 5), (110, -110, 110)])
+@pytest.mark.parametrize("eq,ek,ev", [(60, -60, 0), (-60, 60, 0), (-100, 100, 0), (0, 0, 100), (0, 0, -100), (-40, -80, 5), (110, -110, 110), (0, 0, 119), (-110, 98, -118)])
 def test_paged_sizes_of_operands(fdx, new, eq, ek, ev, kind):
     """Operands far from one in size: the result scales."""
     def change(k, v):
@@ -504,6 +504,28 @@ def test_paged_scores_of_a_few_hundred(fdx, new):
         q[:, ::64] = 1
         # a score is one product, off by less than 2^-22 * 333 = 8e-5 where it is largest
         close(fdx.mha_paged(f.cache, q, [new], heads), f.reference(q, [new], heads), 8e-5)
+
+
+@pytest.mark.parametrize("new", [1, 12, 100])
+@pytest.mark.parametrize("up", [1, -1])
+def test_paged_jumps_of_scores_and_values(fdx, new, up):
+    """From one token to another scores rise by thousands and values shrink by 2^180, or the other way round: sums of the tokens that went before are
+    gone, and nothing passes fp32's range on the way."""
+    n, first = 300, 150
+
+    def jump(k, v):
+        k[:] = 0
+        k[:first, ::64] = -4000 * up
+        k[first:, ::64] = 4000 * up
+        v[:first] *= np.float32(2.0 ** (90 * up))
+        v[first:] *= np.float32(2.0 ** (-90 * up))
+    f, heads = Filled(fdx, [n], 2, 64, 64, 16, "i8", 2, change=jump), 4
+    q = np.zeros((new, heads * 64), np.float32)
+    q[:, ::64] = 3
+    want = f.reference(q, [new], heads)
+    # all scores that count are the same number: what is left are the errors of means of values
+    assert np.isfinite(want).all()
+    close(fdx.mha_paged(f.cache, q, [new], heads).astype(np.float64) * 2.0 ** (90 * up), want * 2.0 ** (90 * up))
 
 
 @pytest.mark.parametrize("new", [1, 12, 100])
