@@ -707,8 +707,10 @@ class PagedCache:
         self.lens = want.astype(np.int32)
 
     def release(self, seq):
-        self.free += [int(page) for page in self.table[seq] if page >= 0]
+        mine = [int(page) for page in self.table[seq] if page >= 0]
         self.table[seq], self.lens[seq] = -1, 0
+        held = set(self.table.ravel().tolist())   # sequences that kv_fork made of one share pages
+        self.free += [page for page in mine if page not in held]
 
     def pages(self):
         """The cache as the entry points take it (fdx_kv_pages, fdx_kv_pages8)."""
