@@ -76,6 +76,7 @@ struct Few8 {
     int rows;        // of a sequence and key head at most
     int unit;        // blocks that shares are counted in: one, or so many that there are fewer than 2^31
     int kv_heads;
+    int2* split;     // [sequence] the share that it begins in, how many it has
 
     __device__ __forceinline__ int64_t row_of(int share, int head, int slot, int row) const
     {
@@ -90,27 +91,15 @@ constexpr int kLeastShare = 8; // blocks: two turns of each wave
 struct FewSequence {
     int first, count, keys, ahead, units;
 };
-__device__ __forceinline__ FewSequence few_sequence(const RaggedParams& p, const Few8& few, int i, bool& cut)
+__device__ __forceinline__ FewSequence few_sequence(const RaggedParams& p, const Few8& few, int i)
 {
-    cut = false;
     if (i >= p.n_seqs)
         return { 0, 0, 0, 0, 0 };
     const Sequence s = sequence_of<kPagedF32>(p, i, packed_span(p.starts, i, p.tokens));
-    cut = s.cut;
     if (s.span.count == 0 || !s.few)
         return { 0, 0, 0, 0, 0 };
     const int blocks = (s.keys + 31) / 32;
     return { s.span.first, s.span.count, s.keys, s.ahead, blocks > 0 ? (blocks - 1) / few.unit + 1 : 1 };
-}
-// units of the sequences in front of `before`
-__device__ __forceinline__ int units_before(const RaggedParams& p, const Few8& few, int before)
-{
-    const int lane = threadIdx.x & 63;
-    int sum = 0;
-    bool cut;
-    for (int i = lane; i < before; i += 64)
-        sum += few_sequence(p, few, i, cut).units;
-    return __builtin_amdgcn_readlane(wave_prefix(sum), 63);
 }
 __device__ __forceinline__ int share_of(const Few8& few, int all)
 {
@@ -455,25 +444,44 @@ __device__ __forceinline__ void few8_body(const RaggedParams& p, const Scales8& 
     const int kv_head = wg % p.kv_heads, mine = wg / p.kv_heads;
     if (p.error_flag && wg == 0)
         for (int i = threadIdx.x; i < p.n_seqs; i += 256)
-            raise_flag(p, !packed_start_ok(p.starts, i, p.tokens));
-    int at = 0, end = 0, front = 0; // units; those in front of sequences i0 ..
-    for (int i0 = 0; i0 < p.n_seqs; i0 += 64) {
+            raise_flag(p, !packed_start_ok(p.starts, i, p.tokens) || sequence_of<kPagedF32>(p, i, packed_span(p.starts, i, p.tokens)).cut);
+    int at = 0, end = 0, share = 1, from = 0, front = 0; // units; those in front of sequences i0 ..
+    auto deal = [&](int all) {
+        share = share_of(few, all);
+        if ((int64_t)mine * share >= all)
+            return false;
+        at = mine * share;
+        end = all - at < share ? all : at + share;
+        return true;
+    };
+    if (p.n_seqs > 64) { // 64 runs of sequences, sixteen a wave: where the share begins among them
+        const int lane = threadIdx.x & 63, length = (p.n_seqs / 64 + 64) & ~63;
+        for (int j = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); j < 64; j += 4) {
+            int sum = 0;
+            for (int64_t i = (int64_t)j * length; i < (int64_t)(j + 1) * length && i < p.n_seqs; i += 64)
+                sum += few_sequence(p, few, (int)i + lane).units;
+            sum = wave_prefix(sum);
+            if (lane == 63)
+                meet.seqs[0][j] = sum;
+        }
+        __syncthreads();
+        const int up_to = wave_prefix(meet.seqs[0][lane]);
+        __syncthreads();
+        if (!deal(__builtin_amdgcn_readlane(up_to, 63)))
+            return;
+        const int run = __builtin_popcountll(__ballot(up_to <= at));
+        front = run > 0 ? __builtin_amdgcn_readlane(up_to, run - 1) : 0;
+        from = run * length;
+    }
+    for (int i0 = from; i0 < p.n_seqs; i0 += 64) {
         int tid = threadIdx.x;
         asm volatile("" : "+v"(tid));
         const int lane = tid & 63;
-        bool cut;
-        const FewSequence of_lane = few_sequence(p, few, i0 + lane, cut);
+        const FewSequence of_lane = few_sequence(p, few, i0 + lane);
         const int up_to = front + wave_prefix(of_lane.units), before = front;
         front = __builtin_amdgcn_readlane(up_to, 63);
-        if (wg == 0)
-            raise_flag(p, cut);
-        if (i0 == 0) {
-            const int all = p.n_seqs <= 64 ? front : units_before(p, few, p.n_seqs), share = share_of(few, all);
-            if ((int64_t)mine * share >= all)
-                return;
-            at = mine * share;
-            end = all - at < share ? all : at + share;
-        }
+        if (p.n_seqs <= 64 && !deal(front))
+            return;
         if (at >= front)
             continue;
         if (tid < 64) { // no register keeps it through the segments
@@ -492,6 +500,8 @@ __device__ __forceinline__ void few8_body(const RaggedParams& p, const Scales8& 
             const int first = of > 0 ? number(0, of - 1) : before, last = number(0, of);
             const Sequence s { { number(1, of), number(2, of) }, number(3, of), number(4, of), i0 + of, true, INT_MAX, false };
             const int stop = end < last ? end : last;
+            if (few.split && kv_head == 0 && at == first && me == 0)
+                few.split[i0 + of] = int2 { mine, (last - 1) / share - mine + 1 };
             few8_segment<D, KIND, WIDE>(p, scales, few, meet, s, kv_head, (at - first) * few.unit, (stop - first) * few.unit, mine,
                 at == first && stop == last ? -1 : (at > first ? 0 : 1));
             at = stop;
@@ -696,7 +706,7 @@ __device__ __forceinline__ void tile8_body(const RaggedParams& p, const Scales8&
                 }
             }
         const Pow2 sq = pow2_for<1>(exponent(max_halves(top)) + 6); // at most 2^9: scores before to_log2 stay in fp32's range for keys up to 2^100
-        to_log2 = sq.down * (p.scale * kLog2e); // above zero: -infinity stays what it is
+        to_log2 = sq.down * (p.scale * kLog2e); // 2^-129 or more: -infinity stays what it is
 #pragma unroll
         for (int u = 0; u < STEPS; ++u)
             split2x8(x[u], sq.up, qh[u], ql[u]);
@@ -1067,10 +1077,8 @@ __global__ __launch_bounds__(256) void paged8_join_kernel(RaggedParams p, Few8 f
         sum_parts<H>(p, FEW ? wave : 0, FEW ? 4 : 1, (visible + s.range - 1) / s.range, [&](int i, int h) { return p.tile.out(i, first + head_of(h), p.dv); },
             [&](int i, int h) { return p.tile.size(i, first + head_of(h), p.dv); }, r);
     } else {
-        bool cut;
-        const int units = few_sequence(p, few, index, cut).units;
-        const int share = share_of(few, units_before(p, few, p.n_seqs)), first = units_before(p, few, index);
-        const int from = first / share, parts = (first + units - 1) / share - from + 1;
+        const int2 split = few.split[index];
+        const int from = split.x, parts = split.y;
         if (parts == 1)
             return;
         auto id = [&](int i, int h) {
@@ -1114,7 +1122,7 @@ struct Plan8 {
     RaggedPlan tiles;
     Few8 few;
     unsigned few_wgs;
-    size_t few_floats;
+    size_t split_at, few_floats; // where Few8::split is, what all has, in floats
 };
 static Plan8 plan8(int tokens, int max_new, int heads, const fdx_kv_pages* c)
 {
@@ -1130,8 +1138,10 @@ static Plan8 plan8(int tokens, int max_new, int heads, const fdx_kv_pages* c)
             r.few.unit *= 2;
         r.few.kv_heads = c->kv_heads;
         r.few_wgs = (unsigned)(r.few.shares * c->kv_heads);
-        if (r.few.shares > 1)
-            r.few_floats = ((size_t)r.few_wgs * 2 * r.few.rows * (2 + (size_t)c->dv) + 3) & ~(size_t)3;
+        if (r.few.shares > 1) {
+            r.split_at = ((size_t)r.few_wgs * 2 * r.few.rows * (2 + (size_t)c->dv) + 3) & ~(size_t)3;
+            r.few_floats = r.split_at + (((size_t)c->n_seqs * 2 + 3) & ~(size_t)3);
+        }
     }
     return r;
 }
@@ -1201,6 +1211,7 @@ extern "C" fdx_status fdx_mha_paged8_f32(const float* q, int64_t ldq, const int3
         return st;
     Plan8 plan = plan8(tokens, max_new, heads, &c);
     plan.few.parts = static_cast<float*>(scratch_dev);
+    plan.few.split = plan.few.shares > 1 ? reinterpret_cast<int2*>(plan.few.parts + plan.split_at) : nullptr;
     p.few_rows = plan.tiles.few_rows;
     p.few = { nullptr, 0, 1, INT_MAX, 0, 0 }; // no ranges: sequences with few rows are cut in shares
     p.tile = { plan.few.parts + plan.few_floats, plan.tiles.tile_part, plan.tiles.tile_ranges, plan.tiles.tile_keys, plan.tiles.tile_whole, 0 };

@@ -361,7 +361,20 @@ def test_lengths_of_sequences_without_new_tokens(fdx, heads):
         close(out.to_host((2, heads * 64)), f.reference(q, [1, 0, 1], heads))
 
 
-@pytest.mark.parametrize("n_seqs", [65, 200])
+@pytest.mark.parametrize("at", [0, 63, 64, 130, 299])
+def test_lengths_out_of_range_among_many(fdx, at):
+    n, heads = 300, 4
+    f = Filled(fdx, [5] * n, 2, 32, 32, 16, "i8", 8)
+    q = np.random.default_rng(1).standard_normal((n, heads * 32)).astype(np.float32)
+    dq, out = fdx.DevBuf.from_host(q), fdx.DevBuf.from_host(np.zeros((n, heads * 32), np.float32))
+    for bad, new in ((-1, 1), (6, 1), (5, 1), (6, 0)):
+        lens = np.full(n, 5)
+        lens[at] = bad
+        starts = np.minimum(np.arange(n + 1), n) if new else np.arange(n + 1) - (np.arange(n + 1) > at)
+        assert call_paged(fdx, f.cache, dq.ptr, heads * 32, starts, n, 1, heads, out.ptr, heads * 32, lens=lens) == (bad != 5), (bad, new)
+
+
+@pytest.mark.parametrize("n_seqs", [65, 200, 1300, 4200])
 @pytest.mark.parametrize("heads,kv", [(4, 2), (6, 6)])
 def test_shares_over_many_sequences(fdx, n_seqs, heads, kv):
     """Long sequences beside short ones and ones without tokens, more than a wave has lanes: every key counts once, whoever has it."""
