@@ -285,6 +285,19 @@ extern "C" fdx_status fdx_beam_select_f32(const float* logits, int64_t ld, int n
     FDX_REQUIRE(end_id < vocab && (end_id >= 0 || (!done && !new_done)), "beam_select: end_id is no token");
     FDX_REQUIRE(scratch_dev && (reinterpret_cast<uintptr_t>(scratch_dev) & 15) == 0, "beam_select: scratch missing or not 16-byte aligned");
     const int64_t rows = (int64_t)n_seqs * beams;
+    const size_t in_bytes = 4 * (size_t)rows, out_bytes = 4 * (size_t)n_seqs * keep, x_bytes = 4 * ((size_t)(rows - 1) * ld + vocab);
+    const void* const outs[] = { new_scores, new_done, parents, tokens }; // the first two may take the place of what a sequence's workgroup has read
+    const void* const ins[] = { scores, done };
+    for (int i = 0; i < 4; ++i) {
+        if (!outs[i])
+            continue;
+        bool meets = overlap(outs[i], out_bytes, logits, x_bytes);
+        for (int j = 0; j < 2; ++j)
+            meets = meets || (ins[j] && !(i == j && outs[i] == ins[j] && keep == beams) && overlap(outs[i], out_bytes, ins[j], in_bytes));
+        for (int j = i + 1; j < 4; ++j)
+            meets = meets || overlap(outs[i], out_bytes, outs[j], out_bytes);
+        FDX_REQUIRE(!meets, "beam_select: results overlap an input or each other");
+    }
     const BeamPlan plan = beam_plan(rows, beams, vocab, keep);
     int width = 1;
     while (width < plan.parts)

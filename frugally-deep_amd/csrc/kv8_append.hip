@@ -240,7 +240,7 @@ extern "C" fdx_status fdx_kv8_append_f32(const float* k, int64_t ldk, const floa
     const int strip = (int)blocks * cache->block;
     FDX_REQUIRE((int64_t)cache->block * (k_chunks > v_chunks ? k_chunks : v_chunks) < ((int64_t)1 << 30), "kv8_append: blocks of more than 2^30 elements of a head");
     const int64_t items = ((int64_t)tokens / strip + 2 * (int64_t)c.n_seqs + 1) * 2 * c.kv_heads;
-    FDX_REQUIRE(items < ((int64_t)1 << 32), "kv8_append: blocks * key heads too many for one launch");
+    FDX_REQUIRE(items < ((int64_t)1 << 25), "kv8_append: strips * key heads too many for one launch");
     const Append8Params p { k, v, ldk, ldv, starts, tokens, c, cache->k_scale, cache->v_scale, cache->block, strip, wide, make_divisor(c.page_size),
         make_divisor(cache->block), make_divisor(strip), make_divisor(k_chunks), make_divisor(v_chunks), make_divisor(2 * c.kv_heads), error_flag_dev };
     const dim3 grid((unsigned)((items + 3) / 4));

@@ -133,7 +133,8 @@ __global__ __launch_bounds__(kForkThreads) void kv_fork_small_kernel(ForkParams 
             const int e = e0 + z * threads < entries ? e0 + z * threads : e0;
             seq[z] = quotient(e, p.by_width);
             entry[z] = e - seq[z] * p.width;
-            filled[z] = length_of[seq[z]] - entry[z] * (int)p.page_size.by; // rows from this entry's first on
+            const int64_t left = length_of[seq[z]] - (int64_t)entry[z] * (int)p.page_size.by; // tables may be far wider than max_len
+            filled[z] = left > 0 ? (int)left : 0; // rows from this entry's first on
             at[z] = filled[z] > 0 ? p.table[(int64_t)parent_of[seq[z]] * p.width + entry[z]] : -1;
         }
 #pragma unroll
@@ -354,16 +355,11 @@ static ForkScratch fork_scratch(const fdx_kv_pages* c)
     return r;
 }
 
-static bool overlap(const void* a, size_t na, const void* b, size_t nb)
-{
-    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-    return x < y + nb && y < x + na;
-}
-
 static fdx_status fork_launch(const char* who, const fdx_kv_pages* c, size_t size, const fdx_kv_pages8* eight, const int32_t* parents,
     const int32_t* grow, int32_t* new_table, int32_t* new_lens, int32_t* free_pages, void* scratch_dev, int* error_flag_dev)
 {
     FDX_REQUIRE(parents && new_table && new_lens, "%s: null pointer", who);
+    FDX_REQUIRE(c->n_seqs <= (1 << 23), "%s: more than 2^23 sequences", who);
     FDX_REQUIRE((int64_t)c->n_seqs * c->table_width < ((int64_t)1 << 31), "%s: a table of more than 2^31 entries", who);
     FDX_REQUIRE(scratch_dev && (reinterpret_cast<uintptr_t>(scratch_dev) & 15) == 0, "%s: scratch missing or not 16-byte aligned", who);
     const size_t table_bytes = (size_t)c->n_seqs * c->table_width * 4, lens_bytes = (size_t)c->n_seqs * 4;

@@ -1,6 +1,7 @@
 // Where the rows of ragged batches lie: spans of packed rows, tiles of them, places in a paged cache.  Plain integer
 // arithmetic on numbers that device memory holds and nobody has checked: whatever they are, what comes out is in range.
 #pragma once
+#include <cstddef>
 #include <cstdint>
 
 #if defined(__HIPCC__)
@@ -25,6 +26,13 @@ inline Divisor make_divisor(int by)
     return { (uint32_t)by, (uint32_t)(((uint64_t)1 << (31 + l)) / (uint32_t)by + 1), 31 + l };
 }
 FDX_HD int quotient(int n, const Divisor& d) { return (int)((uint64_t)(uint32_t)n * d.mul >> d.shift); }
+
+// whether na bytes at a and nb bytes at b have one in common
+inline bool overlap(const void* a, size_t na, const void* b, size_t nb)
+{
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y + nb && y < x + na;
+}
 
 struct Span {
     int first, count;

@@ -443,7 +443,8 @@ typedef struct fdx_kv_pages8 {
  * from s0, codes c of earlier tokens become c * (s0 / s), rounded the same way.  All in fp32.  So a value is off by at most half a step of
  * its block's largest value, and by half a step more for every time that the scale has grown since.  An infinity or a NaN makes its
  * block's scale NaN, and its codes 0: the block's keys (values) of that head are NaN until a call starts the block anew.
- * No two sequences of one call may write to the same block (fdx_kv8_fork gives each its own).  error_flag_dev as there.
+ * No two sequences of one call may write to the same block (fdx_kv8_fork gives each its own).  error_flag_dev as there.  A wave takes up to 64
+ * blocks of a sequence and head: (tokens / (positions of those) + 2 n_seqs + 1) * 2 * kv_heads < 2^25.
  */
 fdx_status fdx_kv8_append_f32(const float* k, int64_t ldk, const float* v, int64_t ldv, const int32_t* starts, int tokens,
     const fdx_kv_pages8* cache, int* error_flag_dev);
@@ -451,7 +452,7 @@ fdx_status fdx_kv8_append_f32(const float* k, int64_t ldk, const float* v, int64
  * fdx_mha_paged_f32 for such a cache: the same sums over code * scale, the same arguments, refusals and error_flag_dev.
  * Precision: fp32 sums, exact codes; queries are held as two fp16 values: 22 bits of an element not below 2^-11 of the largest of its
  * row and head, 2^-34 of that largest below.  So is a row's probability times the scale of the value, of the largest such product.  Keys up to
- * 2^100.  A row that sees a block whose scale is NaN, or whose query holds an infinity or a NaN, gets NaN;
+ * 2^100, scores in fp32's range; codes as the call above writes them (no -128, no NaN of FDX_KV_E4M3).  A row that sees a block whose scale is NaN, or whose query holds an infinity or a NaN, gets NaN;
  * rows that do not see it keep their sums.
  */
 size_t fdx_mha_paged8_scratch_bytes(int tokens, int max_new, int heads, const fdx_kv_pages8* cache);
@@ -471,7 +472,8 @@ fdx_status fdx_mha_paged8_f32(const float* q, int64_t ldq, const int32_t* starts
  * new_table and new_lens take their place afterwards; they overlap no input.
  * A parent of n_seqs or more, a length out of 0 .. max_len, a negative grow or one beyond max_len (both count as 0), a kept page number that
  * is none of the cache, and a lack of free pages (-1 in new_table) set error_flag_dev (may be NULL) to 1 on the device.
- * scratch_dev: fdx_kv_fork_scratch_bytes bytes, 16-byte aligned, as for fdx_mha_packed_f32.  n_seqs * table_width < 2^31.
+ * scratch_dev: fdx_kv_fork_scratch_bytes bytes, 16-byte aligned, as for fdx_mha_packed_f32.  n_seqs * table_width < 2^31,
+ * n_seqs <= 2^23.
  */
 size_t fdx_kv_fork_scratch_bytes(const fdx_kv_pages* cache);
 fdx_status fdx_kv_fork(const fdx_kv_pages* cache, const int32_t* parents, const int32_t* grow, int32_t* new_table, int32_t* new_lens,
@@ -493,7 +495,8 @@ fdx_status fdx_kv8_fork(const fdx_kv_pages8* cache, const int32_t* parents, cons
  * end_id: 0 .. vocab - 1, or negative if no token ends a beam (done and new_done are NULL then).
  * Logits and scores of -infinity are no continuations; places that are left over get row -1, token -1, score -infinity, done 0.  Rows that
  * hold a NaN or +infinity, and scores that are one, give no continuations either, and set error_flag_dev (may be NULL) to 1 on the device.
- * 1 <= keep <= 32, keep <= beams * vocab, beams <= 32.  scratch_dev: fdx_beam_select_scratch_bytes bytes, as for fdx_mha_packed_f32.
+ * Results overlap no input and not each other; but where keep is beams, new_scores may be scores and new_done may be done.
+ * 1 <= keep <= 32, keep <= beams * vocab, beams <= 32, n_seqs * beams <= 2^23.  scratch_dev: fdx_beam_select_scratch_bytes bytes, as for fdx_mha_packed_f32.
  */
 size_t fdx_beam_select_scratch_bytes(int n_seqs, int beams, int vocab, int keep);
 fdx_status fdx_beam_select_f32(const float* logits, int64_t ld, int n_seqs, int beams, int vocab, const float* scores, const int32_t* done,

@@ -84,8 +84,9 @@ def test_append(fdx):
     for change, text in ((dict(k=None), "null"), (dict(v=None), "null"), (dict(starts=None), "null"), (dict(ldk=127), "overlap"), (dict(ldv=0), "overlap"),
                          (dict(tokens=0), "tokens"), (dict(tokens=-4), "tokens"), (dict(tokens=(1 << 24) + 1), "tokens")):
         refused(fdx, append(fdx, ctypes.byref(pages8(fdx)), **change), INVALID, text)
-    c = pages8(fdx, kv_heads=1 << 20, dk=1, dv=1, block=1)
-    refused(fdx, append(fdx, ctypes.byref(c), tokens=1 << 20, ldk=1 << 20, ldv=1 << 20), INVALID, "too many")
+    for change in (dict(kv_heads=1 << 20, dk=1, dv=1, block=1), dict(n_seqs=1 << 23)):
+        c = pages8(fdx, **change)
+        refused(fdx, append(fdx, ctypes.byref(c), tokens=1 << 20, ldk=1 << 20, ldv=1 << 20), INVALID, "too many")
     c = pages8(fdx, n_pages=1, page_size=1 << 24, kv_heads=1, dk=65, dv=65, block=1 << 24)
     refused(fdx, append(fdx, ctypes.byref(c)), INVALID, "2^30 elements")
 
@@ -115,6 +116,8 @@ def test_fork(fdx):
         refused(fdx, fork8(fdx, ctypes.byref(c), **change), INVALID, text)
     c = pages8(fdx, n_seqs=1 << 20, table_width=1 << 11)
     refused(fdx, fork8(fdx, ctypes.byref(c)), INVALID, "2^31")
+    c = pages8(fdx, n_seqs=(1 << 23) + 1)
+    refused(fdx, fork8(fdx, ctypes.byref(c)), INVALID, "2^23")
     assert fdx.lib.fdx_kv_fork_scratch_bytes(None) == 0 and fdx.lib.fdx_kv8_fork_scratch_bytes(None) == 0
     assert fdx.lib.fdx_kv8_fork_scratch_bytes(ctypes.byref(pages8(fdx, n_pages=0))) == 0
 
@@ -129,6 +132,15 @@ def test_beams(fdx):
                          (dict(end_id=100), "end_id"), (dict(end_id=-1), "end_id"), (dict(end_id=-1, done=None), "end_id"), (dict(end_id=-1, new_done=None), "end_id"),
                          (dict(scratch=None), "scratch"), (dict(scratch=ctypes.c_void_p((1 << 20) + 4)), "scratch")):
         refused(fdx, call(**change), INVALID, text)
+    at = [ctypes.c_void_p((i + 2) << 20) for i in range(7)]
+    apart = dict(zip(("x", "scores", "done", "parents", "tokens", "new_scores", "new_done"), at))
+    outs = ("parents", "tokens", "new_scores", "new_done")
+    same = [dict(apart, **{a: apart[b]}) for a in outs for b in apart if a != b]   # keep is not beams
+    same += [dict(apart, keep=4, **{a: apart[b]}) for a in outs for b in apart if a != b and (a, b) not in (("new_scores", "scores"), ("new_done", "done"))]
+    near = [dict(apart, new_scores=ctypes.c_void_p(apart["scores"].value + by), keep=4) for by in (-44, -4, 4, 44)]
+    near += [dict(apart, new_done=ctypes.c_void_p(apart["x"].value + 4 * (11 * 100 + 99))), dict(apart, tokens=ctypes.c_void_p(apart["x"].value - 92))]
+    for change in same + near:
+        refused(fdx, call(**change), INVALID, "overlap")
     for args in ((0, 4, 100, 8), (3, 0, 100, 8), (3, 4, 0, 8), (3, 4, 100, 0), (-1, 4, 100, 8)):
         assert fdx.lib.fdx_beam_select_scratch_bytes(*args) == 0
 
@@ -162,6 +174,19 @@ def test_python_calls(fdx, monkeypatch):
         fdx.beam_select(x, np.zeros((2, 3)), 3, np.zeros((2, 3)))
     got = fdx.beam_select(np.zeros((0, 3, 10)), np.zeros((0, 3)), 4)
     assert sorted(got) == ["parents", "scores", "tokens"] and got["scores"].shape == (0, 4)
+
+
+def test_release_of_shared_pages(fdx, monkeypatch):
+    """A page is free when no sequence has it."""
+    monkeypatch.setattr(fdx, "DevBuf", HostBuf)
+    c = fdx.PagedCache(9, 4, 2, 8, 6, 3, 20, "e4m3", 2)
+    c.table[0, :2], c.table[1, :2], c.table[2, :1] = [5, 1], [5, 7], [3]   # 0 and 1 have page 5 in common, as kv_fork leaves them
+    c.lens[:] = [7, 6, 2]
+    c.free = [8, 6, 4, 2, 0]
+    c.release(1)
+    assert c.free == [8, 6, 4, 2, 0, 7] and c.lens.tolist() == [7, 0, 2] and (c.table[1] == -1).all()
+    c.release(0)
+    assert c.free == [8, 6, 4, 2, 0, 7, 5, 1]
 
 
 def test_fork_that_fails_leaves_the_cache(fdx, monkeypatch):

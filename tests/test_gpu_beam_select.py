@@ -205,6 +205,24 @@ def test_strides_and_alignment(fdx, shift, pad):
     assert (new.to_host((n * keep + 3,))[-3:] == 5).all() and (scratch.to_host((need + 16,), np.uint8)[need:] == 0xff).all()
 
 
+@pytest.mark.parametrize("n,beams,vocab", [(3, 4, 5000), (300, 7, 300), (2, 32, 20000)])
+def test_results_in_the_place_of_scores(fdx, n, beams, vocab):
+    """Where as many are kept as there were, the new scores and ends may take the old ones' place."""
+    import ctypes
+    r = np.random.default_rng(n)
+    done = (r.random((n, beams)) < 0.3).astype(np.int32)
+    x, scores = r.standard_normal((n, beams, vocab)).astype(np.float32), -r.uniform(0, 3, (n, beams)).astype(np.float32)
+    want = fdx.beam_select(x, scores, beams, done, 11)
+    dx, ds, dd = fdx.DevBuf.from_host(x), fdx.DevBuf.from_host(scores), fdx.DevBuf.from_host(done, np.int32)
+    out = [fdx.DevBuf(4 * n * beams) for _ in range(2)]
+    scratch = fdx.DevBuf(fdx.lib.fdx_beam_select_scratch_bytes(n, beams, vocab, beams))
+    fdx.check(fdx.lib.fdx_beam_select_f32(dx.ptr, ctypes.c_int64(vocab), n, beams, vocab, ds.ptr, dd.ptr, 11, beams, out[0].ptr, out[1].ptr, ds.ptr, dd.ptr,
+                                          scratch.ptr, None))
+    fdx.sync()
+    assert np.array_equal(ds.to_host((n, beams)), want["scores"]) and np.array_equal(dd.to_host((n, beams), np.int32), want["done"])
+    assert np.array_equal(out[0].to_host((n, beams), np.int32), want["parents"]) and np.array_equal(out[1].to_host((n, beams), np.int32), want["tokens"])
+
+
 def test_runs_are_equal(fdx):
     r = np.random.default_rng(13)
     x, scores = r.standard_normal((16, 4, 50257)).astype(np.float32), -r.uniform(0, 3, (16, 4)).astype(np.float32)

@@ -208,6 +208,34 @@ def test_fork_sizes(fdx, n_pages, n, width):
         table, lens = p.step(table.astype(np.int32), lens, r.integers(-1, n, n).astype(np.int32), np.ones(n, np.int32), width * page)
 
 
+def test_fork_of_wide_tables(fdx):
+    """Entries of the table whose positions would be beyond 32 bits: nobody has a page there."""
+    page, width = 1 << 20, 4100
+    table = np.full((3, width), -1)
+    table[0, 0], table[1, 0], table[2, 0] = 1, 3, 4
+    for more in (4095, 4096, 4097):
+        table[:, more] = 2   # what it holds there is nothing to anyone
+    for n in (1, 3):
+        p = Pages(fdx, "i8", 6, page, 1, 1, 1, 1 << 10)
+        p.step(table[:n], np.array([page - 5, 1 << 10, page])[:n], np.array([0, 0, 2])[:n] % n, np.array([5, 0, 0])[:n], page)
+
+
+def test_release_after_a_fork(fdx):
+    """Pages that sequences share stay theirs when one of them ends."""
+    r = np.random.default_rng(8)
+    kv, d, heads = 2, 16, 4
+    c = fdx.PagedCache(8, 4, kv, d, d, 3, 24, "e4m3")
+    k, v = (r.standard_normal((10, kv * d)).astype(np.float32) for _ in range(2))
+    fdx.kv_append(c, k, v, [10, 0, 0])
+    q = r.standard_normal((1, heads * d)).astype(np.float32)
+    want = fdx.mha_paged(c, q, [1, 0, 0], heads)
+    fdx.kv_fork(c, [0, 0, -1])
+    c.release(0)
+    assert len(set(c.free)) == len(c.free) == 5 and not set(c.free) & set(c.table.ravel().tolist())
+    fdx.kv_append(c, np.ones((20, kv * d), np.float32), np.ones((20, kv * d), np.float32), [0, 0, 20])
+    assert np.array_equal(fdx.mha_paged(c, q, [0, 1, 0], heads), want)
+
+
 def test_python_fork(fdx):
     """kv_fork on a PagedCache: appended tokens go to each sequence's own pages, and attention sees what its ancestors wrote."""
     r = np.random.default_rng(6)
