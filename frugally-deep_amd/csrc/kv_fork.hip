@@ -126,28 +126,39 @@ __global__ __launch_bounds__(kForkThreads) void kv_fork_small_kernel(ForkParams 
     __syncthreads();
     const int entries = p.n_seqs * p.width;
     constexpr int W = 8; // loads of a thread that are on their way together
+    struct Entry {
+        int seq, at, filled; // rows from this entry's first on
+    };
+    auto entry = [&](int e) {
+        const int seq = quotient(e, p.by_width), at = e - seq * p.width;
+        const int64_t left = length_of[seq] - (int64_t)at * (int)p.page_size.by; // tables may be far wider than max_len
+        return Entry { seq, at, left > 0 ? (int)left : 0 };
+    };
     for (int e0 = tid; e0 < entries; e0 += W * threads) {
-        int at[W], seq[W], entry[W], filled[W];
+        int there[W];
 #pragma unroll
         for (int z = 0; z < W; ++z) {
-            const int e = e0 + z * threads < entries ? e0 + z * threads : e0;
-            seq[z] = quotient(e, p.by_width);
-            entry[z] = e - seq[z] * p.width;
-            const int64_t left = length_of[seq[z]] - (int64_t)entry[z] * (int)p.page_size.by; // tables may be far wider than max_len
-            filled[z] = left > 0 ? (int)left : 0; // rows from this entry's first on
-            at[z] = filled[z] > 0 ? p.table[(int64_t)parent_of[seq[z]] * p.width + entry[z]] : -1;
+            const int i = e0 + z * threads;
+            there[z] = -1;
+            if (i < entries) {
+                const Entry e = entry(i);
+                if (e.filled > 0)
+                    there[z] = p.table[(int64_t)parent_of[e.seq] * p.width + e.at];
+            }
         }
 #pragma unroll
         for (int z = 0; z < W; ++z) {
-            if (z > 0 && e0 + z * threads >= entries)
+            const int i = e0 + z * threads;
+            if (i >= entries)
                 break;
-            const int page = filled[z] > 0 ? checked_page(p, at[z], odd) : -1;
-            const bool full = filled[z] >= (int)p.page_size.by;
+            const Entry e = entry(i);
+            const int page = e.filled > 0 ? checked_page(p, there[z], odd) : -1;
+            const bool full = e.filled >= (int)p.page_size.by;
             if (full && page >= 0)
                 atomicOr(used + (page >> 5), 1u << (page & 31));
-            if (filled[z] > 0 && !full)
-                page_of[seq[z]] = page;
-            p.new_table[(int64_t)seq[z] * p.width + entry[z]] = full ? page : -1;
+            if (e.filled > 0 && !full)
+                page_of[e.seq] = page;
+            p.new_table[i] = full ? page : -1;
         }
     }
     __syncthreads();
@@ -299,7 +310,8 @@ __global__ __launch_bounds__(kForkThreads) void kv_fork_rest_kernel(ForkParams p
 
 struct ForkCopyParams {
     const int4* plan;
-    char *k, *v, *k_scale, *v_scale;
+    char *k, *v;
+    float *k_scale, *v_scale;
     int64_t k_row, v_row;      // bytes
     int page_size, block, kv_heads; // block 0: no scales
     int wide;                  // rows are whole 16-byte vectors
@@ -307,36 +319,45 @@ struct ForkCopyParams {
 
 constexpr int kCopyThreads = 256, kCopyBytes = 16384;
 
+// `bytes` bytes in vectors of T, four of a thread on their way together
 template <typename T>
-__device__ __forceinline__ void copy_bytes(const char* from, char* to, int64_t first, int64_t last)
+__device__ __forceinline__ void copy_bytes(const char* from, char* to, int bytes)
 {
-    for (int64_t i = first + threadIdx.x * (int64_t)sizeof(T); i < last; i += kCopyThreads * (int64_t)sizeof(T))
-        *reinterpret_cast<T*>(to + i) = *reinterpret_cast<const T*>(from + i);
+    constexpr int W = 4, kStep = kCopyThreads * (int)sizeof(T);
+    for (int at = threadIdx.x * (int)sizeof(T); at < bytes; at += W * kStep) {
+        T x[W];
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+            x[i] = *reinterpret_cast<const T*>(from + (at + i * kStep < bytes ? at + i * kStep : at));
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+            if (at + i * kStep < bytes)
+                *reinterpret_cast<T*>(to + at + i * kStep) = x[i];
+    }
 }
 
-// A workgroup takes 16 KB of the filled rows of one sequence's page, keys and values one behind the other.
+// A workgroup takes 16 KB of the filled rows of one sequence's page, of keys (z 0) or values (z 1).
 __global__ __launch_bounds__(kCopyThreads) void kv_fork_copy_kernel(ForkCopyParams p)
 {
     const int4 plan = p.plan[blockIdx.x];
     if (plan.y < 0 || plan.x < 0 || plan.z <= 0)
         return;
-    const int64_t from = (int64_t)plan.x * p.page_size, to = (int64_t)plan.y * p.page_size;
-    auto part = [&](char* base, int64_t row, int64_t first) {
-        const int64_t all = plan.z * row, last = first + kCopyBytes < all ? first + kCopyBytes : all;
+    const bool values = blockIdx.z > 0;
+    const int64_t row = values ? p.v_row : p.k_row, all = plan.z * row;
+    const int64_t from = (int64_t)plan.x * p.page_size * row, to = (int64_t)plan.y * p.page_size * row;
+    char* base = values ? p.v : p.k;
+    for (int64_t first = (int64_t)blockIdx.y * kCopyBytes; first < all; first += (int64_t)gridDim.y * kCopyBytes) {
+        const int bytes = all - first < kCopyBytes ? (int)(all - first) : kCopyBytes;
         if (p.wide)
-            copy_bytes<f32x4>(base + from * row, base + to * row, first, last);
+            copy_bytes<f32x4>(base + from + first, base + to + first, bytes);
         else
-            copy_bytes<char>(base + from * row, base + to * row, first, last);
-    };
-    for (int64_t first = (int64_t)blockIdx.y * kCopyBytes; first < plan.z * p.k_row; first += (int64_t)gridDim.y * kCopyBytes)
-        part(p.k, p.k_row, first);
-    for (int64_t first = (int64_t)blockIdx.y * kCopyBytes; first < plan.z * p.v_row; first += (int64_t)gridDim.y * kCopyBytes)
-        part(p.v, p.v_row, first);
+            copy_bytes<char>(base + from + first, base + to + first, bytes);
+    }
     if (p.block > 0 && blockIdx.y == 0) {
-        const int64_t row = 4 * (int64_t)p.kv_heads, bytes = (plan.z + p.block - 1) / p.block * row;
-        const int64_t a = (int64_t)plan.x * (p.page_size / p.block) * row, b = (int64_t)plan.y * (p.page_size / p.block) * row;
-        copy_bytes<float>(p.k_scale + a, p.k_scale + b, 0, bytes);
-        copy_bytes<float>(p.v_scale + a, p.v_scale + b, 0, bytes);
+        float* scales = values ? p.v_scale : p.k_scale;
+        const int64_t a_page = (int64_t)(p.page_size / p.block) * p.kv_heads, count = (int64_t)((plan.z + p.block - 1) / p.block) * p.kv_heads;
+        for (int64_t i = threadIdx.x; i < count; i += kCopyThreads)
+            scales[plan.y * a_page + i] = scales[plan.x * a_page + i];
     }
 }
 
@@ -380,8 +401,8 @@ static fdx_status fork_launch(const char* who, const fdx_kv_pages* c, size_t siz
         error_flag_dev };
     const int64_t k_row = (int64_t)c->kv_heads * c->dk * (int64_t)size, v_row = (int64_t)c->kv_heads * c->dv * (int64_t)size;
     const bool wide = ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v) | (uintptr_t)k_row | (uintptr_t)v_row) & 15) == 0;
-    const ForkCopyParams copy { p.plan, static_cast<char*>(c->k), static_cast<char*>(c->v), eight ? reinterpret_cast<char*>(eight->k_scale) : nullptr,
-        eight ? reinterpret_cast<char*>(eight->v_scale) : nullptr, k_row, v_row, c->page_size, eight ? eight->block : 0, c->kv_heads, wide };
+    const ForkCopyParams copy { p.plan, static_cast<char*>(c->k), static_cast<char*>(c->v), eight ? eight->k_scale : nullptr,
+        eight ? eight->v_scale : nullptr, k_row, v_row, c->page_size, eight ? eight->block : 0, c->kv_heads, wide };
     const int64_t parts = ((k_row > v_row ? k_row : v_row) * c->page_size + kCopyBytes - 1) / kCopyBytes;
     profile_begin();
     const int64_t entries = (int64_t)c->n_seqs * c->table_width;
@@ -393,7 +414,7 @@ static fdx_status fork_launch(const char* who, const fdx_kv_pages* c, size_t siz
         hipLaunchKernelGGL(kv_fork_mark_kernel, dim3((unsigned)((entries + 255) / 256)), dim3(256), 0, stream(), p);
         hipLaunchKernelGGL(kv_fork_rest_kernel, dim3(1), dim3(kForkThreads), 0, stream(), p);
     }
-    hipLaunchKernelGGL(kv_fork_copy_kernel, dim3((unsigned)c->n_seqs, (unsigned)(parts < 64 ? parts : 64)), dim3(kCopyThreads), 0, stream(), copy);
+    hipLaunchKernelGGL(kv_fork_copy_kernel, dim3((unsigned)c->n_seqs, (unsigned)(parts < 64 ? parts : 64), 2), dim3(kCopyThreads), 0, stream(), copy);
     profile_end("kv_fork", 0.0, 2.0 * table_bytes);
     FDX_LAUNCH_CHECK();
     return FDX_OK;
