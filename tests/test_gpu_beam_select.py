@@ -145,6 +145,24 @@ def test_equal_logits(fdx, vocab):
     check(fdx, x, scores, 32, near_ok=True)
 
 
+@pytest.mark.parametrize("n,beams,vocab,keep", [(2, 32, 5000, 32), (1, 4, 70000, 32), (1, 16, 20000, 16), (3, 8, 4096, 32), (40, 16, 9000, 32), (1, 1, 131072, 32), (2, 2, 33, 31)])
+@pytest.mark.parametrize("what", ["equal", "steps", "one beam"])
+def test_lists_of_one_order(fdx, n, beams, vocab, keep, what):
+    """All that is kept in one list, or as many from each, or all totals the same."""
+    x, scores = np.zeros((n, beams, vocab), np.float32), np.zeros((n, beams), np.float32)
+    if what == "steps":
+        x[:, :, :] = -np.arange(vocab) % 7
+    if what == "one beam":
+        x[:, :, :] = np.random.default_rng(keep).permutation(vocab).astype(np.float32) / 64
+        scores[:, :] = -1000 * ((np.arange(beams) + 1) % beams)
+    got = fdx.beam_select(x, scores, keep)
+    total = x[0].astype(np.float64) + scores[0][:, None]   # less the same number for every beam
+    order = np.argsort(-total.ravel(), kind="stable")[:keep]   # equal ones by beam, then by token
+    rows, tokens = order // vocab, order % vocab
+    assert (got["parents"] - beams * np.arange(n)[:, None] == rows).all(), (got["parents"], rows)
+    assert (got["tokens"] == tokens).all(), (got["tokens"], tokens)
+
+
 def test_logits_near_each_other(fdx):
     """Logits of one row that differ in their last bit, whose totals are the same in fp32: the larger first."""
     vocab = 6000
