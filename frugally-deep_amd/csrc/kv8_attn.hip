@@ -552,7 +552,7 @@ struct TileLds8 {
     __shared__ int lds##_absent;                                                                                            \
     const TileLds8 lds { lds##_ks0, lds##_ks1, lds##_vs0, lds##_vs1, lds##_scale0, lds##_scale1, lds##_rows_of, &lds##_absent }
 
-template <int D, int KIND, bool WIDE>
+template <int D, int KIND, bool WIDE, bool SIXTEENS>
 __device__ __forceinline__ void tile8_body(const RaggedParams& p, const Scales8& scales, const Place& place_in, const TileLds8& lds)
 {
     typedef Tile8<D> S;
@@ -786,16 +786,34 @@ __device__ __forceinline__ void tile8_body(const RaggedParams& p, const Scales8&
             const int limit = (visible < k_end ? visible : k_end) - j0; // keys of the tile that this lane's row sees
             const bool some_hidden = j0 + KT > wave_all_see || j0 + KT > k_end, some_gone = __builtin_amdgcn_readfirstlane(absent) != 0;
             auto hidden = [&](int key) { return key >= limit || (some_gone && rows_of[(t * KT + key) & (2 * kAhead - 1)] < 0); };
-            float mx = -INFINITY;
+            // by key i of a set of sixteen, register i of a half; SIXTEENS: such a set has one scale, which then meets its largest score and what scores are
+            // multiplied by
+            float kf[2 * HALVES], vf[2 * HALVES];
+            bool apart = !SIXTEENS;
+            if constexpr (SIXTEENS) {
+                float most_f = 0.f;
 #pragma unroll
-            for (int kb = 0; kb < HALVES; ++kb)
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const f32x4 by = *reinterpret_cast<const f32x4*>(scale + kb * 32 + 8 * g + 4 * half);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        sc[kb][4 * g + i] *= by[i];
+                for (int g = 0; g < 2 * HALVES; ++g) {
+                    kf[g] = scale[16 * g];
+                    vf[g] = scale[KT + 16 * g];
+                    most_f = fmaxf(most_f, kf[g]);
                 }
+                apart = __any(!(most_f * to_log2 < INFINITY)); // products of three numbers in fp32's range, of which two may pass it
+            }
+            if (apart) {
+#pragma unroll
+                for (int kb = 0; kb < HALVES; ++kb)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const f32x4 by = *reinterpret_cast<const f32x4*>(scale + kb * 32 + 8 * g + 4 * half);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            sc[kb][4 * g + i] *= by[i];
+                    }
+#pragma unroll
+                for (int g = 0; g < 2 * HALVES; ++g)
+                    kf[g] = 1.f;
+            }
             if (some_hidden || some_gone) {
 #pragma unroll
                 for (int kb = 0; kb < HALVES; ++kb)
@@ -805,14 +823,25 @@ __device__ __forceinline__ void tile8_body(const RaggedParams& p, const Scales8&
                         sc[kb][e] = h ? -INFINITY : sc[kb][e];
                         seen = seen || !h;
                     }
+                if constexpr (SIXTEENS) // a scale of NaN is for the rows that see it
+#pragma unroll
+                    for (int g = 0; g < 2 * HALVES; ++g) {
+                        kf[g] = hidden(16 * g) ? 1.f : kf[g];
+                        vf[g] = hidden(16 * g) ? 0.f : vf[g];
+                    }
             } else {
                 seen = true;
             }
+            float mx = -INFINITY;
 #pragma unroll
-            for (int kb = 0; kb < HALVES; ++kb)
+            for (int g = 0; g < 2 * HALVES; ++g) {
+                float of = -INFINITY;
 #pragma unroll
-                for (int e = 0; e < 16; e += 2)
-                    mx = fmaxf(fmaxf(mx, sc[kb][e]), sc[kb][e + 1]);
+                for (int e = 8 * (g & 1); e < 8 * (g & 1) + 8; e += 2)
+                    of = fmaxf(fmaxf(of, sc[g >> 1][e]), sc[g >> 1][e + 1]);
+                mx = fmaxf(mx, SIXTEENS ? of * kf[g] : of);
+                kf[g] = SIXTEENS ? __builtin_elementwise_maximum(kf[g] * to_log2, 0x1p-126f) : to_log2; // above zero for -infinity; NaN stays NaN
+            }
             mx = max_halves(mx) * to_log2;
             float corr = 1.f;
             if (__any(mx > m_run + 4.f)) {
@@ -828,31 +857,42 @@ __device__ __forceinline__ void tile8_body(const RaggedParams& p, const Scales8&
             for (int kb = 0; kb < HALVES; ++kb)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    sc[kb][e] = __builtin_amdgcn_exp2f(fmaf(sc[kb][e], to_log2, base));
+                    sc[kb][e] = __builtin_amdgcn_exp2f(fmaf(sc[kb][e], kf[2 * kb + (e >> 3)], base));
                     rs += sc[kb][e];
                 }
             l_run += rs; // the other half of the tile's keys lies in lane + 32: they meet at the end
+            if constexpr (SIXTEENS) {
 #pragma unroll
-            for (int kb = 0; kb < HALVES; ++kb)
+                for (int g = 0; g < 2 * HALVES; ++g) {
+                    float of = 0.f;
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const f32x4 by = *reinterpret_cast<const f32x4*>(scale + KT + kb * 32 + 8 * g + 4 * half);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        sc[kb][4 * g + i] *= by[i];
+                    for (int e = 8 * (g & 1); e < 8 * (g & 1) + 8; e += 2)
+                        of = fmaxf(fmaxf(of, sc[g >> 1][e]), sc[g >> 1][e + 1]);
+                    most = fmaxf(most, of * vf[g]);
                 }
-            if (some_hidden || some_gone) { // a scale of NaN is for the rows that see it
+            } else {
 #pragma unroll
                 for (int kb = 0; kb < HALVES; ++kb)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        sc[kb][e] = hidden(kb * 32 + 8 * (e >> 2) + 4 * half + (e & 3)) ? 0.f : sc[kb][e];
+                    for (int g = 0; g < 4; ++g) {
+                        const f32x4 by = *reinterpret_cast<const f32x4*>(scale + KT + kb * 32 + 8 * g + 4 * half);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            sc[kb][4 * g + i] *= by[i];
+                    }
+                if (some_hidden || some_gone) { // a scale of NaN is for the rows that see it
+#pragma unroll
+                    for (int kb = 0; kb < HALVES; ++kb)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            sc[kb][e] = hidden(kb * 32 + 8 * (e >> 2) + 4 * half + (e & 3)) ? 0.f : sc[kb][e];
+                }
+#pragma unroll
+                for (int kb = 0; kb < HALVES; ++kb)
+#pragma unroll
+                    for (int e = 0; e < 16; e += 2)
+                        most = fmaxf(fmaxf(most, sc[kb][e]), sc[kb][e + 1]);
             }
-#pragma unroll
-            for (int kb = 0; kb < HALVES; ++kb)
-#pragma unroll
-                for (int e = 0; e < 16; e += 2)
-                    most = fmaxf(fmaxf(most, sc[kb][e]), sc[kb][e + 1]);
             most = max_halves(most);
             if (__any(most > w_most * 16.f || corr != 1.f)) {
                 w_most = fmaxf(w_most, most);
@@ -865,6 +905,24 @@ __device__ __forceinline__ void tile8_body(const RaggedParams& p, const Scales8&
                     for (int e = 0; e < 16; ++e)
                         oacc[d][e] *= by;
             }
+            if constexpr (SIXTEENS) {
+                float most_f = 0.f;
+#pragma unroll
+                for (int g = 0; g < 2 * HALVES; ++g)
+                    most_f = __builtin_elementwise_maximum(most_f, vf[g]); // NaN stays NaN
+                if (__any(!(most_f * power.up < INFINITY))) {
+#pragma unroll
+                    for (int g = 0; g < 2 * HALVES; ++g) {
+#pragma unroll
+                        for (int e = 8 * (g & 1); e < 8 * (g & 1) + 8; ++e)
+                            sc[g >> 1][e] *= vf[g];
+                        vf[g] = 1.f;
+                    }
+                }
+            }
+#pragma unroll
+            for (int g = 0; g < 2 * HALVES; ++g)
+                vf[g] = SIXTEENS ? vf[g] * power.up : power.up;
             __builtin_amdgcn_s_setprio(1); // beside another workgroup's wave that is not at its products (416 -> 406 us)
             scores(next, ks);
             // O^T += V^T P^T
@@ -875,7 +933,7 @@ __device__ __forceinline__ void tile8_body(const RaggedParams& p, const Scales8&
                 for (int j = 0; j < 8; ++j)
                     x[j] = sc[u >> 1][8 * (u & 1) + j];
                 f16x8 ph, pl;
-                split2x8(x, power.up, ph, pl);
+                split2x8(x, vf[u], ph, pl);
 #pragma unroll
                 for (int d = 0; d < DB; ++d) {
                     const f16x8 v = values(vs, 16 * u, d);
@@ -946,21 +1004,21 @@ __device__ __forceinline__ void tile8_body(const RaggedParams& p, const Scales8&
         }
 }
 
-template <int D, int KIND, bool WIDE>
+template <int D, int KIND, bool WIDE, bool SIXTEENS>
 __global__ __launch_bounds__(256, 2) void paged8_tile_kernel(RaggedParams p, Scales8 scales)
 {
     FDX_TILE8_LDS(D, lds);
-    tile8_body<D, KIND, WIDE>(p, scales, Place { blockIdx.x, blockIdx.y, gridDim.x }, lds);
+    tile8_body<D, KIND, WIDE, SIXTEENS>(p, scales, Place { blockIdx.x, blockIdx.y, gridDim.x }, lds);
 }
 
 // Both in one launch: what is bound by memory runs beside what is bound by the matrix and vector units.  Tiles, which take longest, come first.
-template <int D, int KIND>
+template <int D, int KIND, bool SIXTEENS>
 __global__ __launch_bounds__(256, 2) void paged8_mixed_kernel(RaggedParams p, Scales8 scales, Few8 few, unsigned tile_x, unsigned tile_wgs)
 {
     FDX_TILE8_LDS(D, lds);
     __shared__ __attribute__((aligned(16))) unsigned char q[2 * D / 32 * 2 * 1024];
     if (blockIdx.x < tile_wgs) {
-        tile8_body<D, KIND, true>(p, scales, Place { blockIdx.x % tile_x, blockIdx.x / tile_x, tile_x }, lds);
+        tile8_body<D, KIND, true, SIXTEENS>(p, scales, Place { blockIdx.x % tile_x, blockIdx.x / tile_x, tile_x }, lds);
     } else {
         static_assert(16 * (D + 4) * sizeof(float) <= sizeof(lds_ks0) && 16 * (D + 4) * sizeof(float) <= sizeof(lds_vs0)
                 && (2 * 4 * 16 + 5 * 64) * sizeof(float) <= sizeof(lds_rows_of), "fits into the tiles' LDS");
@@ -1158,8 +1216,14 @@ static void paged8_launch(const RaggedParams& p, const Plan8& plan, const Scales
     const bool wide = (all & 15) == 0 && ((p.ldq | p.ldo) & 3) == 0 && ((p.dk | p.dv) & 15) == 0 && rows * (ld >> 4) < ((int64_t)1 << 32);
     const unsigned tile_x = (unsigned)plan.tiles.tiles, tile_y = (unsigned)(plan.tiles.tile_ranges > 0 ? plan.tiles.tile_ranges : 1);
     const uint64_t tile_wgs = (uint64_t)tile_x * tile_y, all_wgs = tile_wgs + plan.few_wgs;
+    // Blocks of whole sixteens (ranges start at multiples of 64): two multiplications less a score.  us without / with, 128 new tokens of 1000, 12 heads of
+    // 64: 25.8 / 23.6; two of 2000 of 3000, 16 / 4 heads of 64, 125.6 / 119.8; four of 1000 of 3000, 32 / 8 heads of 128, 386.5 / 380.2.
+    const bool sixteens = scales.block.by % 16 == 0;
     if (wide && tile_wgs > 0 && plan.few_wgs > 0 && all_wgs < (1u << 23)) {
-        hipLaunchKernelGGL((paged8_mixed_kernel<D, KIND>), dim3((unsigned)all_wgs), dim3(256), 0, stream(), p, scales, plan.few, tile_x, (unsigned)tile_wgs);
+        if (sixteens)
+            hipLaunchKernelGGL((paged8_mixed_kernel<D, KIND, true>), dim3((unsigned)all_wgs), dim3(256), 0, stream(), p, scales, plan.few, tile_x, (unsigned)tile_wgs);
+        else
+            hipLaunchKernelGGL((paged8_mixed_kernel<D, KIND, false>), dim3((unsigned)all_wgs), dim3(256), 0, stream(), p, scales, plan.few, tile_x, (unsigned)tile_wgs);
     } else {
         if (plan.few_wgs > 0) {
             if (wide)
@@ -1168,10 +1232,13 @@ static void paged8_launch(const RaggedParams& p, const Plan8& plan, const Scales
                 hipLaunchKernelGGL((paged8_few_kernel<D, KIND, false>), dim3(plan.few_wgs), dim3(256), 0, stream(), p, scales, plan.few);
         }
         if (tile_wgs > 0) {
-            if (wide)
-                hipLaunchKernelGGL((paged8_tile_kernel<D, KIND, true>), dim3(tile_x, tile_y), dim3(256), 0, stream(), p, scales);
+            const dim3 grid(tile_x, tile_y);
+            if (wide && sixteens)
+                hipLaunchKernelGGL((paged8_tile_kernel<D, KIND, true, true>), grid, dim3(256), 0, stream(), p, scales);
+            else if (wide)
+                hipLaunchKernelGGL((paged8_tile_kernel<D, KIND, true, false>), grid, dim3(256), 0, stream(), p, scales);
             else
-                hipLaunchKernelGGL((paged8_tile_kernel<D, KIND, false>), dim3(tile_x, tile_y), dim3(256), 0, stream(), p, scales);
+                hipLaunchKernelGGL((paged8_tile_kernel<D, KIND, false, false>), grid, dim3(256), 0, stream(), p, scales);
         }
     }
     if (plan.few.shares > 1 || tile_y > 1) {

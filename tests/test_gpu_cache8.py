@@ -439,7 +439,7 @@ def test_paged_queries_of_nan(fdx, new, what):
 
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("new", [[1, 1], [3, 40], [140, 1]])
-@pytest.mark.parametrize("eq,ek,ev", [(60, -60, 0), (-60, 60, 0), (-100, 100, 0), (0, 0, 100), (0, 0, -100), (-40, -80, 5), (110, -110, 110), (0, 0, 119), (-110, 98, -118)])
+@pytest.mark.parametrize("eq,ek,ev", [(60, -60, 0), (-60, 60, 0), (-100, 100, 0), (0, 0, 100), (0, 0, -100), (-40, -80, 5), (110, -110, 110), (0, 0, 119), (-110, 98, -118), (-60, -100, 7), (-100, -110, -100)])
 def test_paged_sizes_of_operands(fdx, new, eq, ek, ev, kind):
     """Operands far from one in size: the result scales."""
     def change(k, v):
@@ -539,6 +539,23 @@ def test_paged_jumps_of_scores_and_values(fdx, new, up):
     # all scores that count are the same number: what is left are the errors of means of values
     assert np.isfinite(want).all()
     close(fdx.mha_paged(f.cache, q, [new], heads).astype(np.float64) * 2.0 ** (90 * up), want * 2.0 ** (90 * up))
+
+
+@pytest.mark.parametrize("new", [3, 100])
+@pytest.mark.parametrize("eq,ek,ev", [(80, 80, 60), (80, 80, -60), (-80, 60, 110)])
+def test_paged_products_that_are_zero(fdx, new, eq, ek, ev):
+    """Queries and keys whose product would be far out of range, and has no terms; values near fp32's end beside ones near its beginning."""
+    n, heads, kv, d = 300, 4, 2, 64
+
+    def change(k, v):
+        k[:] *= np.float32(2.0 ** ek)
+        k[:, ::2] = 0
+        v[::2] *= np.float32(2.0 ** ev)
+        v[1::2] *= np.float32(2.0 ** -ev)
+    f = Filled(fdx, [n], kv, d, d, 16, "i8", 16, change=change)
+    q = (2.0 ** eq * np.random.default_rng(9).standard_normal((new, heads * d))).astype(np.float32)
+    q[:, 1::2] = 0
+    close(fdx.mha_paged(f.cache, q, [new], heads).astype(np.float64) * 2.0 ** -abs(ev), f.reference(q, [new], heads) * 2.0 ** -abs(ev))
 
 
 @pytest.mark.parametrize("new", [1, 12, 100])
