@@ -1135,6 +1135,8 @@ __global__ __launch_bounds__(256) void paged8_join_kernel(RaggedParams p, Few8 f
         sum_parts<H>(p, FEW ? wave : 0, FEW ? 4 : 1, (visible + s.range - 1) / s.range, [&](int i, int h) { return p.tile.out(i, first + head_of(h), p.dv); },
             [&](int i, int h) { return p.tile.size(i, first + head_of(h), p.dv); }, r);
     } else {
+        if (few.shares <= 1) // no sequence is shared, and nothing is kept of where they begin
+            return;
         const int2 split = few.split[index];
         const int from = split.x, parts = split.y;
         if (parts == 1)

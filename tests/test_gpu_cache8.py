@@ -361,6 +361,23 @@ def test_lengths_of_sequences_without_new_tokens(fdx, heads):
         close(out.to_host((2, heads * 64)), f.reference(q, [1, 0, 1], heads))
 
 
+@pytest.mark.parametrize("context,heads,kv", [([190, 150], 8, 8), ([190, 150, 30], 4, 2), ([300, 20], 4, 4), ([384], 4, 4), ([700, 700], 4, 4), ([190, 150], 600, 600)])
+@pytest.mark.parametrize("new", [35, 1])
+def test_whole_sequences_beside_tiles_in_ranges(fdx, context, heads, kv, new):
+    """Tiles whose ranges are joined, and decode steps that nobody shares; a call that says more new tokens than any sequence has."""
+    d = 8 if kv > 8 else 128
+    f = Filled(fdx, context, kv, d, d, 16, "i8", 8)
+    counts = [new] + [1] * (len(context) - 1)
+    rows = sum(counts) + (0 if new > 1 else 40)   # rows behind the last sequence
+    q = np.random.default_rng(3).standard_normal((rows, heads * d)).astype(np.float32)
+    dq, out = fdx.DevBuf.from_host(q), fdx.DevBuf.from_host(np.full((rows, heads * d), 7, np.float32))
+    print("paged8 whole sequences", context, heads, kv, new, flush=True)
+    assert call_paged(fdx, f.cache, dq.ptr, heads * d, np.cumsum([0] + counts), rows, 35, heads, out.ptr, heads * d) == 0
+    got, n = out.to_host((rows, heads * d)), sum(counts)
+    close(got[:n], f.reference(q[:n], counts, heads))
+    assert (got[n:] == 7).all()
+
+
 @pytest.mark.parametrize("at", [0, 63, 64, 130, 299])
 def test_lengths_out_of_range_among_many(fdx, at):
     n, heads = 300, 4
