@@ -22,6 +22,9 @@ namespace fdx {
 //  * Codes are fp16 values exactly; a query is held as two fp16 values (f16_split.hpp), and so are its probabilities times their values' scales, by a
 //    power that keeps the largest of them so far in fp16's range: a row has sums of its own power, and none depends on keys that it does not see.
 //  * A key's scale meets its score; lane (c, g) has looked up one scale, and a lane's number in its row of sixteen names it for all of them.
+// Bound by memory: a wave has its next block on its way beside the one it works on.  64 sequences of 4000 keys, 32 / 8 heads of 128 (528 MB), 107 us,
+// 4.9 TB/s; 64 of 300 to 7900 (315 MB) 84, 3.8 TB/s: beginnings and ends of segments, two or three a workgroup, take a sixth; one token over 100 003 keys (205
+// MB) 49, 4.2.  A third block on its way 91 -> 94 us; three workgroups a CU would spill 37 registers.
 template <int D, bool WIDE>
 struct Block8 {
     static constexpr int NK = D / 64, DL = D / 16;
@@ -85,7 +88,10 @@ struct Few8 {
     __device__ __forceinline__ float* out(int64_t row, int dv) const { return parts + row * dv; }
     __device__ __forceinline__ float* size(int64_t row, int dv) const { return parts + (int64_t)shares * kv_heads * 2 * rows * dv + row * 2; }
 };
-constexpr int kLeastShare = 8; // blocks: two turns of each wave
+// Blocks of a share at least, a turn of each wave; up to kWhole are not shared, which saves the join's launch.  us with 8 and 8 / with 4 and 12, one token:
+// 12 heads of 64, 300 keys 13.0 / 9.7, 1000 13.2 / 11.8; 32 / 8 heads of 128, 300 keys 15.0 / 11.8, 380 and eight tokens 19.7 / 18.5, 2000 15.3 / 13.3, 8000
+// 16.8 / 17.4; 64 sequences of 50 to 400 32.5 / 27.7.  With up to 16 whole, 400 keys and eight tokens take 19.9 instead of 16.0.
+constexpr int kLeastShare = 4, kWhole = 12;
 
 // one of the sequences with few rows: its new rows, its keys, its units of blocks.  One that sees no key has a unit all the same: its rows get zeros.
 struct FewSequence {
@@ -530,6 +536,8 @@ __global__ __launch_bounds__(256, WIDE ? 2 : 1) void paged8_few_kernel(RaggedPar
 //  * A query row is brought to fp16's range by a power of two and held as two fp16 values (f16_split.hpp).  So are its probabilities times
 //    the values' scales, by a power that keeps the largest of them so far between 2^6 and 2^15: a row has sums of its own power, and none
 //    depends on keys that it does not see.  A key's scale meets its score.
+// Vector instructions (60 % of the time) and matrix instructions (44 %) mostly add up: four sequences that bring 1000 tokens to 3000 keys, 32 / 8
+// heads of 128 (164 GFLOP), 380 us, 430 TFLOP/s, where two products for one leave 620.
 //  * LDS holds two tiles.  While the probabilities of tile t meet its values, the scores of tile t + 1 are multiplied; tile t + 2's keys and tile
 //    t + 1's values go to LDS, what comes behind them to registers; one barrier a tile.
 template <int D>
@@ -1189,7 +1197,9 @@ static Plan8 plan8(int tokens, int max_new, int heads, const fdx_kv_pages* c)
     Plan8 r {};
     r.tiles = paged_plan(tokens, max_new, heads, c);
     if (r.tiles.few_ranges > 0) {
-        const int64_t most = (int64_t)c->n_seqs * (((int64_t)c->max_len + 31) / 32), shares = (most + kLeastShare - 1) / kLeastShare;
+        const int64_t most = (int64_t)c->n_seqs * (((int64_t)c->max_len + 31) / 32), shares = most <= kWhole ? 1 : (most + kLeastShare - 1) / kLeastShare;
+        // us with as many as fit, two workgroups a CU or three / with others: 64 of 4000, 32 / 8 heads of 128, 512 118, 768 156; 64 of 100 to 8000, 12 heads of
+        // 64, 768 90, 512 and 1024 102
         const int fit = (c->dk <= 64 && c->dv <= 64 ? 768 : 512) / c->kv_heads;
         r.few.shares = fit < 1 ? 1 : (shares < fit ? (int)shares : fit);
         r.few.rows = (int)(r.tiles.few_part / ((int64_t)c->n_seqs * c->kv_heads));
