@@ -361,6 +361,23 @@ def test_lengths_of_sequences_without_new_tokens(fdx, heads):
         close(out.to_host((2, heads * 64)), f.reference(q, [1, 0, 1], heads))
 
 
+@pytest.mark.parametrize("n,new", [(40, 1), (130, 2), (40, 35)])
+def test_shares_of_the_longest_cache(fdx, n, new):
+    """A cache that says 2^30 positions: blocks are counted in sets."""
+    page, kv, heads, d, width = 4096, 1, 2, 16, 1 << 18
+    r = np.random.default_rng(n)
+    context = np.where(r.random(n) < 0.2, r.integers(1000, 4000, n), r.integers(40, 200, n)).tolist()
+    f = Filled(fdx, context, kv, d, d, page, "e4m3", 32)
+    q = r.standard_normal((n * new, heads * d)).astype(np.float32)
+    table = np.full((n, width), -1, np.int32)
+    table[:, 0] = f.cache.table[:, 0]
+    dq, out = fdx.DevBuf.from_host(q), fdx.DevBuf.from_host(np.zeros((n * new, heads * d), np.float32))
+    print("paged8 longest cache", n, new, flush=True)
+    assert call_paged(fdx, f.cache, dq.ptr, heads * d, np.arange(n + 1) * new, n * new, new, heads, out.ptr, heads * d, table=table, table_width=width,
+                      max_len=1 << 30) == 0
+    close(out.to_host((n * new, heads * d)), f.reference(q, [new] * n, heads))
+
+
 @pytest.mark.parametrize("context,heads,kv", [([190, 150], 8, 8), ([190, 150, 30], 4, 2), ([300, 20], 4, 4), ([384], 4, 4), ([700, 700], 4, 4), ([190, 150], 600, 600)])
 @pytest.mark.parametrize("new", [35, 1])
 def test_whole_sequences_beside_tiles_in_ranges(fdx, context, heads, kv, new):
