@@ -174,6 +174,7 @@ __global__ __launch_bounds__(256) void beam_select_kernel(BeamParams p)
     }
     const int head_list = quotient(tid, p.by_deep), deep = (int)p.by_deep.by, n_heads = lists * deep; // up to kBeamLists
     const uint64_t first_key = tid < n_heads ? keys[head_list * p.keep + tid - head_list * deep] : 0; // on its way beside the sums (rows that are not read have left anything)
+    const uint64_t my_key = tid < lists * p.keep ? keys[tid] : 0;
     // the rows' sums: p.width threads a beam, one a part
     for (int b = tid / p.width; b < p.beams; b += 256 / p.width) {
         const int64_t row = row0 + b;
@@ -224,7 +225,7 @@ __global__ __launch_bounds__(256) void beam_select_kernel(BeamParams p)
         const int list = quotient(i, p.by_keep);
         if (better(least, heads.at(list * deep)))
             continue;
-        const Continuation c = listed(list, i - list * p.keep, keys[i]);
+        const Continuation c = listed(list, i - list * p.keep, i == tid ? my_key : keys[i]);
         if (c.total > -INFINITY && !better(least, c))
             items.put(atomicAdd(&count, 1), c);
     }
