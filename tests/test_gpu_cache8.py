@@ -435,9 +435,10 @@ def test_paged_more_new_tokens_than_said(fdx):
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("new", [1, 4, 16, 50, 100])
 @pytest.mark.parametrize("which", [0, 1])
-def test_paged_blocks_of_nan(fdx, new, which, kind):
+@pytest.mark.parametrize("block,d", [(4, 64), (16, 64), (16, 128)])
+def test_paged_blocks_of_nan(fdx, new, which, kind, block, d):
     """A block whose scale is NaN: NaN for the rows that see a token of it (of its key head), nothing for the others, whatever tile they share."""
-    heads, kv, d, block = 4, 2, 64, 4
+    heads, kv = 4, 2
     f = Filled(fdx, [150, 40], kv, d, d, 16, kind, block)
     q = np.random.default_rng(2).standard_normal((new + 1, heads * d)).astype(np.float32)
     base = f.reference(q, [new, 1], heads)
@@ -474,12 +475,13 @@ def test_paged_queries_of_nan(fdx, new, what):
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("new", [[1, 1], [3, 40], [140, 1]])
 @pytest.mark.parametrize("eq,ek,ev", [(60, -60, 0), (-60, 60, 0), (-100, 100, 0), (0, 0, 100), (0, 0, -100), (-40, -80, 5), (110, -110, 110), (0, 0, 119), (-110, 98, -118), (-60, -100, 7), (-100, -110, -100)])
-def test_paged_sizes_of_operands(fdx, new, eq, ek, ev, kind):
+@pytest.mark.parametrize("block", [8, 16])
+def test_paged_sizes_of_operands(fdx, new, eq, ek, ev, kind, block):
     """Operands far from one in size: the result scales."""
     def change(k, v):
         k *= np.float32(2.0 ** ek)
         v *= np.float32(2.0 ** ev)
-    f, heads = Filled(fdx, [200, 141], 2, 64, 64, 16, kind, 8, change=change), 4
+    f, heads = Filled(fdx, [200, 141], 2, 64, 64, 16, kind, block, change=change), 4
     q = np.ldexp(np.random.default_rng(5).standard_normal((sum(new), heads * 64)).astype(np.float32), eq).astype(np.float32)
     print("paged8 sizes", new, eq, ek, ev, kind, flush=True)
     got = fdx.mha_paged(f.cache, q, new, heads)
@@ -555,9 +557,14 @@ def test_paged_scores_of_a_few_hundred(fdx, new):
 
 @pytest.mark.parametrize("new", [1, 12, 100])
 @pytest.mark.parametrize("up", [1, -1])
-def test_paged_jumps_of_scores_and_values(fdx, new, up):
+@pytest.mark.parametrize("block", [2, 16])
+def test_paged_jumps_of_scores_and_values(fdx, new, up, block):
     """From one token to another scores rise by thousands and values shrink by 2^180, or the other way round: sums of the tokens that went before are
-    gone, and nothing passes fp32's range on the way."""
+    gone, and nothing passes fp32's range on the way.
+
+    Blocks of sixteen have both sorts of tokens in one, with the larger ones' scale s and the smaller ones' codes 0.  A probability times its value's scale
+    is held to 2^-34 of the row's largest such product, which is s times the probability that all n tokens that count have in common: a sum of n
+    products with codes up to 127, over n such probabilities, is off by up to 127 * 2^-34 s.  A step of the block itself is s."""
     n, first = 300, 150
 
     def jump(k, v):
@@ -566,13 +573,19 @@ def test_paged_jumps_of_scores_and_values(fdx, new, up):
         k[first:, ::64] = 4000 * up
         v[:first] *= np.float32(2.0 ** (90 * up))
         v[first:] *= np.float32(2.0 ** (-90 * up))
-    f, heads = Filled(fdx, [n], 2, 64, 64, 16, "i8", 2, change=jump), 4
+    f, heads = Filled(fdx, [n], 2, 64, 64, 16, "i8", block, change=jump), 4
     q = np.zeros((new, heads * 64), np.float32)
     q[:, ::64] = 3
     want = f.reference(q, [new], heads)
     # all scores that count are the same number: what is left are the errors of means of values
     assert np.isfinite(want).all()
-    close(fdx.mha_paged(f.cache, q, [new], heads).astype(np.float64) * 2.0 ** (90 * up), want * 2.0 ** (90 * up))
+    got = fdx.mha_paged(f.cache, q, [new], heads).astype(np.float64)
+    count = [p for p in range(n) if (p >= first) == (up > 0)]
+    most = max(float(f.host.scales[1][f.row_of(0)(p) // block].max()) for p in count)
+    off, step = np.abs(got - want), 127 * 2.0 ** -34 * most
+    print("off %.2e of %.2e, step %.2e" % (off.max(), np.abs(want).max(), step), flush=True)
+    assert off.max() <= step + 2e-5 * np.abs(want).max()
+    assert np.linalg.norm(off * 2.0 ** (90 * up)) <= 2.0 ** (90 * up) * step * np.sqrt(off.size) + 2e-6 * np.linalg.norm(want * 2.0 ** (90 * up))
 
 
 @pytest.mark.parametrize("new", [3, 100])
