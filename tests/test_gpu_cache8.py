@@ -676,3 +676,37 @@ def test_offsets_beyond_32_bits(fdx, kind):
             rows = 2 * s * page + np.arange(length)
             close(got[at:at + n], attend(q[at:at + n], host.values(rows, 0), host.values(rows, 1), kv, kv, np.arange(length - n, length) + 1))
             at += n
+
+
+def test_two_threads(fdx):
+    """Calls of two host threads, each with a cache of its own."""
+    import threading
+    heads, want, got, errors = 4, [None, None], [None, None], []
+    r = np.random.default_rng(11)
+    k, v, q = (r.standard_normal((2, n, w)).astype(np.float32) for n, w in ((500, 128), (500, 128), (2, heads * 64)))
+    logits, scores = r.standard_normal((2, 3, 4, 3001)).astype(np.float32), -r.random((2, 3, 4)).astype(np.float32)
+
+    def steps(i):
+        c = fdx.PagedCache(60, 16, 2, 64, 64, 2, 400, ("i8", "e4m3")[i], 8)
+        out = []
+        for at in range(0, 500, 100):
+            fdx.kv_append(c, k[i, at:at + 100], v[i, at:at + 100], [40 + i, 60 - i])
+            out.append(fdx.mha_paged(c, q[i], [1, 1], heads))
+            best = fdx.beam_select(logits[i], scores[i], 4)
+            out += [best[key] for key in sorted(best)]
+            fdx.kv_fork(c, [0, 1] if at % 200 else [1, 0])
+        return out
+
+    def work(i):
+        try:
+            for _ in range(5):
+                got[i] = steps(i)
+        except Exception as e:   # reported below, by the test's own thread
+            errors.append(e)
+    want = [steps(0), steps(1)]
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not errors, errors
+    for a, b in zip(want, got):
+        assert all(np.array_equal(x, y) for x, y in zip(a, b)) and len(a) == len(b)
