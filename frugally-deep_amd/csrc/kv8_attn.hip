@@ -291,7 +291,8 @@ __device__ __forceinline__ void few8_segment(const RaggedParams& p, const Scales
         }
         float mx = fmaxf(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])), fmaxf(fmaxf(sc[4], sc[5]), fmaxf(sc[6], sc[7])));
         float corr = 1.f;
-        if (__any(mx > m_run + 8.f)) { // the maximum moves when a score passes it by 2^8
+        // The maximum moves when a score passes it by 4: what is added is below 2^4, and 2^4 times a value's scale, up to 2^128 / 127, is in fp32's range
+        if (__any(mx > m_run + 4.f)) {
             const float m_new = fmaxf(m_run, most_of_row(mx));
             corr = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run - m_new);
             m_run = m_new;

@@ -710,3 +710,21 @@ def test_two_threads(fdx):
     assert not errors, errors
     for a, b in zip(want, got):
         assert all(np.array_equal(x, y) for x, y in zip(a, b)) and len(a) == len(b)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("new", [1, 12, 100])
+@pytest.mark.parametrize("keys,rise", [(300, 7.9), (300, 3.9), (900, 7.9), (3000, 7.5)])
+def test_paged_values_near_the_end_of_fp32(fdx, keys, rise, new, kind):
+    """Values up to 3.2e38 behind scores that rise by less than a power of 2^8 on the way: sums are means, none passes fp32's range.  The keys of
+    either half have one score, so its error is common to them: what is left are the errors of means of values."""
+    def change(k, v):
+        k[:] = 0
+        k[keys // 2:, ::64] = rise * np.log(2) * 8
+        v[:] = np.float32(3.2e38) * np.random.default_rng(2).uniform(-1, 1, v.shape).astype(np.float32)
+    f, heads = Filled(fdx, [keys], 2, 64, 64, 16, kind, 16, change=change), 4
+    q = np.zeros((new, heads * 64), np.float32)
+    q[:, ::64] = 1
+    print("paged8 largest values", keys, rise, new, kind, flush=True)
+    got, want = fdx.mha_paged(f.cache, q, [new], heads), f.reference(q, [new], heads)
+    close(np.ldexp(got.astype(np.float64), -127), np.ldexp(want, -127))
