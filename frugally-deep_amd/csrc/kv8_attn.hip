@@ -852,6 +852,21 @@ __device__ __forceinline__ void tile8_body(const RaggedParams& p, const Scales8&
                 kf[g] = SIXTEENS ? __builtin_elementwise_maximum(kf[g] * to_log2, 0x1p-126f) : to_log2; // above zero for -infinity; NaN stays NaN
             }
             mx = max_halves(mx) * to_log2;
+            // The largest score is rounded three times, the exponents' multiply-adds once: up to 2^22 they are less than one apart, of 2^31 further than
+            // exponentials reach, and a row would add infinities, or nothing.  From 2^22 on scores are multiplied out first; the largest is one of them.
+            if (__builtin_expect(__any(fabsf(mx) >= 0x1p22f && mx > -INFINITY), 0)) {
+                mx = -INFINITY;
+#pragma unroll
+                for (int g = 0; g < 2 * HALVES; ++g) {
+#pragma unroll
+                    for (int e = 8 * (g & 1); e < 8 * (g & 1) + 8; ++e) {
+                        sc[g >> 1][e] *= kf[g];
+                        mx = fmaxf(mx, sc[g >> 1][e]);
+                    }
+                    kf[g] = 1.f;
+                }
+                mx = max_halves(mx);
+            }
             float corr = 1.f;
             if (__any(mx > m_run + 4.f)) {
                 const float m_new = mx > m_run + 4.f ? mx : m_run;

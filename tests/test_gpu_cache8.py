@@ -728,3 +728,27 @@ def test_paged_values_near_the_end_of_fp32(fdx, keys, rise, new, kind):
     print("paged8 largest values", keys, rise, new, kind, flush=True)
     got, want = fdx.mha_paged(f.cache, q, [new], heads), f.reference(q, [new], heads)
     close(np.ldexp(got.astype(np.float64), -127), np.ldexp(want, -127))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("new", [1, 12, 100])
+@pytest.mark.parametrize("block", [8, 16])
+@pytest.mark.parametrize("eq,ek", [(16, 0), (20, 0), (24, 0), (30, 0), (0, 60), (60, 50), (-20, 90)])
+def test_paged_scores_far_from_zero(fdx, eq, ek, block, new, kind):
+    """Scores from 2^17 to 2^114, either sign, whose differences are thousands and more: the keys of the largest one, which are several and have the
+    same codes, share the weight.  What is left are the errors of means of values."""
+    n = 300
+
+    def change(k, v):
+        r = np.random.default_rng(4)
+        k[:] = 0
+        c = r.integers(-126, 127, (n, 1)) if kind == "i8" else 16 * r.integers(-27, 28, (n, 1))
+        c[::8] = 127 if kind == "i8" else 448   # every block has the same scale, and codes are exact
+        c[4::8] = -c[::8][:len(c[4::8])]
+        k[:, ::64] = np.ldexp(c.astype(np.float32), ek)
+    f, heads = Filled(fdx, [n], 2, 64, 64, 16, kind, block, change=change), 4
+    r = np.random.default_rng(5)
+    q = np.zeros((new, heads * 64), np.float32)
+    q[:, ::64] = np.ldexp(r.uniform(0.5, 1.5, (new, heads)) * r.choice([-1, 1], (new, heads)), eq)
+    print("paged8 far scores", eq, ek, block, new, kind, flush=True)
+    close(fdx.mha_paged(f.cache, q, [new], heads), f.reference(q, [new], heads))
