@@ -172,7 +172,10 @@ __device__ __forceinline__ void few8_segment(const RaggedParams& p, const Scales
     // the query: step (i, h) has depths 64 i + 16 g + 8 h ..
     // In LDS, which leaves registers to the blocks on their way; waves that share rows write the same.
     f16x8* q_at = reinterpret_cast<f16x8*>(meet.q) + (r_first > 0 ? 4 * NK * 64 : 0) + lane;
-    float to_log2;
+    // Scores over codes are up to 2^15 * 448 * 128 < 2^31 times to_log2, which may pass fp32's range before a small scale brings them back: factors above 2^90
+    // leave 2^30 for behind the scale.
+    float to_log2, behind;
+    bool some_behind;
     const bool q_ok = r_first + c < count;
     const int q_token = quotient(q_ok ? r_first + c : 0, p.by_group);
     const int visible = q_ok ? visible_keys(p, s, q_token) : 0;
@@ -204,6 +207,9 @@ __device__ __forceinline__ void few8_segment(const RaggedParams& p, const Scales
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         const Pow2 sq = pow2_for<1>(exponent(max_halves(top)));
         to_log2 = sq.down * (p.scale * kLog2e);
+        behind = to_log2 > 0x1p90f ? 0x1p30f : 1.f;
+        to_log2 = to_log2 > 0x1p90f ? to_log2 * 0x1p-30f : to_log2;
+        some_behind = __any(behind != 1.f);
 #pragma unroll
         for (int u = 0; u < 2 * NK; ++u)
         {
@@ -260,6 +266,11 @@ __device__ __forceinline__ void few8_segment(const RaggedParams& p, const Scales
         sc[5] *= dpp_move<0x155>(x.scale);
         sc[6] *= dpp_move<0x156>(x.scale);
         sc[7] *= dpp_move<0x157>(x.scale);
+        if (__builtin_expect(some_behind, 0)) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                sc[i] *= behind;
+        }
         vs[0] = dpp_move<0x158>(x.scale);
         vs[1] = dpp_move<0x159>(x.scale);
         vs[2] = dpp_move<0x15A>(x.scale);

@@ -752,3 +752,19 @@ def test_paged_scores_far_from_zero(fdx, eq, ek, block, new, kind):
     q[:, ::64] = np.ldexp(r.uniform(0.5, 1.5, (new, heads)) * r.choice([-1, 1], (new, heads)), eq)
     print("paged8 far scores", eq, ek, block, new, kind, flush=True)
     close(fdx.mha_paged(f.cache, q, [new], heads), f.reference(q, [new], heads))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("new", [[1, 1], [3, 40], [140, 1]])
+@pytest.mark.parametrize("e", [108, 114, 118, 122, 124])
+@pytest.mark.parametrize("d", [64, 128])
+def test_paged_queries_near_the_end_of_fp32(fdx, new, e, kind, d):
+    """Queries up to 2^126 and keys as small: scores of ordinary size, though a sum over codes alone passes fp32's range."""
+    def change(k, v):
+        k *= np.float32(2.0 ** -e)
+    f, heads = Filled(fdx, [200, 141], 2, d, d, 16, kind, 16, change=change), 4
+    q = np.random.default_rng(5).standard_normal((sum(new), heads * d)).astype(np.float32)
+    q = np.ldexp(np.clip(q, -3.5, 3.5), e).astype(np.float32)
+    q[-1, :d] = np.ldexp(q[-1, :d], -2 * e)   # a row of small ones beside them
+    print("paged8 largest queries", new, e, kind, d, flush=True)
+    close(fdx.mha_paged(f.cache, q, new, heads), f.reference(q, new, heads))
