@@ -2,7 +2,6 @@
 #pragma once
 #include <cmath>
 #include <cstdint>
-#include <type_traits>
 
 #include "common.hpp"
 #include "kv_pages.hpp"
@@ -233,57 +232,6 @@ __device__ __forceinline__ void raise_flag(const RaggedParams& p, bool on)
 {
     if (on && p.error_flag)
         *p.error_flag = 1;
-}
-
-// A row's sums over several ranges of keys, by one wave: sum of 2^(m - M) l o over them, divided by that of 2^(m - M) l, into the row's place.
-// out(i), size(i): where the sums of range i are.
-template <class Out, class Size>
-__device__ __forceinline__ void join_parts(const RaggedParams& p, int row, int head, int parts, const Out& out, const Size& size)
-{
-    const int lane = threadIdx.x & 63;
-    // a lane a range for the sizes, then all lanes a range at a time for the rows, up to sixteen of them on their way together
-    float top = -INFINITY;
-    for (int i0 = 0; i0 < parts; i0 += 64)
-        if (i0 + lane < parts)
-            top = fmaxf(top, size(i0 + lane)[0]);
-    top = wave_all<true>(top);
-    const float m = top == -INFINITY ? 0.f : top;
-    float l = 0.f, o0 = 0.f, o1 = 0.f;
-    for (int i0 = 0; i0 < parts; i0 += 64) {
-        float w = 0.f;
-        if (i0 + lane < parts) {
-            const float* at = size(i0 + lane);
-            w = at[1] * __builtin_amdgcn_exp2f(at[0] - m);
-        }
-        l += wave_all<false>(w);
-        const int count = parts - i0 < 64 ? parts - i0 : 64;
-        auto add = [&](int i, auto width) { // ranges i .. i + width - 1
-            constexpr int W = decltype(width)::value;
-            float x0[W], x1[W];
-#pragma unroll
-            for (int z = 0; z < W; ++z) {
-                const float* from = out(i0 + (i + z < count ? i + z : i));
-                x0[z] = from[lane < p.dv ? lane : 0];
-                x1[z] = from[64 + lane < p.dv ? 64 + lane : 0];
-            }
-#pragma unroll
-            for (int z = 0; z < W; ++z) {
-                const float wi = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), i + z < count ? i + z : i));
-                o0 = fmaf(i + z < count ? wi : 0.f, x0[z], o0);
-                o1 = fmaf(i + z < count ? wi : 0.f, x1[z], o1);
-            }
-        };
-        int i = 0;
-        for (; count - i > 4; i += 16)
-            add(i, std::integral_constant<int, 16>());
-        if (i < count)
-            add(i, std::integral_constant<int, 4>());
-    }
-    float* to = p.out + (int64_t)row * p.ldo + (int64_t)head * p.dv;
-    if (lane < p.dv)
-        to[lane] = finish(o0, l, top != -INFINITY);
-    if (64 + lane < p.dv)
-        to[64 + lane] = finish(o1, l, top != -INFINITY);
 }
 
 } // namespace fdx

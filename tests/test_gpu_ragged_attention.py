@@ -952,3 +952,41 @@ def test_packed_split_once_values_beside_infinities_and_nan(fdx, what, name, row
     ok = np.isfinite(want)
     assert np.array_equal(np.isfinite(got), ok)
     close(got[ok], want[ok])
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("parts", [2, 3, 4, 5, 6, 7, 9, 12, 15, 16, 17, 18])
+def test_paged_infinite_values_in_one_of_several_ranges(fdx, parts, kind):
+    """One token over ranges of 256 keys, a value of one of them infinite: so is the mean of its depth, and nothing else, whichever range it is."""
+    n, kv, d, heads = 256 * parts, 2, 64, 4
+    r = np.random.default_rng(parts)
+    k, v = (r.standard_normal((n, kv * d)).astype(np.float32) for _ in range(2))
+    q = r.standard_normal((1, heads * d)).astype(np.float32)
+    cache = fdx.PagedCache(-(-n // 64), 64, kv, d, d, 1, n, kind)
+    base = attend(q, *((k, v) if kind == "f32" else (bf16(k), bf16(v))), heads, kv, [n]).reshape(heads, d)
+    for part in range(parts):
+        x, what = v.copy(), (-1) ** part * np.inf
+        x[256 * part + 5, 7] = what
+        cache.release(0)
+        fdx.kv_append(cache, k, x, [n])
+        print("paged infinity in a range", parts, part, kind, flush=True)
+        got = fdx.mha_paged(cache, q, [1], heads).reshape(heads, d)
+        assert (got[:2, 7] == what).all(), (part, got[:2, 7])   # heads of key head 0
+        got[:2, 7] = base[:2, 7]
+        close(got, base)
+
+
+@pytest.mark.parametrize("n", [700, 1100, 2000])
+def test_packed_infinite_values_in_one_of_several_ranges(fdx, n):
+    """The same for a prompt whose tiles are cut in ranges."""
+    r, heads = np.random.default_rng(8), 6
+    q, k, v = (r.standard_normal((n, h * 64)).astype(np.float32) for h in (heads, 1, 1))
+    base = packed_reference(q, k, v, [n], heads, 1, True).reshape(n, heads, 64)
+    for row in range(5, n, 128):
+        x = v.copy()
+        x[row, 7] = np.inf
+        print("packed infinity in a range", n, row, flush=True)
+        got = fdx.mha_packed(q, k, x, [n], heads, 1, 64, 64).reshape(n, heads, 64)
+        assert (got[row:, :, 7] == np.inf).all() and np.isfinite(got[:row]).all()
+        got[row:, :, 7] = base[row:, :, 7]
+        close(got, base)
