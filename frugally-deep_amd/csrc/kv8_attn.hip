@@ -1299,6 +1299,9 @@ extern "C" size_t fdx_mha_paged8_scratch_bytes(int tokens, int max_new, int head
     if (!c || tokens <= 0 || max_new <= 0 || heads <= 0 || c->kv_heads <= 0 || heads % c->kv_heads != 0 || c->dk <= 0 || c->dv <= 0 || c->n_seqs <= 0
         || c->max_len <= 0)
         return 0;
+    // what the call refuses has no plan, whose numbers would leave their types
+    if ((int64_t)tokens * heads > (1 << 25) || (int64_t)c->n_seqs * c->kv_heads > (1 << 22) || c->max_len > (1 << 30) || c->dk > 128 || c->dv > 128)
+        return 0;
     const Plan8 plan = plan8(tokens, max_new, heads, c);
     return sizeof(float) * (plan.few_floats + plan.tiles.tile_floats(c->dv));
 }

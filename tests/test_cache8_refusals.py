@@ -221,3 +221,23 @@ def test_the_definition(fdx):
     h.append(lambda p: p, 0, np.float32([[[1, -0.5]], [[2, 0]], [[127, 1]]]), 0)
     h.append(lambda p: p, 3, np.float32([[[254, 3]]]), 0)
     assert h.scales[0].ravel()[:2].tolist() == [np.float32(2) / np.float32(127), 2.0] and decode(h.codes[0][2:4, 0], "i8").tolist() == [[64, 0], [127, 2]]
+
+
+def test_paged_sizes_beyond_every_limit(fdx):
+    """Numbers that the call refuses are refused whatever they are, and need no scratch memory."""
+    most = 2 ** 31 - 1
+    for n_seqs in ((1 << 21) + 1, (1 << 30) - 1, 1 << 30, most):
+        for max_len in (1, 64):
+            c = ctypes.byref(pages8(fdx, n_seqs=n_seqs, max_len=max_len))
+            assert fdx.lib.fdx_mha_paged8_scratch_bytes(5, 2, 4, c) == 0
+            refused(fdx, paged(fdx, c), INVALID, "too many")
+    c = ctypes.byref(pages8(fdx, n_pages=1, page_size=1 << 24, table_width=most, max_len=most, n_seqs=most, block=1))
+    assert fdx.lib.fdx_mha_paged8_scratch_bytes(5, 2, 4, c) == 0
+    refused(fdx, paged(fdx, c), INVALID, "2^30")
+    for tokens, max_new, heads in ((most, most, 2), (5, most, most - 1), (most, most, most - 1)):
+        c = ctypes.byref(pages8(fdx))
+        assert fdx.lib.fdx_mha_paged8_scratch_bytes(tokens, max_new, heads, c) == 0
+        refused(fdx, paged(fdx, c, tokens=tokens, max_new=max_new, heads=heads), INVALID, "too many")
+    c = ctypes.byref(pages8(fdx, kv_heads=1 << 23, dk=1, dv=1))
+    assert fdx.lib.fdx_mha_paged8_scratch_bytes(5, 2, 1 << 23, c) == 0
+    refused(fdx, paged(fdx, c, heads=1 << 23), INVALID, "too many")
