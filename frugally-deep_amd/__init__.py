@@ -790,6 +790,9 @@ def beam_select(logits, scores, keep, done=None, end_id=-1):
     n, beams, vocab = logits.shape
     if done is not None and np.shape(done) != (n, beams):
         raise FdxError("done of shape %s for %d sequences of %d beams" % (np.shape(done), n, beams))
+    keep, end_id = int(_whole("keep", keep)), max(int(_whole("end_id", end_id)), -1)
+    if not -2 ** 31 <= keep < 2 ** 31 or end_id >= 2 ** 31:
+        raise FdxError("keep %d or end_id %d beyond 32 bits" % (keep, end_id))
     if n == 0:
         return dict({key: np.zeros((0, keep), np.int32) for key in ("parents", "tokens", "done")[:3 if end_id >= 0 else 2]},
                     scores=np.zeros((0, keep), np.float32))

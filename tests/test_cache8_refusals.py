@@ -241,3 +241,22 @@ def test_paged_sizes_beyond_every_limit(fdx):
     c = ctypes.byref(pages8(fdx, kv_heads=1 << 23, dk=1, dv=1))
     assert fdx.lib.fdx_mha_paged8_scratch_bytes(5, 2, 1 << 23, c) == 0
     refused(fdx, paged(fdx, c, heads=1 << 23), INVALID, "too many")
+
+
+def test_beams_of_numbers_beyond_32_bits(fdx, monkeypatch):
+    """No number reaches the library as another one: those that 32 bits cannot hold are refused, every negative end_id is none."""
+    monkeypatch.setattr(fdx, "DevBuf", HostBuf)
+    x, scores = np.zeros((2, 3, 10), np.float32), np.zeros((2, 3))
+    for change in (dict(keep=2 ** 32 + 3), dict(keep=-2 ** 32 + 3), dict(keep=2 ** 31), dict(end_id=2 ** 32 + 7), dict(end_id=2 ** 31), dict(end_id=2.5), dict(keep=1.5)):
+        with pytest.raises(fdx.FdxError, match="32 bits|whole numbers"):
+            fdx.beam_select(x, scores, **dict(dict(keep=3), **change))
+    seen = []
+
+    def call(*args):
+        seen.append(args[7:9])
+        return INVALID
+    monkeypatch.setattr(fdx.lib, "fdx_beam_select_f32", call)
+    for end_id, want in ((-1, -1), (-2 ** 32 + 7, -1), (np.int64(7), 7)):
+        with pytest.raises(fdx.FdxError):
+            fdx.beam_select(x, scores, np.int64(3), None, end_id)
+        assert seen[-1] == (want, 3) and all(type(a) is int for a in seen[-1])
