@@ -3,8 +3,8 @@
 // Which pages are kept is a bit each; the free ones are then the zeros, taken from the lowest on by ranks: of the sequences' needs (a prefix
 // sum) and of the zeros (prefix sums over the words' counts), so nothing depends on the order in which threads arrive.  A chain of a dozen
 // dependent steps, bound by their latency: one workgroup takes them all where its LDS holds a number for each sequence and a bit for each page
-// (64 groups of eight beams, 24 000 entries of the table: 14 us; through memory 28), so that the steps meet at barriers instead of launches.  Larger
-// tables are marked by a launch of their own.  The copies follow in a launch, at the memory's rate (33 MB read and written 8 us).  Of the 14 us nine are the
+// (64 groups of eight beams, 24 000 entries of the table: 14 us), so that the steps meet at barriers instead of launches.  Larger tables are marked
+// by a launch of their own (kSmallEntries).  The copies follow in a launch, at the memory's rate (33 MB read and written 8 us).  Of the 14 us nine are the
 // table's passage: more loads of a thread at once, the next ones beside the marks, or a wave's lanes on one sequence took 16 to 20.
 #include <climits>
 
@@ -64,7 +64,10 @@ __device__ __forceinline__ void agent_store(int32_t* at, int v) { __hip_atomic_s
 constexpr int kForkThreads = 1024;
 // what a workgroup's LDS is laid out for: a sequence a thread, and a hash table of twice as many pages
 constexpr int kSmallSeqs = kForkThreads, kSmallWords = 4096, kHash = 2 * kSmallSeqs;
-constexpr int64_t kSmallEntries = 1 << 17;
+// Entries of a table (sequences times its width, capacity that nobody uses too) that one workgroup walks, 8192 in some 3 us; marks by a launch of their own
+// cost two more launches and dependent loads.  us of the call in one workgroup / through memory: 512 sequences, 6144 entries 14.5 / 21.6, 24 064 18.2 / 30.5,
+// 40 960 24.2 / 31.6, 60 416 31.4 / 31.6, 81 920 38.4 / 34.5, 131 072 57.8 / 36.8; 1024 sequences, 61 440 33.7 / 36.9, 131 072 59.6 / 41.4, 260 096 104.3 / 50.9.
+constexpr int64_t kSmallEntries = 1 << 16;
 
 // entry j of a sequence in the table: the page that it shares, -1 if none
 __device__ __forceinline__ int checked_page(const ForkParams& p, int at, bool& odd)

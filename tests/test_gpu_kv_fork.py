@@ -277,3 +277,21 @@ def test_python_fork(fdx):
         fdx.kv_append(c, np.zeros((6, 4), np.float32), np.zeros((6, 4), np.float32), [6, 0, 0])
         fdx.kv_fork(c, [0, 0, 0])
     assert c.lens.tolist() == [6, 0, 0] and len(c.free) == 1
+
+
+@pytest.mark.parametrize("n,width", [(1024, 63), (1024, 64), (1024, 65), (512, 128), (513, 128), (512, 256), (1, 65536), (1, 65537)])
+def test_fork_of_tables_beside_the_border_of_its_forms(fdx, n, width):
+    """Tables of 64 512 to 131 072 entries, the most that one workgroup walks (65 536) among them; sequences of any length in them."""
+    r = np.random.default_rng(width)
+    page = 4
+    lens = r.integers(0, np.where(r.random(n) < 0.9, min(width, 12), width) * page - 1).astype(np.int32)
+    counts = -(-lens.astype(np.int64) // page)
+    total = int(counts.sum())
+    order, at = r.permutation(total + 3 * n + 5), np.cumsum(counts) - counts
+    table = np.full((n, width), -1, np.int32)
+    for i in range(n):
+        table[i, :counts[i]] = order[at[i]:at[i] + counts[i]]
+    p = Pages(fdx, "i8", len(order), page, 1, 4, 4, 2)
+    print("fork border", n, width, len(order), flush=True)
+    for _ in range(2):
+        table, lens = p.step(table, lens, r.integers(-1, n, n).astype(np.int32), np.ones(n, np.int32), width * page)
