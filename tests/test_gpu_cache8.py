@@ -768,3 +768,42 @@ def test_paged_queries_near_the_end_of_fp32(fdx, new, e, kind, d):
     q[-1, :d] = np.ldexp(q[-1, :d], -2 * e)   # a row of small ones beside them
     print("paged8 largest queries", new, e, kind, d, flush=True)
     close(fdx.mha_paged(f.cache, q, new, heads), f.reference(q, new, heads))
+
+
+def test_two_threads_at_every_repetition(fdx):
+    """As test_two_threads, all repetitions of either thread compared, and begun together."""
+    import threading
+    heads, times, errors = 4, 6, []
+    r = np.random.default_rng(12)
+    k, v, q = (r.standard_normal((2, n, w)).astype(np.float32) for n, w in ((500, 128), (500, 128), (42, heads * 64)))
+    logits, scores = r.standard_normal((2, 3, 4, 3001)).astype(np.float32), -r.random((2, 3, 4)).astype(np.float32)
+
+    def steps(i):
+        c = fdx.PagedCache(70, 16, 2, 64, 64, 2, 400, ("e4m3", "i8")[i], 8)
+        out = []
+        for at in range(0, 500, 100):
+            fdx.kv_append(c, k[i, at:at + 100], v[i, at:at + 100], [40 + i, 60 - i])
+            out += [fdx.mha_paged(c, q[i, :2], [1, 1], heads), fdx.mha_paged(c, q[i], [41, 1], heads)]
+            best = fdx.beam_select(logits[i], scores[i], 4)
+            out += [best[key] for key in sorted(best)]
+            fdx.kv_fork(c, [0, 1] if at % 200 else [1, 0])
+            out += [c.table.copy(), c.lens.copy()]
+        return out
+    want, got, together = [steps(0), steps(1)], [[], []], threading.Barrier(2)
+
+    def work(i):
+        try:
+            for _ in range(times):
+                together.wait(60)
+                got[i].append(steps(i))
+        except Exception as e:   # reported below, by the test's own thread
+            errors.append(e)
+            together.abort()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not errors, errors
+    for i in range(2):
+        assert len(got[i]) == times
+        for one in got[i]:
+            assert len(one) == len(want[i]) and all(np.array_equal(x, y) for x, y in zip(one, want[i]))
