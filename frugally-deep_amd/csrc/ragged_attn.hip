@@ -1219,14 +1219,18 @@ __global__ __launch_bounds__(256) void ragged_join_kernel(RaggedParams p)
             top = fmaxf(top, part.size(i0 + lane, id, p.dv)[0]);
     top = wave_all<true>(top);
     const float m = top == -INFINITY ? 0.f : top;
-    float l = 0.f, o0 = 0.f, o1 = 0.f;
+    auto weight = [&](int i) {
+        const float* at = part.size(i, id, p.dv);
+        return at[1] * __builtin_amdgcn_exp2f(at[0] - m);
+    };
+    float w = lane < parts ? weight(lane) : 0.f, l = wave_all<false>(w), o0 = 0.f, o1 = 0.f;
+    for (int i0 = 64; i0 < parts; i0 += 64)
+        l += wave_all<false>(i0 + lane < parts ? weight(i0 + lane) : 0.f);
+    // Weights come to less than one, so that a sum is in fp32's range where its mean is; a power of two leaves every result as it was.
+    const float down = l > 0.f && l < 0x1p120f ? __builtin_bit_cast(float, (uint32_t)(253 - exponent(l)) << 23) : 1.f;
+    l *= down;
     for (int i0 = 0; i0 < parts; i0 += 64) {
-        float w = 0.f;
-        if (i0 + lane < parts) {
-            const float* at = part.size(i0 + lane, id, p.dv);
-            w = at[1] * __builtin_amdgcn_exp2f(at[0] - m);
-        }
-        l += wave_all<false>(w);
+        w = (i0 == 0 ? w : (i0 + lane < parts ? weight(i0 + lane) : 0.f)) * down;
         const int count = parts - i0 < 64 ? parts - i0 : 64;
         auto add = [&](int i, auto width) { // ranges i .. i + width - 1
             constexpr int W = decltype(width)::value;

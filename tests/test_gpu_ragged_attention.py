@@ -990,3 +990,34 @@ def test_packed_infinite_values_in_one_of_several_ranges(fdx, n):
         assert (got[row:, :, 7] == np.inf).all() and np.isfinite(got[:row]).all()
         got[row:, :, 7] = base[row:, :, 7]
         close(got, base)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("new", [1, 12, 100])
+@pytest.mark.parametrize("keys,least", [(300, -1), (900, -1), (900, 0.99), (3000, 0.9)])
+def test_paged_values_near_the_end_of_fp32(fdx, keys, least, new, kind):
+    """Values up to 3.2e38, also all of one sign, over one range of keys and over several: results are means, none passes fp32's range.  The keys of
+    either half have one score, so its error is common to them."""
+    heads, kv, d = 4, 2, 64
+    k, v = np.zeros((keys, kv * d), np.float32), (3.2e38 * np.random.default_rng(2).uniform(least, 1, (keys, kv * d))).astype(np.float32)
+    k[keys // 2:, ::d] = 7.9 * np.log(2) * 8
+    cache = fdx.PagedCache(-(-keys // 16), 16, kv, d, d, 1, keys, kind)
+    fdx.kv_append(cache, k, v, [keys])
+    q = np.zeros((new, heads * d), np.float32)
+    q[:, ::d] = 1
+    print("paged largest values", keys, least, new, kind, flush=True)
+    got = fdx.mha_paged(cache, q, [new], heads).astype(np.float64)
+    want = attend(q, *((k, v) if kind == "f32" else (bf16(k), bf16(v))), heads, kv, np.arange(keys - new, keys) + 1)
+    close(np.ldexp(got, -127), np.ldexp(want, -127))
+
+
+@pytest.mark.parametrize("n,heads", [(300, 6), (700, 6), (2000, 6), (2100, 1)])
+@pytest.mark.parametrize("least", [-1, 0.99])
+def test_packed_values_near_the_end_of_fp32(fdx, n, heads, least):
+    """The same for prompts."""
+    r = np.random.default_rng(3)
+    q, k = (r.standard_normal((n, h * 64)).astype(np.float32) for h in (heads, 1))
+    v = (3.2e38 * r.uniform(least, 1, (n, 64))).astype(np.float32)
+    print("packed largest values", n, heads, least, flush=True)
+    got = fdx.mha_packed(q, k, v, [n], heads, 1, 64, 64).astype(np.float64)
+    close(np.ldexp(got, -127), np.ldexp(packed_reference(q, k, v, [n], heads, 1, True), -127))
