@@ -1,6 +1,6 @@
 // The best continuations of a sequence's beams over the vocabulary.
 //
-//   total(b, t) = score_b + x[b, t] - (m_b + log sum exp(x[b, :] - m_b)), the best `keep` of beams * vocab
+//   total(b, t) = score_b + (x[b, t] - m_b) - log sum exp(x[b, :] - m_b), the best `keep` of beams * vocab
 // A row's order is its logits', so its `keep` likeliest are all that can be among the best.  Two launches: a workgroup reads a row, or a part of one,
 // once, and leaves its sum and its list (score_lists.hpp); then a workgroup a sequence brings the lists together.
 //  * Totals of different beams decide an order, so sums are held in 64 bits (a thread's chunk in 32: some 20 terms of one size) and totals are taken in
@@ -161,7 +161,7 @@ __global__ __launch_bounds__(256) void beam_select_kernel(BeamParams p)
 {
     __shared__ Continuations<kMostTop * kMostTop> items;
     __shared__ Continuations<kBeamLists> heads; // of each list the first `deep`
-    __shared__ double before_of[kMostBeams], log_sum_of[kMostBeams];
+    __shared__ double before_of[kMostBeams], most_of[kMostBeams]; // a beam's score less its sum's logarithm, its largest logit
     __shared__ int ended_of[kMostBeams], count;
     __shared__ Continuation threshold;
     const int tid = threadIdx.x;
@@ -194,8 +194,10 @@ __global__ __launch_bounds__(256) void beam_select_kernel(BeamParams p)
             z += __shfl_xor(z, w, 64);
         if (part == 0) {
             const bool bad = !(score < INFINITY) || (reads && !(z < INFINITY)); // a NaN or an infinity: no continuation
-            before_of[b] = bad || !finite || (reads && z == 0.0) ? -INFINITY : (double)score;
-            log_sum_of[b] = reads && z > 0.0 ? most + log(z) : 0.0;
+            // The largest logit stays apart: beside one of 10^12 or more the logarithm has no room, beside fp32's lowest value, which masks are made of, none at all.
+            const bool sums = reads && z > 0.0;
+            before_of[b] = bad || !finite || (reads && z == 0.0) ? -INFINITY : sums ? (double)score - log(z) : (double)score;
+            most_of[b] = sums ? most : 0.0;
             ended_of[b] = finite && done;
             if (bad && p.error_flag)
                 *p.error_flag = 1;
@@ -209,7 +211,7 @@ __global__ __launch_bounds__(256) void beam_select_kernel(BeamParams p)
             return list == b * p.parts && j == 0 ? Continuation { before, 1, b } : Continuation { -INFINITY, 0, b };
         if (key == 0 || before == -INFINITY)
             return { -INFINITY, 0, b };
-        return { before + ((double)bits_score((uint32_t)(key >> 32)) - log_sum_of[b]), key, b };
+        return { before + ((double)bits_score((uint32_t)(key >> 32)) - most_of[b]), key, b };
     };
     if (tid < n_heads)
         heads.put(tid, listed(head_list, tid - head_list * deep, first_key));

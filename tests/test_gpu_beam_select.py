@@ -248,3 +248,38 @@ def test_runs_are_equal(fdx):
     for _ in range(3):
         again = fdx.beam_select(x, scores, 8, None, 3)
         assert all(np.array_equal(first[key], again[key]) for key in first)
+
+
+@pytest.mark.parametrize("vocab", [7, 300, 20000])
+@pytest.mark.parametrize("value", [-3.4028235e38, 3.4028235e38, -1e30, 1e20, -1e13])
+def test_rows_of_one_far_value(fdx, value, vocab):
+    """Every token of a row has one logit of any size, as where a mask of fp32's lowest value leaves nothing: each has the probability 1 / vocab, which beams
+    with ordinary logits are compared with."""
+    far = np.full(vocab, value, np.float32)
+    x, _ = draw(12, 2, 3, vocab, keep=4)
+    x[0, 1], x[1, 0], x[1, 2] = far, far, far
+    scores = np.array([[-4, -3, -5], [-1, -3, -1.5]], np.float32)
+    got = fdx.beam_select(x, scores, 6)
+    for s in range(2):
+        every = []
+        for b in range(3):
+            row = x[s, b].astype(np.float64) - x[s, b].astype(np.float64).max()
+            every += [(float(scores[s, b]) + total, b, t) for t, total in enumerate(row - np.log(np.exp(row).sum()))]
+        every = sorted(every, key=lambda c: (-c[0], c[1], c[2]))[:6]
+        want = np.array([c[0] for c in every])
+        print("beam far value", value, vocab, got["scores"][s], want, flush=True)
+        assert got["parents"][s].tolist() == [3 * s + c[1] for c in every] and got["tokens"][s].tolist() == [c[2] for c in every]
+        assert (np.abs(got["scores"][s] - want) <= 4e-7 + 2.0 ** -23 * np.abs(want)).all()
+
+
+@pytest.mark.parametrize("vocab", [300, 20000])
+def test_masks_of_the_lowest_value(fdx, vocab):
+    """Rows with some tokens at fp32's lowest value beside ones with -infinity there: the same selection, the same scores; a row of nothing else is as likely
+    as any other of equal logits."""
+    r = np.random.default_rng(13)
+    x, scores = draw(14, 4, 3, vocab, keep=6)
+    out = r.random(x.shape) < 0.9
+    x[out] = -np.inf
+    y = np.where(out, np.finfo(np.float32).min, x)
+    a, b = fdx.beam_select(x, scores, 6), fdx.beam_select(y, scores, 6)
+    assert all(np.array_equal(a[key], b[key]) for key in a)
