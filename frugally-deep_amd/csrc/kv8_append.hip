@@ -154,13 +154,13 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Append8Params p)
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    float by = 1.f; // of the first block's earlier codes
+    float by = 1.f; // of the first block's earlier codes; below zero where they become 0
     if (lane < blocks && row0 >= 0) {
         const float most = __builtin_bit_cast(float, most_of[wave][lane]);
         const bool odd = !(most < INFINITY) || !(before < INFINITY);
         const float now = odd ? NAN : fmaxf(fmaxf(most / most_code<KIND>(), kLeastScale), before);
         up_of[wave][lane] = odd ? 0.f : 1.f / now;
-        by = odd ? 0.f : before / now;
+        by = odd ? -1.f : before / now;
         *scale = now;
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -191,7 +191,7 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Append8Params p)
             const int r = quotient(e, by_chunks);
             uint8_t* at = to + (first_row + r) * a_row + (e - r * chunks) * W;
             float y[4] = { 0.f, 0.f, 0.f, 0.f };
-            if (by != 0.f) {
+            if (by >= 0.f) { // where a scale has grown 2^150-fold this is zero, and codes are zeros of their own sign
                 from_codes<KIND>(W == 4 ? *reinterpret_cast<uint32_t*>(at) : *at, y);
 #pragma unroll
                 for (int i = 0; i < W; ++i)

@@ -807,3 +807,22 @@ def test_two_threads_at_every_repetition(fdx):
         assert len(got[i]) == times
         for one in got[i]:
             assert len(one) == len(want[i]) and all(np.array_equal(x, y) for x, y in zip(one, want[i]))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("d", [64, 13])
+def test_append_of_scales_beyond_each_other(fdx, d, kind):
+    """A block whose scale grows so far that what was there in front has no size beside it: earlier codes are zeros of their own sign, as rounding makes
+    them; and where a NaN joins them, zeros."""
+    for first, then in ((-120, 60), (-149, 127), (-60, 100), (-126, 24), (-120, 28)):
+        r = np.random.default_rng(-first)
+        c, host = fdx.PagedCache(1, 8, 2, d, d, 1, 8, kind, 8), HostCache(1, 8, 2, d, d, kind, 8)
+        for at, e in enumerate((first, then, first, None)):
+            x = np.ldexp(r.uniform(-1.9, 1.9, (2, 2 * d)), 0 if e is None else e).astype(np.float32)
+            if e is None:
+                x[1, 3] = np.nan
+            print("append8 scales", first, then, at, d, kind, flush=True)
+            fdx.kv_append(c, x, -x, [2])
+            for which, y in enumerate((x, -x)):
+                host.append(lambda p: p, 2 * at, y.reshape(2, 2, d), which)
+            same(c, host)
