@@ -10,7 +10,8 @@
 //    continuations reach it, and of a list whose first is behind it none does.  Those that reach it, twice as many as are kept on random logits and
 //    keep * keep at most, are ordered by counting the better ones of each.  32 sequences of 16 beams, 32 kept of 50 257 tokens, 32 lists:
 //    282 us where all of 32 lists were ordered, 53 so.
-// 64 sequences of 8 beams over 50 257 tokens (103 MB): rows 28 to 31 us, 3.3 TB/s, the selection 7; four rows take the same 7 each, two launches of dependent steps.
+// 64 sequences of 8 beams over 50 257 tokens, a sixth of which have ended (86 MB): rows 27 us, 3.2 TB/s, the selection 7; four rows take the same 7 each, two
+// launches of dependent steps.
 // The next chunk's logits on their way take registers: 35 -> 39 us, with half the chunk 38.
 #include "score_lists.hpp"
 #include "kv_pages.hpp"

@@ -22,7 +22,7 @@ namespace fdx {
 //  * Codes are fp16 values exactly; a query is held as two fp16 values (f16_split.hpp), and so are its probabilities times their values' scales, by a
 //    power that keeps the largest of them so far in fp16's range: a row has sums of its own power, and none depends on keys that it does not see.
 //  * A key's scale meets its score; lane (c, g) has looked up one scale, and a lane's number in its row of sixteen names it for all of them.
-// Bound by memory: a wave has its next block on its way beside the one it works on.  64 sequences of 4000 keys, 32 / 8 heads of 128 (528 MB), 107 us,
+// Bound by memory: a wave has its next block on its way beside the one it works on.  64 sequences of 4000 keys, 32 / 8 heads of 128 (528 MB), 106 us,
 // 4.9 TB/s; 64 of 300 to 7900 (315 MB) 84, 3.8 TB/s: beginnings and ends of segments, two or three a workgroup, take a sixth; one token over 100 003 keys (205
 // MB) 49, 4.2.  A third block on its way 91 -> 94 us; three workgroups a CU would spill 37 registers.
 template <int D, bool WIDE>
@@ -549,7 +549,7 @@ __global__ __launch_bounds__(256, WIDE ? 2 : 1) void paged8_few_kernel(RaggedPar
 //    the values' scales, by a power that keeps the largest of them so far between 2^6 and 2^15: a row has sums of its own power, and none
 //    depends on keys that it does not see.  A key's scale meets its score.
 // Vector instructions (60 % of the time) and matrix instructions (44 %) mostly add up: four sequences that bring 1000 tokens to 3000 keys, 32 / 8
-// heads of 128 (164 GFLOP), 380 us, 430 TFLOP/s, where two products for one leave 620.
+// heads of 128 (164 GFLOP), 371 us, 442 TFLOP/s, where two products for one leave 620.
 //  * LDS holds two tiles.  While the probabilities of tile t meet its values, the scores of tile t + 1 are multiplied; tile t + 2's keys and tile
 //    t + 1's values go to LDS, what comes behind them to registers; one barrier a tile.
 template <int D>
@@ -958,7 +958,7 @@ __device__ __forceinline__ void tile8_body(const RaggedParams& p, const Scales8&
 #pragma unroll
             for (int g = 0; g < 2 * HALVES; ++g)
                 vf[g] = SIXTEENS ? vf[g] * power.up : power.up;
-            __builtin_amdgcn_s_setprio(1); // beside another workgroup's wave that is not at its products (416 -> 406 us)
+            __builtin_amdgcn_s_setprio(1); // beside another workgroup's wave that is not at its products (four of 1000 of 3000 keys 391 -> 371 us)
             scores(next, ks);
             // O^T += V^T P^T
 #pragma unroll
@@ -1248,7 +1248,8 @@ constexpr int64_t kFewJoins = 1024; // rows that are joined by a workgroup each
 template <int D, int KIND>
 static void paged8_launch(const RaggedParams& p, const Plan8& plan, const Scales8& scales)
 {
-    // codes of a row and head are whole 16-byte vectors, those of q and out whole float4; rows start below 2^32 times 16 bytes
+    // codes of a row and head are whole 16-byte vectors, those of q and out whole float4; rows start below 2^32 times 16 bytes.  Where one is not so,
+    // codes are read byte by byte: 64 sequences of 4000 keys, 16 / 8 heads, 783 us at depth 100, 143 at 112.
     const uintptr_t all = reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.k)
         | reinterpret_cast<uintptr_t>(p.v);
     const int64_t rows = (int64_t)p.n_pages * p.page_size.by, ld = p.ldk > p.ldv ? p.ldk : p.ldv;
@@ -1256,7 +1257,7 @@ static void paged8_launch(const RaggedParams& p, const Plan8& plan, const Scales
     const unsigned tile_x = (unsigned)plan.tiles.tiles, tile_y = (unsigned)(plan.tiles.tile_ranges > 0 ? plan.tiles.tile_ranges : 1);
     const uint64_t tile_wgs = (uint64_t)tile_x * tile_y, all_wgs = tile_wgs + plan.few_wgs;
     // Blocks of whole sixteens (ranges start at multiples of 64): two multiplications less a score.  us without / with, 128 new tokens of 1000, 12 heads of
-    // 64: 25.8 / 23.6; two of 2000 of 3000, 16 / 4 heads of 64, 125.6 / 119.8; four of 1000 of 3000, 32 / 8 heads of 128, 386.5 / 380.2.
+    // 64: 25.8 / 23.5; two of 2000 of 3000, 16 / 4 heads of 64, 124.2 / 117.8; four of 1000 of 3000, 32 / 8 heads of 128, 379.8 / 370.8.
     const bool sixteens = scales.block.by % 16 == 0;
     if (wide && tile_wgs > 0 && plan.few_wgs > 0 && all_wgs < (1u << 23)) {
         if (sixteens)
