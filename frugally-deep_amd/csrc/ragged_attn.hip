@@ -1226,7 +1226,7 @@ __global__ __launch_bounds__(256) void ragged_join_kernel(RaggedParams p)
     float w = lane < parts ? weight(lane) : 0.f, l = wave_all<false>(w), o0 = 0.f, o1 = 0.f;
     for (int i0 = 64; i0 < parts; i0 += 64)
         l += wave_all<false>(i0 + lane < parts ? weight(i0 + lane) : 0.f);
-    // Weights come to less than one, so that a sum is in fp32's range where its mean is; a power of two leaves every result as it was.
+    // Weights come to less than one, so that a sum is in fp32's range where its mean is; a power of two rounds no result that is a normal number otherwise.
     const float down = l > 0.f && l < 0x1p120f ? __builtin_bit_cast(float, (uint32_t)(253 - exponent(l)) << 23) : 1.f;
     l *= down;
     for (int i0 = 0; i0 < parts; i0 += 64) {
